@@ -28,6 +28,7 @@
 #include "../../include/asmllm.h"
 #include "decode_persistent.cuh"
 #include "matvec.cuh"
+#include "serving.cuh"
 #include "tiles.cuh"
 
 using namespace asmllm;
@@ -854,6 +855,231 @@ ASMLLM_API int asm_rows_advance_async(const int64_t* keys, int32_t rows, int32_t
     return rc;
   const cudaError_t e = launch_rows_advance(reinterpret_cast<const long long*>(keys), rows, tokens, max_tokens, pos,
                                             n_prompt, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_error(e, name);
+  return ASM_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Serving operators (rope_append.cu, attention_prompt.cu, attention_paged.cu,
+// rows_sample.cu)
+// ---------------------------------------------------------------------------
+namespace {
+
+// The view's own arguments -> KvArgs; pointers are looked at in check_kv_pointers.
+int check_kv(const char* name, const asm_kv_t* d, bool need_table, KvArgs* out) {
+  if (!d) return set_error(ASM_E_INVALID, "%s: null key-value descriptor", name);
+  if (d->dtype != ASM_DT_F16 && d->dtype != ASM_DT_BF16)
+    return set_error(ASM_E_UNSUPPORTED, "%s: cache type %d (fp16 or bf16)", name, d->dtype);
+  if (d->head_dim != 64 && d->head_dim != 128)
+    return set_error(ASM_E_UNSUPPORTED, "%s: head_dim %d (64 or 128)", name, d->head_dim);
+  if (d->batch < 0 || d->n_kv_heads <= 0 || d->n_pages <= 0 || d->page_size <= 0)
+    return set_error(ASM_E_INVALID, "%s: need batch >= 0 and n_kv_heads, n_pages, page_size > 0", name);
+  if (need_table && !d->table) return set_error(ASM_E_INVALID, "%s: null page table", name);
+  KvArgs& kv = *out;
+  if (d->table) {
+    if (d->page_size < 16 || d->page_size > 256 || (d->page_size & (d->page_size - 1)))
+      return set_error(ASM_E_UNSUPPORTED, "%s: page_size %d (a power of two from 16 to 256)", name, d->page_size);
+    if (d->table_width <= 0 || d->table_stride < d->table_width)
+      return set_error(ASM_E_INVALID, "%s: need 0 < table_width <= table_stride", name);
+    while ((1 << kv.page_shift) < d->page_size) ++kv.page_shift;
+  } else if (d->n_pages != 1) {
+    return set_error(ASM_E_INVALID, "%s: packed keys are one page (n_pages %d)", name, d->n_pages);
+  }
+  const int64_t s[3] = {d->page_stride, d->token_stride, d->head_stride};
+  for (int i = 0; i < 3; ++i)
+    if (s[i] <= 0 || s[i] % 8 || s[i] >= (1ll << 38))
+      return set_error(ASM_E_INVALID, "%s: key-value strides must be positive multiples of 8 elements", name);
+  if ((uintptr_t)d->k % 16 || (uintptr_t)d->v % 16)
+    return set_error(ASM_E_INVALID, "%s: k and v must be 16-byte aligned", name);
+  kv.k = d->k;
+  kv.v = d->v;
+  kv.page_stride = d->page_stride;
+  kv.token_stride = d->token_stride;
+  kv.head_stride = d->head_stride;
+  kv.table = d->table;
+  kv.table_stride = d->table_stride;
+  kv.len = d->len;
+  kv.cu = d->cu;
+  kv.batch = d->batch;
+  kv.n_pages = d->n_pages;
+  kv.page_size = d->page_size;
+  kv.width = d->table_width;
+  kv.n_kv = d->n_kv_heads;
+  kv.head_dim = d->head_dim;
+  kv.dtype = d->dtype;
+  return ASM_OK;
+}
+
+int check_kv_pointers(const char* name, const KvArgs& kv) {
+  int rc;
+  if ((rc = require_device(name, kv.k, "k")) || (rc = require_device(name, kv.v, "v"))) return rc;
+  if (kv.table) {
+    if ((rc = require_device(name, kv.table, "page table")) || (rc = require_device(name, kv.len, "lengths"))) return rc;
+  } else if ((rc = require_device(name, kv.cu, "key offsets"))) {
+    return rc;
+  }
+  return ASM_OK;
+}
+
+int check_heads(const char* name, int n_heads, int n_kv) {
+  if (n_heads <= 0 || n_heads % n_kv || n_heads > 65535)
+    return set_error(ASM_E_INVALID, "%s: n_heads %d is not a multiple of n_kv_heads %d", name, n_heads, n_kv);
+  return ASM_OK;
+}
+
+int check_query(const char* name, const void* q, int64_t row_stride, int64_t head_stride, const void* out,
+                int out_dtype, int cache_dtype) {
+  if (row_stride <= 0 || row_stride % 8 || head_stride <= 0 || head_stride % 8 || (uintptr_t)q % 16 ||
+      (uintptr_t)out % 16)
+    return set_error(ASM_E_INVALID, "%s: q strides must be positive multiples of 8, q and out 16-byte aligned", name);
+  if (out_dtype != ASM_DT_F32 && out_dtype != cache_dtype)
+    return set_error(ASM_E_UNSUPPORTED, "%s: out is fp32 or of the cache's type", name);
+  return ASM_OK;
+}
+
+}  // namespace
+
+ASMLLM_API int asm_rope_append_async(const void* qkv, int32_t qkv_dtype, int64_t qkv_stride, const float* rope_cs,
+                                     int32_t rope_len, const int32_t* cu_q, int32_t rows, int32_t n_heads,
+                                     void* q_out, const asm_kv_t* kvd, void* stream) {
+  const char* name = "asm_rope_append_async";
+  KvArgs kv;
+  int rc;
+  if ((rc = check_kv(name, kvd, true, &kv)) || (rc = check_heads(name, n_heads, kv.n_kv))) return rc;
+  if (rows < 0 || rope_len <= 0 || (!cu_q && rows != kv.batch))
+    return set_error(ASM_E_INVALID, "%s: need rows >= 0 (the batch without cu_q) and rope_len > 0", name);
+  if (qkv_dtype != ASM_DT_F32 && qkv_dtype != kv.dtype)
+    return set_error(ASM_E_UNSUPPORTED, "%s: qkv is fp32 or of the cache's type", name);
+  if (qkv_stride < (int64_t)(n_heads + 2 * kv.n_kv) * kv.head_dim || qkv_stride % 8)
+    return set_error(ASM_E_INVALID, "%s: qkv_stride %lld too small or not a multiple of 8", name, (long long)qkv_stride);
+  if ((uintptr_t)qkv % 16 || (uintptr_t)rope_cs % 16 || (uintptr_t)q_out % 16)
+    return set_error(ASM_E_INVALID, "%s: misaligned buffer", name);
+  if (rows == 0 || kv.batch == 0) return ASM_OK;
+  if ((rc = check_kv_pointers(name, kv)) || (rc = require_device(name, qkv, "qkv")) ||
+      (rc = require_device(name, rope_cs, "rope_cs")) || (rc = require_device(name, q_out, "q_out")) ||
+      (cu_q && (rc = require_device(name, cu_q, "cu_q"))))
+    return rc;
+  RopeAppendArgs a;
+  a.qkv = qkv;
+  a.src_dtype = qkv_dtype;
+  a.qkv_stride = qkv_stride;
+  a.rope_cs = rope_cs;
+  a.rope_len = rope_len;
+  a.cu_q = cu_q;
+  a.rows = rows;
+  a.n_heads = n_heads;
+  a.q_out = q_out;
+  const cudaError_t e = launch_rope_append(a, kv, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_error(e, name);
+  return ASM_OK;
+}
+
+ASMLLM_API int asm_attention_prompt_async(const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                                          const int32_t* cu_q, int32_t rows, int32_t n_heads, float scale, void* out,
+                                          int32_t out_dtype, const asm_kv_t* kvd, void* stream) {
+  const char* name = "asm_attention_prompt_async";
+  KvArgs kv;
+  int rc;
+  if ((rc = check_kv(name, kvd, false, &kv)) || (rc = check_heads(name, n_heads, kv.n_kv)) ||
+      (rc = check_query(name, q, q_row_stride, q_head_stride, out, out_dtype, kv.dtype)))
+    return rc;
+  if (rows < 0 || rows > (1 << 22) || kv.batch > (1 << 15))
+    return set_error(rows < 0 ? ASM_E_INVALID : ASM_E_UNSUPPORTED, "%s: rows %d (0..2^22) of %d sequences (..2^15)",
+                     name, rows, kv.batch);
+  if (rows == 0 || kv.batch == 0) return ASM_OK;
+  if ((rc = check_kv_pointers(name, kv)) || (rc = require_device(name, q, "q")) ||
+      (rc = require_device(name, out, "out")) || (rc = require_device(name, cu_q, "cu_q")))
+    return rc;
+  PromptArgs a;
+  a.q = q;
+  a.q_row_stride = q_row_stride;
+  a.q_head_stride = q_head_stride;
+  a.out = out;
+  a.out_dtype = out_dtype;
+  a.cu_q = cu_q;
+  a.rows = rows;
+  a.n_heads = n_heads;
+  a.scale = scale;
+  const cudaError_t e = launch_attention_prompt(a, kv, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_error(e, name);
+  return ASM_OK;
+}
+
+ASMLLM_API int64_t asm_attention_paged_workspace(int32_t batch, int32_t n_heads, int32_t n_kv_heads,
+                                                 int32_t head_dim) {
+  if (batch < 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || (head_dim != 64 && head_dim != 128)) {
+    set_error(ASM_E_INVALID, "asm_attention_paged_workspace: need batch >= 0, n_heads a multiple of n_kv_heads, "
+                             "head_dim 64 or 128");
+    return -1;
+  }
+  return (int64_t)attention_paged_workspace(batch, n_heads, n_kv_heads, head_dim);
+}
+
+ASMLLM_API int asm_attention_paged_async(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t n_heads,
+                                         float scale, void* out, int32_t out_dtype, const asm_kv_t* kvd,
+                                         void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* name = "asm_attention_paged_async";
+  KvArgs kv;
+  int rc;
+  if ((rc = check_kv(name, kvd, true, &kv)) || (rc = check_heads(name, n_heads, kv.n_kv)) ||
+      (rc = check_query(name, q, q_row_stride, q_head_stride, out, out_dtype, kv.dtype)))
+    return rc;
+  if (kv.batch > (1 << 15)) return set_error(ASM_E_UNSUPPORTED, "%s: batch %d (at most 2^15)", name, kv.batch);
+  const size_t need = attention_paged_workspace(kv.batch, n_heads, kv.n_kv, kv.head_dim);
+  if (workspace_bytes < 0 || (size_t)workspace_bytes < need || (uintptr_t)workspace % 16)
+    return set_error(ASM_E_INVALID, "%s: workspace of %lld bytes, %zu needed (16-byte aligned)", name,
+                     (long long)workspace_bytes, need);
+  if (kv.batch == 0) return ASM_OK;
+  if ((rc = check_kv_pointers(name, kv)) || (rc = require_device(name, q, "q")) ||
+      (rc = require_device(name, out, "out")) || (need && (rc = require_device(name, workspace, "workspace"))))
+    return rc;
+  PagedArgs a;
+  a.q = q;
+  a.q_row_stride = q_row_stride;
+  a.q_head_stride = q_head_stride;
+  a.out = out;
+  a.out_dtype = out_dtype;
+  a.n_heads = n_heads;
+  a.scale = scale;
+  a.workspace = workspace;
+  const cudaError_t e = launch_attention_paged(a, kv, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_error(e, name);
+  return ASM_OK;
+}
+
+ASMLLM_API int asm_rows_sample_async(const void* logits, int32_t dtype, int32_t rows, int32_t n, int64_t stride,
+                                     const float* u, const float* temperature, const int32_t* top_k,
+                                     const float* top_p, const float* min_p, int32_t* tokens, void* stream) {
+  const char* name = "asm_rows_sample_async";
+  if (rows < 0 || n <= 0 || stride < n)
+    return set_error(ASM_E_INVALID, "%s: need rows >= 0, n > 0, stride >= n", name);
+  if (n > kSampleMaxN) return set_error(ASM_E_UNSUPPORTED, "%s: n=%d (at most %d)", name, n, kSampleMaxN);
+  if (dtype != ASM_DT_F32 && dtype != ASM_DT_F16 && dtype != ASM_DT_BF16)
+    return set_error(ASM_E_UNSUPPORTED, "%s: logits type %d", name, dtype);
+  if ((uintptr_t)logits % (dtype == ASM_DT_F32 ? 4 : 2))
+    return set_error(ASM_E_INVALID, "%s: misaligned buffer", name);
+  if (rows == 0) return ASM_OK;
+  int rc;
+  if ((rc = require_device(name, logits, "logits")) || (rc = require_device(name, u, "u")) ||
+      (rc = require_device(name, tokens, "tokens")) ||
+      (temperature && (rc = require_device(name, temperature, "temperature"))) ||
+      (top_k && (rc = require_device(name, top_k, "top_k"))) ||
+      (top_p && (rc = require_device(name, top_p, "top_p"))) ||
+      (min_p && (rc = require_device(name, min_p, "min_p"))))
+    return rc;
+  SampleArgs a;
+  a.logits = logits;
+  a.dtype = dtype;
+  a.stride = stride;
+  a.rows = rows;
+  a.n = n;
+  a.u = u;
+  a.temperature = temperature;
+  a.top_k = top_k;
+  a.top_p = top_p;
+  a.min_p = min_p;
+  a.tokens = tokens;
+  const cudaError_t e = launch_rows_sample(a, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_error(e, name);
   return ASM_OK;
 }

@@ -21,6 +21,7 @@ _lib = None
 
 ASM_OK, ASM_E_INVALID, ASM_E_UNSUPPORTED, ASM_E_CUDA, ASM_E_NOT_DEVICE = 0, 1, 2, 3, 4
 FMT_Q4_0, FMT_Q8_0 = 2, 8
+DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 
 vp, i64, c_int = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
 i32, f32 = ctypes.c_int32, ctypes.c_float
@@ -65,6 +66,14 @@ class DecodeModel(ctypes.Structure):
                                      "h", "img_h", "counters", "logits", "best", "tokens", "pos")])
 
 
+class Kv(ctypes.Structure):
+    """asm_kv_t (include/asmllm.h): keys and values of a batch, paged or packed."""
+    _fields_ = ([("k", vp), ("v", vp), ("page_stride", i64), ("token_stride", i64), ("head_stride", i64), ("table", vp),
+                 ("table_stride", i64), ("len", vp), ("cu", vp)]
+                + [(n, i32) for n in ("batch", "n_pages", "page_size", "table_width", "n_kv_heads", "head_dim", "dtype",
+                                      "reserved")])
+
+
 class Rows(ctypes.Structure):
     """asm_rows_t (include/asmllm.h): one batched RMSNorm / embed / residual step."""
     _fields_ = [("rows", i32), ("dim", i32), ("x", vp), ("delta", vp), ("embed", vp), ("tokens", vp), ("pos", vp),
@@ -103,6 +112,11 @@ SIGNATURES = {
     "asm_attention_batch_async": ([vp, i64, vp, vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, f32, vp], c_int),
     "asm_rows_argmax_async": ([vp, i32, i32, i64, i32, vp, vp], c_int),
     "asm_rows_advance_async": ([vp, i32, vp, i32, vp, i32, vp], c_int),
+    "asm_rope_append_async": ([vp, i32, i64, vp, i32, vp, i32, i32, vp, ctypes.POINTER(Kv), vp], c_int),
+    "asm_attention_prompt_async": ([vp, i64, i64, vp, i32, i32, f32, vp, i32, ctypes.POINTER(Kv), vp], c_int),
+    "asm_attention_paged_workspace": ([i32, i32, i32, i32], i64),
+    "asm_attention_paged_async": ([vp, i64, i64, i32, f32, vp, i32, ctypes.POINTER(Kv), vp, i64, vp], c_int),
+    "asm_rows_sample_async": ([vp, i32, i32, i32, i64, vp, vp, vp, vp, vp, vp, vp], c_int),
     # additions
     "asm_matmul_q8q8": ([vp, vp, vp, vp, i64, i64], None),
     "asm_quantize_q8_0": ([vp, vp, vp, i64], None),

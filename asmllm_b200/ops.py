@@ -373,6 +373,7 @@ __all__ = [
     "threadpool_shutdown", "threadpool_get_num_threads", "max_k", "matvec", "quantize_q8_0_dev",
     "block_sums_dev", "gguf_split_dev", "act_image_bytes", "act_image_dev", "matvec_image",
     "mark_static", "unmark_static", "device_error", "set_option",
+    "rope_append", "attention_prompt", "attention_paged", "attention_paged_workspace", "rows_sample",
 ]
 
 
@@ -546,3 +547,219 @@ def rows_advance(keys, tokens, pos, n_prompt: int, stream=None):
 def key_index(keys):
     """Index part of signed-orderable argmax keys (host or device int64 tensor)."""
     return ((keys ^ (-(1 << 63))) & 0xFFFFFFFF).neg().add(0xFFFFFFFF)
+
+
+# --------------------------------------------------------------------------
+# Serving operators: prompts of different lengths, a paged cache, sampling
+# --------------------------------------------------------------------------
+
+
+def _dt(dtype):
+    torch = _torch()
+    return {torch.float32: native.DT_F32, torch.float16: native.DT_F16, torch.bfloat16: native.DT_BF16}[dtype]
+
+
+def _empty(shape, dtype, device, stream):
+    """A new output that belongs to the stream the kernel runs on."""
+    torch = _torch()
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _dense(t, name, ndim, dtypes):
+    """A CUDA tensor of `ndim` axes whose last one is dense (the others may be strided)."""
+    torch = _torch()
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name}: expected a CUDA tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name}: dtype {t.dtype} not in {tuple(dtypes)}")
+    if t.dim() != ndim or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name}: expected {ndim} axes, the last one dense; got {tuple(t.shape)} "
+                         f"with strides {t.stride()}")
+
+
+def _step(t, axis, default):
+    """Stride of an axis; `default` where it has one entry and the stride means nothing."""
+    return t.stride(axis) if t.shape[axis] > 1 else default
+
+
+def _kv_view(k, v, kv_len=None, page_table=None, cu_k=None):
+    """native.Kv of paged k, v [pages, page_size, heads, head_dim] or packed k, v [rows, heads, head_dim]."""
+    torch = _torch()
+    nd = 4 if page_table is not None else 3
+    for t, name in ((k, "k"), (v, "v")):
+        _dense(t, name, nd, (torch.float16, torch.bfloat16))
+    if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or any(
+            a != b and n > 1 for a, b, n in zip(k.stride(), v.stride(), k.shape)):
+        raise ValueError(f"k and v must agree in shape, strides, type and device: {tuple(k.shape)} {k.stride()} "
+                         f"{k.dtype}, {tuple(v.shape)} {v.stride()} {v.dtype}")
+    d = native.Kv()
+    d.k, d.v = k.data_ptr(), v.data_ptr()
+    hd = k.shape[-1]
+    d.head_dim, d.n_kv_heads, d.dtype = hd, k.shape[-2], _dt(k.dtype)
+    d.head_stride = _step(k, -2, hd)
+    d.token_stride = _step(k, -3, hd)
+    if page_table is not None:
+        _dense(page_table, "page_table", 2, (torch.int32,))
+        _check_dev(kv_len, (torch.int32,), "kv_len")
+        if kv_len.numel() != page_table.shape[0]:
+            raise ValueError(f"kv_len has {kv_len.numel()} entries, page_table {page_table.shape[0]} rows")
+        d.batch, d.table_width = page_table.shape
+        d.table, d.table_stride = page_table.data_ptr(), _step(page_table, 0, page_table.shape[1])
+        d.len = kv_len.data_ptr()
+        d.n_pages, d.page_size = k.shape[0], k.shape[1]
+        d.page_stride = _step(k, 0, hd)
+    else:
+        _check_dev(cu_k, (torch.int32,), "cu_k")
+        d.batch = cu_k.numel() - 1
+        d.cu = cu_k.data_ptr()
+        d.n_pages, d.page_size, d.page_stride = 1, k.shape[0], hd
+    return d
+
+
+def _out_for(q, out, out_dtype, stream):
+    torch = _torch()
+    if out is None:
+        dt = out_dtype or q.dtype
+        if dt not in (q.dtype, torch.float32):
+            raise TypeError(f"out_dtype {dt}: fp32 or q's type")
+        return _empty(tuple(q.shape), dt, q.device, stream)
+    _check_dev(out, (q.dtype, torch.float32), "out")
+    if out.shape != q.shape or (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError(f"out: {tuple(out.shape)} {out.dtype}, expected {tuple(q.shape)} {out_dtype or q.dtype}")
+    return out
+
+
+def rope_append(qkv, rope_cs, kv_len, page_table, k_pages, v_pages, n_heads: int, *, cu_q=None, q_out=None,
+                stream=None):
+    """Rotary positions on the query and key heads of qkv [T, (nh + 2 nkv) * hd] (fp32 or the cache's
+    type) and append of keys and values to their pages (asm_rope_append_async).
+
+    Row t of sequence s (cu_q int32 [B + 1]; without it row s is sequence s) is the position
+    kv_len[s] - (rows of s) + (t - cu_q[s]): kv_len counts the new rows already.  k_pages, v_pages
+    [pages, page_size, nkv, hd] fp16 or bf16 (any strides, hd dense), page_table int32 [B, n], rope_cs fp32
+    [positions, hd/2, 2] (decode.rope_table).  Returns the rotated queries [T, nh, hd] in the cache's
+    type; rows at or past cu_q[B] are not written."""
+    torch = _torch()
+    _dense(k_pages, "k_pages", 4, (torch.float16, torch.bfloat16))
+    _dense(qkv, "qkv", 2, (torch.float32, k_pages.dtype))
+    _check_dev(rope_cs, (torch.float32,), "rope_cs")
+    kv = _kv_view(k_pages, v_pages, kv_len, page_table)
+    T, hd = qkv.shape[0], kv.head_dim
+    if qkv.shape[1] != (n_heads + 2 * kv.n_kv_heads) * hd:
+        raise ValueError(f"qkv has {qkv.shape[1]} columns, expected ({n_heads} + 2 * {kv.n_kv_heads}) * {hd}")
+    if rope_cs.shape[1:] != (hd // 2, 2):
+        raise ValueError(f"rope_cs {tuple(rope_cs.shape)}: expected [positions, {hd // 2}, 2]")
+    if cu_q is not None:
+        _check_dev(cu_q, (torch.int32,), "cu_q")
+        if cu_q.numel() != kv.batch + 1:
+            raise ValueError(f"cu_q has {cu_q.numel()} entries, expected {kv.batch + 1}")
+    elif T != kv.batch:
+        raise ValueError(f"{T} rows for {kv.batch} sequences: pass cu_q")
+    if q_out is None:
+        q_out = _empty((T, n_heads, hd), k_pages.dtype, qkv.device, stream)
+    else:
+        _check_dev(q_out, (k_pages.dtype,), "q_out")
+        if q_out.shape != (T, n_heads, hd):
+            raise ValueError(f"q_out {tuple(q_out.shape)}: expected {(T, n_heads, hd)}")
+    native.check(native.lib().asm_rope_append_async(
+        _ptr(qkv), _dt(qkv.dtype), _step(qkv, 0, qkv.shape[1]), _ptr(rope_cs), rope_cs.shape[0],
+        None if cu_q is None else _ptr(cu_q), T, n_heads, _ptr(q_out), ctypes.byref(kv), _stream_handle(stream)))
+    return q_out
+
+
+def attention_prompt(q, k, v, cu_q, *, cu_k=None, kv_len=None, page_table=None, scale: float | None = None, out=None,
+                     out_dtype=None, stream=None):
+    """Causal attention of packed prompts q [T, nh, hd], fp16 or bf16 (asm_attention_prompt_async).
+
+    Sequence s owns rows cu_q[s] .. cu_q[s + 1] - 1 (int32 [B + 1]).  Keys and values are packed
+    [Tk, nkv, hd] with offsets cu_k (cu_q where they are the prompt's own), or the pages of a cache
+    [pages, page_size, nkv, hd] with page_table int32 [B, n] and kv_len int32 [B].  The last row of a
+    sequence sees all its keys; earlier rows one less each; a row without keys gives zeros.  scale
+    defaults to hd ** -0.5.  out [T, nh, hd] in q's type or fp32; rows at or past cu_q[B] are not written."""
+    torch = _torch()
+    _dense(q, "q", 3, (torch.float16, torch.bfloat16))
+    _check_dev(cu_q, (torch.int32,), "cu_q")
+    if (page_table is None) != (kv_len is None) or (page_table is not None and cu_k is not None):
+        raise ValueError("pass page_table and kv_len (paged) or cu_k (packed)")
+    kv = _kv_view(k, v, kv_len, page_table, cu_q if cu_k is None else cu_k)
+    if cu_q.numel() != kv.batch + 1:
+        raise ValueError(f"cu_q has {cu_q.numel()} entries for {kv.batch} sequences")
+    _same_heads(q, k)
+    out = _out_for(q, out, out_dtype, stream)
+    native.check(native.lib().asm_attention_prompt_async(
+        _ptr(q), _step(q, 0, q.shape[1] * q.shape[2]), _step(q, 1, q.shape[2]), _ptr(cu_q), q.shape[0], q.shape[1],
+        q.shape[2] ** -0.5 if scale is None else scale, _ptr(out), _dt(out.dtype), ctypes.byref(kv),
+        _stream_handle(stream)))
+    return out
+
+
+def _same_heads(q, k):
+    if q.dtype != k.dtype or q.shape[-1] != k.shape[-1] or q.device != k.device:
+        raise ValueError(f"q {q.dtype} of head_dim {q.shape[-1]} against keys {k.dtype} of {k.shape[-1]}")
+    if k.shape[-2] == 0 or q.shape[-2] == 0 or q.shape[-2] % k.shape[-2]:
+        raise ValueError(f"{q.shape[-2]} query heads are not a multiple of {k.shape[-2]} KV heads")
+
+
+def attention_paged_workspace(batch: int, n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    """Bytes of scratch one attention_paged call needs (asm_attention_paged_workspace)."""
+    n = int(native.lib().asm_attention_paged_workspace(batch, n_heads, n_kv_heads, head_dim))
+    if n < 0:
+        native.check()
+    return n
+
+
+def attention_paged(q, k_pages, v_pages, page_table, kv_len, *, scale: float | None = None, out=None, out_dtype=None,
+                    workspace=None, stream=None):
+    """Attention of one new token per sequence, q [B, nh, hd] fp16 or bf16, over a paged cache
+    (asm_attention_paged_async): k_pages, v_pages [pages, page_size, nkv, hd], page_table int32 [B, n],
+    kv_len int32 [B] (the new token counted).  kv_len 0 gives zeros.  out [B, nh, hd] in q's type or fp32.
+    workspace: uint8 of attention_paged_workspace bytes, one per call that may overlap another (a call
+    without one takes it from torch's allocator)."""
+    torch = _torch()
+    _dense(q, "q", 3, (torch.float16, torch.bfloat16))
+    if page_table is None:
+        raise ValueError("page_table is required")
+    kv = _kv_view(k_pages, v_pages, kv_len, page_table)
+    _same_heads(q, k_pages)
+    B, nh, hd = q.shape
+    if B != kv.batch:
+        raise ValueError(f"q has {B} rows for {kv.batch} sequences")
+    out = _out_for(q, out, out_dtype, stream)
+    if workspace is None:
+        workspace = _empty(attention_paged_workspace(B, nh, kv.n_kv_heads, hd), torch.uint8, q.device, stream)
+    else:
+        _check_dev(workspace, (torch.uint8,), "workspace")
+    native.check(native.lib().asm_attention_paged_async(
+        _ptr(q), _step(q, 0, nh * hd), _step(q, 1, hd), nh, hd ** -0.5 if scale is None else scale, _ptr(out),
+        _dt(out.dtype), ctypes.byref(kv), _ptr(workspace), workspace.numel(), _stream_handle(stream)))
+    return out
+
+
+def rows_sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, stream=None):
+    """The next token of each row of logits [B, V] (fp32, fp16 or bf16; V <= 262144) from the given
+    numbers u fp32 [B] in [0, 1) (asm_rows_sample_async).
+
+    temperature, top_p, min_p fp32 [B] and top_k int32 [B], each optional (1, 1, 0, off).  top_k first,
+    then top_p of what is left, then min_p of the largest probability; ties go to the lower index; the
+    word is the first, in index order, whose cumulative probability exceeds u.  temperature 0: the first
+    maximum.  NaN is never chosen; a row of NaN and -inf gives -1.  Returns int32 [B]."""
+    torch = _torch()
+    _dense(logits, "logits", 2, (torch.float32, torch.float16, torch.bfloat16))
+    B, V = logits.shape
+    for t, name, dt in ((u, "u", torch.float32), (temperature, "temperature", torch.float32),
+                        (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
+                        (min_p, "min_p", torch.float32), (tokens, "tokens", torch.int32)):
+        if t is None and name != "u":
+            continue
+        _check_dev(t, (dt,), name)
+        if t.shape != (B,):
+            raise ValueError(f"{name}: shape {tuple(t.shape)}, expected ({B},)")
+    if tokens is None:
+        tokens = _empty((B,), torch.int32, logits.device, stream)
+    opt = [None if t is None else _ptr(t) for t in (temperature, top_k, top_p, min_p)]
+    native.check(native.lib().asm_rows_sample_async(_ptr(logits), _dt(logits.dtype), B, V, _step(logits, 0, V), _ptr(u),
+                                                    *opt, _ptr(tokens), _stream_handle(stream)))
+    return tokens

@@ -638,6 +638,100 @@ ASMLLM_API int asm_rows_argmax_async(const float* logits, int32_t rows, int32_t 
 ASMLLM_API int asm_rows_advance_async(const int64_t* keys, int32_t rows, int32_t* tokens, int32_t max_tokens,
                                       int32_t* pos, int32_t n_prompt, void* stream);
 
+/* Serving operators: prompts of different lengths, a paged key-value cache and
+ * sampling.  The reference runs one sequence with a fixed cache and takes the
+ * argmax (src/runtime/generate.py:252-326, 410-411); these have no counterpart
+ * there.  All are stream-ordered and capturable in CUDA graphs (after one eager
+ * call per shape), take device pointers of the current device, and keep nothing
+ * between calls. */
+#define ASM_DT_F32 0
+#define ASM_DT_F16 1
+#define ASM_DT_BF16 2
+
+/* Keys and values of `batch` sequences, 16-bit (dtype ASM_DT_F16 or _BF16),
+ * head_dim 64 or 128.  Element d of head j at (page, offset) is
+ * k[page*page_stride + offset*token_stride + j*head_stride + d]; strides in
+ * elements, multiples of 8, the same for k and v; k and v 16-byte aligned.
+ *   Paged (table set): position p of sequence s is at page
+ *     table[s*table_stride + p/page_size], offset p % page_size; page_size a
+ *     power of two from 16 to 256; len[s] positions are held.  Page numbers
+ *     at or past ceil(len[s]/page_size) are not read.
+ *   Packed (table NULL): one page (n_pages 1) of page_size rows; sequence s
+ *     holds rows cu[s] .. cu[s+1] - 1.
+ * Lengths and page numbers live on the device.  A length above
+ * table_width*page_size or below 0, packed offsets that are out of range, or a
+ * page number outside [0, n_pages) sets ASM_DEVERR_DECODE_RANGE (see
+ * asm_device_error): the length is clipped, the positions of a bad page count
+ * as zero keys and values, and nothing is read outside the pool. */
+typedef struct asm_kv {
+  void* k;
+  void* v;
+  int64_t page_stride, token_stride, head_stride;
+  const int32_t* table;  /* [batch][table_stride], table_width columns used */
+  int64_t table_stride;
+  const int32_t* len;    /* [batch] (paged) */
+  const int32_t* cu;     /* [batch + 1] (packed) */
+  int32_t batch, n_pages, page_size, table_width;
+  int32_t n_kv_heads, head_dim, dtype, reserved;
+} asm_kv_t;
+
+/* Rotary positions and cache append: qkv [rows][(n_heads + 2 n_kv_heads) *
+ * head_dim] (query heads, key heads, value heads; row stride qkv_stride
+ * elements; fp32 or the cache's type).  Row t belongs to the sequence s with
+ * cu_q[s] <= t < cu_q[s+1] (cu_q NULL: rows == batch, row s is sequence s) and
+ * sits at position p = len[s] - (cu_q[s+1] - cu_q[s]) + (t - cu_q[s]); len
+ * counts the new rows already.  Query and key heads are rotated in
+ * interleaved pairs with rope_cs[p] (fp32 [rope_len][head_dim/2][2], as
+ * asm_attention_decode_async), rounded to the cache's type and written to
+ * q_out [rows][n_heads][head_dim] and to the row's page; values are rounded
+ * and written beside the keys.  p < 0: zero query, nothing appended.  p past
+ * the table, the rotary table or the pool: the same, and
+ * ASM_DEVERR_DECODE_RANGE.  Rows at or past cu_q[batch] are left as they are.  Two rows must not share a
+ * slot (a page that is appended to belongs to one sequence). */
+ASMLLM_API int asm_rope_append_async(const void* qkv, int32_t qkv_dtype, int64_t qkv_stride, const float* rope_cs,
+                                     int32_t rope_len, const int32_t* cu_q, int32_t rows, int32_t n_heads,
+                                     void* q_out, const asm_kv_t* kv, void* stream);
+
+/* Causal attention of packed prompts: q [rows][n_heads][head_dim] of the
+ * cache's type (row and head strides in elements, multiples of 8), positions
+ * as above (bottom-right aligned: the last row of a sequence sees all its
+ * keys), query head h on KV head h / (n_heads / n_kv_heads).  out
+ * [rows][n_heads][head_dim], fp32 or the cache's type.  Rows without a key
+ * give zeros; rows at or past cu_q[batch] are left as they are.  Scores,
+ * maxima and sums are fp32; the weights are rounded to the 16-bit type for
+ * the product with the values, which costs about as much as one rounding of
+ * the output.  What a row does not attend to -- later positions, other
+ * sequences, the rest of a page -- does not reach it, whatever it holds. */
+ASMLLM_API int asm_attention_prompt_async(const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                                          const int32_t* cu_q, int32_t rows, int32_t n_heads, float scale, void* out,
+                                          int32_t out_dtype, const asm_kv_t* kv, void* stream);
+
+/* Attention of one new token per sequence over its pages: q [batch][n_heads]
+ * [head_dim] (strides as above), out [batch][n_heads][head_dim], fp32 or the
+ * cache's type; len[s] == 0 gives zeros.  fp32 throughout (the weights enter
+ * the product as two 16-bit parts).  workspace: asm_attention_paged_workspace
+ * bytes of device memory, 16-byte aligned, whose content need not be set or
+ * kept; calls that may overlap need one each. */
+ASMLLM_API int64_t asm_attention_paged_workspace(int32_t batch, int32_t n_heads, int32_t n_kv_heads,
+                                                 int32_t head_dim);
+ASMLLM_API int asm_attention_paged_async(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t n_heads,
+                                         float scale, void* out, int32_t out_dtype, const asm_kv_t* kv,
+                                         void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The next token of each row of logits (n values at r*stride; fp32, fp16 or
+ * bf16; n <= 262144) from one given number u[r] in [0, 1).  Words are ordered
+ * by (logit descending, index ascending); with w = exp((x - max)/temperature):
+ * top_k > 0 keeps the first top_k words; of those, top_p keeps each word
+ * whose predecessors' mass is below top_p times the mass kept so far; min_p
+ * keeps the words with w >= min_p; the first word always stays.  tokens[r] =
+ * the first kept word, in index order, whose cumulative mass exceeds u[r]
+ * times the kept mass.  temperature <= 0: the first maximum, as
+ * asm_rows_argmax_async.  NaN is never chosen; a row of NaN and -inf gives -1.
+ * temperature, top_k, top_p, min_p: [rows] each, or NULL for 1, off, 1, 0. */
+ASMLLM_API int asm_rows_sample_async(const void* logits, int32_t dtype, int32_t rows, int32_t n, int64_t stride,
+                                     const float* u, const float* temperature, const int32_t* top_k,
+                                     const float* top_p, const float* min_p, int32_t* tokens, void* stream);
+
 /* Q5_0 x fp32 on device pointers (see asm_matmul_q5), stream ordered. */
 ASMLLM_API int asm_matmul_q5_async(const uint8_t* ql, const uint8_t* qh, const float* scales,
                                    const float* x, float* y, int64_t M, int64_t K, void* stream);

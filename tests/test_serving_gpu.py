@@ -1,0 +1,789 @@
+"""The serving operators on the GPU (ops.rope_append, attention_prompt, attention_paged, rows_sample)
+against plain implementations in 64 bits.
+
+Tolerances count roundings.  u = eps/2 of the 16-bit type, u32 = 2^-24.
+  * A score is a sum of hd exact products in fp32: off by at most hd * 2^-23 * sum|q||k| * scale (the
+    tensor core truncates), and its scaled copy by 2^-22 of its size; the weight exp(s - m) follows
+    with twice that (its own and the maximum's), and 2^-22 of the exponential itself.
+  * Prompt: each weight is rounded once to 16 bits (u); paged: to twice 16 bits (2 u^2, and 2^-38 of the
+    largest weight where fp16 runs out of exponent).
+  * Sums of n terms in fp32, in chains of at most n: n * 2^-23 at most (it is far less).
+  * The output is rounded once (u of its type).
+So |out - exact| <= A * sum_j p_j |v_j| + u_out |exact|, A collecting the relative errors of the weights
+(twice: in the weighted sum and in the sum of weights)."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+from asmllm_b200 import decode as D
+from asmllm_b200 import native, ops
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = ["float16", "bfloat16"]
+
+
+def half_step(torch, dt):
+    return torch.finfo(dt).eps / 2
+
+
+@pytest.fixture(autouse=True)
+def clean_error_word(cuda):
+    ops.device_error()
+    yield
+    assert ops.device_error() == 0
+
+
+# ------------------------------------------------------------------ helpers
+def make_pages(torch, dense_k, dense_v, page, layout="token", extra=3, seed=0, width_extra=2):
+    """Pages (NaN wherever no position lives) of per-sequence keys and values [n, nkv, hd]."""
+    nkv, hd, dt = dense_k[0].shape[1], dense_k[0].shape[2], dense_k[0].dtype
+    need = [-(-k.shape[0] // page) for k in dense_k]
+    total = sum(need) + extra
+    g = torch.Generator().manual_seed(seed)
+    perm = torch.randperm(total, generator=g).tolist()
+    if layout == "token":  # [page][offset][head][hd]
+        mk = lambda: torch.full((total, page, nkv, hd), float("nan"), dtype=dt, device="cuda")  # noqa: E731
+    elif layout == "head":  # [page][head][offset][hd]
+        mk = lambda: torch.full((total, nkv, page, hd), float("nan"), dtype=dt,  # noqa: E731
+                                device="cuda").transpose(1, 2)
+    else:  # keys and values side by side in one pool, heads padded
+        mk = lambda: torch.full((total, page, nkv, hd + 16), float("nan"), dtype=dt,  # noqa: E731
+                                device="cuda")[..., :hd]
+    kp, vp = mk(), mk()
+    table = torch.full((len(need), max(need + [1]) + width_extra), -7, dtype=torch.int32)  # not to be read
+    at = 0
+    for s, n in enumerate(need):
+        for i in range(n):
+            pg = perm[at]
+            at += 1
+            table[s, i] = pg
+            rows = dense_k[s][i * page:(i + 1) * page]
+            kp[pg, :rows.shape[0]] = rows
+            vp[pg, :rows.shape[0]] = dense_v[s][i * page:(i + 1) * page]
+    return kp, vp, table.cuda()
+
+
+def exact_attention(torch, q, k, v, scale, first):
+    """64-bit causal attention of q [n, nh, hd] whose row i sees keys 0 .. first + i; also sum p|v| and A's score part."""
+    n, nh, hd = q.shape
+    m, nkv = k.shape[0], k.shape[1]
+    g = nh // nkv
+    out = torch.zeros(n, nh, hd, dtype=torch.float64, device="cuda")
+    pv = torch.zeros_like(out)
+    serr = torch.zeros(n, nh, 1, dtype=torch.float64, device="cuda")
+    if m == 0:
+        return out, pv, serr
+    keep = torch.arange(m, device="cuda")[None] <= (first + torch.arange(n, device="cuda"))[:, None]
+    for h in range(nh):
+        Q, K, V = q[:, h].double(), k[:, h // g].double(), v[:, h // g].double()
+        s = (Q @ K.T * scale).masked_fill(~keep, -math.inf)
+        mx = s.amax(-1, keepdim=True)
+        mx = torch.where(torch.isinf(mx), torch.zeros_like(mx), mx)
+        p = torch.exp(s - mx)
+        l = p.sum(-1, keepdim=True)
+        p = p / torch.where(l == 0, torch.ones_like(l), l)
+        out[:, h] = p @ V
+        pv[:, h] = p @ V.abs()
+        mag = (Q.abs() @ K.abs().T * scale).masked_fill(~keep, 0)
+        serr[:, h, 0] = (mag.amax(-1) * hd * 2.0 ** -23 + s.masked_fill(~keep, 0).abs().amax(-1) * 2.0 ** -22)
+    return out, pv, serr
+
+
+def close(torch, got, want, pv, serr, n, weight, dt, what=""):
+    A = 2 * (2 * serr + 2.0 ** -22 + weight + n * 2.0 ** -23)
+    u = half_step(torch, got.dtype)
+    tiny = 2.0 ** -24 if got.dtype == torch.float16 else 0.0  # fp16 subnormal steps
+    tol = A * pv + u * (want.abs() + A * pv) + tiny
+    err = (got.double() - want).abs()
+    bad = ~(err <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} outside, worst {float((err / tol).max()):.3g} of it"
+
+
+def paged_weight(torch, dt, n):
+    u = half_step(torch, dt)
+    return 2 * u * u + (n * 2.0 ** -38 if dt == torch.float16 else 0.0)
+
+
+def prompt_weight(torch, dt, n):
+    return half_step(torch, dt) + (n * 2.0 ** -32 if dt == torch.float16 else 0.0)
+
+
+def rand(torch, *shape, dt, seed, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dt)
+
+
+# ------------------------------------------------------------------ rotary and append
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("src", ["float32", "same"])
+@pytest.mark.parametrize("nh,nkv,hd", [(4, 2, 128), (5, 1, 64), (32, 32, 128)])
+@pytest.mark.parametrize("page,layout", [(16, "token"), (64, "head"), (256, "padded")])
+def test_rope_append(cuda, dtype, src, nh, nkv, hd, page, layout):
+    torch = cuda
+    dt = getattr(torch, dtype)
+    q_len, kv_len = [3, 1, 0, 40, 5], [3, 17, 9, 300, 2]  # the last has more rows than positions
+    T, tail = sum(q_len), 4
+    x = rand(torch, T + tail, (nh + 2 * nkv) * hd, dt=torch.float32 if src == "float32" else dt, seed=1)
+    rope = torch.from_numpy(D.rope_table(512, hd, 10000.0)).cuda()
+    empty = [torch.full((n, nkv, hd), float("nan"), dtype=dt, device="cuda") for n in kv_len]
+    kp, vp, table = make_pages(torch, empty, empty, page, layout)
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(q_len)]), dtype=torch.int32, device="cuda")
+    kv = torch.tensor(kv_len, dtype=torch.int32, device="cuda")
+    q_out = torch.full((T + tail, nh, hd), 77.0, dtype=dt, device="cuda")
+    before = (kp.clone(), vp.clone())
+    ops.rope_append(x, rope, kv, table, kp, vp, nh, cu_q=cu, q_out=q_out)
+    torch.cuda.synchronize()
+    assert (q_out[T:] == 77.0).all()  # rows behind the last sequence
+    xs = x.float().view(T + tail, nh + 2 * nkv, hd)
+    want_k, want_v = before
+    t = 0
+    for s, (n, m) in enumerate(zip(q_len, kv_len)):
+        for i in range(n):
+            p = m - n + i
+            if p < 0:
+                assert (q_out[t] == 0).all()
+            else:
+                c, d = rope[p, :, 0], rope[p, :, 1]
+                z = xs[t, :nh + nkv].unflatten(-1, (hd // 2, 2))
+                # the same fp32 roundings, one by one; then one to 16 bits
+                z = torch.stack([z[..., 0] * c - z[..., 1] * d, z[..., 0] * d + z[..., 1] * c], -1).flatten(-2).to(dt)
+                assert torch.equal(q_out[t], z[:nh])
+                pg = int(table[s, p // page])
+                want_k[pg, p % page] = z[nh:]
+                want_v[pg, p % page] = xs[t, nh + nkv:].to(dt)
+            t += 1
+    same = lambda a, b: torch.equal(torch.nan_to_num(a.float(), nan=123.0), torch.nan_to_num(b.float(), nan=123.0))  # noqa: E731
+    assert same(kp, want_k) and same(vp, want_v)
+
+
+def test_rope_append_one_row_per_sequence_and_strided_input(cuda):
+    torch = cuda
+    B, nh, nkv, hd = 7, 8, 2, 128
+    big = rand(torch, B, (nh + 2 * nkv) * hd + 64, dt=torch.float32, seed=2)
+    x = big[:, :(nh + 2 * nkv) * hd]
+    rope = torch.from_numpy(D.rope_table(128, hd, 10000.0)).cuda()
+    kv_len = [1, 16, 17, 100, 33, 0, 128]  # no position: nothing to write
+    empty = [torch.zeros(n, nkv, hd, dtype=torch.float16, device="cuda") for n in kv_len]
+    kp, vp, table = make_pages(torch, empty, empty, 16)
+    kv = torch.tensor(kv_len, dtype=torch.int32, device="cuda")
+    a = ops.rope_append(x, rope, kv, table, kp, vp, nh)
+    b = ops.rope_append(x.contiguous(), rope, kv, table, kp.clone(), vp.clone(), nh,
+                        cu_q=torch.arange(B + 1, dtype=torch.int32, device="cuda"))
+    torch.cuda.synchronize()
+    assert torch.equal(a, b)
+    assert (a[5] == 0).all() and not (a[4] == 0).all()
+
+
+def test_rope_append_refuses_positions_and_pages_on_the_device(cuda):
+    torch = cuda
+    nh, nkv, hd = 4, 2, 128
+    x = rand(torch, 4, (nh + 2 * nkv) * hd, dt=torch.float32, seed=3)
+    rope = torch.from_numpy(D.rope_table(32, hd, 10000.0)).cuda()
+    kp = torch.zeros(4, 16, nkv, hd, dtype=torch.float16, device="cuda")
+    vp = torch.zeros_like(kp)
+    table = torch.tensor([[0, 1, 9], [9, 1, 2], [2, -1, 3], [3, 1, 2]], dtype=torch.int32, device="cuda")
+    # past the rotary table; page 9 of 4; page -1; past the table's width
+    kv = torch.tensor([40, 4, 20, 49], dtype=torch.int32, device="cuda")
+    q = ops.rope_append(x, rope, kv, table, kp, vp, nh)
+    assert ops.device_error() == native.DEVERR_DECODE_RANGE
+    assert (q == 0).all() and (kp == 0).all() and (vp == 0).all()
+
+
+# ------------------------------------------------------------------ paged attention
+PAGED = [
+    # nh, nkv, hd, page, lengths
+    (32, 32, 128, 16, [1, 2, 15, 16, 17, 63, 64, 65]),
+    (64, 8, 128, 16, [512, 0, 1, 700, 333, 1024, 64, 129]),
+    (8, 1, 128, 64, [5000, 1, 0]),
+    (8, 1, 64, 32, [4097, 31]),
+    (12, 4, 64, 128, [129, 128, 127, 1, 0, 640]),
+    (40, 2, 128, 256, [300, 256, 255, 1]),  # 20 query heads on one KV head
+    (5, 5, 128, 16, [77]),
+    (33, 1, 128, 32, [999, 40]),            # 33 on one
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nh,nkv,hd,page,lens", PAGED)
+@pytest.mark.parametrize("out", ["same", "float32"])
+def test_attention_paged(cuda, dtype, nh, nkv, hd, page, lens, out):
+    torch = cuda
+    dt = getattr(torch, dtype)
+    k = [rand(torch, n, nkv, hd, dt=dt, seed=10 + i) for i, n in enumerate(lens)]
+    v = [rand(torch, n, nkv, hd, dt=dt, seed=50 + i) for i, n in enumerate(lens)]
+    layout = ["token", "head", "padded"][len(lens) % 3]
+    kp, vp, table = make_pages(torch, k, v, page, layout)
+    q = rand(torch, len(lens), nh, hd, dt=dt, seed=99, scale=2.0)
+    kv = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    odt = dt if out == "same" else torch.float32
+    got = ops.attention_paged(q, kp, vp, table, kv, out_dtype=odt)
+    again = ops.attention_paged(q, kp, vp, table, kv, out_dtype=odt)
+    torch.cuda.synchronize()
+    assert got.dtype == odt and torch.equal(got, again)  # the same bits every time
+    for i, n in enumerate(lens):
+        want, pv, serr = exact_attention(torch, q[i:i + 1], k[i], v[i], hd ** -0.5, n - 1)
+        close(torch, got[i:i + 1], want, pv, serr, max(1, n), paged_weight(torch, dt, n), dt, f"sequence {i} of {n}")
+
+
+def test_attention_paged_long_tail_of_small_weights(cuda):
+    # one key far above 60000 others whose weights are near 2^-25 of it: together they still count
+    torch = cuda
+    n, hd = 60001, 128
+    q = torch.zeros(1, 1, hd, dtype=torch.float16, device="cuda")
+    q[..., 0] = 1.0
+    k = torch.zeros(n, 1, hd, dtype=torch.float16, device="cuda")
+    k[1234, 0, 0] = 17.5
+    v = torch.ones(n, 1, hd, dtype=torch.float16, device="cuda")
+    v[1234] = 0.0
+    kp, vp, table = make_pages(torch, [k], [v], 64)
+    kv = torch.tensor([n], dtype=torch.int32, device="cuda")
+    got = ops.attention_paged(q, kp, vp, table, kv, scale=1.0, out_dtype=torch.float32)
+    want, pv, serr = exact_attention(torch, q, k, v, 1.0, n - 1)
+    close(torch, got, want, pv, serr, n, paged_weight(torch, torch.float16, n), torch.float16)
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    got = ops.attention_prompt(q, kp, vp, cu, kv_len=kv, page_table=table, scale=1.0, out_dtype=torch.float32)
+    # n weights of fp16 with 2^-32 of the largest as their step
+    close(torch, got, want, pv, serr, n, prompt_weight(torch, torch.float16, n), torch.float16)
+
+
+def test_attention_paged_strided_query_scale_and_out(cuda):
+    torch = cuda
+    nh, nkv, hd, lens = 8, 2, 128, [100, 7]
+    k = [rand(torch, n, nkv, hd, dt=torch.bfloat16, seed=i) for i, n in enumerate(lens)]
+    v = [rand(torch, n, nkv, hd, dt=torch.bfloat16, seed=9 + i) for i, n in enumerate(lens)]
+    kp, vp, table = make_pages(torch, k, v, 16)
+    kv = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    rows = rand(torch, 2, nh + 5, hd + 8, dt=torch.bfloat16, seed=3)
+    q = rows[:, 2:2 + nh, :hd]
+    ws = torch.empty(ops.attention_paged_workspace(2, nh, nkv, hd), dtype=torch.uint8, device="cuda").fill_(255)
+    out = torch.full((2, nh, hd), float("nan"), device="cuda")
+    got = ops.attention_paged(q, kp, vp, table, kv, scale=0.3, out=out, workspace=ws)
+    assert got is out
+    for i, n in enumerate(lens):
+        want, pv, serr = exact_attention(torch, q[i:i + 1], k[i], v[i], 0.3, n - 1)
+        close(torch, got[i:i + 1], want, pv, serr, n, paged_weight(torch, torch.bfloat16, n), torch.bfloat16)
+
+
+def test_attention_nonfinite_inputs_of_attended_positions_show(cuda):
+    torch = cuda
+    n, hd = 200, 128
+    k, v = (rand(torch, n, 1, hd, dt=torch.float16, seed=i) for i in (1, 2))
+    v[150, 0, 3] = float("inf")
+    k[20, 0, 0] = float("nan")
+    kp, vp, table = make_pages(torch, [k, v], [v, v], 16)
+    q = rand(torch, 2, 2, hd, dt=torch.float16, seed=5)
+    kv = torch.tensor([n, n], dtype=torch.int32, device="cuda")
+    got = ops.attention_paged(q, kp, vp, table, kv)
+    assert torch.isnan(got[0]).all()           # a NaN key reaches every value of its sequence
+    got = ops.attention_paged(q[:1], kp, vp, table[:1], torch.tensor([20], dtype=torch.int32, device="cuda"))
+    assert torch.isfinite(got).all()           # ... unless it is behind the sequence's end
+
+
+def test_attention_paged_bad_pages_and_lengths_are_reported(cuda):
+    torch = cuda
+    k = [rand(torch, 64, 2, 128, dt=torch.float16, seed=i) for i in range(3)]
+    kp, vp, table = make_pages(torch, k, k, 16, width_extra=0)
+    q = rand(torch, 3, 4, 128, dt=torch.float16, seed=7)
+    kv = torch.tensor([64, 64, 64], dtype=torch.int32, device="cuda")
+    good = ops.attention_paged(q, kp, vp, table, kv)
+    for bad in (-1, kp.shape[0], 2 ** 31 - 1):
+        t = table.clone()
+        t[1, 2] = bad
+        got = ops.attention_paged(q, kp, vp, t, kv)
+        assert ops.device_error() == native.DEVERR_DECODE_RANGE
+        assert torch.equal(got[0], good[0]) and torch.equal(got[2], good[2]) and torch.isfinite(got[1]).all()
+    got = ops.attention_paged(q, kp, vp, table, torch.tensor([64, 65, -3], dtype=torch.int32, device="cuda"))
+    assert ops.device_error() == native.DEVERR_DECODE_RANGE
+    assert torch.equal(got[:2], good[:2]) and (got[2] == 0).all()
+
+
+def test_attention_paged_offsets_past_32_bits(cuda):
+    # a pool of over 2^32 bytes and over 2^31 elements; only two far pages are filled
+    torch = cuda
+    pages, page, hd = 2 ** 31 // (16 * 128) + 40, 16, 128
+    kp = torch.empty(pages, page, 1, hd, dtype=torch.float16, device="cuda")
+    vp = torch.empty_like(kp)
+    k, v = (rand(torch, 30, 1, hd, dt=torch.float16, seed=i) for i in (1, 2))
+    where = [pages - 1, 5]
+    for i, pg in enumerate(where):
+        rows = k[16 * i:16 * i + 16]
+        kp[pg, :rows.shape[0]] = rows
+        vp[pg, :rows.shape[0]] = v[16 * i:16 * i + 16]
+    table = torch.tensor([where], dtype=torch.int32, device="cuda")
+    kv = torch.tensor([30], dtype=torch.int32, device="cuda")
+    q = rand(torch, 1, 1, hd, dt=torch.float16, seed=3)
+    got = ops.attention_paged(q, kp, vp, table, kv, out_dtype=torch.float32)
+    want, pv, serr = exact_attention(torch, q, k, v, hd ** -0.5, 29)
+    close(torch, got, want, pv, serr, 30, paged_weight(torch, torch.float16, 30), torch.float16)
+    got = ops.attention_prompt(q, kp, vp, torch.tensor([0, 1], dtype=torch.int32, device="cuda"), kv_len=kv,
+                               page_table=table)
+    close(torch, got, want, pv, serr, 30, prompt_weight(torch, torch.float16, 30), torch.float16)
+    rope = torch.from_numpy(D.rope_table(64, hd, 10000.0)).cuda()
+    x = rand(torch, 1, 3 * hd, dt=torch.float32, seed=4)
+    kv = torch.tensor([16], dtype=torch.int32, device="cuda")  # offset 15 of the last page
+    ops.rope_append(x, rope, kv, table, kp, vp, 1)
+    assert torch.equal(vp[pages - 1, 15, 0], x[0, 2 * hd:].half())
+
+
+# ------------------------------------------------------------------ prompt attention
+PROMPT = [
+    # nh, nkv, hd, q lengths, extra keys before them (paged only), page (0: packed)
+    (4, 4, 128, [1], None, 0),
+    (2, 2, 128, [64, 65, 63, 1, 128, 127, 129], None, 0),
+    (4, 2, 128, [300, 0, 5, 257, 256, 255], None, 0),
+    (6, 2, 64, [33, 513, 1, 100], None, 0),      # three query heads per KV head
+    (8, 1, 64, [1025, 7], None, 0),
+    (32, 32, 128, [130], None, 0),
+    (8, 1, 128, [40, 1, 130, 3], [0, 700, 17, 255], 16),
+    (4, 4, 128, [200, 129, 1], [56, 1, 1000], 64),
+    (8, 2, 64, [128, 128], [128, 0], 128),
+    (5, 1, 128, [260, 9], [300, 4], 256),
+    (16, 2, 128, [1, 1, 1, 2], [0, 300, 15, 16], 32),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nh,nkv,hd,q_len,prefix,page", PROMPT)
+@pytest.mark.parametrize("out", ["same", "float32"])
+def test_attention_prompt(cuda, dtype, nh, nkv, hd, q_len, prefix, page, out):
+    torch = cuda
+    dt = getattr(torch, dtype)
+    T, tail = sum(q_len), 70
+    kv_len = [n + p for n, p in zip(q_len, prefix or [0] * len(q_len))]
+    q = rand(torch, T + tail, nh, hd, dt=dt, seed=1, scale=2.0)
+    cu_h = np.concatenate([[0], np.cumsum(q_len)])
+    cu = torch.tensor(cu_h, dtype=torch.int32, device="cuda")
+    odt = dt if out == "same" else torch.float32
+    got = torch.full((T + tail, nh, hd), 55.0, dtype=odt, device="cuda")
+    if page:
+        k = [rand(torch, n, nkv, hd, dt=dt, seed=20 + i) for i, n in enumerate(kv_len)]
+        v = [rand(torch, n, nkv, hd, dt=dt, seed=60 + i) for i, n in enumerate(kv_len)]
+        kp, vp, table = make_pages(torch, k, v, page, ["token", "head", "padded"][len(q_len) % 3])
+        kv = torch.tensor(kv_len, dtype=torch.int32, device="cuda")
+        call = lambda: ops.attention_prompt(q, kp, vp, cu, kv_len=kv, page_table=table, out=got)  # noqa: E731
+    else:
+        K, V = (rand(torch, T + 30, nkv, hd, dt=dt, seed=i) for i in (2, 3))
+        K[T:] = float("nan")  # behind the last sequence
+        V[T:] = float("nan")
+        k, v = ([X[cu_h[i]:cu_h[i + 1]] for i in range(len(q_len))] for X in (K, V))
+        call = lambda: ops.attention_prompt(q, K, V, cu, cu_k=cu, out=got)  # noqa: E731
+    call()
+    first = got.clone()
+    call()
+    torch.cuda.synchronize()
+    assert torch.equal(first, got)
+    assert (got[T:] == 55.0).all()
+    for i, (n, m) in enumerate(zip(q_len, kv_len)):
+        rows = slice(int(cu_h[i]), int(cu_h[i + 1]))
+        want, pv, serr = exact_attention(torch, q[rows], k[i], v[i], hd ** -0.5, m - n)
+        close(torch, got[rows], want, pv, serr, max(m, 1), prompt_weight(torch, dt, m), dt, f"sequence {i}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_prompt_long(cuda, dtype):
+    torch = cuda
+    dt = getattr(torch, dtype)
+    n, nh, hd = 4100, 2, 128
+    q = rand(torch, n, nh, hd, dt=dt, seed=1, scale=2.0)
+    k, v = (rand(torch, n, 1, hd, dt=dt, seed=i) for i in (2, 3))
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    got = ops.attention_prompt(q, k, v, cu)
+    want, pv, serr = exact_attention(torch, q, k, v, hd ** -0.5, 0)
+    close(torch, got, want, pv, serr, n, prompt_weight(torch, dt, n), dt)
+
+
+@pytest.mark.parametrize("step", [0.05, 0.5, 5.0])
+def test_attention_prompt_rising_scores(cuda, step):
+    # every key's score is above all before it: the running maximum rises in every tile
+    torch = cuda
+    n, hd = 700, 128
+    q = torch.zeros(n, 1, hd, dtype=torch.float16, device="cuda")
+    q[..., 0] = 1.0
+    q[..., 1] = 1.0
+    k = torch.zeros_like(q)
+    x = torch.arange(n, device="cuda").float() * step
+    k[:, 0, 0] = x.half()
+    k[:, 0, 1] = (x - k[:, 0, 0].float()).half()
+    v = rand(torch, n, 1, hd, dt=torch.float16, seed=3)
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    for sign in (1.0, -1.0):
+        got = ops.attention_prompt(q * sign, k, v, cu, scale=1.0)
+        want, pv, serr = exact_attention(torch, q * sign, k, v, 1.0, 0)
+        close(torch, got, want, pv, serr, n, prompt_weight(torch, torch.float16, n), torch.float16)
+
+
+@pytest.mark.parametrize("page", [0, 16])
+def test_attention_prompt_later_values_do_not_reach_earlier_rows(cuda, page):
+    torch = cuda
+    q_len, nh, nkv, hd = [150, 300], 4, 2, 128
+    T = sum(q_len)
+    q = rand(torch, T, nh, hd, dt=torch.bfloat16, seed=1)
+    k, v = (rand(torch, T, nkv, hd, dt=torch.bfloat16, seed=i) for i in (2, 3))
+    cu = torch.tensor([0, 150, 450], dtype=torch.int32, device="cuda")
+
+    def call(k, v):
+        if not page:
+            return ops.attention_prompt(q, k, v, cu)
+        kp, vp, table = make_pages(torch, [k[:150], k[150:]], [v[:150], v[150:]], page)
+        kv = torch.tensor(q_len, dtype=torch.int32, device="cuda")
+        return ops.attention_prompt(q, kp, vp, cu, kv_len=kv, page_table=table)
+
+    good = call(k, v)
+    k2, v2 = k.clone(), v.clone()
+    v2[100, 0, 5] = float("nan")    # position 100 of the first sequence, KV head 0
+    v2[150 + 200, 1, 7] = float("inf")  # position 200 of the second, KV head 1
+    k2[150 + 250, 0] = float("nan")     # position 250, KV head 0
+    got = call(k2, v2)
+    assert torch.isfinite(good).all()
+    u = half_step(torch, torch.bfloat16)
+    # rows before the position: computed another way at most, each way within 2u of the exact value
+    same = lambda a, b: ((a.float() - b.float()).abs() <= 4 * u * (1 + b.float().abs())).all()  # noqa: E731
+    assert same(got[:100], good[:100]) and torch.equal(got[:150, 2:], good[:150, 2:])
+    assert torch.isnan(got[100:150, :2, 5]).all()
+    assert same(got[100:150, :2, 6:], good[100:150, :2, 6:])
+    assert same(got[150:350], good[150:350])
+    assert (~torch.isfinite(got[350:, 2:, 7])).all()
+    assert same(got[150:400, :2], good[150:400, :2]) and torch.isnan(got[400:, :2]).all()
+
+
+def test_attention_prompt_rows_without_keys_and_strided_inputs(cuda):
+    torch = cuda
+    nh, nkv, hd = 4, 2, 128
+    buf = rand(torch, 90, (nh + 2 * nkv) * hd + 8, dt=torch.float16, seed=1)
+    heads = buf[:, :(nh + 2 * nkv) * hd].unflatten(1, (nh + 2 * nkv, hd))
+    q, k, v = heads[:, :nh], heads[:, nh:nh + nkv], heads[:, nh + nkv:]
+    cu_q = torch.tensor([0, 50, 90], dtype=torch.int32, device="cuda")
+    cu_k = torch.tensor([0, 20, 90], dtype=torch.int32, device="cuda")  # 20 keys for 50 rows; 70 for 40
+    got = ops.attention_prompt(q, k, v, cu_q, cu_k=cu_k)
+    assert (got[:30] == 0).all()
+    for a, b, ka, kb in ((30, 50, 0, 20), (50, 90, 20, 90)):
+        want, pv, serr = exact_attention(torch, q[a:b], k[ka:kb], v[ka:kb], hd ** -0.5, (kb - ka) - (b - a))
+        close(torch, got[a:b], want, pv, serr, kb - ka, prompt_weight(torch, torch.float16, 100), torch.float16)
+
+
+def test_attention_prompt_many_sequences(cuda):
+    torch = cuda
+    nh, nkv, hd = 2, 1, 128
+    rng = np.random.default_rng(0)
+    q_len = rng.integers(0, 9, 1000)
+    q_len[500] = 400
+    T = int(q_len.sum())
+    q = rand(torch, T, nh, hd, dt=torch.bfloat16, seed=1)
+    k, v = (rand(torch, T, nkv, hd, dt=torch.bfloat16, seed=i) for i in (2, 3))
+    cu_h = np.concatenate([[0], np.cumsum(q_len)])
+    got = ops.attention_prompt(q, k, v, torch.tensor(cu_h, dtype=torch.int32, device="cuda"))
+    for s in list(range(0, 1000, 37)) + [500, 999]:
+        a, b = int(cu_h[s]), int(cu_h[s + 1])
+        want, pv, serr = exact_attention(torch, q[a:b], k[a:b], v[a:b], hd ** -0.5, 0)
+        close(torch, got[a:b], want, pv, serr, max(1, b - a), prompt_weight(torch, torch.bfloat16, b - a),
+              torch.bfloat16, f"sequence {s}")
+
+
+def test_attention_prompt_bad_offsets_and_pages_are_reported(cuda):
+    torch = cuda
+    q = rand(torch, 60, 2, 128, dt=torch.float16, seed=1)
+    k = rand(torch, 60, 1, 128, dt=torch.float16, seed=2)
+    cu = torch.tensor([0, 30, 60], dtype=torch.int32, device="cuda")
+    good = ops.attention_prompt(q, k, k, cu)
+    for bad in ([0, 30, 61], [-1, 30, 60], [0, 61, 60]):
+        got = ops.attention_prompt(q, k, k, cu, cu_k=torch.tensor(bad, dtype=torch.int32, device="cuda"))
+        assert ops.device_error() == native.DEVERR_DECODE_RANGE
+        if bad[1] == 30:
+            ok = slice(0, 30) if bad[0] == 0 else slice(30, 60)
+            assert torch.equal(got[ok], good[ok])
+    kp, vp, table = make_pages(torch, [k[:30], k[30:]], [k[:30], k[30:]], 16, width_extra=0)
+    kv = torch.tensor([30, 30], dtype=torch.int32, device="cuda")
+    table[0, 1] = 99
+    got = ops.attention_prompt(q, kp, vp, cu, kv_len=kv, page_table=table)
+    assert ops.device_error() == native.DEVERR_DECODE_RANGE
+    assert torch.equal(got[30:], good[30:]) and torch.isfinite(got).all()
+
+
+# ------------------------------------------------------------------ sampling
+def sample_ref(x, u, T, k, p, mp):
+    """One row in 64 bits: numpy, the definition word by word."""
+    x = x.astype(np.float64)
+    x[np.isnan(x)] = -np.inf
+    m = x.max()
+    if m == -np.inf:
+        return -1
+    order = np.argsort(-x, kind="stable")
+    if not T > 0:
+        return int(order[0])
+    with np.errstate(invalid="ignore"):
+        w = np.where(x == m, 1.0, np.exp((x - m) / T))
+    keep = order[:k] if k > 0 else order
+    c = np.cumsum(w[keep])
+    n = int(np.sum(c - w[keep] < float(p) * c[-1])) if p < 1 else len(keep)
+    keep = keep[:max(1, n)]
+    keep = np.concatenate([keep[:1], keep[1:][w[keep[1:]] >= mp]])
+    keep.sort()
+    c = np.cumsum(w[keep])
+    return int(keep[np.searchsorted(c, float(u) * c[-1], side="right")]) if float(u) * c[-1] < c[-1] else int(
+        keep[np.nonzero(w[keep])[0][-1]])
+
+
+def f32(v):
+    return float(np.float32(v))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("V", [1, 2, 31, 1000, 32000, 50257, 128256])
+def test_rows_sample(cuda, dtype, V):
+    torch = cuda
+    rng = np.random.default_rng(V)
+    B = 40
+    x = torch.from_numpy((rng.standard_normal((B, V)) * rng.uniform(0.2, 6, (B, 1))).astype(np.float32)).cuda().to(
+        getattr(torch, dtype))
+    par = dict(temperature=rng.choice([0.0, 0.3, 0.8, 1.0, 2.5], B), top_k=rng.choice([0, 1, 2, 40, V, V + 9, -3], B),
+               top_p=rng.choice([1.0, 0.95, 0.5, 0.01, 0.0, 2.0], B), min_p=rng.choice([0.0, 0.0, 0.05, 0.9, 1.0], B))
+    u = rng.random(B).astype(np.float32)
+    u[:3] = [0.0, np.nextafter(np.float32(1), np.float32(0)), 0.5]
+    dev = {n: torch.tensor(a, dtype=torch.int32 if n == "top_k" else torch.float32, device="cuda")
+           for n, a in par.items()}
+    got = ops.rows_sample(x, torch.from_numpy(u).cuda(), **dev).cpu().numpy()
+    xs = x.float().cpu().numpy()
+    want = [sample_ref(xs[r].copy(), u[r], f32(par["temperature"][r]), int(par["top_k"][r]), f32(par["top_p"][r]),
+                       f32(par["min_p"][r])) for r in range(B)]
+    np.testing.assert_array_equal(got, want)
+
+
+def test_rows_sample_ties_masks_and_infinities(cuda):
+    torch = cuda
+    inf, nan = float("inf"), float("nan")
+    V = 300
+    rows, want = [], []
+
+    def add(x, token, u=0.0, T=1.0, k=0, p=1.0, mp=0.0):
+        rows.append((x, u, T, k, p, mp))
+        want.append(token)
+
+    flat = np.zeros(V, np.float32)
+    add(flat, 0, u=0.0)
+    add(flat, 150, u=0.5)                     # cumulative mass 151/300 is the first above 1/2
+    add(flat, 9, u=0.999, k=10)               # ties: the lowest indices are the first ten
+    add(flat, 37, u=0.999, p=0.125)           # 38 of 300 words reach an eighth of the mass
+    add(flat, 4, u=0.9, k=10, p=0.5)          # five of the ten
+    mask = np.full(V, -inf, np.float32)
+    add(mask, -1)
+    add(np.full(V, nan, np.float32), -1, T=0.0)
+    one = mask.copy()
+    one[77] = -1e30
+    add(one, 77, u=0.7)
+    add(one, 77, T=0.0)
+    lowest = np.full(V, np.finfo(np.float32).min, np.float32)
+    lowest[5] = 0.0
+    add(lowest, 5, u=0.9999)
+    add(np.full(V, np.finfo(np.float32).min, np.float32), 150, u=0.5)  # all at the type's lowest value
+    holes = flat.copy()
+    holes[::2] = nan
+    add(holes, 1, u=0.0)
+    add(holes, 151, u=0.5)                    # the 76th of 150 words
+    big = flat.copy()
+    big[[10, 20]] = inf
+    add(big, 10, u=0.3)
+    add(big, 20, u=0.6)
+    add(big, 10, T=0.0)
+    signed = flat.copy()
+    signed[::3] = -0.0                        # the two zeros are one value
+    add(signed, 4, u=0.9, k=5)
+    add(flat, 0, u=0.9, p=0.0)
+    add(flat, 0, u=-1.0)
+    add(flat, 299, u=2.0)                     # a number outside [0, 1): the nearest word
+    add(flat, 299, u=0.999, T=inf)
+    add(flat, 0, u=0.9, T=-1.0)
+    B = len(rows)
+    x = torch.from_numpy(np.stack([r[0] for r in rows])).cuda()
+    col = lambda i, dt: torch.tensor([r[i] for r in rows], dtype=dt, device="cuda")  # noqa: E731
+    args = dict(temperature=col(2, torch.float32), top_k=col(3, torch.int32), top_p=col(4, torch.float32),
+                min_p=col(5, torch.float32))
+    got = ops.rows_sample(x, col(1, torch.float32), **args)
+    assert got.tolist() == want
+    wide = torch.full((B, V + 13), inf, device="cuda")  # a strided view: what is beside it is not read
+    wide[:, 5:5 + V] = x
+    got = ops.rows_sample(wide[:, 5:5 + V], col(1, torch.float32), **args)
+    assert got.tolist() == want
+
+
+def test_rows_sample_greedy_is_rows_argmax_and_defaults(cuda):
+    torch = cuda
+    x = rand(torch, 9, 32000, dt=torch.float32, seed=4).mul_(4).round_()  # many equal maxima
+    u = torch.rand(9, device="cuda")
+    keys = torch.zeros(9, dtype=torch.int64, device="cuda")
+    ops.rows_argmax(x, keys)
+    got = ops.rows_sample(x, u, temperature=torch.zeros(9, device="cuda"))
+    assert torch.equal(got.long(), ops.key_index(keys))
+    got = ops.rows_sample(x, u)
+    xs = x.cpu().numpy()
+    assert got.tolist() == [sample_ref(xs[r].copy(), u[r].item(), 1.0, 0, 1.0, 0.0) for r in range(9)]
+
+
+def test_rows_sample_frequencies(cuda):
+    # 20000 evenly spaced numbers over one row: every word comes up as often as its probability says, to one
+    torch = cuda
+    V, N = 50, 20000
+    x = rand(torch, 1, V, dt=torch.float32, seed=8).expand(N, V).contiguous()
+    u = ((torch.arange(N, device="cuda").double() + 0.5) / N).float()
+    got = torch.bincount(ops.rows_sample(x, u).long(), minlength=V).double()
+    want = torch.softmax(x[0].double(), 0) * N
+    assert (got - want).abs().max() <= 2.0
+
+
+# ------------------------------------------------------------------ streams, graphs, the operators together
+def test_side_stream_and_graph_replay(cuda):
+    torch = cuda
+    nh, nkv, hd, B, page = 8, 2, 128, 3, 16
+    lens = [40, 17, 90]
+    k = [rand(torch, n, nkv, hd, dt=torch.float16, seed=i) for i, n in enumerate(lens)]
+    kp, vp, table = make_pages(torch, k, k, page)
+    rope = torch.from_numpy(D.rope_table(256, hd, 10000.0)).cuda()
+    x = rand(torch, B, (nh + 2 * nkv) * hd, dt=torch.float32, seed=5)
+    kv = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    logits = rand(torch, B, 1000, dt=torch.float32, seed=6)
+    u = torch.rand(B, device="cuda")
+    cu = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device="cuda")
+
+    def step(stream=None):
+        q = ops.rope_append(x, rope, kv, table, kp, vp, nh, stream=stream)
+        a = ops.attention_paged(q, kp, vp, table, kv, stream=stream)
+        b = ops.attention_prompt(q, kp, vp, cu, kv_len=kv, page_table=table, stream=stream)
+        return q, a, b, ops.rows_sample(logits, u, top_k=cu[1:], stream=stream)
+
+    want = [t.clone() for t in step()]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    got = step(side)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs = []
+    for _ in range(2):  # two graphs at once, replayed in turn and on two streams
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res = step()
+        graphs.append((g, res))
+    for _ in range(2):
+        for g, _ in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for _, res in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(res, want))
+    # other contents in the same buffers: nothing was kept from the capture
+    x.mul_(-0.5)
+    kv.copy_(torch.tensor([39, 3, 88], dtype=torch.int32))
+    logits.neg_()
+    want = [t.clone() for t in step()]
+    for (g, _), s in zip(graphs, (torch.cuda.Stream(), torch.cuda.Stream())):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            g.replay()
+    torch.cuda.synchronize()
+    for _, res in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(res, want))
+
+
+def test_prompts_of_different_lengths_then_sampled_decode(cuda):
+    """A two-layer model served as a user would: ragged prompts in one pass into a paged cache, then sampled
+    tokens step by step.  Every attention is held to the 64-bit one over a dense record of the rotated keys
+    and values, every token to the sampling's definition, and the logits to the lockstep decoder's."""
+    torch = cuda
+    from asmllm_b200 import batch_decode as BD
+
+    shape = D.LlamaShape(n_layers=2, dim=512, n_heads=4, n_kv_heads=2, head_dim=128, ffn=1536, vocab=1000)
+    ctx, page, n_new = 64, 16, 5
+    sh = D.shard_plan(shape, 1, 0)
+    W = D.make_weights(shape, sh, 3, native.FMT_Q4_0, torch.device("cuda"))
+    rng = np.random.default_rng(1)
+    prompts = [rng.integers(0, shape.vocab, n) for n in (7, 1, 19)]
+    B = len(prompts)
+    nh, nkv, hd = shape.n_heads, shape.n_kv_heads, shape.head_dim
+    rope = torch.from_numpy(D.rope_table(ctx, hd, shape.theta)).cuda()
+    pools = [[torch.full((B * 4, page, nkv, hd), float("nan"), dtype=torch.float16, device="cuda") for _ in "kv"]
+             for _ in range(shape.n_layers)]
+    table = torch.randperm(B * 4, generator=torch.Generator().manual_seed(0)).view(B, 4).int().cuda()
+
+    record = [[[] for _ in range(B)] for _ in range(shape.n_layers)]  # per layer and sequence: (keys, values) so far
+
+    def check_attention(li, qkv, q, got, starts, first):
+        """The attention of one layer against 64 bits; starts: row offsets, first: the first position of each."""
+        x = qkv.view(-1, nh + 2 * nkv, hd)
+        for s in range(B):
+            a, b = starts[s], starts[s + 1]
+            p = torch.arange(first[s], first[s] + b - a, device="cuda")
+            c, d = rope[p, None, :, 0], rope[p, None, :, 1]
+            z = x[a:b, :nh + nkv].unflatten(-1, (hd // 2, 2))
+            z = torch.stack([z[..., 0] * c - z[..., 1] * d, z[..., 0] * d + z[..., 1] * c], -1).flatten(-2).half()
+            assert torch.equal(q[a:b], z[:, :nh])
+            record[li][s].append((z[:, nh:], x[a:b, nh + nkv:].half()))
+            k, v = (torch.cat([r[i] for r in record[li][s]]) for i in (0, 1))
+            want, pv, serr = exact_attention(torch, q[a:b], k, v, hd ** -0.5, first[s])
+            n = k.shape[0]
+            close(torch, got[a:b], want, pv, serr, n, prompt_weight(torch, torch.float16, n), torch.float16)
+
+    def forward(ids, cu, kv_len, last):
+        """Logits of rows `last` of the packed token ids."""
+        starts = cu.tolist() if cu is not None else list(range(B + 1))
+        first = [int(kv_len[s]) - (starts[s + 1] - starts[s]) for s in range(B)]
+        x = W["embed"][ids].contiguous()
+        T = x.shape[0]
+        delta = None
+        for li, L in enumerate(W["layers"]):
+            t = torch.empty(ops.act_tiles_bytes(T, shape.dim), dtype=torch.uint8, device="cuda")
+            ops.rows_norm_tiles(x, t, L["attn_norm"], shape.eps, delta=delta)
+            qkv = ops.gemm_tiles(native.FMT_Q4_0, *L["wqkv"], t, T)
+            k, v = pools[li]
+            q = ops.rope_append(qkv, rope, kv_len, table, k, v, nh, cu_q=cu)
+            if cu is None:
+                a = ops.attention_paged(q, k, v, table, kv_len, out_dtype=torch.float32)
+            else:
+                a = ops.attention_prompt(q, k, v, cu, kv_len=kv_len, page_table=table, out_dtype=torch.float32)
+            check_attention(li, qkv, q, a, starts, first)
+            o = ops.gemm(native.FMT_Q4_0, *L["wo"], a.view(T, nh * hd))
+            ops.rows_norm_tiles(x, t, L["ffn_norm"], shape.eps, delta=o)
+            gu = ops.gemm_tiles(native.FMT_Q4_0, *L["wgu"], t, T)
+            th = torch.empty(ops.act_tiles_bytes(T, shape.ffn), dtype=torch.uint8, device="cuda")
+            ops.rows_swiglu_tiles(gu, th)
+            delta = ops.gemm_tiles(native.FMT_Q4_0, *L["wdown"], th, T)
+        t = torch.empty(ops.act_tiles_bytes(T, shape.dim), dtype=torch.uint8, device="cuda")
+        ops.rows_norm_tiles(x, t, W["final_norm"], shape.eps, delta=delta)
+        return ops.gemm_tiles(native.FMT_Q4_0, *W["lm_head"], t, T)[last]
+
+    lens = [len(p) for p in prompts]
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+    kv = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ids = torch.from_numpy(np.concatenate(prompts)).cuda()
+    temperature = torch.tensor([0.0, 0.8, 1.0], device="cuda")
+    top_k = torch.tensor([0, 20, 0], dtype=torch.int32, device="cuda")
+    top_p = torch.tensor([1.0, 1.0, 0.9], device="cuda")
+    numbers = torch.rand(n_new, B, generator=torch.Generator().manual_seed(2)).cuda()
+    steps, tokens = [], []
+    logits = forward(ids, cu, kv, cu[1:].long() - 1)
+    for i in range(n_new):
+        steps.append(logits.clone())
+        tok = ops.rows_sample(logits, numbers[i], temperature=temperature, top_k=top_k, top_p=top_p)
+        tokens.append(tok)
+        kv += 1
+        logits = forward(tok.long(), None, kv, slice(None))
+    tokens = torch.stack(tokens, 1).cpu().numpy()
+    for i in range(n_new):
+        for s in range(B):
+            assert tokens[s, i] == sample_ref(steps[i][s].cpu().numpy(), numbers[i, s].item(), temperature[s].item(),
+                                              int(top_k[s]), top_p[s].item(), 0.0)
+    for s in range(B):  # the lockstep decoder, teacher-forced with the same tokens
+        forced = np.concatenate([prompts[s], tokens[s]])
+        dec = BD.BatchDecoder(shape, 1, ctx=ctx, weights=W)
+        dec.reset(forced[None])
+        for i in range(len(forced) - 1):
+            dec.step()
+            j = i - (len(prompts[s]) - 1)
+            if j >= 0:
+                a, b = steps[j][s].cpu().numpy(), dec.logits[0].cpu().numpy()
+                # The lockstep decoder keeps q in fp32; the rounding to fp16 here tips Q8_0 quants by one
+                # step, at most 1/127 of the block's largest value for each of its 32: sqrt(32)/127 of the
+                # vector's norm, at each of the nine quantised vectors (four a layer and the lm_head's).
+                # A wrong position, page or mask gives about 1.
+                assert np.linalg.norm(a - b) <= 9 * math.sqrt(32) / 127 * np.linalg.norm(b)
+        dec.close()
