@@ -220,7 +220,8 @@ def test_attention_paged(cuda, dtype, nh, nkv, hd, page, lens, out):
     q = rand(torch, len(lens), nh, hd, dt=dt, seed=99, scale=2.0)
     kv = torch.tensor(lens, dtype=torch.int32, device="cuda")
     odt = dt if out == "same" else torch.float32
-    got = ops.attention_paged(q, kp, vp, table, kv, out_dtype=odt)
+    ws = torch.empty(ops.attention_paged_workspace(len(lens), nh, nkv, hd), dtype=torch.uint8, device="cuda")
+    got = ops.attention_paged(q, kp, vp, table, kv, out_dtype=odt, workspace=ws.fill_(255))  # NaN to begin with
     again = ops.attention_paged(q, kp, vp, table, kv, out_dtype=odt)
     torch.cuda.synchronize()
     assert got.dtype == odt and torch.equal(got, again)  # the same bits every time
