@@ -6,16 +6,43 @@
 // (t - cu_q[s]), n_s the sequence's key count, and
 //   out[t][h] = sum_{j <= p} softmax_j(scale q[t][h] . k[j][h / g]) v[j][h / g];
 // p < 0: zeros.
+//
+// 4 head_dim flops per row, head and key: bound by the tensor cores, and next
+// to them by the one exponential per row, head and key.  A work item is two
+// 128-row query tiles that read the same keys: the same rows of two heads of
+// a group (even groups), or 256 rows of one head.  Per 128 keys and query
+// tile the tensor core computes S = Q K^T into tensor memory, one thread per
+// row takes maximum, exponentials and sum, writes the weights P (16 bits)
+// over S, and the tensor core adds P V to the output, which stays in tensor
+// memory.  While one tile's weights are computed the tensor core works on the
+// other's.  The output is rescaled only when a row's maximum has risen by
+// more than 2^kLazy since it was last set (the weights then still fit 16
+// bits and the division by the sum cancels the factor).
+//
+// CTA (one per SM, persistent), 12 warps:
+//   0-3, 4-7  softmax, rescale and output of query tile 0 and 1
+//   8         tcgen05.mma issue; zeroes the values behind a sequence's end
+//   9         tensor copies: Q (2 tiles), then K and V tiles into one ring
+//   10        scheduler: the work items in order of falling key count
+// Every wait is bounded: a role that gives up sets the device error word and
+// an abort flag, all roles leave, and tensor memory is released.
+#include <type_traits>
+
 #include "matvec.cuh"
 #include "mma16.cuh"
+#include "pipeline.cuh"
 #include "serving.cuh"
+#include "tensor_map.cuh"
+#include "tmem.cuh"
 
 namespace asmllm {
 
 namespace {
 
-constexpr int kTile = 64;   // query rows per CTA (16 per warp) and positions per tile
-constexpr int kWarps = 4;
+constexpr int kRows = 128;  // rows of a query tile, positions of a key tile
+constexpr float kLazy = 6.0f;
+constexpr float kPShift = 8.0f;  // weights are 2^kPShift exp(s - m): fp16 keeps those down to 2^-32 of the largest
+constexpr int kThreads = 384;
 
 // A row whose output is not finite, computed again key by key by one warp:
 // in a matrix product a later position's infinite or NaN value meets the
@@ -58,167 +85,548 @@ __device__ void attend_row(const PromptArgs& a, const KvArgs& kv, int t, int h, 
   }
 }
 
+
+// One work item, written by the scheduler.
+struct Item {
+  int s;       // sequence; -1: no more
+  int t0;      // first query row
+  int rows;    // query rows from t0 (at most 128 with two heads, 256 with one)
+  int base;    // position of row t0
+  int n;       // keys of the sequence
+  int head;    // first query head
+  int key0;    // packed: first key row of the sequence
+  int tiles[2];  // key tiles of each query tile
+};
+
+template <int HD>
+struct Cfg {
+  static constexpr int kTile = kRows * HD * 2;  // bytes of a Q, K or V tile
+  static constexpr int kStages = HD == 128 ? 5 : 8;
+  static constexpr int kRing = 2 * kTile;
+  static constexpr int kBars = kRing + kStages * kTile;
+  static constexpr int kNBars = 2 * kStages + 2 + 8 + 4 + 1;
+  static constexpr int kItems = kBars + kNBars * 8 + 16;
+  static constexpr int kSmem = kItems + 2 * (int)sizeof(Item) + 16 + 1024;
+  static constexpr uint32_t kO = 2 * kRows;  // tensor memory: S0, S1, then the two outputs
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+// Operand descriptors, 128-byte swizzle.  Q and K: rows of 128 bytes (64
+// values along the product's K), eight rows 1024 bytes apart.  V: the product
+// runs over its rows; 64 values are contiguous, the next 64 a half tile away.
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((kRows * 128) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+
+// Tiles of sequence (base, q rows, R rows a tile) with at least w key tiles.
+__device__ __forceinline__ int tiles_at_least(int base, int q, int R, int w) {
+  const int n = (q + R - 1) / R;
+  if (w <= 0) return n;
+  const int x = kRows * (w - 1) - base;  // a tile counts when its last row + 1 is above x
+  if (q <= x) return 0;
+  return n - (x < 0 ? 0 : min(x / R, n - 1));
+}
+
 template <class T, class O, int HD>
-__global__ void __launch_bounds__(kWarps * 32) attention_prompt_kernel(const PromptArgs a, const KvArgs kv,
-                                                                       unsigned* __restrict__ err) {
-  constexpr int kChunks = HD / 8;
+__global__ void __launch_bounds__(kThreads, 1)
+attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                        const __grid_constant__ CUtensorMap vmap, const PromptArgs a, const KvArgs kv, int pair,
+                        int box_rows, unsigned* __restrict__ err) {
+  using C = Cfg<HD>;
+  constexpr int kHalves = HD / 64, S = C::kStages;
+  constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
+  constexpr uint32_t kIdescS = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((kRows >> 3) << 17) | ((kRows >> 4) << 24);
+  constexpr uint32_t kIdescO =
+      (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((kRows >> 4) << 24);
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  const uint32_t sk = smem_u32(smem), sv = sk + kTile * HD * 2;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBars);
+  uint64_t* kv_full = bars;
+  uint64_t* kv_empty = kv_full + S;
+  uint64_t* q_full = kv_empty + S;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_empty + 1;   // [2] scores of a tile are in tensor memory
+  uint64_t* p_full = s_full + 2;    // [2] its weights are
+  uint64_t* o_full = p_full + 2;    // [2] the item's output is complete
+  uint64_t* o_empty = o_full + 2;   // [2] and has been read
+  uint64_t* i_full = o_empty + 2;   // [2] work items
+  uint64_t* i_empty = i_full + 2;
+  uint64_t* drain = i_empty + 2;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile uint32_t* s_abort = s_tmem + 1;
+  Item* items = reinterpret_cast<Item*>(smem + C::kItems);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(smem_u32(kv_full + i), 1);
+      mbar_init(smem_u32(kv_empty + i), 1);
+    }
+    mbar_init(smem_u32(q_full), 1);
+    mbar_init(smem_u32(q_empty), 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(s_full + i), 1);
+      mbar_init(smem_u32(p_full + i), 4);
+      mbar_init(smem_u32(o_full + i), 1);
+      mbar_init(smem_u32(o_empty + i), 4);
+      mbar_init(smem_u32(i_full + i), 1);
+      mbar_init(smem_u32(i_empty + i), 10);  // 8 softmax warps, the issuer, the loader
+    }
+    mbar_init(smem_u32(drain), 1);
+    *s_abort = 0u;
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
   pdl_trigger();
   pdl_wait();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int h = blockIdx.x, j = h / (a.n_heads / kv.n_kv);
-  // which sequence and tile block blockIdx.y is
-  int s = 0, tile = blockIdx.y, qb = 0, qe = 0;
-  for (; s < kv.batch; ++s) {
-    q_range(a.cu_q, s, a.rows, &qb, &qe);
-    const int nt = (qe - qb + kTile - 1) / kTile;
-    if (tile < nt) break;
-    tile -= nt;
-  }
-  if (s == kv.batch) return;
-  bool clipped;
-  const int n = kv_length(kv, s, &clipped);
-  if (clipped && tid == 0) atomicOr(err, kErrDecodeRange);
-  const int t0 = qb + tile * kTile;               // first query row of the tile
-  const int base = n - (qe - qb) + tile * kTile;  // its position
-  const int rows = min(kTile, qe - t0);
-  const int stop = min(n, base + rows);           // positions the tile attends to
-  const float sl2 = a.scale * 1.4426950408889634f;
-  const int r = lane >> 2, c2 = (lane & 3) * 2;
 
-  uint32_t qf[HD / 16][4];
-  auto ld = [&](int row, int col) -> uint32_t {
-    if (row >= rows) return 0u;
-    return __ldcg(reinterpret_cast<const unsigned*>(static_cast<const T*>(a.q) + (long long)(t0 + row) * a.q_row_stride +
-                                                    (long long)h * a.q_head_stride + col));
+  auto fail = [&]() {
+    *s_abort = 1u;
+    atomicOr(err, kErrRingTimeout);
   };
-#pragma unroll
-  for (int ks = 0; ks < HD / 16; ++ks) {
-    qf[ks][0] = ld(warp * 16 + r, ks * 16 + c2);
-    qf[ks][1] = ld(warp * 16 + r + 8, ks * 16 + c2);
-    qf[ks][2] = ld(warp * 16 + r, ks * 16 + c2 + 8);
-    qf[ks][3] = ld(warp * 16 + r + 8, ks * 16 + c2 + 8);
-  }
-  float o[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-#pragma unroll
-  for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+  // Warp-wide wait; false (in every lane) when the role has to leave.
+  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    const bool ok = mbar_wait_bounded(smem_u32(bar), parity);
+    if (!ok) fail();
+    return !__any_sync(kFull, !ok || *s_abort);
+  };
+  // Work item k; false when there is none left.
+  auto take_item = [&](int k, Item* it) -> bool {
+    if (!wait(i_full + (k & 1), (k >> 1) & 1)) return false;
+    *it = items[k & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(i_empty + (k & 1)));
+    return it->s >= 0;
+  };
+  const int R = pair ? kRows : 2 * kRows, units = pair ? a.n_heads / 2 : a.n_heads;
 
-  for (int p0 = 0; p0 < stop; p0 += kTile) {
-    __syncthreads();
-    for (int i = tid; i < kTile * kChunks; i += kWarps * 32) {
-      const int row = i / kChunks, c = i % kChunks;
-      const long long off = p0 + row < stop ? kv_offset(kv, s, p0 + row) : -1;
-      uint4 kk = make_uint4(0u, 0u, 0u, 0u), vv = kk;
-      if (off >= 0) {
-        kk = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(kv.k) + off + j * kv.head_stride) + c);
-        vv = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(kv.v) + off + j * kv.head_stride) + c);
-      } else if (p0 + row < stop) {
-        atomicOr(err, kErrDecodeRange);
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 10) {
+      // ---------------- scheduler ----------------
+      // Items are numbered by falling key-tile count, heads fastest; CTA b takes numbers b, 2G-1-b, 2G+b, ...
+      constexpr int kHeld = 4;  // sequences per lane kept in registers
+      int hq[kHeld], hb[kHeld];
+      bool any_clipped = false;
+      auto load = [&](int s, int* q, int* b) {
+        int qb, qe;
+        bool clipped;
+        q_range(a.cu_q, s, a.rows, &qb, &qe);
+        const int n = kv_length(kv, s, &clipped);
+        any_clipped |= clipped;
+        *q = qe - qb;
+        *b = n - (qe - qb);
+      };
+#pragma unroll
+      for (int e = 0; e < kHeld; ++e) {
+        hq[e] = hb[e] = 0;
+        if (lane + 32 * e < kv.batch) load(lane + 32 * e, hq + e, hb + e);
       }
-      *reinterpret_cast<uint4*>(smem + tile_chunk<kTile>(row, c)) = kk;
-      *reinterpret_cast<uint4*>(smem + kTile * HD * 2 + tile_chunk<kTile>(row, c)) = vv;
-    }
-    __syncthreads();
-    float sc[kTile / 8][4] = {};
+      // sum over the sequences of f(q rows, base)
+      auto total = [&](auto f) -> int {
+        int x = 0;
 #pragma unroll
-    for (int ks = 0; ks < HD / 16; ++ks)
-#pragma unroll
-      for (int kt = 0; kt < kTile / 16; ++kt) {
-        uint32_t b[4];
-        ldsm4(b, key_frag<kTile>(sk, kt * 16, ks, lane));
-        mma16816<T>(sc[2 * kt], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], b[0], b[1]);
-        mma16816<T>(sc[2 * kt + 1], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], b[2], b[3]);
-      }
-    uint32_t pf[kTile / 8][2];
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int last = base + warp * 16 + r + 8 * q;  // this row's position
-      float t = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < kTile / 8; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int p = p0 + i * 8 + c2 + e;
-          float& x = sc[i][2 * q + e];
-          x = (p <= last && p < n) ? x * sl2 : -INFINITY;
-          t = fmaxf(t, x);
+        for (int e = 0; e < kHeld; ++e) x += f(hq[e], hb[e]);
+        for (int s = lane + 32 * kHeld; s < kv.batch; s += 32) {
+          int q, b;
+          load(s, &q, &b);
+          x += f(q, b);
         }
-      t = fmaxf(t, __shfl_xor_sync(kFull, t, 1));
-      t = fmaxf(t, __shfl_xor_sync(kFull, t, 2));
-      const float mn = fmaxf(m[q], t), mz = mn == -INFINITY ? 0.0f : mn;
-      const float f = ex2(m[q] - mz);
-      m[q] = mn;
-      float sum = 0.0f;
+        return __reduce_add_sync(kFull, x);
+      };
+      int top = 0;
 #pragma unroll
-      for (int i = 0; i < kTile / 8; ++i) {
-        const float p0f = ex2(sc[i][2 * q] - mz + kShift), p1f = ex2(sc[i][2 * q + 1] - mz + kShift);
-        sum += p0f + p1f;
-        pf[i][q] = pack16<T>(p0f, p1f);
+      for (int e = 0; e < kHeld; ++e) top = max(top, hq[e] > 0 ? hq[e] + hb[e] : 0);
+      for (int s = lane + 32 * kHeld; s < kv.batch; s += 32) {
+        int q, b;
+        load(s, &q, &b);
+        top = max(top, q > 0 ? q + b : 0);
       }
-      l[q] = l[q] * f + sum;
+      top = (__reduce_max_sync(kFull, top) + kRows - 1) / kRows;  // most key tiles of any item
+      if (any_clipped && blockIdx.x == 0) atomicOr(err, kErrDecodeRange);
+      const long long count = (long long)total([&](int q, int) { return (q + R - 1) / R; }) * units;
+      for (int k = 0;; ++k) {
+        const long long G = gridDim.x, at = k * G + ((k & 1) ? G - 1 - blockIdx.x : blockIdx.x);
+        if (k >= 2 && !wait(i_empty + (k & 1), ((k >> 1) - 1) & 1)) break;
+        Item it;
+        it.s = -1;
+        if (at < count) {
+          const int rank = (int)(at / units), unit = (int)(at % units);
+          // the largest w with more than `rank` tiles of at least w key tiles
+          int lo = 0, hi = top;
+          while (lo < hi) {
+            const int w = (lo + hi + 1) >> 1;
+            if (total([&](int q, int b) { return tiles_at_least(b, q, R, w); }) > rank) lo = w; else hi = w - 1;
+          }
+          int left = rank - total([&](int q, int b) { return tiles_at_least(b, q, R, lo + 1); });
+          for (int s0 = 0; s0 < kv.batch; s0 += 32) {
+            int q = 0, b = 0;
+            if (s0 + lane < kv.batch) load(s0 + lane, &q, &b);
+            const int c1 = tiles_at_least(b, q, R, lo), c = c1 - tiles_at_least(b, q, R, lo + 1);
+            int x = c;
 #pragma unroll
-      for (int i = 0; i < HD / 8; ++i) {
-        o[i][2 * q] *= f;
-        o[i][2 * q + 1] *= f;
+            for (int o = 1; o < 32; o <<= 1) {
+              const int y = __shfl_up_sync(kFull, x, o);
+              if (lane >= o) x += y;
+            }
+            const unsigned hit = __ballot_sync(kFull, left < x);
+            if (hit) {
+              const int src = __ffs(hit) - 1;
+              const int tile = (q + R - 1) / R - c1 + (left - (x - c));
+              it.s = s0 + src;
+              it.rows = __shfl_sync(kFull, min(R, q - tile * R), src);
+              it.base = __shfl_sync(kFull, b + tile * R, src);
+              it.n = __shfl_sync(kFull, q + b, src);
+              const int t = __shfl_sync(kFull, tile, src);
+              int qb, qe;
+              q_range(a.cu_q, it.s, a.rows, &qb, &qe);
+              it.t0 = qb + t * R;
+              break;
+            }
+            left -= __shfl_sync(kFull, x, 31);
+          }
+          it.head = pair ? 2 * unit : unit;
+          it.key0 = kv.table ? 0 : __ldcg(kv.cu + it.s);
+          for (int i = 0; i < 2; ++i) {
+            const int rows = pair ? it.rows : min(kRows, it.rows - i * kRows);
+            const int stop = rows <= 0 ? 0 : it.base + (pair ? 0 : i * kRows) + rows;
+            it.tiles[i] = stop <= 0 ? 0 : (stop + kRows - 1) / kRows;
+          }
+        }
+        if (lane == 0) {
+          items[k & 1] = it;
+          mbar_arrive(smem_u32(i_full + (k & 1)));
+        }
+        __syncwarp();
+        if (it.s < 0) break;
+      }
+    } else if (warp == 9) {
+      // ---------------- loader ----------------
+      const int pages = kv.table ? kRows / box_rows : 1;
+      const int my_page = lane / kHalves, half = lane % kHalves;
+      const uint32_t box_bytes = (uint32_t)box_rows * 128u;
+      const int g = a.n_heads / kv.n_kv;
+      int c = 0, nq = 0;
+      Item it;
+      bool ok = true;
+      for (int k = 0; ok && take_item(k, &it); ++k) {
+        const int nm = max(it.tiles[0], it.tiles[1]);
+        if (nm == 0) continue;
+        if (nq > 0 && !(ok = wait(q_empty, (nq - 1) & 1))) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(smem_u32(q_full), 2 * C::kTile);
+          for (int i = 0; i < 2; ++i)
+            for (int h = 0; h < kHalves; ++h)
+              tma_load_4d(smem_u32(smem) + i * C::kTile + h * (kRows * 128), &qmap, h * 64,
+                          it.t0 + (pair ? 0 : i * kRows), it.head + (pair ? i : 0), 0, smem_u32(q_full));
+        }
+        __syncwarp();
+        ++nq;
+        const int head = it.head / g;
+        // page of this lane's box in key tile j: -1 nothing to read, n_pages reads as zeros
+        auto lookup = [&](int j) -> int {
+          const int p = j * kRows + my_page * box_rows;
+          if (my_page >= pages) return -1;
+          if (!kv.table) return 0;
+          if (j >= nm || p >= it.n) return -1;
+          const int page = __ldcg(kv.table + (long long)it.s * kv.table_stride + (p >> kv.page_shift));
+          if ((unsigned)page < (unsigned)kv.n_pages) return page;
+          atomicOr(err, kErrDecodeRange);
+          return kv.n_pages;
+        };
+        int page = lookup(0);
+        for (int j = 0; j < nm && ok; ++j) {
+          const int cur = page;
+          page = j + 1 < nm ? lookup(j + 1) : -1;
+          const unsigned live = __ballot_sync(kFull, cur >= 0);
+          const int p = j * kRows + my_page * box_rows;
+          const int row = kv.table ? p & (kv.page_size - 1) : it.key0 + p;
+          for (int v = 0; v < 2; ++v, ++c) {
+            const int st = c % S;
+            if (c >= S && !(ok = wait(kv_empty + st, ((c / S) - 1) & 1))) break;
+            const uint32_t bar = smem_u32(kv_full + st);
+            if (lane == 0) mbar_arrive_expect_tx(bar, box_bytes * __popc(live));
+            __syncwarp();
+            if (cur >= 0)
+              tma_load_4d(smem_u32(smem) + C::kRing + st * C::kTile + half * (kRows * 128) + my_page * box_bytes,
+                          v ? &vmap : &kmap, half * 64, row, head, cur, bar);
+          }
+        }
+      }
+      // what was issued lands before the CTA may end (bounded)
+      if (nq > 0) mbar_wait_bounded(smem_u32(q_full), (nq - 1) & 1);
+      for (int j = c - S < 0 ? 0 : c - S; j < c; ++j) mbar_wait_bounded(smem_u32(kv_full + j % S), (j / S) & 1);
+    } else if (warp == 8) {
+      // ---------------- matrix products ----------------
+      int c = 0, nq = 0, np[2] = {0, 0}, no[2] = {0, 0};
+      const uint32_t q_addr = smem_u32(smem), ring = q_addr + C::kRing;
+      Item it;
+      bool ok = true, issued = false;
+      auto mma_s = [&](int i, int st) {  // S_i = Q_i K^T
+        if (lane == 0) {
+          const uint64_t qd = desc_k_major(q_addr + i * C::kTile), kd = desc_k_major(ring + st * C::kTile);
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            const uint64_t step = (ks >> 2) * ((kRows * 128) >> 4) + (ks & 3) * 2;
+            umma_ss(tmem + i * kRows, qd + step, kd + step, kIdescS, ks > 0);
+          }
+          umma_commit(smem_u32(s_full + i));
+        }
+        issued = true;
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (lane == 0) umma_commit(smem_u32(bar));
+      };
+      for (int k = 0; ok && take_item(k, &it); ++k) {
+        const int nm = max(it.tiles[0], it.tiles[1]);
+        if (nm == 0) continue;
+        if (!(ok = wait(q_full, nq & 1))) break;
+        ++nq;
+        if (!(ok = wait(kv_full + c % S, (c / S) & 1))) break;
+        for (int i = 0; i < 2; ++i)
+          if (it.tiles[i] > 0) mma_s(i, c % S);
+        commit(kv_empty + c % S);
+        if (nm == 1) commit(q_empty);
+        ++c;
+        for (int j = 0; j < nm && ok; ++j, c += 2) {
+          const int sv = c % S, sk = (c + 1) % S;  // this tile's values, the next one's keys
+          if (!(ok = wait(kv_full + sv, (c / S) & 1))) break;
+          const int valid = it.n - j * kRows;
+          if (valid < kRows) {  // nothing lives behind the sequence's end: zero weights meet zeros there
+            for (int h = 0; h < kHalves; ++h)
+              for (int b = valid * 128 + lane * 16; b < kRows * 128; b += 512)
+                *reinterpret_cast<uint4*>(smem + C::kRing + sv * C::kTile + h * (kRows * 128) + b) =
+                    make_uint4(0u, 0u, 0u, 0u);
+            fence_proxy_async();
+            __syncwarp();
+          }
+          bool have_k = false;
+          for (int i = 0; i < 2 && ok; ++i) {
+            if (j < it.tiles[i]) {
+              if (!(ok = wait(p_full + i, np[i] & 1))) break;
+              ++np[i];
+              if (j == 0) {
+                if (no[i] > 0 && !(ok = wait(o_empty + i, (no[i] - 1) & 1))) break;
+                ++no[i];
+              }
+              tc_fence_after();
+              if (lane == 0) {
+                const uint64_t vd = desc_mn_major(ring + sv * C::kTile);
+#pragma unroll
+                for (int ks = 0; ks < kRows / 16; ++ks)
+                  umma_ts(tmem + C::kO + i * HD, tmem + i * kRows + ks * 8, vd + ks * (2048 >> 4), kIdescO,
+                          j > 0 || ks > 0);
+              }
+              issued = true;
+              if (j == it.tiles[i] - 1) commit(o_full + i);
+            }
+            if (i == 1) commit(kv_empty + sv);
+            if (j + 1 < it.tiles[i]) {
+              if (!have_k && !(ok = wait(kv_full + sk, ((c + 1) / S) & 1))) break;
+              have_k = true;
+              mma_s(i, sk);
+            }
+          }
+          if (!ok) break;
+          if (j + 1 < nm) {
+            commit(kv_empty + sk);
+            if (j + 2 == nm) commit(q_empty);
+          } else {
+            --c;  // there was no next key tile
+          }
+        }
+      }
+      if (issued) {  // the tensor core is done before tensor memory is released
+        commit(drain);
+        if (!mbar_wait_bounded(smem_u32(drain), 0)) fail();
       }
     }
+  } else {
+    // ---------------- softmax ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    const int i = warp >> 2, lrow = 32 * (warp & 3) + lane;
+    const uint32_t ts = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + i * kRows;
+    const uint32_t to = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + C::kO + i * HD;
+    const float sl2 = a.scale * 1.4426950408889634f;
+    int ns = 0, no = 0;
+    Item it;
+    for (int k = 0; take_item(k, &it); ++k) {
+      const int row = lrow + (pair ? 0 : i * kRows), head = it.head + (pair ? i : 0), tiles = it.tiles[i];
+      const int pos = it.base + row;
+      float m = -INFINITY, l = 0.0f;
+      bool ok = true;
+      for (int j = 0; j < tiles; ++j) {
+        if (!(ok = wait(s_full + i, ns & 1))) break;
+        ++ns;
+        tc_fence_after();
+        uint32_t x[kRows];
 #pragma unroll
-    for (int kt = 0; kt < kTile / 16; ++kt)
+        for (int b = 0; b < kRows; b += 32) tmem_ld<32>(ts + b, *reinterpret_cast<uint32_t(*)[32]>(x + b));
+        tmem_wait_ld();
+        const int limit = pos - j * kRows + 1;  // columns below it are attended to
+        if (!__all_sync(kFull, limit >= kRows)) {
 #pragma unroll
-      for (int nt = 0; nt < HD / 16; ++nt) {
-        uint32_t b[4];
-        ldsm4_t(b, value_frag<kTile>(sv, kt * 16, nt, lane));
-        mma16816<T>(o[2 * nt], pf[2 * kt][0], pf[2 * kt][1], pf[2 * kt + 1][0], pf[2 * kt + 1][1], b[0], b[1]);
-        mma16816<T>(o[2 * nt + 1], pf[2 * kt][0], pf[2 * kt][1], pf[2 * kt + 1][0], pf[2 * kt + 1][1], b[2], b[3]);
+          for (int e = 0; e < kRows; ++e)
+            if (e >= limit) x[e] = 0xFF800000u;
+        }
+        float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < kRows; e += 8)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) t[q] = max3(t[q], __uint_as_float(x[e + 2 * q]), __uint_as_float(x[e + 2 * q + 1]));
+        const float mt = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        if (j == 0) {
+          m = mt;
+        } else if (__any_sync(kFull, (mt - m) * sl2 > kLazy || m == -INFINITY)) {
+          const float mn = fmaxf(m, mt), f = m == -INFINITY ? 0.0f : ex2((m - mn) * sl2);
+          m = mn;
+          l *= f;
+          const unsigned long long f2 = pack2(f, f);
+#pragma unroll
+          for (int b = 0; b < HD; b += 32) {
+            uint32_t y[32];
+            tmem_ld<32>(to + b, y);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              float y0, y1;
+              unpack2(mul2(pack2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), f2), y0, y1);
+              y[e] = __float_as_uint(y0);
+              y[e + 1] = __float_as_uint(y1);
+            }
+            tmem_st32(to + b, y);
+          }
+        }
+        const float off = kPShift - (m == -INFINITY ? 0.0f : m * sl2);
+        const unsigned long long sl22 = pack2(sl2, sl2), off2 = pack2(off, off);
+        unsigned long long sum[2] = {0ull, 0ull};
+#pragma unroll
+        for (int b = 0; b < kRows; b += 64) {
+          uint32_t w[32];
+#pragma unroll
+          for (int e = 0; e < 64; e += 2) {
+            float x0, x1;
+            unpack2(fma2(pack2(__uint_as_float(x[b + e]), __uint_as_float(x[b + e + 1])), sl22, off2), x0, x1);
+            x0 = ex2(x0);
+            x1 = ex2(x1);
+            sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(x0, x1));
+            w[e >> 1] = pack16<T>(x0, x1);
+          }
+          tmem_st32(ts + (b >> 1), w);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(p_full + i));
+        float s0, s1;
+        unpack2(add2(sum[0], sum[1]), s0, s1);
+        l += s0 + s1;
       }
-  }
-#pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    l[q] += __shfl_xor_sync(kFull, l[q], 1);
-    l[q] += __shfl_xor_sync(kFull, l[q], 2);
-    const float inv = l[q] == 0.0f ? 0.0f : 1.0f / l[q];
-    const int row = warp * 16 + r + 8 * q;
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < HD / 8; ++i) {
-      const float v0 = o[i][2 * q] * inv, v1 = o[i][2 * q + 1] * inv;
-      bad |= !(fabsf(v0) < INFINITY) || !(fabsf(v1) < INFINITY);
-      if (row < rows) {
-        O* p = static_cast<O*>(a.out) + ((long long)(t0 + row) * a.n_heads + h) * HD + i * 8 + c2;
-        if constexpr (sizeof(O) == 4) *reinterpret_cast<float2*>(p) = make_float2(v0, v1);
-        else *reinterpret_cast<uint32_t*>(p) = pack16<O>(v0, v1);
+      if (!ok) break;
+      const bool mine = row < it.rows;
+      if (tiles == 0) {  // no key for any row of the tile
+        if (mine) {
+          O* out = static_cast<O*>(a.out) + ((long long)(it.t0 + row) * a.n_heads + head) * HD;
+          const float z[8] = {};
+          for (int b = 0; b < HD; b += 8) store8(out + b, z);
+        }
+        continue;
       }
-    }
-    unsigned todo = __ballot_sync(kFull, bad && row < rows);
-    while (todo) {  // one row of the warp at a time
-      const int rr = (__ffs(todo) - 1) >> 2;
-      todo &= ~(0xFu << (4 * rr));
-      const int rw = warp * 16 + rr + 8 * q;
+      if (!wait(o_full + i, no & 1)) break;
+      ++no;
+      tc_fence_after();
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      O* out = static_cast<O*>(a.out) + ((long long)(it.t0 + row) * a.n_heads + head) * HD;
+      bool bad = false;
+#pragma unroll
+      for (int b = 0; b < HD; b += 32) {
+        uint32_t y[32];
+        tmem_ld<32>(to + b, y);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          float v[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            v[q] = __uint_as_float(y[e + q]) * inv;
+            bad |= !(fabsf(v[q]) < INFINITY);
+          }
+          if (mine) store8(out + b + e, v);
+        }
+      }
+      tc_fence_before();
       __syncwarp();
-      attend_row<T, O, HD>(a, kv, t0 + rw, h, s, min(base + rw, n - 1), lane);
+      if (lane == 0) mbar_arrive(smem_u32(o_empty + i));
+      // Rows that are not finite: because of a later position's value?
+      unsigned todo = __ballot_sync(kFull, bad && mine);
+      if (todo) {
+        const int first = __shfl_sync(kFull, pos, __ffs(todo) - 1) + 1, last = min(it.n, tiles * kRows);
+        const long long ho = (long long)(head / (a.n_heads / kv.n_kv)) * kv.head_stride;
+        bool later = false;
+        for (int p = max(0, first); p < last; ++p) {
+          const long long o = kv_offset(kv, it.s, p);
+          if (o < 0) continue;
+          for (int e = lane; e < HD; e += 32) later |= !(fabsf(to_f32(static_cast<const T*>(kv.v)[o + ho + e])) < INFINITY);
+        }
+        if (__any_sync(kFull, later)) {
+          __syncwarp();  // the rows' first stores come before the second ones
+          while (todo) {
+            const int src = __ffs(todo) - 1;
+            todo &= todo - 1;
+            const int rr = __shfl_sync(kFull, row, src);
+            attend_row<T, O, HD>(a, kv, it.t0 + rr, head, it.s, min(it.base + rr, it.n - 1), lane);
+          }
+        }
+      }
     }
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
 template <class T, class O, int HD>
 cudaError_t launch_typed(const PromptArgs& a, const KvArgs& kv, cudaStream_t stream, unsigned* err) {
+  using C = Cfg<HD>;
   auto kernel = attention_prompt_kernel<T, O, HD>;
-  const size_t smem = 2 * kTile * HD * 2 + 1024;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  CUtensorMap qmap, kmap, vmap;
+  const int box_rows = kv.table && kv.page_size < kRows ? kv.page_size : kRows;
+  if (!encode_4d(&qmap, kv.dtype, a.q, HD, (uint64_t)a.rows, (uint64_t)a.n_heads, 1, (uint64_t)a.q_row_stride,
+                 (uint64_t)a.q_head_stride, (uint64_t)a.q_row_stride, kRows) ||
+      !encode_kv_map(&kmap, kv, kv.k, box_rows) || !encode_kv_map(&vmap, kv, kv.v, box_rows))
+    return cudaErrorInvalidValue;
+  int dev = 0, sms = 0;
+  cudaGetDevice(&dev);
+  cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return e;
+  if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem)) != cudaSuccess) return e;
+  const int pair = (a.n_heads / kv.n_kv) % 2 == 0, R = pair ? kRows : 2 * kRows;
+  const long long items = ((long long)a.rows / R + kv.batch) * (pair ? a.n_heads / 2 : a.n_heads);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)a.n_heads, (unsigned)(a.rows / kTile + kv.batch));
-  cfg.blockDim = dim3(kWarps * 32);
-  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3((unsigned)(items < sms ? items : sms));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = g_opt_pdl.load() ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, a, kv, err);
+  return cudaLaunchKernelEx(&cfg, kernel, qmap, kmap, vmap, a, kv, pair, box_rows, err);
 }
 
 template <class T>

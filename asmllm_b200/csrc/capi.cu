@@ -928,7 +928,9 @@ int check_heads(const char* name, int n_heads, int n_kv) {
 }
 
 int check_query(const char* name, const void* q, int64_t row_stride, int64_t head_stride, const void* out,
-                int out_dtype, int cache_dtype) {
+                int out_dtype, int cache_dtype, float scale) {
+  if (!(scale > 0.0f) || scale > 1e30f)
+    return set_error(ASM_E_INVALID, "%s: scale must be positive and finite", name);
   if (row_stride <= 0 || row_stride % 8 || head_stride <= 0 || head_stride % 8 || (uintptr_t)q % 16 ||
       (uintptr_t)out % 16)
     return set_error(ASM_E_INVALID, "%s: q strides must be positive multiples of 8, q and out 16-byte aligned", name);
@@ -981,7 +983,7 @@ ASMLLM_API int asm_attention_prompt_async(const void* q, int64_t q_row_stride, i
   KvArgs kv;
   int rc;
   if ((rc = check_kv(name, kvd, false, &kv)) || (rc = check_heads(name, n_heads, kv.n_kv)) ||
-      (rc = check_query(name, q, q_row_stride, q_head_stride, out, out_dtype, kv.dtype)))
+      (rc = check_query(name, q, q_row_stride, q_head_stride, out, out_dtype, kv.dtype, scale)))
     return rc;
   if (rows < 0 || rows > (1 << 22) || kv.batch > (1 << 15))
     return set_error(rows < 0 ? ASM_E_INVALID : ASM_E_UNSUPPORTED, "%s: rows %d (0..2^22) of %d sequences (..2^15)",
@@ -1022,7 +1024,7 @@ ASMLLM_API int asm_attention_paged_async(const void* q, int64_t q_row_stride, in
   KvArgs kv;
   int rc;
   if ((rc = check_kv(name, kvd, true, &kv)) || (rc = check_heads(name, n_heads, kv.n_kv)) ||
-      (rc = check_query(name, q, q_row_stride, q_head_stride, out, out_dtype, kv.dtype)))
+      (rc = check_query(name, q, q_row_stride, q_head_stride, out, out_dtype, kv.dtype, scale)))
     return rc;
   if (kv.batch > (1 << 15)) return set_error(ASM_E_UNSUPPORTED, "%s: batch %d (at most 2^15)", name, kv.batch);
   const size_t need = attention_paged_workspace(kv.batch, n_heads, kv.n_kv, kv.head_dim);

@@ -695,7 +695,7 @@ ASMLLM_API int asm_rope_append_async(const void* qkv, int32_t qkv_dtype, int64_t
 /* Causal attention of packed prompts: q [rows][n_heads][head_dim] of the
  * cache's type (row and head strides in elements, multiples of 8), positions
  * as above (bottom-right aligned: the last row of a sequence sees all its
- * keys), query head h on KV head h / (n_heads / n_kv_heads).  out
+ * keys), query head h on KV head h / (n_heads / n_kv_heads), scale > 0.  out
  * [rows][n_heads][head_dim], fp32 or the cache's type.  Rows without a key
  * give zeros; rows at or past cu_q[batch] are left as they are.  Scores,
  * maxima and sums are fp32; the weights are rounded to the 16-bit type for
