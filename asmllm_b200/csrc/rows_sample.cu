@@ -42,11 +42,13 @@ namespace cg = cooperative_groups;
 
 typedef unsigned long long u64;
 constexpr int kThreads = 512;
-constexpr int kBins = 2048;   // bins of (m - x) / temperature, 1/64 wide; the last: weighs nothing
-constexpr float kBinsPerUnit = 64.0f;
+constexpr int kBins = 1024;   // bins of (m - x) / temperature, 1/32 wide; the last: weighs nothing
+constexpr float kBinsPerUnit = 32.0f;
 constexpr int kList = 1024;   // words that are put in order by comparing each with each
 constexpr int kIndexBits = 18;
+constexpr int kPart = 15;     // masses are added up in three parts of 15 bits (45 and the top word's one)
 static_assert(kSampleMaxN <= 1 << kIndexBits, "the index fits the order word");
+static_assert(kSampleMaxN / 8 <= 1 << 15, "a slice's sum of 16-bit parts fits 32 bits");
 
 __constant__ double kPow2[64] = {  // 2^(j / 64)
     1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
@@ -67,48 +69,46 @@ __constant__ double kPow2[64] = {  // 2^(j / 64)
     1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951,
 };
 
-// Order of logits as unsigned integers; 0 for NaN, so every number is above it.
-__device__ __forceinline__ unsigned order_key(float v) {
-  const unsigned u = __float_as_uint(v == 0.0f ? 0.0f : v);  // -0 and +0 are one value
-  return v == v ? ((u & 0x80000000u) ? ~u : (u | 0x80000000u)) : 0u;
+// (value, index) as one word, larger = earlier in the order.  Values are never NaN or -0 here.
+__device__ __forceinline__ u64 order_word(float v, int index) {
+  const unsigned u = __float_as_uint(v);
+  return ((u64)((u & 0x80000000u) ? ~u : (u | 0x80000000u)) << kIndexBits) | (u64)((1 << kIndexBits) - 1 - index);
 }
-__device__ __forceinline__ float key_value(unsigned k) {
+__device__ __forceinline__ float word_value(u64 w) {
+  const unsigned k = (unsigned)(w >> kIndexBits);
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
 }
-// (key, index) as one word, larger = earlier in the order.
-__device__ __forceinline__ u64 order_word(unsigned key, int index) {
-  return ((u64)key << kIndexBits) | (u64)((1 << kIndexBits) - 1 - index);
-}
+__device__ __forceinline__ int word_index(u64 w) { return (1 << kIndexBits) - 1 - (int)(w & ((1u << kIndexBits) - 1)); }
 
 struct Shared {
-  u64 hist[2][kBins];
+  unsigned hist[2][3][kBins];  // two in turn; counts use the first part alone
+  u64 coarse[2][32];           // sums of 32 bins each
   u64 list[kList], mass[kList];
   u64 scan[kThreads / 32];
-  u64 out[2], sum;
+  u64 found[3];
   double pow2[64];
   u64 best;      // this CTA's first word
+  u64 sum;       // this CTA's kept mass
   u64 cut;       // the border found by rank 0
   int count[3];  // words in the list of each selection (at most three in a call)
 };
 
 struct Row {
-  unsigned top;      // key of the largest logit
-  float vtop;
+  float vtop;        // the largest logit
   float bin_scale;   // kBinsPerUnit / temperature
   double exp_scale;  // log2(e) / temperature
   const double* pow2;
 
-  __device__ __forceinline__ int bin(unsigned key) const {
-    if (key == top) return 0;
-    const float t = (vtop - key_value(key)) * bin_scale;
-    return key && t < (float)(kBins - 1) ? (int)t : kBins - 1;
+  __device__ __forceinline__ int bin(float v) const {
+    const float t = (vtop - v) * bin_scale;
+    return v == vtop ? 0 : t < (float)(kBins - 1) ? (int)t : kBins - 1;
   }
-  // w = exp((x - m) / temperature) and its fixed-point mass, for a word that is not in the last bin.
+  // w = exp((x - m) / temperature) for a word that is not in the last bin.
   // Table-driven (Tang 1989): x = (64 k + j) / 64 + r in powers of two, |r| <= 1/128, 2^(j/64) from the
   // table and 2^r from its Taylor polynomial; the remainder r^6 ln(2)^6 / 720 is below 2^-54.
-  __device__ __forceinline__ double weight(unsigned key) const {
-    if (key == top) return 1.0;
-    const double y = ((double)key_value(key) - (double)vtop) * exp_scale;
+  __device__ __forceinline__ double weight(float v) const {
+    if (v == vtop) return 1.0;
+    const double y = ((double)v - (double)vtop) * exp_scale;
     const double big = y + 105553116266496.0;  // 1.5 * 2^46: rounds to a multiple of 1/64
     const int n = __double2loint(big);
     const double z = (y - (big - 105553116266496.0)) * 0.6931471805599453;
@@ -120,8 +120,11 @@ struct Row {
     const double t = pow2[n & 63];
     return __hiloint2double(__double2hiint(t) + (n >> 6) * 1048576, __double2loint(t)) * p;
   }
-  __device__ __forceinline__ static u64 fixed(double w) { return __double2ull_rn(w * 35184372088832.0); }  // 2^45
-  __device__ __forceinline__ u64 mass(unsigned key) const { return bin(key) == kBins - 1 ? 0ull : fixed(weight(key)); }
+  // w <= 1 as a multiple of 2^-45: adding 2^7 leaves 45 bits behind the point, rounded to nearest even
+  __device__ __forceinline__ static u64 fixed(double w) {
+    return (u64)__double_as_longlong(w + 128.0) - 0x4060000000000000ull;
+  }
+  __device__ __forceinline__ u64 mass(float v) const { return bin(v) == kBins - 1 ? 0ull : fixed(weight(v)); }
 };
 
 // Inclusive scan over the CTA; every thread also gets the total.
@@ -149,55 +152,102 @@ __device__ __forceinline__ u64 block_scan(u64 v, Shared& sh, u64* total) {
 // One row's slice in a CTA of the cluster and the selections over the whole row.
 struct Slice {
   Shared& sh;
-  const unsigned* keys;
+  const float* val;
   int n, first;  // words first .. first + n - 1 of the row
   cg::cluster_group cluster;
-  int ranks, rank;
+  int ranks;
   Row row;
-  int levels = 0;  // histograms used so far (two buffers in turn)
+  float cut_v = -INFINITY;  // the words at or before (cut_v, cut_i) of the order are kept
+  int cut_i = 1 << kIndexBits;
+  int levels = 0;           // histograms used so far (two buffers in turn)
   int lists = 0;
 
-  __device__ __forceinline__ u64* clear(int bins) {
-    // the other CTAs read this buffer two levels ago and have met at a cluster barrier since
-    u64* h = sh.hist[levels & 1];
-    for (int i = threadIdx.x; i < bins; i += kThreads) h[i] = 0;
+  __device__ __forceinline__ bool keep(float v, int i) const { return v > cut_v || (v == cut_v && first + i <= cut_i); }
+
+  // Empties the next histogram.  The other CTAs read this buffer two histograms ago and have met at a
+  // cluster barrier since.
+  template <bool MASS>
+  __device__ __forceinline__ void clear() {
+    unsigned* h = &sh.hist[levels & 1][0][0];
+    for (int i = threadIdx.x; i < (MASS ? 3 : 1) * kBins; i += kThreads) h[i] = 0;
     __syncthreads();
-    return h;
+  }
+  template <bool MASS>
+  __device__ __forceinline__ void add(int bin, float v) {
+    unsigned* h = &sh.hist[levels & 1][0][bin];
+    if (MASS) {
+      const u64 m = Row::fixed(row.weight(v));
+      atomicAdd(h, (unsigned)m & ((1u << kPart) - 1));
+      atomicAdd(h + kBins, (unsigned)(m >> kPart) & ((1u << kPart) - 1));
+      atomicAdd(h + 2 * kBins, (unsigned)(m >> (2 * kPart)));
+    } else {
+      atomicAdd(h, 1u);
+    }
+  }
+  template <bool MASS>
+  __device__ __forceinline__ static u64 read(const unsigned* h) {
+    return MASS ? (u64)h[0] + ((u64)h[kBins] << kPart) + ((u64)h[2 * kBins] << (2 * kPart)) : (u64)h[0];
   }
 
-  // Adds the cluster's histograms and finds the first bin at which the running sum reaches `want`;
-  // bins means "none".  *before: the sum up to that bin; *total: of all bins.
-  template <int BINS>
-  __device__ int find(u64 want, u64* before, u64* total) {
-    constexpr int E = BINS / kThreads;
+  // Sums the histogram by 32 bins and meets the other CTAs.  Returns the total of the row.
+  template <bool MASS>
+  __device__ u64 publish() {
+    __syncthreads();
+    const unsigned* h = &sh.hist[levels & 1][0][0];
+    u64 v = read<MASS>(h + 2 * threadIdx.x) + read<MASS>(h + 2 * threadIdx.x + 1);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    if ((threadIdx.x & 15) == 0) sh.coarse[levels & 1][threadIdx.x >> 4] = v;
     cluster.sync();
-    u64* h = sh.hist[levels & 1];
-    ++levels;
-    u64 v[E] = {};
-    for (int r = 0; r < ranks; ++r) {
-      const u64* p = cluster.map_shared_rank(h, r) + threadIdx.x * E;
+    if (threadIdx.x < 32) {
+      u64 t = 0;
+      for (int r = 0; r < ranks; ++r) t += cluster.map_shared_rank(&sh, r)->coarse[levels & 1][threadIdx.x];
+      u64 x = t;
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] += p[e];
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 y = __shfl_up_sync(kFull, x, o);
+        if (threadIdx.x >= o) x += y;
+      }
+      sh.mass[threadIdx.x] = x;  // running sums over the row, for find (the list is idle)
     }
-    u64 mine = 0;
+    __syncthreads();
+    return sh.mass[31];
+  }
+
+  // The first bin at which the row's running sum reaches `want` (kBins: none) and the sum before it.
+  template <bool MASS>
+  __device__ int find(u64 want, u64* before) {
+    static_assert(kBins == 1024, "32 sums of 32 bins");
+    if (threadIdx.x < 32) {
+      const unsigned lane = threadIdx.x;
+      const unsigned hit = __ballot_sync(kFull, sh.mass[lane] >= want);
+      int b = kBins;
+      u64 run = 0;
+      if (hit) {
+        const int c = __ffs(hit) - 1;
+        if (c) run = sh.mass[c - 1];
+        u64 t = 0;
+        for (int r = 0; r < ranks; ++r)
+          t += read<MASS>(&cluster.map_shared_rank(&sh, r)->hist[levels & 1][0][32 * c + lane]);
+        u64 x = t;
 #pragma unroll
-    for (int e = 0; e < E; ++e) mine += v[e];
-    if (threadIdx.x == 0) sh.out[0] = (u64)BINS;
-    u64 run = block_scan(mine, sh, total) - mine;
-    if (run < want && run + mine >= want) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if (run < want && run + v[e] >= want) {
-          sh.out[0] = (u64)(threadIdx.x * E + e);
-          sh.out[1] = run;
+        for (int o = 1; o < 32; o <<= 1) {
+          const u64 y = __shfl_up_sync(kFull, x, o);
+          if (lane >= o) x += y;
         }
-        run += v[e];
+        const int e = __ffs(__ballot_sync(kFull, run + x >= want)) - 1;
+        b = 32 * c + e;
+        run += __shfl_sync(kFull, x - t, e);
+      }
+      if (lane == 0) {
+        sh.found[0] = (u64)b;
+        sh.found[1] = run;
       }
     }
+    ++levels;
     __syncthreads();
-    const int b = (int)sh.out[0];
-    *before = sh.out[1];
-    __syncthreads();
+    const int b = (int)sh.found[0];
+    *before = sh.found[1];
     return b;
   }
 
@@ -208,64 +258,54 @@ struct Slice {
     if (i < kList) s0->list[i] = w;
   }
 
-  // The border of the order at `want`: the earliest word such that it and the words before it (of those
-  // at or above `from`) weigh at least `want`, each 1 or its mass.  0 if all together weigh less.
+  // Moves the border to the earliest word such that it and the kept words before it weigh at least
+  // `want` (each 1, or its mass); the histogram of the kept words' bins is published.  No change if all
+  // weigh less.
   template <bool MASS>
-  __device__ u64 border(u64 from, u64 want, u64* total) {
-    u64* h = clear(kBins);
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const unsigned key = keys[i];
-      const int b = row.bin(key);
-      if (b < kBins - 1 && order_word(key, first + i) >= from)
-        atomicAdd(h + b, MASS ? Row::fixed(row.weight(key)) : 1ull);
-    }
-    return border_in(from, want, total, MASS);
-  }
-
-  __device__ u64 border_in(u64 from, u64 want, u64* total, bool by_mass) {
+  __device__ void border(u64 want) {
     u64 before;
-    const int b = find<kBins>(want, &before, total);
-    if (b == kBins) return 0;
+    const int b = find<MASS>(want, &before);
+    if (b == kBins) return;
     for (int i = threadIdx.x; i < n; i += kThreads) {
-      const unsigned key = keys[i];
-      const u64 w = order_word(key, first + i);
-      if (row.bin(key) == b && w >= from) append(w);
+      const float v = val[i];
+      if (row.bin(v) == b && keep(v, i)) append(order_word(v, first + i));
     }
     cluster.sync();
     const int c = cluster.map_shared_rank(&sh, 0)->count[lists];
     ++lists;
+    u64 w = 0;
     if (c <= kList) {
-      if (rank == 0) {
-        for (int i = threadIdx.x; i < c; i += kThreads)
-          sh.mass[i] = by_mass ? row.mass((unsigned)(sh.list[i] >> kIndexBits)) : 1ull;
+      if (cluster.block_rank() == 0) {
+        for (int i = threadIdx.x; i < c; i += kThreads) sh.mass[i] = MASS ? row.mass(word_value(sh.list[i])) : 1ull;
         __syncthreads();
         for (int i = threadIdx.x; i < c; i += kThreads) {
-          const u64 w = sh.list[i];
+          const u64 x = sh.list[i];
           u64 s = before;
           for (int j = 0; j < c; ++j)
-            if (sh.list[j] > w) s += sh.mass[j];
-          if (s < want && s + sh.mass[i] >= want) sh.cut = w;
+            if (sh.list[j] > x) s += sh.mass[j];
+          if (s < want && s + sh.mass[i] >= want) sh.cut = x;
         }
       }
       cluster.sync();
-      return cluster.map_shared_rank(&sh, 0)->cut;
-    }
-    // too many words in one bin (equal logits): digit by digit of the order word, from the top
-    u64 prefix = 0;
-    for (int shift = 32 + kIndexBits - 10; shift >= 0; shift -= 10) {
-      u64* h = clear(1024);
-      for (int i = threadIdx.x; i < n; i += kThreads) {
-        const unsigned key = keys[i];
-        const u64 w = order_word(key, first + i);
-        if (row.bin(key) == b && w >= from && (w >> (shift + 10)) == prefix)
-          atomicAdd(h + (1023 - (int)((w >> shift) & 1023u)), by_mass ? Row::fixed(row.weight(key)) : 1ull);
+      w = cluster.map_shared_rank(&sh, 0)->cut;
+    } else {  // too many words in one bin (equal logits): digit by digit of the order word, from the top
+      for (int shift = 32 + kIndexBits - 10; shift >= 0; shift -= 10) {
+        clear<MASS>();
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+          const float v = val[i];
+          if (row.bin(v) != b || !keep(v, i)) continue;
+          const u64 x = order_word(v, first + i);
+          if ((x >> (shift + 10)) == w) add<MASS>(1023 - (int)((x >> shift) & 1023u), v);
+        }
+        u64 over;
+        publish<MASS>();
+        const int d = find<MASS>(want - before, &over);
+        before += over;
+        w = (w << 10) | (u64)(1023 - d);
       }
-      u64 over, sum;
-      const int d = find<1024>(want - before, &over, &sum);
-      before += over;
-      prefix = (prefix << 10) | (u64)(1023 - d);
     }
-    return prefix;
+    cut_v = word_value(w);
+    cut_i = word_index(w);
   }
 };
 
@@ -273,18 +313,13 @@ template <class T>
 __global__ void __launch_bounds__(kThreads, 2) rows_sample_kernel(const SampleArgs a, int per) {
   extern __shared__ __align__(16) unsigned char s_raw[];
   Shared& sh = *reinterpret_cast<Shared*>(s_raw);
-  unsigned* s_keys = reinterpret_cast<unsigned*>(s_raw + sizeof(Shared));
+  float* s_val = reinterpret_cast<float*>(s_raw + sizeof(Shared));
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int r = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31;
   const int first = min(a.n, rank * per), n = min(a.n, first + per) - first;
   if (tid < 64) sh.pow2[tid] = kPow2[tid];
-  if (tid == 0) {
-    sh.best = 0;
-    sh.cut = 0;
-    sh.count[0] = sh.count[1] = sh.count[2] = 0;
-  }
-  __syncthreads();
+  if (tid < 3) sh.count[tid] = 0;
   pdl_trigger();
   pdl_wait();
   const float temp = a.temperature ? __ldcg(a.temperature + r) : 1.0f;
@@ -292,24 +327,32 @@ __global__ void __launch_bounds__(kThreads, 2) rows_sample_kernel(const SampleAr
   const float tp = a.top_p ? __ldcg(a.top_p + r) : 1.0f, mp = a.min_p ? __ldcg(a.min_p + r) : 0.0f;
   const float u = __ldcg(a.u + r);
 
-  // the slice, as order keys, and its first word
+  // The slice (NaN as -inf: neither weighs anything; -0 as +0) and its first word.
   const T* row = static_cast<const T*>(a.logits) + (long long)r * a.stride + first;
-  u64 best = 0;
-  auto put = [&](int i, float v) {
-    const unsigned key = order_key(v);
-    s_keys[i] = key;
-    const u64 w = key ? order_word(key, first + i) : 0ull;
-    best = w > best ? w : best;
+  float bv = -INFINITY;
+  int bi = 0;
+  auto put = [&](int i, float v) -> float {  // a thread's indices rise, so > keeps its lowest one
+    v = v == v ? v + 0.0f : -INFINITY;
+    if (v > bv) {
+      bv = v;
+      bi = i;
+    }
+    return v;
   };
   int done = 0;
   if ((uintptr_t)row % 16 == 0) {
-    done = n & ~7;
+    constexpr int E = 16 / sizeof(T);
+    done = n & ~(E - 1);
 #pragma unroll 4
-    for (int i = tid * 8; i < done; i += kThreads * 8) {
-      float v[8];
-      load8(row + i, v);
+    for (int i = tid * E; i < done; i += kThreads * E) {
+      const uint4 w = __ldcg(reinterpret_cast<const uint4*>(row + i));
+      const T* p = reinterpret_cast<const T*>(&w);
+      float v[E];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) put(i + e, v[e]);
+      for (int e = 0; e < E; ++e) v[e] = put(i + e, to_f32(p[e]));
+#pragma unroll
+      for (int e = 0; e < E; e += 4)
+        *reinterpret_cast<float4*>(s_val + i + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
     }
   }
 #pragma unroll 4
@@ -320,8 +363,9 @@ __global__ void __launch_bounds__(kThreads, 2) rows_sample_kernel(const SampleAr
       const unsigned short h = __ldcg(reinterpret_cast<const unsigned short*>(row) + i);
       v = to_f32(*reinterpret_cast<const T*>(&h));
     }
-    put(i, v);
+    s_val[i] = put(i, v);
   }
+  u64 best = bv > -INFINITY ? order_word(bv, first + bi) : 0ull;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const u64 t = __shfl_xor_sync(kFull, best, o);
@@ -332,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_sample_kernel(const SampleAr
   if (tid < 32) {
     best = tid < kThreads / 32 ? sh.scan[tid] : 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+    for (int o = 8; o > 0; o >>= 1) {
       const u64 t = __shfl_xor_sync(kFull, best, o);
       best = t > best ? t : best;
     }
@@ -344,34 +388,35 @@ __global__ void __launch_bounds__(kThreads, 2) rows_sample_kernel(const SampleAr
     const u64 t = cluster.map_shared_rank(&sh, q)->best;
     best = t > best ? t : best;
   }
-  const unsigned top = (unsigned)(best >> kIndexBits);
-  const float vtop = key_value(top);
-  const bool none = best == 0 || vtop == -INFINITY;
-  if (none || !(temp > 0.0f)) {
-    if (rank == 0 && tid == 0)
-      a.tokens[r] = none ? -1 : (1 << kIndexBits) - 1 - (int)(best & ((1u << kIndexBits) - 1));
+  if (best == 0 || !(temp > 0.0f)) {
+    if (rank == 0 && tid == 0) a.tokens[r] = best == 0 ? -1 : word_index(best);
     cluster.sync();  // nobody leaves while its shared memory may be read
     return;
   }
-  Slice s{sh, s_keys, n, first, cluster, ranks, rank,
-          Row{top, vtop, kBinsPerUnit / temp, 1.4426950408889634 / (double)temp, sh.pow2}};
+  const float vtop = word_value(best);
+  Slice s{sh, s_val, n, first, cluster, ranks, Row{vtop, kBinsPerUnit / temp, 1.4426950408889634 / (double)temp, sh.pow2}};
   const double least = (double)mp;
-  const bool by_k = k > 0 && k < a.n;
-  u64 from = 0, total;
+  u64 total;
 
-  if (by_k) {
-    u64* h = s.clear(kBins);
-    for (int i = tid; i < n; i += kThreads) {
-      const int b = s.row.bin(s_keys[i]);
-      if (b < kBins - 1) atomicAdd(h + b, 1ull);
-    }
+  if (k > 0 && k < a.n) {
+    auto counts = [&]() {
+      s.template clear<false>();
+#pragma unroll 4
+      for (int i = tid; i < n; i += kThreads) {
+        const int b = s.row.bin(s_val[i]);
+        if (b < kBins - 1) s.template add<false>(b, 0.0f);
+      }
+      s.template publish<false>();
+    };
+    counts();
     if (k <= kList / 2) {
       // the short way: every word down to the border's bin, if they fit the list
       u64 before;
-      int b = s.find<kBins>((u64)k, &before, &total);
+      int b = s.template find<false>((u64)k, &before);
       if (b == kBins) b = kBins - 2;  // fewer than top_k words weigh anything
+#pragma unroll 4
       for (int i = tid; i < n; i += kThreads)
-        if (s.row.bin(s_keys[i]) <= b) s.append(order_word(s_keys[i], first + i));
+        if (s.row.bin(s_val[i]) <= b) s.append(order_word(s_val[i], first + i));
       cluster.sync();
       const int c = cluster.map_shared_rank(&sh, 0)->count[0];
       ++s.lists;
@@ -379,13 +424,15 @@ __global__ void __launch_bounds__(kThreads, 2) rows_sample_kernel(const SampleAr
         cluster.sync();
         if (rank != 0) return;
         u64 sum = 0;
-        u64* rest = sh.hist[0];  // mass of the words before each (the histograms are no longer needed)
-        for (int i = tid; i < c; i += kThreads) sh.mass[i] = s.row.mass((unsigned)(sh.list[i] >> kIndexBits));
+        u64* rest = reinterpret_cast<u64*>(sh.hist);  // mass before each word (the histograms are done with)
+        static_assert(sizeof(sh.hist) >= kList * sizeof(u64), "room");
+        for (int i = tid; i < c; i += kThreads) sh.mass[i] = s.row.mass(word_value(sh.list[i]));
         __syncthreads();
         for (int i = tid; i < c; i += kThreads) {
           const u64 w = sh.list[i];
           int pos = 0;
           u64 m = 0;
+#pragma unroll 4
           for (int j = 0; j < c; ++j)
             if (sh.list[j] > w) {
               ++pos;
@@ -400,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_sample_kernel(const SampleAr
         u64 kept = 0;
         for (int i = tid; i < c; i += kThreads) {
           const bool keep = rest[i] != ~0ull && (rest[i] == 0 || ((double)rest[i] < lim &&
-                            (!(least > 0.0) || s.row.weight((unsigned)(sh.list[i] >> kIndexBits)) >= least)));
+                            (!(least > 0.0) || s.row.weight(word_value(sh.list[i])) >= least)));
           if (!keep) sh.mass[i] = 0;
           kept += sh.mass[i];
         }
@@ -410,64 +457,52 @@ __global__ void __launch_bounds__(kThreads, 2) rows_sample_kernel(const SampleAr
         if (target >= total) target = total - 1;
         for (int i = tid; i < c; i += kThreads) {
           if (sh.mass[i] == 0) continue;
-          const u64 index = sh.list[i] & ((1u << kIndexBits) - 1);  // larger = lower index
+          const int index = word_index(sh.list[i]);
           u64 cum = 0;
+#pragma unroll 4
           for (int j = 0; j < c; ++j)
-            if ((sh.list[j] & ((1u << kIndexBits) - 1)) >= index) cum += sh.mass[j];
-          if (cum > target && cum - sh.mass[i] <= target) a.tokens[r] = (1 << kIndexBits) - 1 - (int)index;
+            if (word_index(sh.list[j]) <= index) cum += sh.mass[j];
+          if (cum > target && cum - sh.mass[i] <= target) a.tokens[r] = index;
         }
         return;
       }
-      // they do not fit: order the border's bin alone, over a new histogram
-      h = s.clear(kBins);
-      for (int i = tid; i < n; i += kThreads) {
-        const int q = s.row.bin(s_keys[i]);
-        if (q < kBins - 1) atomicAdd(h + q, 1ull);
-      }
+      counts();  // they do not fit: put the border's bin alone in order
     }
-    from = s.border_in(0ull, (u64)k, &total, false);
+    s.template border<false>((u64)k);
   }
   if (tp < 1.0f) {
-    // the mass of the words kept so far comes with the histogram, so it is found first with no border
-    u64* h = s.clear(kBins);
+    s.template clear<true>();
+#pragma unroll 2
     for (int i = tid; i < n; i += kThreads) {
-      const unsigned key = s_keys[i];
-      const int b = s.row.bin(key);
-      if (b < kBins - 1 && order_word(key, first + i) >= from) atomicAdd(h + b, Row::fixed(s.row.weight(key)));
+      const float v = s_val[i];
+      const int b = s.row.bin(v);
+      if (b < kBins - 1 && s.keep(v, i)) s.template add<true>(b, v);
     }
-    u64 part = 0;
-    __syncthreads();
-    for (int i = tid; i < kBins; i += kThreads) part += h[i];
-    block_scan(part, sh, &part);
-    if (tid == 0) sh.sum = part;
-    cluster.sync();
-    total = 0;
-    for (int q = 0; q < ranks; ++q) total += cluster.map_shared_rank(&sh, q)->sum;
+    total = s.template publish<true>();
     const double lim = fmax((double)tp * (double)total, 0.0);
-    const u64 want = max(1ull, (u64)ceil(lim));  // the first word whose predecessors and itself reach it is the last
-    const u64 c = s.border_in(from, want, &total, true);
-    from = c > from ? c : from;
+    s.template border<true>(max(1ull, (u64)ceil(lim)));  // the word that brings the sum to top_p is the last
   }
 
-  // mass of the kept words, in index order: a contiguous share per thread (an odd number of words, so
-  // that the shares begin in different banks)
+  // Mass of the kept words, in index order: a contiguous share per thread (an odd number of words, so
+  // that the shares begin in different banks).
   const int share = ((n + kThreads - 1) / kThreads) | 1, i0 = min(n, tid * share), i1 = min(n, i0 + share);
   auto kept = [&](int i) -> u64 {
-    const unsigned key = s_keys[i];
-    if (s.row.bin(key) == kBins - 1 || order_word(key, first + i) < from) return 0ull;
-    const double w = s.row.weight(key);
-    return key == top || !(least > 0.0) || w >= least ? Row::fixed(w) : 0ull;
+    const float v = s_val[i];
+    if (!s.keep(v, i) || s.row.bin(v) == kBins - 1) return 0ull;
+    const double w = s.row.weight(v);
+    return v == vtop || !(least > 0.0) || w >= least ? Row::fixed(w) : 0ull;
   };
   u64 mine = 0;
+#pragma unroll 2
   for (int i = i0; i < i1; ++i) mine += kept(i);
   u64 cta;
   const u64 upto = block_scan(mine, sh, &cta);
-  if (tid == 0) sh.best = cta;
+  if (tid == 0) sh.sum = cta;
   cluster.sync();
   u64 before = 0;
   total = 0;
   for (int q = 0; q < ranks; ++q) {
-    const u64 t = cluster.map_shared_rank(&sh, q)->best;
+    const u64 t = cluster.map_shared_rank(&sh, q)->sum;
     if (q < rank) before += t;
     total += t;
   }
