@@ -517,11 +517,10 @@ cudaError_t launch_typed(const PagedArgs& a, const KvArgs& kv, cudaStream_t stre
   const int box_rows = kv.page_size < kTile ? kv.page_size : kTile;
   if (!encode_kv_map(&kmap, kv, kv.k, box_rows) || !encode_kv_map(&vmap, kv, kv.v, box_rows))
     return cudaErrorInvalidValue;
-  int dev = 0, sms = 0;
-  cudaGetDevice(&dev);
-  cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  static std::atomic<unsigned long long> done{0};
+  int sms = 0;
+  cudaError_t e = kernel_setup(reinterpret_cast<const void*>(kernel), L::kSmem, done, &sms);
   if (e != cudaSuccess) return e;
-  if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem)) != cudaSuccess) return e;
   const int g = a.n_heads / kv.n_kv, zs = (g + 15) / 16;
   const int ctas = 2 * sms < kMaxCtas ? 2 * sms : kMaxCtas;
   cudaLaunchConfig_t cfg = {};

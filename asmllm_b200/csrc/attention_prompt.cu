@@ -609,11 +609,10 @@ cudaError_t launch_typed(const PromptArgs& a, const KvArgs& kv, cudaStream_t str
                  (uint64_t)a.q_head_stride, (uint64_t)a.q_row_stride, kRows) ||
       !encode_kv_map(&kmap, kv, kv.k, box_rows) || !encode_kv_map(&vmap, kv, kv.v, box_rows))
     return cudaErrorInvalidValue;
-  int dev = 0, sms = 0;
-  cudaGetDevice(&dev);
-  cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  static std::atomic<unsigned long long> done{0};
+  int sms = 0;
+  cudaError_t e = kernel_setup(reinterpret_cast<const void*>(kernel), C::kSmem, done, &sms);
   if (e != cudaSuccess) return e;
-  if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem)) != cudaSuccess) return e;
   const int pair = (a.n_heads / kv.n_kv) % 2 == 0, R = pair ? kRows : 2 * kRows;
   const long long items = ((long long)a.rows / R + kv.batch) * (pair ? a.n_heads / 2 : a.n_heads);
   cudaLaunchConfig_t cfg = {};

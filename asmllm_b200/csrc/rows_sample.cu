@@ -529,8 +529,10 @@ cudaError_t launch_typed(const SampleArgs& a, cudaStream_t stream) {
   const int ranks = a.n <= 4096 ? 1 : a.n <= 8192 ? 2 : a.n <= 16384 ? 4 : 8;
   const int per = ((a.n + ranks - 1) / ranks + 7) & ~7;
   const size_t smem = sizeof(Shared) + (size_t)per * sizeof(unsigned);
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)sizeof(Shared) + kSampleMaxN / 8 * (int)sizeof(unsigned));
+  static std::atomic<unsigned long long> done{0};
+  int sms = 0;
+  cudaError_t e = kernel_setup(reinterpret_cast<const void*>(kernel),
+                               (int)(sizeof(Shared) + kSampleMaxN / 8 * sizeof(unsigned)), done, &sms);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.rows * (unsigned)ranks);

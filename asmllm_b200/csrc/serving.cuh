@@ -9,6 +9,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace asmllm {
@@ -86,6 +88,25 @@ cudaError_t launch_attention_prompt(const PromptArgs& a, const KvArgs& kv, cudaS
 size_t attention_paged_workspace(int batch, int n_heads, int n_kv, int head_dim);
 cudaError_t launch_attention_paged(const PagedArgs& a, const KvArgs& kv, cudaStream_t stream);
 cudaError_t launch_rows_sample(const SampleArgs& a, cudaStream_t stream);
+
+// The current device's SM count, and a kernel's shared-memory limit raised
+// once per device (`done`: one flag a device, of this kernel alone).
+inline cudaError_t kernel_setup(const void* kernel, int smem, std::atomic<unsigned long long>& done, int* sms) {
+  static std::atomic<int> count[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!(done.load() >> dev & 1ull)) {
+    int n = 0;
+    if ((e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
+    if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
+    count[dev].store(n);
+    done.fetch_or(1ull << dev);
+  }
+  *sms = count[dev].load();
+  return cudaSuccess;
+}
 
 #ifdef __CUDACC__
 

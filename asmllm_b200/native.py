@@ -112,10 +112,10 @@ SIGNATURES = {
     "asm_attention_batch_async": ([vp, i64, vp, vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, f32, vp], c_int),
     "asm_rows_argmax_async": ([vp, i32, i32, i64, i32, vp, vp], c_int),
     "asm_rows_advance_async": ([vp, i32, vp, i32, vp, i32, vp], c_int),
-    "asm_rope_append_async": ([vp, i32, i64, vp, i32, vp, i32, i32, vp, ctypes.POINTER(Kv), vp], c_int),
-    "asm_attention_prompt_async": ([vp, i64, i64, vp, i32, i32, f32, vp, i32, ctypes.POINTER(Kv), vp], c_int),
+    "asm_rope_append_async": ([vp, i32, i64, vp, i32, vp, i32, i32, vp, vp, vp], c_int),
+    "asm_attention_prompt_async": ([vp, i64, i64, vp, i32, i32, f32, vp, i32, vp, vp], c_int),
     "asm_attention_paged_workspace": ([i32, i32, i32, i32], i64),
-    "asm_attention_paged_async": ([vp, i64, i64, i32, f32, vp, i32, ctypes.POINTER(Kv), vp, i64, vp], c_int),
+    "asm_attention_paged_async": ([vp, i64, i64, i32, f32, vp, i32, vp, vp, i64, vp], c_int),
     "asm_rows_sample_async": ([vp, i32, i32, i32, i64, vp, vp, vp, vp, vp, vp, vp], c_int),
     # additions
     "asm_matmul_q8q8": ([vp, vp, vp, vp, i64, i64], None),

@@ -16,6 +16,7 @@ Argument meanings follow the reference: qweights Q4_0 uint8 [M, K/32, 16]
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import numpy as np
 
@@ -551,12 +552,30 @@ def key_index(keys):
 
 # --------------------------------------------------------------------------
 # Serving operators: prompts of different lengths, a paged cache, sampling
+#
+# A decode step makes hundreds of these calls and the kernels take a few
+# microseconds, so the checks are written for the case that passes: one
+# expression over what the tensors say, and the long way (which names the
+# fault) only where it fails.
 # --------------------------------------------------------------------------
 
+_DT: dict = {}   # torch dtype -> ASM_DT_*
+_H16: dict = {}  # the 16-bit ones alone
+_KV_PACK = struct.Struct("QQqqqQqQQiiiiiiii").pack  # asm_kv_t (native.Kv), field for field
 
-def _dt(dtype):
+
+def _dtypes():
     torch = _torch()
-    return {torch.float32: native.DT_F32, torch.float16: native.DT_F16, torch.bfloat16: native.DT_BF16}[dtype]
+    _H16.update({torch.float16: native.DT_F16, torch.bfloat16: native.DT_BF16})
+    _DT.update({torch.float32: native.DT_F32, **_H16})
+    return _DT
+
+
+def _raw_stream(device: int, stream) -> int:
+    """cudaStream_t of `stream`, or of torch's current stream on the device."""
+    if stream is not None:
+        return stream.cuda_stream
+    return _torch()._C._cuda_getCurrentRawStream(device)
 
 
 def _empty(shape, dtype, device, stream):
@@ -566,6 +585,11 @@ def _empty(shape, dtype, device, stream):
         return torch.empty(shape, dtype=dtype, device=device)
     with torch.cuda.stream(stream):
         return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _call(rc: int) -> None:
+    if rc:
+        native.check(rc)
 
 
 def _dense(t, name, ndim, dtypes):
@@ -580,56 +604,80 @@ def _dense(t, name, ndim, dtypes):
                          f"with strides {t.stride()}")
 
 
-def _step(t, axis, default):
-    """Stride of an axis; `default` where it has one entry and the stride means nothing."""
-    return t.stride(axis) if t.shape[axis] > 1 else default
+def _strides(t):
+    """Strides, those of axes with a single entry replaced by the dense ones (they mean nothing)."""
+    st = t.stride()
+    if 1 in t.shape:
+        st, dense = list(st), 1
+        for i in range(len(st) - 1, -1, -1):
+            if t.shape[i] == 1:
+                st[i] = dense
+            dense = max(dense, st[i] * t.shape[i])
+        st = tuple(st)
+    return st
 
 
-def _kv_view(k, v, kv_len=None, page_table=None, cu_k=None):
-    """native.Kv of paged k, v [pages, page_size, heads, head_dim] or packed k, v [rows, heads, head_dim]."""
+def _vector(t, name, n, device):
+    """int32 [n], contiguous, on the device."""
     torch = _torch()
-    nd = 4 if page_table is not None else 3
-    for t, name in ((k, "k"), (v, "v")):
-        _dense(t, name, nd, (torch.float16, torch.bfloat16))
-    if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or any(
-            a != b and n > 1 for a, b, n in zip(k.stride(), v.stride(), k.shape)):
-        raise ValueError(f"k and v must agree in shape, strides, type and device: {tuple(k.shape)} {k.stride()} "
-                         f"{k.dtype}, {tuple(v.shape)} {v.stride()} {v.dtype}")
-    d = native.Kv()
-    d.k, d.v = k.data_ptr(), v.data_ptr()
-    hd = k.shape[-1]
-    d.head_dim, d.n_kv_heads, d.dtype = hd, k.shape[-2], _dt(k.dtype)
-    d.head_stride = _step(k, -2, hd)
-    d.token_stride = _step(k, -3, hd)
-    if page_table is not None:
-        _dense(page_table, "page_table", 2, (torch.int32,))
-        _check_dev(kv_len, (torch.int32,), "kv_len")
-        if kv_len.numel() != page_table.shape[0]:
-            raise ValueError(f"kv_len has {kv_len.numel()} entries, page_table {page_table.shape[0]} rows")
-        d.batch, d.table_width = page_table.shape
-        d.table, d.table_stride = page_table.data_ptr(), _step(page_table, 0, page_table.shape[1])
-        d.len = kv_len.data_ptr()
-        d.n_pages, d.page_size = k.shape[0], k.shape[1]
-        d.page_stride = _step(k, 0, hd)
-    else:
-        _check_dev(cu_k, (torch.int32,), "cu_k")
-        d.batch = cu_k.numel() - 1
-        d.cu = cu_k.data_ptr()
-        d.n_pages, d.page_size, d.page_stride = 1, k.shape[0], hd
-    return d
+    _check_dev(t, (torch.int32,), name)
+    if t.shape != (n,):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({n},)")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on another device")
 
 
-def _out_for(q, out, out_dtype, stream):
-    torch = _torch()
+def _kv_view(k, v, device, kv_len=None, page_table=None, cu_k=None):
+    """asm_kv_t of paged k, v [pages, page_size, heads, head_dim] or packed k, v [rows, heads, head_dim]."""
+    if not _DT:
+        _dtypes()
+    paged = page_table is not None
+    shape, st = k.shape, _strides(k)
+    if (k.dtype not in _H16 or v.dtype != k.dtype or shape != v.shape or st != _strides(v) or st[-1] != 1
+            or len(st) != (4 if paged else 3) or not k.get_device() == v.get_device() == device >= 0):
+        for t, name in ((k, "k"), (v, "v")):
+            _dense(t, name, 4 if paged else 3, _H16)
+        if shape != v.shape or k.dtype != v.dtype or st != _strides(v):
+            raise ValueError(f"k and v must agree in shape, strides and type: {tuple(k.shape)} {k.stride()} {k.dtype}, "
+                             f"{tuple(v.shape)} {v.stride()} {v.dtype}")
+        raise ValueError("k, v and the rows are on different devices")
+    if paged:
+        batch, width = page_table.shape
+        if (page_table.dtype != _torch().int32 or page_table.get_device() != device
+                or (width > 1 and page_table.stride(1) != 1)):
+            _dense(page_table, "page_table", 2, (_torch().int32,))
+            raise ValueError("page_table is on another device")
+        _vector(kv_len, "kv_len", batch, device)
+        return (_KV_PACK(k.data_ptr(), v.data_ptr(), st[0], st[1], st[2], page_table.data_ptr(),
+                         page_table.stride(0) if batch > 1 else width, kv_len.data_ptr(), 0, batch, shape[0], shape[1],
+                         width, shape[2], shape[3], _H16[k.dtype], 0), batch)
+    batch = cu_k.shape[0] - 1
+    _vector(cu_k, "cu_k", batch + 1, device)
+    return (_KV_PACK(k.data_ptr(), v.data_ptr(), max(st[0], 8), st[0], st[1], 0, 0, 0, cu_k.data_ptr(), batch, 1,
+                     shape[0], 0, shape[1], shape[2], _H16[k.dtype], 0), batch)
+
+
+def _query(q, k, out, out_dtype, stream):
+    """Checks q [rows, heads, head_dim] against k and returns (strides, out)."""
+    if not _DT:
+        _dtypes()
+    shape, st = q.shape, _strides(q)
+    if q.dtype not in _H16 or not q.is_cuda or len(shape) != 3 or st[2] != 1:
+        _dense(q, "q", 3, _H16)
+    heads = k.shape[-2]
+    if q.dtype != k.dtype or shape[2] != k.shape[-1]:
+        raise ValueError(f"q {q.dtype} of head_dim {shape[2]} against keys {k.dtype} of {k.shape[-1]}")
+    if heads == 0 or shape[1] == 0 or shape[1] % heads:
+        raise ValueError(f"{shape[1]} query heads are not a multiple of {heads} KV heads")
     if out is None:
         dt = out_dtype or q.dtype
-        if dt not in (q.dtype, torch.float32):
+        if dt != q.dtype and dt != _torch().float32:
             raise TypeError(f"out_dtype {dt}: fp32 or q's type")
-        return _empty(tuple(q.shape), dt, q.device, stream)
-    _check_dev(out, (q.dtype, torch.float32), "out")
-    if out.shape != q.shape or (out_dtype is not None and out.dtype != out_dtype):
-        raise ValueError(f"out: {tuple(out.shape)} {out.dtype}, expected {tuple(q.shape)} {out_dtype or q.dtype}")
-    return out
+        return st, _empty(shape, dt, q.device, stream)
+    _check_dev(out, (q.dtype, _torch().float32), "out")
+    if out.shape != shape or (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError(f"out: {tuple(out.shape)} {out.dtype}, expected {tuple(shape)} {out_dtype or q.dtype}")
+    return st, out
 
 
 def rope_append(qkv, rope_cs, kv_len, page_table, k_pages, v_pages, n_heads: int, *, cu_q=None, q_out=None,
@@ -643,30 +691,36 @@ def rope_append(qkv, rope_cs, kv_len, page_table, k_pages, v_pages, n_heads: int
     [positions, hd/2, 2] (decode.rope_table).  Returns the rotated queries [T, nh, hd] in the cache's
     type; rows at or past cu_q[B] are not written."""
     torch = _torch()
-    _dense(k_pages, "k_pages", 4, (torch.float16, torch.bfloat16))
-    _dense(qkv, "qkv", 2, (torch.float32, k_pages.dtype))
+    if page_table is None:
+        raise ValueError("page_table is required")
+    device = qkv.get_device() if isinstance(qkv, torch.Tensor) else -1
+    if device < 0:
+        raise TypeError("qkv: expected a CUDA tensor")
+    kv, batch = _kv_view(k_pages, v_pages, device, kv_len, page_table)
+    dt = k_pages.dtype
+    nkv, hd = k_pages.shape[2:]
+    if qkv.dtype not in (torch.float32, dt) or qkv.dim() != 2 or qkv.stride(1) != 1:
+        _dense(qkv, "qkv", 2, (torch.float32, dt))
+    T = qkv.shape[0]
+    if qkv.shape[1] != (n_heads + 2 * nkv) * hd:
+        raise ValueError(f"qkv has {qkv.shape[1]} columns, expected ({n_heads} + 2 * {nkv}) * {hd}")
     _check_dev(rope_cs, (torch.float32,), "rope_cs")
-    kv = _kv_view(k_pages, v_pages, kv_len, page_table)
-    T, hd = qkv.shape[0], kv.head_dim
-    if qkv.shape[1] != (n_heads + 2 * kv.n_kv_heads) * hd:
-        raise ValueError(f"qkv has {qkv.shape[1]} columns, expected ({n_heads} + 2 * {kv.n_kv_heads}) * {hd}")
     if rope_cs.shape[1:] != (hd // 2, 2):
         raise ValueError(f"rope_cs {tuple(rope_cs.shape)}: expected [positions, {hd // 2}, 2]")
     if cu_q is not None:
-        _check_dev(cu_q, (torch.int32,), "cu_q")
-        if cu_q.numel() != kv.batch + 1:
-            raise ValueError(f"cu_q has {cu_q.numel()} entries, expected {kv.batch + 1}")
-    elif T != kv.batch:
-        raise ValueError(f"{T} rows for {kv.batch} sequences: pass cu_q")
+        _vector(cu_q, "cu_q", batch + 1, device)
+    elif T != batch:
+        raise ValueError(f"{T} rows for {batch} sequences: pass cu_q")
     if q_out is None:
-        q_out = _empty((T, n_heads, hd), k_pages.dtype, qkv.device, stream)
+        q_out = _empty((T, n_heads, hd), dt, qkv.device, stream)
     else:
-        _check_dev(q_out, (k_pages.dtype,), "q_out")
+        _check_dev(q_out, (dt,), "q_out")
         if q_out.shape != (T, n_heads, hd):
             raise ValueError(f"q_out {tuple(q_out.shape)}: expected {(T, n_heads, hd)}")
-    native.check(native.lib().asm_rope_append_async(
-        _ptr(qkv), _dt(qkv.dtype), _step(qkv, 0, qkv.shape[1]), _ptr(rope_cs), rope_cs.shape[0],
-        None if cu_q is None else _ptr(cu_q), T, n_heads, _ptr(q_out), ctypes.byref(kv), _stream_handle(stream)))
+    _call((native._lib or native.lib()).asm_rope_append_async(
+        qkv.data_ptr(), _DT[qkv.dtype], qkv.stride(0) if T > 1 else qkv.shape[1], rope_cs.data_ptr(),
+        rope_cs.shape[0], None if cu_q is None else cu_q.data_ptr(), T, n_heads, q_out.data_ptr(), kv,
+        _raw_stream(device, stream)))
     return q_out
 
 
@@ -678,29 +732,19 @@ def attention_prompt(q, k, v, cu_q, *, cu_k=None, kv_len=None, page_table=None, 
     [Tk, nkv, hd] with offsets cu_k (cu_q where they are the prompt's own), or the pages of a cache
     [pages, page_size, nkv, hd] with page_table int32 [B, n] and kv_len int32 [B].  The last row of a
     sequence sees all its keys; earlier rows one less each; a row without keys gives zeros.  scale
-    defaults to hd ** -0.5.  out [T, nh, hd] in q's type or fp32; rows at or past cu_q[B] are not written."""
-    torch = _torch()
-    _dense(q, "q", 3, (torch.float16, torch.bfloat16))
-    _check_dev(cu_q, (torch.int32,), "cu_q")
+    (positive) defaults to hd ** -0.5.  out [T, nh, hd] in q's type or fp32; rows at or past cu_q[B] are
+    not written."""
     if (page_table is None) != (kv_len is None) or (page_table is not None and cu_k is not None):
         raise ValueError("pass page_table and kv_len (paged) or cu_k (packed)")
-    kv = _kv_view(k, v, kv_len, page_table, cu_q if cu_k is None else cu_k)
-    if cu_q.numel() != kv.batch + 1:
-        raise ValueError(f"cu_q has {cu_q.numel()} entries for {kv.batch} sequences")
-    _same_heads(q, k)
-    out = _out_for(q, out, out_dtype, stream)
-    native.check(native.lib().asm_attention_prompt_async(
-        _ptr(q), _step(q, 0, q.shape[1] * q.shape[2]), _step(q, 1, q.shape[2]), _ptr(cu_q), q.shape[0], q.shape[1],
-        q.shape[2] ** -0.5 if scale is None else scale, _ptr(out), _dt(out.dtype), ctypes.byref(kv),
-        _stream_handle(stream)))
+    device = q.get_device()
+    kv, batch = _kv_view(k, v, device, kv_len, page_table, cu_q if cu_k is None else cu_k)
+    _vector(cu_q, "cu_q", batch + 1, device)
+    st, out = _query(q, k, out, out_dtype, stream)
+    T, nh, hd = q.shape
+    _call((native._lib or native.lib()).asm_attention_prompt_async(
+        q.data_ptr(), st[0], st[1], cu_q.data_ptr(), T, nh, hd ** -0.5 if scale is None else scale, out.data_ptr(),
+        _DT[out.dtype], kv, _raw_stream(device, stream)))
     return out
-
-
-def _same_heads(q, k):
-    if q.dtype != k.dtype or q.shape[-1] != k.shape[-1] or q.device != k.device:
-        raise ValueError(f"q {q.dtype} of head_dim {q.shape[-1]} against keys {k.dtype} of {k.shape[-1]}")
-    if k.shape[-2] == 0 or q.shape[-2] == 0 or q.shape[-2] % k.shape[-2]:
-        raise ValueError(f"{q.shape[-2]} query heads are not a multiple of {k.shape[-2]} KV heads")
 
 
 def attention_paged_workspace(batch: int, n_heads: int, n_kv_heads: int, head_dim: int) -> int:
@@ -715,26 +759,26 @@ def attention_paged(q, k_pages, v_pages, page_table, kv_len, *, scale: float | N
                     workspace=None, stream=None):
     """Attention of one new token per sequence, q [B, nh, hd] fp16 or bf16, over a paged cache
     (asm_attention_paged_async): k_pages, v_pages [pages, page_size, nkv, hd], page_table int32 [B, n],
-    kv_len int32 [B] (the new token counted).  kv_len 0 gives zeros.  out [B, nh, hd] in q's type or fp32.
-    workspace: uint8 of attention_paged_workspace bytes, one per call that may overlap another (a call
-    without one takes it from torch's allocator)."""
-    torch = _torch()
-    _dense(q, "q", 3, (torch.float16, torch.bfloat16))
+    kv_len int32 [B] (the new token counted).  kv_len 0 gives zeros.  scale (positive) defaults to
+    hd ** -0.5.  out [B, nh, hd] in q's type or fp32.  workspace: uint8 of attention_paged_workspace bytes,
+    one per call that may overlap another (a call without one takes it from torch's allocator)."""
     if page_table is None:
         raise ValueError("page_table is required")
-    kv = _kv_view(k_pages, v_pages, kv_len, page_table)
-    _same_heads(q, k_pages)
+    device = q.get_device()
+    kv, batch = _kv_view(k_pages, v_pages, device, kv_len, page_table)
+    st, out = _query(q, k_pages, out, out_dtype, stream)
     B, nh, hd = q.shape
-    if B != kv.batch:
-        raise ValueError(f"q has {B} rows for {kv.batch} sequences")
-    out = _out_for(q, out, out_dtype, stream)
+    if B != batch:
+        raise ValueError(f"q has {B} rows for {batch} sequences")
+    lib = native._lib or native.lib()
     if workspace is None:
-        workspace = _empty(attention_paged_workspace(B, nh, kv.n_kv_heads, hd), torch.uint8, q.device, stream)
+        workspace = _empty(lib.asm_attention_paged_workspace(B, nh, k_pages.shape[2], hd), _torch().uint8, q.device,
+                           stream)
     else:
-        _check_dev(workspace, (torch.uint8,), "workspace")
-    native.check(native.lib().asm_attention_paged_async(
-        _ptr(q), _step(q, 0, nh * hd), _step(q, 1, hd), nh, hd ** -0.5 if scale is None else scale, _ptr(out),
-        _dt(out.dtype), ctypes.byref(kv), _ptr(workspace), workspace.numel(), _stream_handle(stream)))
+        _check_dev(workspace, (_torch().uint8,), "workspace")
+    _call(lib.asm_attention_paged_async(
+        q.data_ptr(), st[0], st[1], nh, hd ** -0.5 if scale is None else scale, out.data_ptr(), _DT[out.dtype], kv,
+        workspace.data_ptr(), workspace.numel(), _raw_stream(device, stream)))
     return out
 
 
@@ -747,19 +791,26 @@ def rows_sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=No
     word is the first, in index order, whose cumulative probability exceeds u.  temperature 0: the first
     maximum.  NaN is never chosen; a row of NaN and -inf gives -1.  Returns int32 [B]."""
     torch = _torch()
-    _dense(logits, "logits", 2, (torch.float32, torch.float16, torch.bfloat16))
-    B, V = logits.shape
-    for t, name, dt in ((u, "u", torch.float32), (temperature, "temperature", torch.float32),
-                        (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
-                        (min_p, "min_p", torch.float32), (tokens, "tokens", torch.int32)):
-        if t is None and name != "u":
-            continue
-        _check_dev(t, (dt,), name)
-        if t.shape != (B,):
-            raise ValueError(f"{name}: shape {tuple(t.shape)}, expected ({B},)")
+    if not _DT:
+        _dtypes()
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in _DT or not logits.is_cuda or logits.dim() != 2 or (
+            logits.stride(1) != 1):
+        _dense(logits, "logits", 2, _DT)
+    B, V = shape = logits.shape
+    device = logits.get_device()
     if tokens is None:
-        tokens = _empty((B,), torch.int32, logits.device, stream)
-    opt = [None if t is None else _ptr(t) for t in (temperature, top_k, top_p, min_p)]
-    native.check(native.lib().asm_rows_sample_async(_ptr(logits), _dt(logits.dtype), B, V, _step(logits, 0, V), _ptr(u),
-                                                    *opt, _ptr(tokens), _stream_handle(stream)))
+        tokens = _empty(shape[:1], torch.int32, logits.device, stream)
+    f32, i32, ptr = torch.float32, torch.int32, []
+    for t, name, dt in ((u, "u", f32), (temperature, "temperature", f32), (top_k, "top_k", i32), (top_p, "top_p", f32),
+                        (min_p, "min_p", f32), (tokens, "tokens", i32)):
+        if t is None and name != "u":
+            ptr.append(None)
+            continue
+        if not isinstance(t, torch.Tensor) or t.dtype != dt or t.get_device() != device or t.shape != shape[:1] or (
+                B > 1 and t.stride(0) != 1):
+            _check_dev(t, (dt,), name)
+            raise ValueError(f"{name}: shape {tuple(t.shape)} on device {t.get_device()}, expected ({B},) on {device}")
+        ptr.append(t.data_ptr())
+    _call((native._lib or native.lib()).asm_rows_sample_async(logits.data_ptr(), _DT[logits.dtype], B, V,
+                                             logits.stride(0) if B > 1 else V, *ptr, _raw_stream(device, stream)))
     return tokens
