@@ -375,7 +375,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       Item it;
       bool ok = true, issued = false;
       auto mma_s = [&](int i, int st) {  // S_i = Q_i K^T
-        if (lane == 0) {
+        if (elect_one()) {
           const uint64_t qd = desc_k_major(q_addr + i * C::kTile), kd = desc_k_major(ring + st * C::kTile);
 #pragma unroll
           for (int ks = 0; ks < HD / 16; ++ks) {
@@ -387,7 +387,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         issued = true;
       };
       auto commit = [&](uint64_t* bar) {
-        if (lane == 0) umma_commit(smem_u32(bar));
+        if (elect_one()) umma_commit(smem_u32(bar));
       };
       for (int k = 0; ok && take_item(k, &it); ++k) {
         const int nm = max(it.tiles[0], it.tiles[1]);
@@ -422,7 +422,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                 ++no[i];
               }
               tc_fence_after();
-              if (lane == 0) {
+              if (elect_one()) {
                 const uint64_t vd = desc_mn_major(ring + sv * C::kTile);
 #pragma unroll
                 for (int ks = 0; ks < kRows / 16; ++ks)
