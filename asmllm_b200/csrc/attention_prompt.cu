@@ -21,9 +21,11 @@
 //
 // CTA (one per SM, persistent), 12 warps:
 //   0-3, 4-7  softmax, rescale and output of query tile 0 and 1
-//   8         tcgen05.mma issue; zeroes the values behind a sequence's end
+//   8         tcgen05.mma issue, by one elected thread (behind lane == 0 each
+//             product went through a loop over lanes: 400 cycles instead of 100)
 //   9         tensor copies: Q (2 tiles), then K and V tiles into one ring
 //   10        scheduler: the work items in order of falling key count
+//   11        zeroes the values behind a sequence's end
 // Every wait is bounded: a role that gives up sets the device error word and
 // an abort flag, all roles leave, and tensor memory is released.
 #include <type_traits>
@@ -104,22 +106,25 @@ struct Cfg {
   static constexpr int kStages = HD == 128 ? 5 : 8;
   static constexpr int kRing = 2 * kTile;
   static constexpr int kBars = kRing + kStages * kTile;
-  static constexpr int kNBars = 2 * kStages + 2 + 8 + 4 + 1;
+  static constexpr int kNBars = 2 * kStages + 2 + 8 + 4 + 3;
   static constexpr int kItems = kBars + kNBars * 8 + 16;
   static constexpr int kSmem = kItems + 2 * (int)sizeof(Item) + 16 + 1024;
   static constexpr uint32_t kO = 2 * kRows;  // tensor memory: S0, S1, then the two outputs
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
-// Operand descriptors, 128-byte swizzle.  Q and K: rows of 128 bytes (64
+// Operand descriptors, 128-byte swizzle: the low word is the address and the
+// leading offset, the high word the rest.  Q and K: rows of 128 bytes (64
 // values along the product's K), eight rows 1024 bytes apart.  V: the product
-// runs over its rows; 64 values are contiguous, the next 64 a half tile away.
-__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((kRows * 128) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         (1ull << 46) | (2ull << 61);
+// runs over its rows, eight of them 1024 bytes apart; 64 values are
+// contiguous, the next 64 a half tile away (the leading offset).
+constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
+constexpr uint32_t kLeading = ((kRows * 128) >> 4) << 16;
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr) { return ((addr >> 4) & 0x3FFFu) | kLeading; }
+__device__ __forceinline__ uint64_t desc64(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
 }
 
 // Tiles of sequence (base, q rows, R rows a tile) with at least w key tiles.
@@ -155,7 +160,9 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
   uint64_t* o_empty = o_full + 2;   // [2] and has been read
   uint64_t* i_full = o_empty + 2;   // [2] work items
   uint64_t* i_empty = i_full + 2;
-  uint64_t* drain = i_empty + 2;
+  uint64_t* v_clean = i_empty + 2;  // an item's last value tile is zero behind the sequence's end
+  uint64_t* v_dirty = v_clean + 1;  // the tile that needs it has landed
+  uint64_t* drain = v_dirty + 1;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drain + 1);
   volatile uint32_t* s_abort = s_tmem + 1;
   Item* items = reinterpret_cast<Item*>(smem + C::kItems);
@@ -179,8 +186,10 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       mbar_init(smem_u32(o_full + i), 1);
       mbar_init(smem_u32(o_empty + i), 4);
       mbar_init(smem_u32(i_full + i), 1);
-      mbar_init(smem_u32(i_empty + i), 10);  // 8 softmax warps, the issuer, the loader
+      mbar_init(smem_u32(i_empty + i), 11);  // 8 softmax warps, the issuer, the loader, the cleaner
     }
+    mbar_init(smem_u32(v_clean), 1);
+    mbar_init(smem_u32(v_dirty), 1);
     mbar_init(smem_u32(drain), 1);
     *s_abort = 0u;
     fence_mbar_init();
@@ -368,88 +377,110 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       // what was issued lands before the CTA may end (bounded)
       if (nq > 0) mbar_wait_bounded(smem_u32(q_full), (nq - 1) & 1);
       for (int j = c - S < 0 ? 0 : c - S; j < c; ++j) mbar_wait_bounded(smem_u32(kv_full + j % S), (j / S) & 1);
-    } else if (warp == 8) {
-      // ---------------- matrix products ----------------
-      int c = 0, nq = 0, np[2] = {0, 0}, no[2] = {0, 0};
-      const uint32_t q_addr = smem_u32(smem), ring = q_addr + C::kRing;
+    } else if (warp == 11) {
+      // ---------------- cleaner: zeroes the values behind a sequence's end ----------------
+      // (zero weights meet zeros there, whatever the page or the next sequence holds)
+      int c = 0, nd = 0;
       Item it;
+      for (int k = 0; take_item(k, &it); ++k) {
+        const int nm = max(it.tiles[0], it.tiles[1]), valid = it.n - (nm - 1) * kRows;
+        c += 2 * nm;
+        if (nm == 0 || valid >= kRows) continue;
+        const int sv = (c - 1) % S;  // the item's last value tile
+        if (!wait(v_dirty, nd & 1)) break;  // the issuer has seen the tile land
+        ++nd;
+        for (int h = 0; h < kHalves; ++h)
+          for (int b = valid * 128 + lane * 16; b < kRows * 128; b += 512)
+            *reinterpret_cast<uint4*>(smem + C::kRing + sv * C::kTile + h * (kRows * 128) + b) =
+                make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(v_clean));
+      }
+    } else if (elect_one()) {
+      // ---------------- matrix products (one thread) ----------------
+      const uint32_t q_lo = desc_lo(smem_u32(smem)), ring_lo = desc_lo(smem_u32(smem) + C::kRing);
+      constexpr uint32_t kTileLo = C::kTile >> 4;
+      int st = 0, nq = 0, np[2] = {0, 0}, no[2] = {0, 0}, nc = 0;
+      uint32_t ph = 0;  // ring stage and its parity
       bool ok = true, issued = false;
-      auto mma_s = [&](int i, int st) {  // S_i = Q_i K^T
-        if (elect_one()) {
-          const uint64_t qd = desc_k_major(q_addr + i * C::kTile), kd = desc_k_major(ring + st * C::kTile);
-#pragma unroll
-          for (int ks = 0; ks < HD / 16; ++ks) {
-            const uint64_t step = (ks >> 2) * ((kRows * 128) >> 4) + (ks & 3) * 2;
-            umma_ss(tmem + i * kRows, qd + step, kd + step, kIdescS, ks > 0);
-          }
-          umma_commit(smem_u32(s_full + i));
+      auto step = [&]() {
+        if (++st == S) {
+          st = 0;
+          ph ^= 1;
         }
+      };
+      auto mma_s = [&](int i, int stage) {  // S_i = Q_i K^T
+        const uint32_t ql = q_lo + i * kTileLo, kl = ring_lo + stage * kTileLo;
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * ((kRows * 128) >> 4) + (ks & 3) * 2;
+          umma_ss(tmem + i * kRows, desc64(ql + off, kDescHi), desc64(kl + off, kDescHi), kIdescS, ks > 0);
+        }
+        umma_commit(smem_u32(s_full + i));
         issued = true;
       };
-      auto commit = [&](uint64_t* bar) {
-        if (elect_one()) umma_commit(smem_u32(bar));
-      };
-      for (int k = 0; ok && take_item(k, &it); ++k) {
-        const int nm = max(it.tiles[0], it.tiles[1]);
+      Item it;
+      for (int k = 0; ok; ++k) {
+        if (!(ok = mbar_wait_bounded(smem_u32(i_full + (k & 1)), (k >> 1) & 1))) break;
+        it = items[k & 1];
+        mbar_arrive(smem_u32(i_empty + (k & 1)));
+        if (it.s < 0) break;
+        const int n0 = it.tiles[0], n1 = it.tiles[1], nm = max(n0, n1);
         if (nm == 0) continue;
-        if (!(ok = wait(q_full, nq & 1))) break;
+        if (!(ok = mbar_wait_bounded(smem_u32(q_full), nq & 1))) break;
         ++nq;
-        if (!(ok = wait(kv_full + c % S, (c / S) & 1))) break;
-        for (int i = 0; i < 2; ++i)
-          if (it.tiles[i] > 0) mma_s(i, c % S);
-        commit(kv_empty + c % S);
-        if (nm == 1) commit(q_empty);
-        ++c;
-        for (int j = 0; j < nm && ok; ++j, c += 2) {
-          const int sv = c % S, sk = (c + 1) % S;  // this tile's values, the next one's keys
-          if (!(ok = wait(kv_full + sv, (c / S) & 1))) break;
-          const int valid = it.n - j * kRows;
-          if (valid < kRows) {  // nothing lives behind the sequence's end: zero weights meet zeros there
-            for (int h = 0; h < kHalves; ++h)
-              for (int b = valid * 128 + lane * 16; b < kRows * 128; b += 512)
-                *reinterpret_cast<uint4*>(smem + C::kRing + sv * C::kTile + h * (kRows * 128) + b) =
-                    make_uint4(0u, 0u, 0u, 0u);
-            fence_proxy_async();
-            __syncwarp();
+        if (!(ok = mbar_wait_bounded(smem_u32(kv_full + st), ph))) break;
+        if (n0 > 0) mma_s(0, st);
+        if (n1 > 0) mma_s(1, st);
+        umma_commit(smem_u32(kv_empty + st));
+        if (nm == 1) umma_commit(smem_u32(q_empty));
+        step();
+        for (int j = 0; j < nm; ++j) {
+          const int sv = st;  // this tile's values; the next stage holds the next tile's keys
+          if (!(ok = mbar_wait_bounded(smem_u32(kv_full + sv), ph))) break;
+          if (j == nm - 1 && it.n < nm * kRows) {
+            mbar_arrive(smem_u32(v_dirty));
+            if (!(ok = mbar_wait_bounded(smem_u32(v_clean), nc & 1))) break;
+            ++nc;
           }
-          bool have_k = false;
-          for (int i = 0; i < 2 && ok; ++i) {
-            if (j < it.tiles[i]) {
-              if (!(ok = wait(p_full + i, np[i] & 1))) break;
+          step();
+          const bool more = j + 1 < nm;
+          const uint32_t vl = ring_lo + sv * kTileLo;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int ni = i ? n1 : n0;
+            if (j < ni) {
+              if (!(ok = mbar_wait_bounded(smem_u32(p_full + i), np[i] & 1))) break;
               ++np[i];
               if (j == 0) {
-                if (no[i] > 0 && !(ok = wait(o_empty + i, (no[i] - 1) & 1))) break;
+                if (no[i] > 0 && !(ok = mbar_wait_bounded(smem_u32(o_empty + i), (no[i] - 1) & 1))) break;
                 ++no[i];
               }
               tc_fence_after();
-              if (elect_one()) {
-                const uint64_t vd = desc_mn_major(ring + sv * C::kTile);
 #pragma unroll
-                for (int ks = 0; ks < kRows / 16; ++ks)
-                  umma_ts(tmem + C::kO + i * HD, tmem + i * kRows + ks * 8, vd + ks * (2048 >> 4), kIdescO,
-                          j > 0 || ks > 0);
-              }
-              issued = true;
-              if (j == it.tiles[i] - 1) commit(o_full + i);
+              for (int ks = 0; ks < kRows / 16; ++ks)
+                umma_ts(tmem + C::kO + i * HD, tmem + i * kRows + ks * 8, desc64(vl + ks * (2048 >> 4), kDescHi), kIdescO,
+                        ks > 0 || j > 0);
+              if (j == ni - 1) umma_commit(smem_u32(o_full + i));
             }
-            if (i == 1) commit(kv_empty + sv);
-            if (j + 1 < it.tiles[i]) {
-              if (!have_k && !(ok = wait(kv_full + sk, ((c + 1) / S) & 1))) break;
-              have_k = true;
-              mma_s(i, sk);
+            if (i == 1) umma_commit(smem_u32(kv_empty + sv));
+            if (j + 1 < ni) {
+              if (!(ok = mbar_wait_bounded(smem_u32(kv_full + st), ph))) break;
+              mma_s(i, st);
             }
           }
           if (!ok) break;
-          if (j + 1 < nm) {
-            commit(kv_empty + sk);
-            if (j + 2 == nm) commit(q_empty);
-          } else {
-            --c;  // there was no next key tile
+          if (more) {
+            umma_commit(smem_u32(kv_empty + st));
+            if (j + 2 == nm) umma_commit(smem_u32(q_empty));
+            step();
           }
         }
       }
+      if (!ok) fail();
       if (issued) {  // the tensor core is done before tensor memory is released
-        commit(drain);
+        umma_commit(smem_u32(drain));
         if (!mbar_wait_bounded(smem_u32(drain), 0)) fail();
       }
     }
