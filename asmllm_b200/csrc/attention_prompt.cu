@@ -88,6 +88,25 @@ __device__ void attend_row(const PromptArgs& a, const KvArgs& kv, int t, int h, 
 }
 
 
+// Transposes the 4 x 4 matrix of 16-byte pieces that four consecutive lanes hold (lane = row, w = columns).
+__device__ __forceinline__ uint4 shfl_xor4(uint4 v, int mask) {
+  return make_uint4(__shfl_xor_sync(kFull, v.x, mask), __shfl_xor_sync(kFull, v.y, mask),
+                    __shfl_xor_sync(kFull, v.z, mask), __shfl_xor_sync(kFull, v.w, mask));
+}
+__device__ __forceinline__ void transpose4(uint4 (&w)[4], int lane) {
+  const bool odd = lane & 1, high = lane & 2;
+#pragma unroll
+  for (int q = 0; q < 4; q += 2) {  // 2 x 2 blocks of neighbours
+    const uint4 t = shfl_xor4(odd ? w[q] : w[q + 1], 1);
+    if (odd) w[q] = t; else w[q + 1] = t;
+  }
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {  // and of pairs
+    const uint4 t = shfl_xor4(high ? w[q] : w[q + 2], 2);
+    if (high) w[q] = t; else w[q + 2] = t;
+  }
+}
+
 // One work item, written by the scheduler.
 struct Item {
   int s;       // sequence; -1: no more
@@ -106,7 +125,7 @@ struct Cfg {
   static constexpr int kStages = HD == 128 ? 5 : 8;
   static constexpr int kRing = 2 * kTile;
   static constexpr int kBars = kRing + kStages * kTile;
-  static constexpr int kNBars = 2 * kStages + 2 + 8 + 4 + 3;
+  static constexpr int kNBars = 2 * kStages + 4 + 8 + 4 + 3;
   static constexpr int kItems = kBars + kNBars * 8 + 16;
   static constexpr int kSmem = kItems + 2 * (int)sizeof(Item) + 16 + 1024;
   static constexpr uint32_t kO = 2 * kRows;  // tensor memory: S0, S1, then the two outputs
@@ -152,9 +171,9 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBars);
   uint64_t* kv_full = bars;
   uint64_t* kv_empty = kv_full + S;
-  uint64_t* q_full = kv_empty + S;
-  uint64_t* q_empty = q_full + 1;
-  uint64_t* s_full = q_empty + 1;   // [2] scores of a tile are in tensor memory
+  uint64_t* q_full = kv_empty + S;  // [2]
+  uint64_t* q_empty = q_full + 2;   // [2]
+  uint64_t* s_full = q_empty + 2;   // [2] scores of a tile are in tensor memory
   uint64_t* p_full = s_full + 2;    // [2] its weights are
   uint64_t* o_full = p_full + 2;    // [2] the item's output is complete
   uint64_t* o_empty = o_full + 2;   // [2] and has been read
@@ -178,9 +197,9 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       mbar_init(smem_u32(kv_full + i), 1);
       mbar_init(smem_u32(kv_empty + i), 1);
     }
-    mbar_init(smem_u32(q_full), 1);
-    mbar_init(smem_u32(q_empty), 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(q_full + i), 1);
+      mbar_init(smem_u32(q_empty + i), 1);
       mbar_init(smem_u32(s_full + i), 1);
       mbar_init(smem_u32(p_full + i), 4);
       mbar_init(smem_u32(o_full + i), 1);
@@ -327,22 +346,24 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       const int my_page = lane / kHalves, half = lane % kHalves;
       const uint32_t box_bytes = (uint32_t)box_rows * 128u;
       const int g = a.n_heads / kv.n_kv;
-      int c = 0, nq = 0;
+      int c = 0, nq[2] = {0, 0};
       Item it;
       bool ok = true;
       for (int k = 0; ok && take_item(k, &it); ++k) {
         const int nm = max(it.tiles[0], it.tiles[1]);
         if (nm == 0) continue;
-        if (nq > 0 && !(ok = wait(q_empty, (nq - 1) & 1))) break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(smem_u32(q_full), 2 * C::kTile);
-          for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2 && ok; ++i) {
+          if (it.tiles[i] == 0) continue;
+          if (nq[i] > 0 && !(ok = wait(q_empty + i, (nq[i] - 1) & 1))) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(smem_u32(q_full + i), C::kTile);
             for (int h = 0; h < kHalves; ++h)
               tma_load_4d(smem_u32(smem) + i * C::kTile + h * (kRows * 128), &qmap, h * 64,
-                          it.t0 + (pair ? 0 : i * kRows), it.head + (pair ? i : 0), 0, smem_u32(q_full));
+                          it.t0 + (pair ? 0 : i * kRows), it.head + (pair ? i : 0), 0, smem_u32(q_full + i));
+          }
+          __syncwarp();
+          ++nq[i];
         }
-        __syncwarp();
-        ++nq;
         const int head = it.head / g;
         // page of this lane's box in key tile j: -1 nothing to read, n_pages reads as zeros
         auto lookup = [&](int j) -> int {
@@ -375,7 +396,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         }
       }
       // what was issued lands before the CTA may end (bounded)
-      if (nq > 0) mbar_wait_bounded(smem_u32(q_full), (nq - 1) & 1);
+      for (int i = 0; i < 2; ++i)
+        if (nq[i] > 0) mbar_wait_bounded(smem_u32(q_full + i), (nq[i] - 1) & 1);
       for (int j = c - S < 0 ? 0 : c - S; j < c; ++j) mbar_wait_bounded(smem_u32(kv_full + j % S), (j / S) & 1);
     } else if (warp == 11) {
       // ---------------- cleaner: zeroes the values behind a sequence's end ----------------
@@ -401,82 +423,91 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       // ---------------- matrix products (one thread) ----------------
       const uint32_t q_lo = desc_lo(smem_u32(smem)), ring_lo = desc_lo(smem_u32(smem) + C::kRing);
       constexpr uint32_t kTileLo = C::kTile >> 4;
-      int st = 0, nq = 0, np[2] = {0, 0}, no[2] = {0, 0}, nc = 0;
+      int st = 0, nq[2] = {0, 0}, np[2] = {0, 0}, no[2] = {0, 0}, nc = 0, k = 0;
       uint32_t ph = 0;  // ring stage and its parity
       bool ok = true, issued = false;
-      auto step = [&]() {
-        if (++st == S) {
-          st = 0;
-          ph ^= 1;
+      auto get = [&](uint64_t* bar, uint32_t parity) { return ok = ok && mbar_wait_bounded(smem_u32(bar), parity); };
+      // the next item with keys; false when there is none
+      auto next_item = [&](Item* it) -> bool {
+        for (;; ++k) {
+          if (!get(i_full + (k & 1), (k >> 1) & 1)) return false;
+          *it = items[k & 1];
+          mbar_arrive(smem_u32(i_empty + (k & 1)));
+          if (it->s < 0) return false;
+          if (max(it->tiles[0], it->tiles[1]) > 0) {
+            ++k;
+            return true;
+          }
         }
       };
-      auto mma_s = [&](int i, int stage) {  // S_i = Q_i K^T
-        const uint32_t ql = q_lo + i * kTileLo, kl = ring_lo + stage * kTileLo;
+      // S_i = Q_i K^T for key tile j of an item, its keys in ring stage st
+      auto scores = [&](int i, const Item& it, int j) {
+        if (j >= it.tiles[i]) return;
+        if (j == 0 && !get(q_full + i, nq[i]++ & 1)) return;
+        if (!get(kv_full + st, ph)) return;
+        const uint32_t ql = q_lo + i * kTileLo, kl = ring_lo + st * kTileLo;
 #pragma unroll
         for (int ks = 0; ks < HD / 16; ++ks) {
           const uint32_t off = (ks >> 2) * ((kRows * 128) >> 4) + (ks & 3) * 2;
           umma_ss(tmem + i * kRows, desc64(ql + off, kDescHi), desc64(kl + off, kDescHi), kIdescS, ks > 0);
         }
         umma_commit(smem_u32(s_full + i));
+        if (j == it.tiles[i] - 1) umma_commit(smem_u32(q_empty + i));
         issued = true;
       };
-      Item it;
-      for (int k = 0; ok; ++k) {
-        if (!(ok = mbar_wait_bounded(smem_u32(i_full + (k & 1)), (k >> 1) & 1))) break;
-        it = items[k & 1];
-        mbar_arrive(smem_u32(i_empty + (k & 1)));
-        if (it.s < 0) break;
-        const int n0 = it.tiles[0], n1 = it.tiles[1], nm = max(n0, n1);
-        if (nm == 0) continue;
-        if (!(ok = mbar_wait_bounded(smem_u32(q_full), nq & 1))) break;
-        ++nq;
-        if (!(ok = mbar_wait_bounded(smem_u32(kv_full + st), ph))) break;
-        if (n0 > 0) mma_s(0, st);
-        if (n1 > 0) mma_s(1, st);
+      auto release = [&]() {
         umma_commit(smem_u32(kv_empty + st));
-        if (nm == 1) umma_commit(smem_u32(q_empty));
-        step();
-        for (int j = 0; j < nm; ++j) {
-          const int sv = st;  // this tile's values; the next stage holds the next tile's keys
-          if (!(ok = mbar_wait_bounded(smem_u32(kv_full + sv), ph))) break;
-          if (j == nm - 1 && it.n < nm * kRows) {
-            mbar_arrive(smem_u32(v_dirty));
-            if (!(ok = mbar_wait_bounded(smem_u32(v_clean), nc & 1))) break;
-            ++nc;
-          }
-          step();
-          const bool more = j + 1 < nm;
-          const uint32_t vl = ring_lo + sv * kTileLo;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int ni = i ? n1 : n0;
-            if (j < ni) {
-              if (!(ok = mbar_wait_bounded(smem_u32(p_full + i), np[i] & 1))) break;
-              ++np[i];
-              if (j == 0) {
-                if (no[i] > 0 && !(ok = mbar_wait_bounded(smem_u32(o_empty + i), (no[i] - 1) & 1))) break;
-                ++no[i];
-              }
-              tc_fence_after();
-#pragma unroll
-              for (int ks = 0; ks < kRows / 16; ++ks)
-                umma_ts(tmem + C::kO + i * HD, tmem + i * kRows + ks * 8, desc64(vl + ks * (2048 >> 4), kDescHi), kIdescO,
-                        ks > 0 || j > 0);
-              if (j == ni - 1) umma_commit(smem_u32(o_full + i));
-            }
-            if (i == 1) umma_commit(smem_u32(kv_empty + sv));
-            if (j + 1 < ni) {
-              if (!(ok = mbar_wait_bounded(smem_u32(kv_full + st), ph))) break;
-              mma_s(i, st);
-            }
-          }
-          if (!ok) break;
-          if (more) {
-            umma_commit(smem_u32(kv_empty + st));
-            if (j + 2 == nm) umma_commit(smem_u32(q_empty));
-            step();
-          }
+        if (++st == S) {
+          st = 0;
+          ph ^= 1;
         }
+      };
+      Item it, nx;
+      bool live = next_item(&it);
+      if (live) {
+        scores(0, it, 0);
+        scores(1, it, 0);
+        release();
+      }
+      for (int j = 0; live && ok;) {
+        // this step's values are in stage st, the next step's keys -- of this item or the next -- behind them
+        const int nm = max(it.tiles[0], it.tiles[1]), sv = st;
+        const uint32_t pv = ph, vl = ring_lo + sv * kTileLo;
+        if (!get(kv_full + sv, pv)) break;
+        if (j == nm - 1 && it.n < nm * kRows) {
+          mbar_arrive(smem_u32(v_dirty));
+          if (!get(v_clean, nc++ & 1)) break;
+        }
+        if (++st == S) {
+          st = 0;
+          ph ^= 1;
+        }
+        const bool last = j == nm - 1;
+        if (last) live = next_item(&nx);
+        else nx = it;
+        const int jn = last ? 0 : j + 1;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (j < it.tiles[i]) {
+            if (!get(p_full + i, np[i]++ & 1)) break;
+            if (j == 0) {
+              if (no[i] > 0 && !get(o_empty + i, (no[i] - 1) & 1)) break;
+              ++no[i];
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int ks = 0; ks < kRows / 16; ++ks)
+              umma_ts(tmem + C::kO + i * HD, tmem + i * kRows + ks * 8, desc64(vl + ks * (2048 >> 4), kDescHi), kIdescO,
+                      ks > 0 || j > 0);
+            if (j == it.tiles[i] - 1) umma_commit(smem_u32(o_full + i));
+          }
+          if (i == 1) umma_commit(smem_u32(kv_empty + sv));
+          if (live) scores(i, nx, jn);
+        }
+        if (!ok) break;
+        if (live) release();
+        it = nx;
+        j = jn;
       }
       if (!ok) fail();
       if (issued) {  // the tensor core is done before tensor memory is released
@@ -579,22 +610,37 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       ++no;
       tc_fence_after();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      O* out = static_cast<O*>(a.out) + ((long long)(it.t0 + row) * a.n_heads + head) * HD;
       bool bad = false;
+      // A thread holds a row; its 16-byte pieces are exchanged within four lanes, so that a store writes 64
+      // bytes of a row at a time (16 bytes a row kept the load-store unit busy for 5000 cycles an item).
+      constexpr int kPer = 16 / sizeof(O);  // values of a piece
+      O* out4 = static_cast<O*>(a.out) + ((long long)(it.t0 + (row & ~3)) * a.n_heads + head) * HD + (lane & 3) * kPer;
+      const int rows4 = it.rows - (row & ~3);  // rows of the four lanes that exist
 #pragma unroll
       for (int b = 0; b < HD; b += 32) {
         uint32_t y[32];
         tmem_ld<32>(to + b, y);
         tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          float v[8];
+        for (int e = 0; e < 32; e += 4 * kPer) {
+          uint4 w[4];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            v[q] = __uint_as_float(y[e + q]) * inv;
-            bad |= !(fabsf(v[q]) < INFINITY);
+          for (int q = 0; q < 4; ++q) {
+            float v[kPer];
+#pragma unroll
+            for (int z = 0; z < kPer; ++z) {
+              v[z] = __uint_as_float(y[e + q * kPer + z]) * inv;
+              bad |= !(fabsf(v[z]) < INFINITY);
+            }
+            if constexpr (sizeof(O) == 4)
+              w[q] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+            else
+              w[q] = make_uint4(pack16<O>(v[0], v[1]), pack16<O>(v[2], v[3]), pack16<O>(v[4], v[5]), pack16<O>(v[6], v[7]));
           }
-          if (mine) store8(out + b + e, v);
+          transpose4(w, lane);  // now w[q] is piece lane % 4 of the four lanes' row q
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (q < rows4) *reinterpret_cast<uint4*>(out4 + (long long)q * a.n_heads * HD + b + e) = w[q];
         }
       }
       tc_fence_before();
