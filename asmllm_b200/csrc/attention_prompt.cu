@@ -51,7 +51,7 @@ constexpr int kThreads = 384;
 // row's zero weight and turns its output to NaN, although the row does not
 // attend to that position.  Lane l holds values l, l + 32, ...
 template <class T, class O, int HD>
-__device__ void attend_row(const PromptArgs& a, const KvArgs& kv, int t, int h, int s, int last, int lane) {
+__device__ __forceinline__ void attend_row(const PromptArgs& a, const KvArgs& kv, int t, int h, int s, int last, int lane) {
   constexpr int E = HD / 32;
   const T* q = static_cast<const T*>(a.q) + (long long)t * a.q_row_stride + (long long)h * a.q_head_stride;
   const long long ho = (long long)(h / (a.n_heads / kv.n_kv)) * kv.head_stride;
@@ -118,6 +118,29 @@ struct Item {
   int key0;    // packed: first key row of the sequence
   int tiles[2];  // key tiles of each query tile
 };
+
+// Rows `todo` of a warp's 32 (lane by lane) are not finite: computed again if that may be a later position's doing.
+template <class T, class O, int HD>
+__device__ __forceinline__ void mend_rows(const PromptArgs& a, const KvArgs& kv, const Item& it, int i, int pair, int tiles,
+                                       int lrow, unsigned todo, int lane) {
+  const int row = lrow + (pair ? 0 : i * kRows), head = it.head + (pair ? i : 0);
+  const int first = __shfl_sync(kFull, it.base + row, __ffs(todo) - 1) + 1, last = min(it.n, tiles * kRows);
+  const long long ho = (long long)(head / (a.n_heads / kv.n_kv)) * kv.head_stride;
+  bool later = false;
+#pragma unroll 1
+  for (int p = max(0, first); p < last; ++p) {
+    const long long o = kv_offset(kv, it.s, p);
+    if (o < 0) continue;
+    for (int e = lane; e < HD; e += 32) later |= !(fabsf(to_f32(static_cast<const T*>(kv.v)[o + ho + e])) < INFINITY);
+  }
+  if (!__any_sync(kFull, later)) return;
+  __syncwarp();  // the rows' first stores come before the second ones
+  while (todo) {
+    const int rr = __shfl_sync(kFull, row, __ffs(todo) - 1);
+    todo &= todo - 1;
+    attend_row<T, O, HD>(a, kv, it.t0 + rr, head, it.s, min(it.base + rr, it.n - 1), lane);
+  }
+}
 
 template <int HD>
 struct Cfg {
@@ -267,6 +290,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         int x = 0;
 #pragma unroll
         for (int e = 0; e < kHeld; ++e) x += f(hq[e], hb[e]);
+#pragma unroll 1
         for (int s = lane + 32 * kHeld; s < kv.batch; s += 32) {
           int q, b;
           load(s, &q, &b);
@@ -277,6 +301,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       int top = 0;
 #pragma unroll
       for (int e = 0; e < kHeld; ++e) top = max(top, hq[e] > 0 ? hq[e] + hb[e] : 0);
+#pragma unroll 1
       for (int s = lane + 32 * kHeld; s < kv.batch; s += 32) {
         int q, b;
         load(s, &q, &b);
@@ -423,7 +448,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       // ---------------- matrix products (one thread) ----------------
       const uint32_t q_lo = desc_lo(smem_u32(smem)), ring_lo = desc_lo(smem_u32(smem) + C::kRing);
       constexpr uint32_t kTileLo = C::kTile >> 4;
-      int st = 0, nq[2] = {0, 0}, np[2] = {0, 0}, no[2] = {0, 0}, nc = 0, k = 0;
+      int st = 0, nc = 0, k = 0;
+      uint32_t nq = 0, np = 0, no = 3;  // parities, one bit a tile (nobody has to empty the first outputs)
       uint32_t ph = 0;  // ring stage and its parity
       bool ok = true, issued = false;
       auto get = [&](uint64_t* bar, uint32_t parity) { return ok = ok && mbar_wait_bounded(smem_u32(bar), parity); };
@@ -442,8 +468,12 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       };
       // S_i = Q_i K^T for key tile j of an item, its keys in ring stage st
       auto scores = [&](int i, const Item& it, int j) {
-        if (j >= it.tiles[i]) return;
-        if (j == 0 && !get(q_full + i, nq[i]++ & 1)) return;
+        const int tiles = i ? it.tiles[1] : it.tiles[0];
+        if (j >= tiles) return;
+        if (j == 0) {
+          if (!get(q_full + i, nq >> i & 1)) return;
+          nq ^= 1u << i;
+        }
         if (!get(kv_full + st, ph)) return;
         const uint32_t ql = q_lo + i * kTileLo, kl = ring_lo + st * kTileLo;
 #pragma unroll
@@ -452,7 +482,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
           umma_ss(tmem + i * kRows, desc64(ql + off, kDescHi), desc64(kl + off, kDescHi), kIdescS, ks > 0);
         }
         umma_commit(smem_u32(s_full + i));
-        if (j == it.tiles[i] - 1) umma_commit(smem_u32(q_empty + i));
+        if (j == tiles - 1) umma_commit(smem_u32(q_empty + i));
         issued = true;
       };
       auto release = [&]() {
@@ -464,44 +494,43 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       };
       Item it, nx;
       bool live = next_item(&it);
-      if (live) {
-        scores(0, it, 0);
-        scores(1, it, 0);
-        release();
-      }
-      for (int j = 0; live && ok;) {
-        // this step's values are in stage st, the next step's keys -- of this item or the next -- behind them
+      nx = it;
+      // Step j of an item: values of its key tile j into the outputs, then the scores of the next key tile,
+      // of this item or the next.  Step -1 has no values: the first item's first scores.
+      for (int j = -1; live && ok;) {
         const int nm = max(it.tiles[0], it.tiles[1]), sv = st;
-        const uint32_t pv = ph, vl = ring_lo + sv * kTileLo;
-        if (!get(kv_full + sv, pv)) break;
-        if (j == nm - 1 && it.n < nm * kRows) {
-          mbar_arrive(smem_u32(v_dirty));
-          if (!get(v_clean, nc++ & 1)) break;
-        }
-        if (++st == S) {
-          st = 0;
-          ph ^= 1;
-        }
         const bool last = j == nm - 1;
+        const uint32_t vl = ring_lo + sv * kTileLo;
+        if (j >= 0) {  // this step's values are in stage st, the next step's keys behind them
+          if (!get(kv_full + sv, ph)) break;
+          if (last && it.n < nm * kRows) {
+            mbar_arrive(smem_u32(v_dirty));
+            if (!get(v_clean, nc++ & 1)) break;
+          }
+          if (++st == S) {
+            st = 0;
+            ph ^= 1;
+          }
+        }
         if (last) live = next_item(&nx);
-        else nx = it;
         const int jn = last ? 0 : j + 1;
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < 2; ++i) {
-          if (j < it.tiles[i]) {
-            if (!get(p_full + i, np[i]++ & 1)) break;
-            if (j == 0) {
-              if (no[i] > 0 && !get(o_empty + i, (no[i] - 1) & 1)) break;
-              ++no[i];
+          if (j >= 0 && j < (i ? it.tiles[1] : it.tiles[0])) {
+            if (!get(p_full + i, np >> i & 1)) break;
+            np ^= 1u << i;
+            if (j == 0) {  // the last item's output has been read (the first time: there is none)
+              if (!get(o_empty + i, no >> i & 1)) break;
+              no ^= 1u << i;
             }
             tc_fence_after();
 #pragma unroll
             for (int ks = 0; ks < kRows / 16; ++ks)
               umma_ts(tmem + C::kO + i * HD, tmem + i * kRows + ks * 8, desc64(vl + ks * (2048 >> 4), kDescHi), kIdescO,
                       ks > 0 || j > 0);
-            if (j == it.tiles[i] - 1) umma_commit(smem_u32(o_full + i));
+            if (j == (i ? it.tiles[1] : it.tiles[0]) - 1) umma_commit(smem_u32(o_full + i));
           }
-          if (i == 1) umma_commit(smem_u32(kv_empty + sv));
+          if (j >= 0 && i == 1) umma_commit(smem_u32(kv_empty + sv));
           if (live) scores(i, nx, jn);
         }
         if (!ok) break;
@@ -556,7 +585,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
           m = mn;
           l *= f;
           const unsigned long long f2 = pack2(f, f);
-#pragma unroll
+#pragma unroll 1
           for (int b = 0; b < HD; b += 32) {
             uint32_t y[32];
             tmem_ld<32>(to + b, y);
@@ -602,6 +631,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         if (mine) {
           O* out = static_cast<O*>(a.out) + ((long long)(it.t0 + row) * a.n_heads + head) * HD;
           const float z[8] = {};
+#pragma unroll 1
           for (int b = 0; b < HD; b += 8) store8(out + b, z);
         }
         continue;
@@ -616,7 +646,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       constexpr int kPer = 16 / sizeof(O);  // values of a piece
       O* out4 = static_cast<O*>(a.out) + ((long long)(it.t0 + (row & ~3)) * a.n_heads + head) * HD + (lane & 3) * kPer;
       const int rows4 = it.rows - (row & ~3);  // rows of the four lanes that exist
-#pragma unroll
+#pragma unroll 1
       for (int b = 0; b < HD; b += 32) {
         uint32_t y[32];
         tmem_ld<32>(to + b, y);
@@ -647,26 +677,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(o_empty + i));
       // Rows that are not finite: because of a later position's value?
-      unsigned todo = __ballot_sync(kFull, bad && mine);
-      if (todo) {
-        const int first = __shfl_sync(kFull, pos, __ffs(todo) - 1) + 1, last = min(it.n, tiles * kRows);
-        const long long ho = (long long)(head / (a.n_heads / kv.n_kv)) * kv.head_stride;
-        bool later = false;
-        for (int p = max(0, first); p < last; ++p) {
-          const long long o = kv_offset(kv, it.s, p);
-          if (o < 0) continue;
-          for (int e = lane; e < HD; e += 32) later |= !(fabsf(to_f32(static_cast<const T*>(kv.v)[o + ho + e])) < INFINITY);
-        }
-        if (__any_sync(kFull, later)) {
-          __syncwarp();  // the rows' first stores come before the second ones
-          while (todo) {
-            const int src = __ffs(todo) - 1;
-            todo &= todo - 1;
-            const int rr = __shfl_sync(kFull, row, src);
-            attend_row<T, O, HD>(a, kv, it.t0 + rr, head, it.s, min(it.base + rr, it.n - 1), lane);
-          }
-        }
-      }
+      const unsigned todo = __ballot_sync(kFull, bad && mine);
+      if (todo) mend_rows<T, O, HD>(a, kv, it, i, pair, tiles, lrow, todo, lane);
     }
   }
   tc_fence_before();
