@@ -148,7 +148,7 @@ struct Cfg {
   static constexpr int kStages = HD == 128 ? 5 : 8;
   static constexpr int kRing = 2 * kTile;
   static constexpr int kBars = kRing + kStages * kTile;
-  static constexpr int kNBars = 2 * kStages + 4 + 8 + 4 + 3;
+  static constexpr int kNBars = 2 * kStages + 4 + 10 + 4 + 3;
   static constexpr int kItems = kBars + kNBars * 8 + 16;
   static constexpr int kSmem = kItems + 2 * (int)sizeof(Item) + 16 + 1024;
   static constexpr uint32_t kO = 2 * kRows;  // tensor memory: S0, S1, then the two outputs
@@ -197,8 +197,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
   uint64_t* q_full = kv_empty + S;  // [2]
   uint64_t* q_empty = q_full + 2;   // [2]
   uint64_t* s_full = q_empty + 2;   // [2] scores of a tile are in tensor memory
-  uint64_t* p_full = s_full + 2;    // [2] its weights are
-  uint64_t* o_full = p_full + 2;    // [2] the item's output is complete
+  uint64_t* p_full = s_full + 2;    // [2][2] the weights of its first and second 64 keys are
+  uint64_t* o_full = p_full + 4;    // [2] the item's output is complete
   uint64_t* o_empty = o_full + 2;   // [2] and has been read
   uint64_t* i_full = o_empty + 2;   // [2] work items
   uint64_t* i_empty = i_full + 2;
@@ -224,7 +224,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       mbar_init(smem_u32(q_full + i), 1);
       mbar_init(smem_u32(q_empty + i), 1);
       mbar_init(smem_u32(s_full + i), 1);
-      mbar_init(smem_u32(p_full + i), 4);
+      mbar_init(smem_u32(p_full + 2 * i), 4);
+      mbar_init(smem_u32(p_full + 2 * i + 1), 4);
       mbar_init(smem_u32(o_full + i), 1);
       mbar_init(smem_u32(o_empty + i), 4);
       mbar_init(smem_u32(i_full + i), 1);
@@ -249,6 +250,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
   };
   // Warp-wide wait; false (in every lane) when the role has to leave.
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    if (__all_sync(kFull, mbar_try_wait(smem_u32(bar), parity))) return true;
     const bool ok = mbar_wait_bounded(smem_u32(bar), parity);
     if (!ok) fail();
     return !__any_sync(kFull, !ok || *s_abort);
@@ -517,17 +519,21 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
           if (j >= 0 && j < (i ? it.tiles[1] : it.tiles[0])) {
-            if (!get(p_full + i, np >> i & 1)) break;
-            np ^= 1u << i;
             if (j == 0) {  // the last item's output has been read (the first time: there is none)
               if (!get(o_empty + i, no >> i & 1)) break;
               no ^= 1u << i;
             }
-            tc_fence_after();
 #pragma unroll
-            for (int ks = 0; ks < kRows / 16; ++ks)
-              umma_ts(tmem + C::kO + i * HD, tmem + i * kRows + ks * 8, desc64(vl + ks * (2048 >> 4), kDescHi), kIdescO,
-                      ks > 0 || j > 0);
+            for (int h = 0; h < 2; ++h) {  // the first 64 keys while the weights of the others are computed
+              if (!get(p_full + 2 * i + h, np >> i & 1)) break;
+              tc_fence_after();
+#pragma unroll
+              for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
+                umma_ts(tmem + C::kO + i * HD, tmem + i * kRows + ks * 8, desc64(vl + ks * (2048 >> 4), kDescHi),
+                        kIdescO, ks > 0 || j > 0);
+            }
+            if (!ok) break;
+            np ^= 1u << i;
             if (j == (i ? it.tiles[1] : it.tiles[0]) - 1) umma_commit(smem_u32(o_full + i));
           }
           if (j >= 0 && i == 1) umma_commit(smem_u32(kv_empty + sv));
@@ -616,11 +622,11 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
             w[e >> 1] = pack16<T>(x0, x1);
           }
           tmem_st32(ts + (b >> 1), w);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(p_full + 2 * i + (b >> 6)));
         }
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(p_full + i));
         float s0, s1;
         unpack2(add2(sum[0], sum[1]), s0, s1);
         l += s0 + s1;
