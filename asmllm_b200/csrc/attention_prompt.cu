@@ -45,13 +45,16 @@ constexpr int kRows = 128;  // rows of a query tile, positions of a key tile
 constexpr float kLazy = 6.0f;
 constexpr float kPShift = 8.0f;  // weights are 2^kPShift exp(s - m): fp16 keeps those down to 2^-32 of the largest
 constexpr int kThreads = 384;
+constexpr int kSplitItems = 2, kSplitTiles = 8;
 
 // A row whose output is not finite, computed again key by key by one warp:
 // in a matrix product a later position's infinite or NaN value meets the
 // row's zero weight and turns its output to NaN, although the row does not
-// attend to that position.  Lane l holds values l, l + 32, ...
+// attend to that position.  Lane l holds values l, l + 32, ...; those from
+// 32 e0 to 32 e1 are written.
 template <class T, class O, int HD>
-__device__ __forceinline__ void attend_row(const PromptArgs& a, const KvArgs& kv, int t, int h, int s, int last, int lane) {
+__device__ __forceinline__ void attend_row(const PromptArgs& a, const KvArgs& kv, int t, int h, int s, int last, int lane,
+                                           int e0, int e1) {
   constexpr int E = HD / 32;
   const T* q = static_cast<const T*>(a.q) + (long long)t * a.q_row_stride + (long long)h * a.q_head_stride;
   const long long ho = (long long)(h / (a.n_heads / kv.n_kv)) * kv.head_stride;
@@ -77,7 +80,7 @@ __device__ __forceinline__ void attend_row(const PromptArgs& a, const KvArgs& kv
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   O* out = static_cast<O*>(a.out) + ((long long)t * a.n_heads + h) * HD;
-  for (int e = 0; e < E; ++e) {
+  for (int e = e0; e < e1; ++e) {
     const float v = o[e] * inv;
     if constexpr (sizeof(O) == 4) out[lane + 32 * e] = v;
     else {
@@ -116,13 +119,30 @@ struct Item {
   int n;       // keys of the sequence
   int head;    // first query head
   int key0;    // packed: first key row of the sequence
-  int tiles[2];  // key tiles of each query tile
+  int tiles[2];  // key tiles of each query tile in this item, from key tile j0 on
+  int j0;
+  int slot;      // -1: the whole of it; else where this part of it goes
 };
+
+// The item that begins in a CTA's share and ends in a later one's, for the join.
+struct Split {
+  Item it;  // whole: j0 = 0, all key tiles; slot: of the first part (CTA c + p, p > 0, has slot 2 (c + p))
+  int parts;  // 0: none
+  int pad[3];
+};
+// A part: unnormalised outputs [2 query tiles][HD / 4][128 rows][4], then (maximum, sum) [2][128].
+template <int HD>
+__host__ __device__ constexpr size_t part_floats() {
+  return (size_t)2 * kRows * HD + 4 * kRows;
+}
+__device__ __forceinline__ int cta_of(long long x, long long total, int ctas) {  // whose share holds x
+  return (int)(((x + 1) * ctas - 1) / total);
+}
 
 // Rows `todo` of a warp's 32 (lane by lane) are not finite: computed again if that may be a later position's doing.
 template <class T, class O, int HD>
 __device__ __forceinline__ void mend_rows(const PromptArgs& a, const KvArgs& kv, const Item& it, int i, int pair, int tiles,
-                                       int lrow, unsigned todo, int lane) {
+                                       int lrow, unsigned todo, int lane, int e0, int e1) {
   const int row = lrow + (pair ? 0 : i * kRows), head = it.head + (pair ? i : 0);
   const int first = __shfl_sync(kFull, it.base + row, __ffs(todo) - 1) + 1, last = min(it.n, tiles * kRows);
   const long long ho = (long long)(head / (a.n_heads / kv.n_kv)) * kv.head_stride;
@@ -131,14 +151,14 @@ __device__ __forceinline__ void mend_rows(const PromptArgs& a, const KvArgs& kv,
   for (int p = max(0, first); p < last; ++p) {
     const long long o = kv_offset(kv, it.s, p);
     if (o < 0) continue;
-    for (int e = lane; e < HD; e += 32) later |= !(fabsf(to_f32(static_cast<const T*>(kv.v)[o + ho + e])) < INFINITY);
+    for (int e = lane + 32 * e0; e < 32 * e1; e += 32) later |= !(fabsf(to_f32(static_cast<const T*>(kv.v)[o + ho + e])) < INFINITY);
   }
   if (!__any_sync(kFull, later)) return;
   __syncwarp();  // the rows' first stores come before the second ones
   while (todo) {
     const int rr = __shfl_sync(kFull, row, __ffs(todo) - 1);
     todo &= todo - 1;
-    attend_row<T, O, HD>(a, kv, it.t0 + rr, head, it.s, min(it.base + rr, it.n - 1), lane);
+    attend_row<T, O, HD>(a, kv, it.t0 + rr, head, it.s, min(it.base + rr, it.n - 1), lane, e0, e1);
   }
 }
 
@@ -182,7 +202,8 @@ template <class T, class O, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap, const PromptArgs a, const KvArgs kv, int pair,
-                        int box_rows, unsigned* __restrict__ err) {
+                        int box_rows, float* __restrict__ parts, Split* __restrict__ splits,
+                        unsigned* __restrict__ err) {
   using C = Cfg<HD>;
   constexpr int kHalves = HD / 64, S = C::kStages;
   constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
@@ -269,7 +290,9 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 10) {
       // ---------------- scheduler ----------------
-      // Items are numbered by falling key-tile count, heads fastest; CTA b takes numbers b, 2G-1-b, 2G+b, ...
+      // Many items: numbered by falling key-tile count, heads fastest; CTA b takes numbers b, 2G-1-b, 2G+b, ...
+      // Few items: the key tiles of all of them in a row are cut into equal shares, one a CTA, and an item that
+      // lies in several shares is joined afterwards.
       constexpr int kHeld = 4;  // sequences per lane kept in registers
       int hq[kHeld], hb[kHeld];
       bool any_clipped = false;
@@ -300,6 +323,110 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         }
         return __reduce_add_sync(kFull, x);
       };
+      // key tiles of the item of query rows [tile R, ...) of a sequence; the first i's own; at least 1 counted
+      auto tiles_in = [&](int base, int rows, int i) -> int {
+        const int r = pair ? rows : min(kRows, rows - i * kRows);
+        const int stop = r <= 0 ? 0 : base + (pair ? 0 : i * kRows) + r;
+        return stop <= 0 ? 0 : (stop + kRows - 1) / kRows;
+      };
+      if (parts) {
+        auto weight = [&](int q, int b, int tile) -> int {
+          return max(1, (b + min((tile + 1) * R, q) + kRows - 1) / kRows);
+        };
+        auto weights = [&](int s) -> long long {  // of a sequence, all heads
+          if (s >= kv.batch) return 0;
+          int q, b;
+          load(s, &q, &b);
+          long long x = 0;
+#pragma unroll 1
+          for (int t = 0; t * R < q; ++t) x += weight(q, b, t);
+          return x * units;
+        };
+        long long sum = 0;
+#pragma unroll 1
+        for (int s0 = 0; s0 < kv.batch; s0 += 32) {
+          long long x = weights(s0 + lane);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(kFull, x, o);
+          sum += x;
+        }
+        if (any_clipped && blockIdx.x == 0) atomicOr(err, kErrDecodeRange);
+        const int cta = blockIdx.x, ctas = (int)min((long long)gridDim.x, sum);
+        long long at = cta < ctas ? sum * cta / ctas : 0;
+        const long long begin = at, end = cta < ctas ? sum * (cta + 1) / ctas : 0;
+        int s = 0, q = 0, b = 0, tile = 0, unit = 0, t = 0;
+        if (at < end) {
+          long long before = 0;
+#pragma unroll 1
+          for (int s0 = 0;; s0 += 32) {  // the sequence that holds `begin`
+            const long long w = weights(s0 + lane);
+            long long x = w;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const long long y = __shfl_up_sync(kFull, x, o);
+              if (lane >= o) x += y;
+            }
+            const unsigned hit = __ballot_sync(kFull, begin < before + x);
+            if (hit) {
+              s = s0 + __ffs(hit) - 1;
+              before += __shfl_sync(kFull, x - w, __ffs(hit) - 1);
+              break;
+            }
+            before += __shfl_sync(kFull, x, 31);
+          }
+          load(s, &q, &b);
+          long long left = begin - before;
+          for (; left >= (long long)weight(q, b, tile) * units; ++tile) left -= (long long)weight(q, b, tile) * units;
+          unit = (int)(left / weight(q, b, tile));
+          t = (int)(left % weight(q, b, tile));
+        }
+        Split mine;
+        mine.parts = 0;
+        for (int k = 0;; ++k) {
+          if (k >= 2 && !wait(i_empty + (k & 1), ((k >> 1) - 1) & 1)) break;
+          Item it;
+          it.s = -1;
+          if (at < end) {
+            const int w = weight(q, b, tile), t1 = (int)min((long long)w, t + (end - at));
+            int qb, qe;
+            q_range(a.cu_q, s, a.rows, &qb, &qe);
+            it.s = s;
+            it.t0 = qb + tile * R;
+            it.rows = min(R, q - tile * R);
+            it.base = b + tile * R;
+            it.n = q + b;
+            it.head = pair ? 2 * unit : unit;
+            it.key0 = kv.table ? 0 : __ldcg(kv.cu + s);
+            const int f0 = tiles_in(it.base, it.rows, 0), f1 = tiles_in(it.base, it.rows, 1);
+            it.j0 = t;
+            it.slot = t == 0 && t1 == w ? -1 : 2 * cta + (at == begin ? 0 : 1);
+            it.tiles[0] = max(0, min(f0, t1) - t);
+            it.tiles[1] = max(0, min(f1, t1) - t);
+            if (t == 0 && t1 < w) {
+              mine.it = it;
+              mine.it.tiles[0] = f0;
+              mine.it.tiles[1] = f1;
+              mine.parts = cta_of(at + w - 1, sum, ctas) - cta + 1;
+            }
+            at += t1 - t;
+            t = 0;
+            if (++unit == units) {
+              unit = 0;
+              if (++tile * R >= q && at < end) {
+                tile = 0;
+                do load(++s, &q, &b); while (q == 0);
+              }
+            }
+          }
+          if (lane == 0) {
+            items[k & 1] = it;
+            mbar_arrive(smem_u32(i_full + (k & 1)));
+          }
+          __syncwarp();
+          if (it.s < 0) break;
+        }
+        if (lane == 0) splits[cta] = mine;
+      } else {
       int top = 0;
 #pragma unroll
       for (int e = 0; e < kHeld; ++e) top = max(top, hq[e] > 0 ? hq[e] + hb[e] : 0);
@@ -354,11 +481,10 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
           }
           it.head = pair ? 2 * unit : unit;
           it.key0 = kv.table ? 0 : __ldcg(kv.cu + it.s);
-          for (int i = 0; i < 2; ++i) {
-            const int rows = pair ? it.rows : min(kRows, it.rows - i * kRows);
-            const int stop = rows <= 0 ? 0 : it.base + (pair ? 0 : i * kRows) + rows;
-            it.tiles[i] = stop <= 0 ? 0 : (stop + kRows - 1) / kRows;
-          }
+          it.j0 = 0;
+          it.slot = -1;
+          it.tiles[0] = tiles_in(it.base, it.rows, 0);
+          it.tiles[1] = tiles_in(it.base, it.rows, 1);
         }
         if (lane == 0) {
           items[k & 1] = it;
@@ -366,6 +492,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         }
         __syncwarp();
         if (it.s < 0) break;
+      }
       }
     } else if (warp == 9) {
       // ---------------- loader ----------------
@@ -394,7 +521,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         const int head = it.head / g;
         // page of this lane's box in key tile j: -1 nothing to read, n_pages reads as zeros
         auto lookup = [&](int j) -> int {
-          const int p = j * kRows + my_page * box_rows;
+          const int p = (it.j0 + j) * kRows + my_page * box_rows;
           if (my_page >= pages) return -1;
           if (!kv.table) return 0;
           if (j >= nm || p >= it.n) return -1;
@@ -408,7 +535,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
           const int cur = page;
           page = j + 1 < nm ? lookup(j + 1) : -1;
           const unsigned live = __ballot_sync(kFull, cur >= 0);
-          const int p = j * kRows + my_page * box_rows;
+          const int p = (it.j0 + j) * kRows + my_page * box_rows;
           const int row = kv.table ? p & (kv.page_size - 1) : it.key0 + p;
           for (int v = 0; v < 2; ++v, ++c) {
             const int st = c % S;
@@ -432,7 +559,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       int c = 0, nd = 0;
       Item it;
       for (int k = 0; take_item(k, &it); ++k) {
-        const int nm = max(it.tiles[0], it.tiles[1]), valid = it.n - (nm - 1) * kRows;
+        const int nm = max(it.tiles[0], it.tiles[1]), valid = it.n - (it.j0 + nm - 1) * kRows;
         c += 2 * nm;
         if (nm == 0 || valid >= kRows) continue;
         const int sv = (c - 1) % S;  // the item's last value tile
@@ -505,7 +632,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         const uint32_t vl = ring_lo + sv * kTileLo;
         if (j >= 0) {  // this step's values are in stage st, the next step's keys behind them
           if (!get(kv_full + sv, ph)) break;
-          if (last && it.n < nm * kRows) {
+          if (last && it.n < (it.j0 + nm) * kRows) {
             mbar_arrive(smem_u32(v_dirty));
             if (!get(v_clean, nc++ & 1)) break;
           }
@@ -572,7 +699,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
 #pragma unroll
         for (int b = 0; b < kRows; b += 32) tmem_ld<32>(ts + b, *reinterpret_cast<uint32_t(*)[32]>(x + b));
         tmem_wait_ld();
-        const int limit = pos - j * kRows + 1;  // columns below it are attended to
+        const int limit = pos - (it.j0 + j) * kRows + 1;  // columns below it are attended to
         if (!__all_sync(kFull, limit >= kRows)) {
 #pragma unroll
           for (int e = 0; e < kRows; ++e)
@@ -633,6 +760,29 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       }
       if (!ok) break;
       const bool mine = row < it.rows;
+      if (it.slot >= 0) {  // a part of an item: as it is, for the join
+        float* part = parts + (size_t)it.slot * part_floats<HD>();
+        __stcg(reinterpret_cast<float2*>(part + (size_t)2 * kRows * HD) + i * kRows + lrow, make_float2(m, l));
+        if (tiles == 0) continue;
+        if (!wait(o_full + i, no & 1)) break;
+        ++no;
+        tc_fence_after();
+        float4* o4 = reinterpret_cast<float4*>(part) + (size_t)i * kRows * (HD / 4) + lrow;
+#pragma unroll 1
+        for (int b = 0; b < HD; b += 32) {
+          uint32_t y[32];
+          tmem_ld<32>(to + b, y);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            __stcg(o4 + (size_t)((b + e) >> 2) * kRows, make_float4(__uint_as_float(y[e]), __uint_as_float(y[e + 1]),
+                                                                   __uint_as_float(y[e + 2]), __uint_as_float(y[e + 3])));
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(o_empty + i));
+        continue;
+      }
       if (tiles == 0) {  // no key for any row of the tile
         if (mine) {
           O* out = static_cast<O*>(a.out) + ((long long)(it.t0 + row) * a.n_heads + head) * HD;
@@ -684,7 +834,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       if (lane == 0) mbar_arrive(smem_u32(o_empty + i));
       // Rows that are not finite: because of a later position's value?
       const unsigned todo = __ballot_sync(kFull, bad && mine);
-      if (todo) mend_rows<T, O, HD>(a, kv, it, i, pair, tiles, lrow, todo, lane);
+      if (todo) mend_rows<T, O, HD>(a, kv, it, i, pair, tiles, lrow, todo, lane, 0, HD / 32);
     }
   }
   tc_fence_before();
@@ -692,6 +842,62 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
   tc_fence_after();
   if (warp == 8)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// Joins the parts of the item that began in CTA blockIdx.x: query tile blockIdx.y, values 32 blockIdx.z ..,
+// in part order.  Thread: a row and 16 of the values.
+template <class T, class O, int HD>
+__global__ void __launch_bounds__(256) attention_prompt_join_kernel(const PromptArgs a, const KvArgs kv, int pair,
+                                                                    const float* __restrict__ parts,
+                                                                    const Split* __restrict__ splits) {
+  pdl_trigger();
+  pdl_wait();
+  const int c = blockIdx.x, i = blockIdx.y, z = blockIdx.z, lrow = threadIdx.x & (kRows - 1), half = threadIdx.x >> 7;
+  const int n = __ldcg(&splits[c].parts);
+  if (n == 0) return;
+  const Item it = splits[c].it;
+  const int row = lrow + (pair ? 0 : i * kRows), tiles = i ? it.tiles[1] : it.tiles[0];
+  const float sl2 = a.scale * 1.4426950408889634f;
+  float m = -INFINITY, l = 0.0f, o[16] = {};
+  for (int p = 0; p < n; ++p) {
+    const float* part = parts + (size_t)(p ? 2 * (c + p) : it.slot) * part_floats<HD>();
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + (size_t)2 * kRows * HD) + i * kRows + lrow);
+    if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // no key of this part for the row: there may be no output either
+    const float mn = fmaxf(m, ml.x), f0 = m == -INFINITY ? 0.0f : ex2((m - mn) * sl2), f1 = ex2((ml.x - mn) * sl2);
+    m = mn;
+    l = l * f0 + ml.y * f1;
+    const float4* o4 = reinterpret_cast<const float4*>(part) + (size_t)i * kRows * (HD / 4) + lrow;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float4 v = __ldcg(o4 + (size_t)(z * 8 + half * 4 + e) * kRows);
+      o[4 * e] = o[4 * e] * f0 + v.x * f1;
+      o[4 * e + 1] = o[4 * e + 1] * f0 + v.y * f1;
+      o[4 * e + 2] = o[4 * e + 2] * f0 + v.z * f1;
+      o[4 * e + 3] = o[4 * e + 3] * f0 + v.w * f1;
+    }
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const bool mine = row < it.rows;
+  bool bad = false;
+  O* out = static_cast<O*>(a.out) + ((long long)(it.t0 + row) * a.n_heads + it.head + (pair ? i : 0)) * HD + z * 32 + half * 16;
+#pragma unroll
+  for (int e = 0; e < 16; e += 8) {
+    float v[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      v[q] = o[e + q] * inv;
+      bad |= !(fabsf(v[q]) < INFINITY);
+    }
+    if (mine) store8(out + e, v);
+  }
+  // a row that is bad in either half is mended by the first (32 values from 32 z on)
+  __shared__ unsigned s_bad[8];
+  const unsigned vote = __ballot_sync(kFull, bad && mine);
+  if ((threadIdx.x & 31) == 0) s_bad[threadIdx.x >> 5] = vote;
+  __syncthreads();
+  const int warp = threadIdx.x >> 5;
+  const unsigned todo = warp < 4 ? s_bad[warp] | s_bad[warp + 4] : 0u;
+  if (todo) mend_rows<T, O, HD>(a, kv, it, i, pair, tiles, lrow, todo, threadIdx.x & 31, z, z + 1);
 }
 
 template <class T, class O, int HD>
@@ -710,8 +916,20 @@ cudaError_t launch_typed(const PromptArgs& a, const KvArgs& kv, cudaStream_t str
   if (e != cudaSuccess) return e;
   const int pair = (a.n_heads / kv.n_kv) % 2 == 0, R = pair ? kRows : 2 * kRows;
   const long long items = ((long long)a.rows / R + kv.batch) * (pair ? a.n_heads / 2 : a.n_heads);
+  // Lengths are on the device; what is known here bounds the items and an item's key tiles.
+  const long long most = ((kv.table ? (long long)kv.width * kv.page_size : kv.page_size) + kRows - 1) / kRows;
+  const bool split = items < kSplitItems * sms && most >= kSplitTiles;
+  float* parts = nullptr;
+  Split* splits = nullptr;
+  if (split) {
+    const size_t floats = (size_t)sms * 2 * part_floats<HD>();
+    void* p = nullptr;
+    if ((e = scratch_alloc_async(&p, floats * sizeof(float) + (size_t)sms * sizeof(Split), stream)) != cudaSuccess) return e;
+    parts = static_cast<float*>(p);
+    splits = reinterpret_cast<Split*>(parts + floats);
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(items < sms ? items : sms));
+  cfg.gridDim = dim3((unsigned)(split || items >= sms ? sms : items));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = stream;
@@ -720,7 +938,16 @@ cudaError_t launch_typed(const PromptArgs& a, const KvArgs& kv, cudaStream_t str
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = g_opt_pdl.load() ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, qmap, kmap, vmap, a, kv, pair, box_rows, err);
+  e = cudaLaunchKernelEx(&cfg, kernel, qmap, kmap, vmap, a, kv, pair, box_rows, parts, splits, err);
+  if (!split) return e;
+  if (e == cudaSuccess) {
+    cfg.gridDim = dim3((unsigned)sms, 2, HD / 32);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, attention_prompt_join_kernel<T, O, HD>, a, kv, pair, parts, splits);
+  }
+  const cudaError_t f = scratch_free_async(parts, stream);
+  return e != cudaSuccess ? e : f;
 }
 
 template <class T>

@@ -344,6 +344,13 @@ PROMPT = [
     (8, 2, 64, [128, 128], [128, 0], 128),
     (5, 1, 128, [260, 9], [300, 4], 256),
     (16, 2, 128, [1, 1, 1, 2], [0, 300, 15, 16], 32),
+    # few items over many keys: their key tiles are dealt out in equal shares and joined
+    (2, 1, 128, [5, 1, 128], [3000, 1290, 0], 64),
+    (1, 1, 64, [300, 1], [2000, 0], 16),
+    (3, 1, 128, [1, 257, 0, 2], [5000, 1100, 0, 127], 128),
+    (8, 1, 128, [130, 64], [4000, 1], 256),
+    (2, 2, 64, [1500], None, 0),
+    (4, 2, 128, [1100, 3, 129], None, 0),
 ]
 
 
@@ -417,8 +424,8 @@ def test_attention_prompt_rising_scores(cuda, step):
         close(torch, got, want, pv, serr, n, prompt_weight(torch, torch.float16, n), torch.float16)
 
 
-@pytest.mark.parametrize("page", [0, 16])
-def test_attention_prompt_later_values_do_not_reach_earlier_rows(cuda, page):
+@pytest.mark.parametrize("page,width", [(0, 0), (16, 0), (16, 100)])  # 100 more columns: dealt out in shares
+def test_attention_prompt_later_values_do_not_reach_earlier_rows(cuda, page, width):
     torch = cuda
     q_len, nh, nkv, hd = [150, 300], 4, 2, 128
     T = sum(q_len)
@@ -429,7 +436,7 @@ def test_attention_prompt_later_values_do_not_reach_earlier_rows(cuda, page):
     def call(k, v):
         if not page:
             return ops.attention_prompt(q, k, v, cu)
-        kp, vp, table = make_pages(torch, [k[:150], k[150:]], [v[:150], v[150:]], page)
+        kp, vp, table = make_pages(torch, [k[:150], k[150:]], [v[:150], v[150:]], page, width_extra=width)
         kv = torch.tensor(q_len, dtype=torch.int32, device="cuda")
         return ops.attention_prompt(q, kp, vp, cu, kv_len=kv, page_table=table)
 
