@@ -95,6 +95,8 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x, units = kv.n_kv * zs, g = a.n_heads / kv.n_kv;
   if (tid == 0) {
+    prefetch_map(&kmap);
+    prefetch_map(&vmap);
     for (int i = 0; i < kStages; ++i) {
       mbar_init(smem_u32(full + i), 1);
       mbar_init(smem_u32(empty + i), kWarps);

@@ -45,7 +45,10 @@ constexpr int kRows = 128;  // rows of a query tile, positions of a key tile
 constexpr float kLazy = 6.0f;
 constexpr float kPShift = 8.0f;  // weights are 2^kPShift exp(s - m): fp16 keeps those down to 2^-32 of the largest
 constexpr int kThreads = 384;
-constexpr int kSplitItems = 2, kSplitTiles = 8;
+// Items are dealt out by key tiles (and joined) where there may be fewer of them than SMs and one may have 16
+// key tiles or more.  Measured (us, by items / by key tiles): 64 items of 4096 keys 61 / 38, 128 of 8192 116 / 87,
+// 96 of 2048 36 / 33; the other way round 128 of 2048 37 / 39, 64 of 1024 22 / 26, 256 of 4096 63 / 97.
+constexpr int kSplitTiles = 16;
 
 // A row whose output is not finite, computed again key by key by one warp:
 // in a matrix product a later position's infinite or NaN value meets the
@@ -198,7 +201,8 @@ __device__ __forceinline__ int tiles_at_least(int base, int q, int R, int w) {
   return n - (x < 0 ? 0 : min(x / R, n - 1));
 }
 
-template <class T, class O, int HD>
+// SPLIT: few items, dealt out by key tiles (an instantiation of its own keeps the code small).
+template <class T, class O, int HD, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap, const PromptArgs a, const KvArgs kv, int pair,
@@ -237,6 +241,9 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (tid == 0) {
+    prefetch_map(&qmap);
+    prefetch_map(&kmap);
+    prefetch_map(&vmap);
     for (int i = 0; i < S; ++i) {
       mbar_init(smem_u32(kv_full + i), 1);
       mbar_init(smem_u32(kv_empty + i), 1);
@@ -294,9 +301,9 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       // Few items: the key tiles of all of them in a row are cut into equal shares, one a CTA, and an item that
       // lies in several shares is joined afterwards.
       constexpr int kHeld = 4;  // sequences per lane kept in registers
-      int hq[kHeld], hb[kHeld];
+      int hq[kHeld], hb[kHeld], hr[kHeld];
       bool any_clipped = false;
-      auto load = [&](int s, int* q, int* b) {
+      auto load = [&](int s, int* q, int* b) -> int {  // query rows, position of the first, its row
         int qb, qe;
         bool clipped;
         q_range(a.cu_q, s, a.rows, &qb, &qe);
@@ -304,11 +311,12 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         any_clipped |= clipped;
         *q = qe - qb;
         *b = n - (qe - qb);
+        return qb;
       };
 #pragma unroll
       for (int e = 0; e < kHeld; ++e) {
-        hq[e] = hb[e] = 0;
-        if (lane + 32 * e < kv.batch) load(lane + 32 * e, hq + e, hb + e);
+        hq[e] = hb[e] = hr[e] = 0;
+        if (!SPLIT && lane + 32 * e < kv.batch) hr[e] = load(lane + 32 * e, hq + e, hb + e);
       }
       // sum over the sequences of f(q rows, base)
       auto total = [&](auto f) -> int {
@@ -329,7 +337,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         const int stop = r <= 0 ? 0 : base + (pair ? 0 : i * kRows) + r;
         return stop <= 0 ? 0 : (stop + kRows - 1) / kRows;
       };
-      if (parts) {
+      if constexpr (SPLIT) {
         auto weight = [&](int q, int b, int tile) -> int {
           return max(1, (b + min((tile + 1) * R, q) + kRows - 1) / kRows);
         };
@@ -453,9 +461,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
             if (total([&](int q, int b) { return tiles_at_least(b, q, R, w); }) > rank) lo = w; else hi = w - 1;
           }
           int left = rank - total([&](int q, int b) { return tiles_at_least(b, q, R, lo + 1); });
-          for (int s0 = 0; s0 < kv.batch; s0 += 32) {
-            int q = 0, b = 0;
-            if (s0 + lane < kv.batch) load(s0 + lane, &q, &b);
+          // which of the tiles with exactly lo key tiles: true in every lane once it is among these sequences
+          auto pick = [&](int s0, int q, int b, int r) -> bool {
             const int c1 = tiles_at_least(b, q, R, lo), c = c1 - tiles_at_least(b, q, R, lo + 1);
             int x = c;
 #pragma unroll
@@ -464,20 +471,27 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
               if (lane >= o) x += y;
             }
             const unsigned hit = __ballot_sync(kFull, left < x);
-            if (hit) {
-              const int src = __ffs(hit) - 1;
-              const int tile = (q + R - 1) / R - c1 + (left - (x - c));
-              it.s = s0 + src;
-              it.rows = __shfl_sync(kFull, min(R, q - tile * R), src);
-              it.base = __shfl_sync(kFull, b + tile * R, src);
-              it.n = __shfl_sync(kFull, q + b, src);
-              const int t = __shfl_sync(kFull, tile, src);
-              int qb, qe;
-              q_range(a.cu_q, it.s, a.rows, &qb, &qe);
-              it.t0 = qb + t * R;
-              break;
+            if (!hit) {
+              left -= __shfl_sync(kFull, x, 31);
+              return false;
             }
-            left -= __shfl_sync(kFull, x, 31);
+            const int src = __ffs(hit) - 1, tile = (q + R - 1) / R - c1 + (left - (x - c));
+            it.s = s0 + src;
+            it.rows = __shfl_sync(kFull, min(R, q - tile * R), src);
+            it.base = __shfl_sync(kFull, b + tile * R, src);
+            it.n = __shfl_sync(kFull, q + b, src);
+            it.t0 = __shfl_sync(kFull, r + tile * R, src);
+            return true;
+          };
+          bool found = false;
+#pragma unroll
+          for (int e = 0; e < kHeld; ++e)
+            if (!found && 32 * e < kv.batch) found = pick(32 * e, hq[e], hb[e], hr[e]);
+#pragma unroll 1
+          for (int s0 = 32 * kHeld; !found && s0 < kv.batch; s0 += 32) {
+            int q = 0, b = 0, r = 0;
+            if (s0 + lane < kv.batch) r = load(s0 + lane, &q, &b);
+            found = pick(s0, q, b, r);
           }
           it.head = pair ? 2 * unit : unit;
           it.key0 = kv.table ? 0 : __ldcg(kv.cu + it.s);
@@ -760,7 +774,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       }
       if (!ok) break;
       const bool mine = row < it.rows;
-      if (it.slot >= 0) {  // a part of an item: as it is, for the join
+      if (SPLIT && it.slot >= 0) {  // a part of an item: as it is, for the join
         float* part = parts + (size_t)it.slot * part_floats<HD>();
         __stcg(reinterpret_cast<float2*>(part + (size_t)2 * kRows * HD) + i * kRows + lrow, make_float2(m, l));
         if (tiles == 0) continue;
@@ -903,22 +917,23 @@ __global__ void __launch_bounds__(256) attention_prompt_join_kernel(const Prompt
 template <class T, class O, int HD>
 cudaError_t launch_typed(const PromptArgs& a, const KvArgs& kv, cudaStream_t stream, unsigned* err) {
   using C = Cfg<HD>;
-  auto kernel = attention_prompt_kernel<T, O, HD>;
   CUtensorMap qmap, kmap, vmap;
   const int box_rows = kv.table && kv.page_size < kRows ? kv.page_size : kRows;
   if (!encode_4d(&qmap, kv.dtype, a.q, HD, (uint64_t)a.rows, (uint64_t)a.n_heads, 1, (uint64_t)a.q_row_stride,
                  (uint64_t)a.q_head_stride, (uint64_t)a.q_row_stride, kRows) ||
       !encode_kv_map(&kmap, kv, kv.k, box_rows) || !encode_kv_map(&vmap, kv, kv.v, box_rows))
     return cudaErrorInvalidValue;
-  static std::atomic<unsigned long long> done{0};
+  static std::atomic<unsigned long long> done[2] = {};
   int sms = 0;
-  cudaError_t e = kernel_setup(reinterpret_cast<const void*>(kernel), C::kSmem, done, &sms);
+  cudaError_t e = kernel_setup(reinterpret_cast<const void*>(attention_prompt_kernel<T, O, HD, false>), C::kSmem, done[0], &sms);
+  if (e == cudaSuccess)
+    e = kernel_setup(reinterpret_cast<const void*>(attention_prompt_kernel<T, O, HD, true>), C::kSmem, done[1], &sms);
   if (e != cudaSuccess) return e;
   const int pair = (a.n_heads / kv.n_kv) % 2 == 0, R = pair ? kRows : 2 * kRows;
   const long long items = ((long long)a.rows / R + kv.batch) * (pair ? a.n_heads / 2 : a.n_heads);
   // Lengths are on the device; what is known here bounds the items and an item's key tiles.
   const long long most = ((kv.table ? (long long)kv.width * kv.page_size : kv.page_size) + kRows - 1) / kRows;
-  const bool split = items < kSplitItems * sms && most >= kSplitTiles;
+  const bool split = items < sms && most >= kSplitTiles;
   float* parts = nullptr;
   Split* splits = nullptr;
   if (split) {
@@ -938,8 +953,10 @@ cudaError_t launch_typed(const PromptArgs& a, const KvArgs& kv, cudaStream_t str
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = g_opt_pdl.load() ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, kernel, qmap, kmap, vmap, a, kv, pair, box_rows, parts, splits, err);
-  if (!split) return e;
+  if (!split) return cudaLaunchKernelEx(&cfg, attention_prompt_kernel<T, O, HD, false>, qmap, kmap, vmap, a, kv, pair,
+                                        box_rows, parts, splits, err);
+  e = cudaLaunchKernelEx(&cfg, attention_prompt_kernel<T, O, HD, true>, qmap, kmap, vmap, a, kv, pair, box_rows, parts,
+                         splits, err);
   if (e == cudaSuccess) {
     cfg.gridDim = dim3((unsigned)sms, 2, HD / 32);
     cfg.blockDim = dim3(256);

@@ -49,6 +49,10 @@ inline bool encode_kv_map(CUtensorMap* map, const KvArgs& kv, const void* base, 
 }
 
 #ifdef __CUDACC__
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
                                             uint32_t mbar) {
   asm volatile(
