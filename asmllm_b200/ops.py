@@ -562,29 +562,24 @@ def key_index(keys):
 _DT: dict = {}   # torch dtype -> ASM_DT_*
 _H16: dict = {}  # the 16-bit ones alone
 _KV_PACK = struct.Struct("QQqqqQqQQiiiiiiii").pack  # asm_kv_t (native.Kv), field for field
+_F32 = _I32 = _U8 = _current_stream = None  # torch's, once it is imported
 
 
 def _dtypes():
+    global _F32, _I32, _U8, _current_stream
     torch = _torch()
+    _F32, _I32, _U8, _current_stream = torch.float32, torch.int32, torch.uint8, torch._C._cuda_getCurrentRawStream
     _H16.update({torch.float16: native.DT_F16, torch.bfloat16: native.DT_BF16})
     _DT.update({torch.float32: native.DT_F32, **_H16})
     return _DT
 
 
-def _raw_stream(device: int, stream) -> int:
-    """cudaStream_t of `stream`, or of torch's current stream on the device."""
-    if stream is not None:
-        return stream.cuda_stream
-    return _torch()._C._cuda_getCurrentRawStream(device)
-
-
-def _empty(shape, dtype, device, stream):
-    """A new output that belongs to the stream the kernel runs on."""
-    torch = _torch()
+def _empty(like, shape, dtype, stream):
+    """A new output beside `like` that belongs to the stream the kernel runs on."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
+    with _torch().cuda.stream(stream):
+        return like.new_empty(shape, dtype=dtype)
 
 
 def _call(rc: int) -> None:
@@ -619,12 +614,12 @@ def _strides(t):
 
 def _vector(t, name, n, device):
     """int32 [n], contiguous, on the device."""
-    torch = _torch()
-    _check_dev(t, (torch.int32,), name)
+    if t.dtype is _I32 and t.shape == (n,) and t.get_device() == device and (n < 2 or t.stride(0) == 1):
+        return
+    _check_dev(t, (_I32,), name)
     if t.shape != (n,):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({n},)")
-    if t.get_device() != device:
-        raise ValueError(f"{name} is on another device")
+    raise ValueError(f"{name} is on another device")
 
 
 def _kv_view(k, v, device, kv_len=None, page_table=None, cu_k=None):
@@ -643,9 +638,9 @@ def _kv_view(k, v, device, kv_len=None, page_table=None, cu_k=None):
         raise ValueError("k, v and the rows are on different devices")
     if paged:
         batch, width = page_table.shape
-        if (page_table.dtype != _torch().int32 or page_table.get_device() != device
+        if (page_table.dtype is not _I32 or page_table.get_device() != device
                 or (width > 1 and page_table.stride(1) != 1)):
-            _dense(page_table, "page_table", 2, (_torch().int32,))
+            _dense(page_table, "page_table", 2, (_I32,))
             raise ValueError("page_table is on another device")
         _vector(kv_len, "kv_len", batch, device)
         return (_KV_PACK(k.data_ptr(), v.data_ptr(), st[0], st[1], st[2], page_table.data_ptr(),
@@ -671,10 +666,10 @@ def _query(q, k, out, out_dtype, stream):
         raise ValueError(f"{shape[1]} query heads are not a multiple of {heads} KV heads")
     if out is None:
         dt = out_dtype or q.dtype
-        if dt != q.dtype and dt != _torch().float32:
+        if dt != q.dtype and dt != _F32:
             raise TypeError(f"out_dtype {dt}: fp32 or q's type")
-        return st, _empty(shape, dt, q.device, stream)
-    _check_dev(out, (q.dtype, _torch().float32), "out")
+        return st, _empty(q, shape, dt, stream)
+    _check_dev(out, (q.dtype, _F32), "out")
     if out.shape != shape or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError(f"out: {tuple(out.shape)} {out.dtype}, expected {tuple(shape)} {out_dtype or q.dtype}")
     return st, out
@@ -690,21 +685,21 @@ def rope_append(qkv, rope_cs, kv_len, page_table, k_pages, v_pages, n_heads: int
     [pages, page_size, nkv, hd] fp16 or bf16 (any strides, hd dense), page_table int32 [B, n], rope_cs fp32
     [positions, hd/2, 2] (decode.rope_table).  Returns the rotated queries [T, nh, hd] in the cache's
     type; rows at or past cu_q[B] are not written."""
-    torch = _torch()
     if page_table is None:
         raise ValueError("page_table is required")
-    device = qkv.get_device() if isinstance(qkv, torch.Tensor) else -1
+    device = qkv.get_device()
     if device < 0:
         raise TypeError("qkv: expected a CUDA tensor")
     kv, batch = _kv_view(k_pages, v_pages, device, kv_len, page_table)
     dt = k_pages.dtype
     nkv, hd = k_pages.shape[2:]
-    if qkv.dtype not in (torch.float32, dt) or qkv.dim() != 2 or qkv.stride(1) != 1:
-        _dense(qkv, "qkv", 2, (torch.float32, dt))
+    if (qkv.dtype is not _F32 and qkv.dtype is not dt) or qkv.dim() != 2 or qkv.stride(1) != 1:
+        _dense(qkv, "qkv", 2, (_F32, dt))
     T = qkv.shape[0]
     if qkv.shape[1] != (n_heads + 2 * nkv) * hd:
         raise ValueError(f"qkv has {qkv.shape[1]} columns, expected ({n_heads} + 2 * {nkv}) * {hd}")
-    _check_dev(rope_cs, (torch.float32,), "rope_cs")
+    if rope_cs.dtype is not _F32 or not rope_cs.is_cuda or not rope_cs.is_contiguous():
+        _check_dev(rope_cs, (_F32,), "rope_cs")
     if rope_cs.shape[1:] != (hd // 2, 2):
         raise ValueError(f"rope_cs {tuple(rope_cs.shape)}: expected [positions, {hd // 2}, 2]")
     if cu_q is not None:
@@ -712,7 +707,7 @@ def rope_append(qkv, rope_cs, kv_len, page_table, k_pages, v_pages, n_heads: int
     elif T != batch:
         raise ValueError(f"{T} rows for {batch} sequences: pass cu_q")
     if q_out is None:
-        q_out = _empty((T, n_heads, hd), dt, qkv.device, stream)
+        q_out = _empty(qkv, (T, n_heads, hd), dt, stream)
     else:
         _check_dev(q_out, (dt,), "q_out")
         if q_out.shape != (T, n_heads, hd):
@@ -720,7 +715,7 @@ def rope_append(qkv, rope_cs, kv_len, page_table, k_pages, v_pages, n_heads: int
     _call((native._lib or native.lib()).asm_rope_append_async(
         qkv.data_ptr(), _DT[qkv.dtype], qkv.stride(0) if T > 1 else qkv.shape[1], rope_cs.data_ptr(),
         rope_cs.shape[0], None if cu_q is None else cu_q.data_ptr(), T, n_heads, q_out.data_ptr(), kv,
-        _raw_stream(device, stream)))
+        _current_stream(device) if stream is None else stream.cuda_stream))
     return q_out
 
 
@@ -743,7 +738,7 @@ def attention_prompt(q, k, v, cu_q, *, cu_k=None, kv_len=None, page_table=None, 
     T, nh, hd = q.shape
     _call((native._lib or native.lib()).asm_attention_prompt_async(
         q.data_ptr(), st[0], st[1], cu_q.data_ptr(), T, nh, hd ** -0.5 if scale is None else scale, out.data_ptr(),
-        _DT[out.dtype], kv, _raw_stream(device, stream)))
+        _DT[out.dtype], kv, _current_stream(device) if stream is None else stream.cuda_stream))
     return out
 
 
@@ -772,13 +767,12 @@ def attention_paged(q, k_pages, v_pages, page_table, kv_len, *, scale: float | N
         raise ValueError(f"q has {B} rows for {batch} sequences")
     lib = native._lib or native.lib()
     if workspace is None:
-        workspace = _empty(lib.asm_attention_paged_workspace(B, nh, k_pages.shape[2], hd), _torch().uint8, q.device,
-                           stream)
+        workspace = _empty(q, (lib.asm_attention_paged_workspace(B, nh, k_pages.shape[2], hd),), _U8, stream)
     else:
-        _check_dev(workspace, (_torch().uint8,), "workspace")
+        _check_dev(workspace, (_U8,), "workspace")
     _call(lib.asm_attention_paged_async(
         q.data_ptr(), st[0], st[1], nh, hd ** -0.5 if scale is None else scale, out.data_ptr(), _DT[out.dtype], kv,
-        workspace.data_ptr(), workspace.numel(), _raw_stream(device, stream)))
+        workspace.data_ptr(), workspace.numel(), _current_stream(device) if stream is None else stream.cuda_stream))
     return out
 
 
@@ -790,27 +784,24 @@ def rows_sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=No
     then top_p of what is left, then min_p of the largest probability; ties go to the lower index; the
     word is the first, in index order, whose cumulative probability exceeds u.  temperature 0: the first
     maximum.  NaN is never chosen; a row of NaN and -inf gives -1.  Returns int32 [B]."""
-    torch = _torch()
     if not _DT:
         _dtypes()
-    if not isinstance(logits, torch.Tensor) or logits.dtype not in _DT or not logits.is_cuda or logits.dim() != 2 or (
-            logits.stride(1) != 1):
+    if logits.dtype not in _DT or not logits.is_cuda or logits.dim() != 2 or logits.stride(1) != 1:
         _dense(logits, "logits", 2, _DT)
     B, V = shape = logits.shape
     device = logits.get_device()
     if tokens is None:
-        tokens = _empty(shape[:1], torch.int32, logits.device, stream)
-    f32, i32, ptr = torch.float32, torch.int32, []
-    for t, name, dt in ((u, "u", f32), (temperature, "temperature", f32), (top_k, "top_k", i32), (top_p, "top_p", f32),
-                        (min_p, "min_p", f32), (tokens, "tokens", i32)):
+        tokens = _empty(logits, shape[:1], _I32, stream)
+    ptr, rows = [], shape[:1]
+    for t, name, dt in ((u, "u", _F32), (temperature, "temperature", _F32), (top_k, "top_k", _I32),
+                        (top_p, "top_p", _F32), (min_p, "min_p", _F32), (tokens, "tokens", _I32)):
         if t is None and name != "u":
             ptr.append(None)
             continue
-        if not isinstance(t, torch.Tensor) or t.dtype != dt or t.get_device() != device or t.shape != shape[:1] or (
-                B > 1 and t.stride(0) != 1):
+        if t.dtype is not dt or t.get_device() != device or t.shape != rows or (B > 1 and t.stride(0) != 1):
             _check_dev(t, (dt,), name)
             raise ValueError(f"{name}: shape {tuple(t.shape)} on device {t.get_device()}, expected ({B},) on {device}")
         ptr.append(t.data_ptr())
     _call((native._lib or native.lib()).asm_rows_sample_async(logits.data_ptr(), _DT[logits.dtype], B, V,
-                                             logits.stride(0) if B > 1 else V, *ptr, _raw_stream(device, stream)))
+                                             logits.stride(0) if B > 1 else V, *ptr, _current_stream(device) if stream is None else stream.cuda_stream))
     return tokens
