@@ -60,16 +60,32 @@ struct Layout {
   static constexpr int kMlOff = kJoinOff + 2 * 8 * kJoinRow * 4;
   static constexpr int kBarOff = kMlOff + 2 * 8 * 8;
   static constexpr int kSmem = kBarOff + 2 * kStages * 8 + 64 + 1024;
+  // A unit's query rows pass through the join buffer: padded by 16 bytes for ldmatrix.
+  static constexpr int kQRow = HD * 2 + 16;
+  static_assert(16 * kQRow <= 2 * 8 * kJoinRow * 4, "the query rows fit the join buffer");
 };
 
 __device__ __forceinline__ int tiles_of(int n) { return (n + kTile - 1) / kTile; }
 
-// First tile of CTA c's range.
-__device__ __forceinline__ long long range_start(long long total, int c, int ctas) { return total * c / ctas; }
-// The CTA whose range holds tile x.
-__device__ __forceinline__ int cta_of(long long x, long long total, int ctas) {
-  return (int)(((x + 1) * ctas - 1) / total);
-}
+// `total` tiles over `ctas` ranges: the first `extra` have one more than the others.
+struct Deal {
+  long long each;
+  int extra;
+  __device__ __forceinline__ Deal(long long total, int ctas) {
+    if (total < (1ll << 32)) {  // a 64-bit division costs hundreds of cycles
+      each = (unsigned)total / (unsigned)ctas;
+      extra = (int)((unsigned)total % (unsigned)ctas);
+    } else {
+      each = total / ctas;
+      extra = (int)(total % ctas);
+    }
+  }
+  __device__ __forceinline__ long long start(int c) const { return c * each + min(c, extra); }
+  __device__ __forceinline__ int cta_of(long long x) const {  // whose range holds tile x
+    const long long big = (each + 1) * extra;
+    return x < big ? (int)(x / (each + 1)) : extra + (int)((x - big) / each);
+  }
+};
 
 // A CTA's walk over its tiles: sequence, unit of the sequence, tile.
 struct Walk {
@@ -88,8 +104,8 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
   uint64_t* empty = full + kStages;
   volatile int* s_abort = reinterpret_cast<int*>(empty + kStages);
-  int* s_start = const_cast<int*>(s_abort) + 1;  // sequence of the range's first tile, and
-  long long* s_first = reinterpret_cast<long long*>(empty + kStages + 2);  // [0] its first tile, [1] total
+  int* s_start = reinterpret_cast<int*>(empty + kStages + 1);  // [0] sequence of the range's first tile, [1] its positions
+  long long* s_first = reinterpret_cast<long long*>(empty + kStages + 2);  // [0] the sequence's first tile, [1] total
   long long* s_part = reinterpret_cast<long long*>(smem + L::kJoinOff);    // per-thread sums (before the join uses it)
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -102,7 +118,6 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
       mbar_init(smem_u32(empty + i), kWarps);
     }
     *s_abort = 0;
-    *s_start = -1;
     fence_mbar_init();
   }
   pdl_trigger();
@@ -111,9 +126,11 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
   // Sum of all tiles and the sequence this range begins in: a contiguous share of the sequences per thread.
   const int per = (kv.batch + kThreads - 1) / kThreads, q0 = min(kv.batch, tid * per), q1 = min(kv.batch, q0 + per);
   long long mine = 0;
+  int held = 0;  // positions of the thread's first sequence
   for (int s = q0; s < q1; ++s) {
     bool clipped;
     const int n = kv_length(kv, s, &clipped);
+    if (s == q0) held = n;
     if (clipped && cta == 0) atomicOr(err, kErrDecodeRange);
     mine += tiles_of(n);
     // a sequence without positions: zeros, written by one CTA
@@ -144,15 +161,17 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
   __syncthreads();
   const long long total = s_first[1];
   const int ctas = (int)min((long long)gridDim.x, total);  // every range in use holds a tile; the other CTAs have none
-  const long long begin = cta < ctas ? range_start(total, cta, ctas) : 0;
-  const long long end = cta < ctas ? range_start(total, cta + 1, ctas) : 0;
+  const Deal deal(total, max(1, ctas));
+  const long long begin = cta < ctas ? deal.start(cta) : 0, end = cta < ctas ? deal.start(cta + 1) : 0;
   if (begin < end && s_part[tid] <= begin && begin < s_part[tid] + mine) {
     long long x = s_part[tid];
     for (int s = q0; s < q1; ++s) {
       bool clipped;
-      const long long w = (long long)tiles_of(kv_length(kv, s, &clipped)) * units;
+      const int n = s == q0 ? held : kv_length(kv, s, &clipped);
+      const long long w = (long long)tiles_of(n) * units;
       if (begin < x + w) {
-        *s_start = s;
+        s_start[0] = s;
+        s_start[1] = n;
         s_first[0] = x;
         break;
       }
@@ -168,11 +187,12 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
     return;
   }
   Walk w;
-  w.s = *s_start;
+  w.s = s_start[0];
   bool clipped;
-  w.n = kv_length(kv, w.s, &clipped);
+  w.n = s_start[1];
   w.nt = tiles_of(w.n);
-  w.u = (int)((begin - s_first[0]) / w.nt);
+  const long long into = begin - s_first[0];
+  w.u = into < (1ll << 32) ? (int)((unsigned)into / (unsigned)w.nt) : (int)(into / w.nt);
   w.first = s_first[0] + (long long)w.u * w.nt;
   w.t = (int)(begin - w.first);
   w.at = begin;
@@ -254,21 +274,37 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
     // one segment: tiles w.t .. of unit (w.s, w.u)
     const int j = w.u / zs, h0 = (w.u % zs) * 16, nh = min(16, g - h0);
     const int t0 = w.t, t1 = (int)min((long long)w.nt, w.t + (w.end - w.at));
+    // The unit's query rows, read once by the CTA (each warp for itself made the same lines of a long
+    // sequence's one unit a bottleneck of 5 to 14 thousand cycles), then as fragments.
     uint32_t qf[HD / 16][ROWS / 4];
     {
       const T* qb = static_cast<const T*>(a.q) + w.s * a.q_row_stride + (long long)(j * g + h0) * a.q_head_stride;
-      auto ld = [&](int row, int col) -> uint32_t {
-        return row < nh ? __ldcg(reinterpret_cast<const unsigned*>(qb + row * a.q_head_stride + col)) : 0u;
-      };
+      unsigned char* sq = smem + L::kJoinOff;
+      for (int e = tid; e < ROWS * (HD / 8); e += kWarps * 32) {
+        const int row = e / (HD / 8), c = e % (HD / 8);
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (row < nh) v = __ldcg(reinterpret_cast<const uint4*>(qb + row * a.q_head_stride) + c);
+        *reinterpret_cast<uint4*>(sq + row * L::kQRow + c * 16) = v;
+      }
+      consumer_bar_sync(kWarps * 32);
+      // matrices of 8 rows x 8 values: [0..1] rows 0-7, [2..3] rows 8-15; each pair the 16 values of a step
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks) {
-        qf[ks][0] = ld(r, ks * 16 + c2);
-        qf[ks][1] = ld(r, ks * 16 + c2 + 8);
         if constexpr (ROWS == 16) {
-          qf[ks][2] = ld(r + 8, ks * 16 + c2);
-          qf[ks][3] = ld(r + 8, ks * 16 + c2 + 8);
+          uint32_t f[4];
+          ldsm4(f, smem_u32(sq) + ((lane & 7) + 8 * (lane >> 4)) * L::kQRow + (2 * ks + ((lane >> 3) & 1)) * 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qf[ks][e] = f[e];
+        } else if ((ks & 1) == 0) {  // two steps at once
+          uint32_t f[4];
+          ldsm4(f, smem_u32(sq) + (lane & 7) * L::kQRow + (2 * ks + (lane >> 3)) * 16);
+          qf[ks][0] = f[0];
+          qf[ks][1] = f[1];
+          qf[ks + 1][0] = f[2];
+          qf[ks + 1][1] = f[3];
         }
       }
+      consumer_bar_sync(kWarps * 32);  // the buffer is the join's again
     }
     // with ROWS == 8, rows 8-15 repeat rows 0-7: their scores are the same numbers
     constexpr int Q1 = ROWS == 16 ? 2 : 0, Q3 = ROWS == 16 ? 3 : 1, R = ROWS / 8;
@@ -441,7 +477,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
     if (t0 == 0 && !whole) {  // a split unit begins here (it is the range's last segment)
       split_unit = w.s * units + w.u;
       split_slot = slot;
-      split_parts = cta_of(w.first + w.nt - 1, total, ctas) - cta + 1;
+      split_parts = deal.cta_of(w.first + w.nt - 1) - cta + 1;
     }
     w.at += t1 - t0;
     next = w.at < w.end;
@@ -457,12 +493,12 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
   }
 }
 
-// Joins the parts of the split unit that began in CTA blockIdx.x, row
-// blockIdx.y: eight warps take every eighth part, each lane HD / 32 values.
+// Joins the parts of the split unit that began in CTA blockIdx.x, row blockIdx.y: all maxima and sums
+// first, so that the outputs (a warp takes every eighth part) are independent loads.
 template <class O, int HD, int ROWS>
 __global__ void __launch_bounds__(256) attention_paged_join_kernel(const PagedArgs a, int n_kv, int zs) {
   constexpr int E = HD / 32;
-  __shared__ float s_o[8][HD], s_m[8], s_l[8];
+  __shared__ float s_o[8][HD], s_f[kMaxCtas], s_red[8], s_sum[8];
   pdl_trigger();
   pdl_wait();
   const float* slots = static_cast<const float*>(a.workspace);
@@ -470,40 +506,61 @@ __global__ void __launch_bounds__(256) attention_paged_join_kernel(const PagedAr
   const int c = blockIdx.x, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4 raw = __ldcg(reinterpret_cast<const int4*>(splits + c));
   if (raw.x < 0) return;
-  const int g = a.n_heads / n_kv, units = n_kv * zs, s = raw.x / units, u = raw.x % units;
+  const int g = a.n_heads / n_kv, units = n_kv * zs, s = raw.x / units, u = raw.x % units, n = raw.y;
   const int h0 = (u % zs) * 16;
   if (row >= g - h0) return;
-  float m = -INFINITY, l = 0.0f, o[E] = {};
-#pragma unroll 4
-  for (int p = warp; p < raw.y; p += 8) {
-    const float* b = slots + (size_t)(p ? 2 * (c + p) : raw.z) * slot_floats(ROWS, HD);
-    const float pm = __ldcg(b + ROWS * HD + row), pl = __ldcg(b + ROWS * HD + ROWS + row);
-    float v[E];
+  auto part = [&](int p) { return slots + (size_t)(p ? 2 * (c + p) : raw.z) * slot_floats(ROWS, HD); };
+  // weights 2^(m_p - max) of the parts (at most two a thread) and the weighted sum
+  float pm[2] = {-INFINITY, -INFINITY}, pl[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = __ldcg(b + row * HD + lane + 32 * e);
-    const float mn = fmaxf(m, pm), mz = mn == -INFINITY ? 0.0f : mn, f0 = ex2(m - mz), f1 = ex2(pm - mz);
-    m = mn;
-    l = l * f0 + pl * f1;
+  for (int e = 0; e < 2; ++e) {
+    const int p = threadIdx.x + 256 * e;
+    if (p < n) {
+      pm[e] = __ldcg(part(p) + ROWS * HD + row);
+      pl[e] = __ldcg(part(p) + ROWS * HD + ROWS + row);
+    }
+  }
+  float m = fmaxf(pm[0], pm[1]);
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * f0 + v[e] * f1;
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+  if (lane == 0) s_red[warp] = m;
+  __syncthreads();
+  m = s_red[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = fmaxf(m, s_red[i]);
+  const float mz = m == -INFINITY ? 0.0f : m;
+  float sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int p = threadIdx.x + 256 * e;
+    if (p < n) {
+      const float f = ex2(pm[e] - mz);
+      s_f[p] = f;
+      sum += f * pl[e];
+    }
+  }
+  sum = warp_sum(sum);
+  if (lane == 0) s_sum[warp] = sum;
+  __syncthreads();
+  float o[E] = {};
+#pragma unroll 8
+  for (int p = warp; p < n; p += 8) {
+    const float* b = part(p) + row * HD + lane;
+    const float f = s_f[p];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = fmaf(f, __ldcg(b + 32 * e), o[e]);
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) s_o[warp][lane + 32 * e] = o[e];
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
-  }
   __syncthreads();
   const int d = threadIdx.x;
   if (d >= HD) return;
-  m = s_m[0];
-  for (int i = 1; i < 8; ++i) m = fmaxf(m, s_m[i]);
-  const float mz = m == -INFINITY ? 0.0f : m;
-  float sum = 0.0f, v = 0.0f;
+  float v = 0.0f;
+  sum = 0.0f;
+#pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float f = ex2(s_m[i] - mz);
-    sum += f * s_l[i];
-    v += f * s_o[i][d];
+    v += s_o[i][d];
+    sum += s_sum[i];
   }
   v *= sum == 0.0f ? 0.0f : 1.0f / sum;
   O* out = static_cast<O*>(a.out) + ((long long)s * a.n_heads + (u / zs) * g + h0 + row) * HD;
