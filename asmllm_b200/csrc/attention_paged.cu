@@ -493,8 +493,9 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
   }
 }
 
-// Joins the parts of the split unit that began in CTA blockIdx.x, row blockIdx.y: all maxima and sums
-// first, so that the outputs (a warp takes every eighth part) are independent loads.
+// Joins the parts of the split unit that began in CTA blockIdx.x.  Up to four parts (ordinary batches have two
+// or three): block y = 0 takes all rows, a warp each.  More (a few long sequences): block y takes row y, its
+// warps every eighth part, all maxima and sums first so that the outputs are independent loads.
 template <class O, int HD, int ROWS>
 __global__ void __launch_bounds__(256) attention_paged_join_kernel(const PagedArgs a, int n_kv, int zs) {
   constexpr int E = HD / 32;
@@ -508,8 +509,39 @@ __global__ void __launch_bounds__(256) attention_paged_join_kernel(const PagedAr
   if (raw.x < 0) return;
   const int g = a.n_heads / n_kv, units = n_kv * zs, s = raw.x / units, u = raw.x % units, n = raw.y;
   const int h0 = (u % zs) * 16;
-  if (row >= g - h0) return;
   auto part = [&](int p) { return slots + (size_t)(p ? 2 * (c + p) : raw.z) * slot_floats(ROWS, HD); };
+  if (n <= 4) {
+    if (blockIdx.y) return;
+    for (int r = warp; r < min(16, g - h0); r += 8) {
+      const float pm = lane < n ? __ldcg(part(lane) + ROWS * HD + r) : -INFINITY;
+      const float pl = lane < n ? __ldcg(part(lane) + ROWS * HD + ROWS + r) : 0.0f;
+      float m = pm;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+      const float f = ex2(pm - (m == -INFINITY ? 0.0f : m)), sum = warp_sum(f * pl);
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      float o[E] = {};
+#pragma unroll 4
+      for (int p = 0; p < n; ++p) {
+        const float w = __shfl_sync(kFull, f, p);
+        const float* b = part(p) + r * HD + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(b + e));
+          o[e] = fmaf(w, v.x, o[e]);
+          o[e + 1] = fmaf(w, v.y, o[e + 1]);
+        }
+      }
+      O* out = static_cast<O*>(a.out) + ((long long)s * a.n_heads + (u / zs) * g + h0 + r) * HD + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        if constexpr (sizeof(O) == 4) *reinterpret_cast<float2*>(out + e) = make_float2(o[e] * inv, o[e + 1] * inv);
+        else *reinterpret_cast<uint32_t*>(out + e) = pack16<O>(o[e] * inv, o[e + 1] * inv);
+      }
+    }
+    return;
+  }
+  if (row >= g - h0) return;
   // weights 2^(m_p - max) of the parts (at most two a thread) and the weighted sum
   float pm[2] = {-INFINITY, -INFINITY}, pl[2] = {0.0f, 0.0f};
 #pragma unroll

@@ -69,8 +69,8 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const RopeAppendArgs a
     float v[8];
     load8(src + h * hd + c, v);
     if (h < nq + nk) {
-      const float4 r0 = __ldg(reinterpret_cast<const float4*>(cs + c));
-      const float4 r1 = __ldg(reinterpret_cast<const float4*>(cs + c) + 1);
+      const float4 r0 = __ldcg(reinterpret_cast<const float4*>(cs + c));
+      const float4 r1 = __ldcg(reinterpret_cast<const float4*>(cs + c) + 1);
       const float f[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
 #pragma unroll
       for (int j = 0; j < 8; j += 2) {
