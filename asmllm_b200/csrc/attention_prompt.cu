@@ -306,7 +306,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       auto load = [&](int s, int* q, int* b) -> int {  // query rows, position of the first, its row
         int qb, qe;
         bool clipped;
-        q_range(a.cu_q, s, a.rows, &qb, &qe);
+        any_clipped |= !q_range(a.cu_q, s, a.rows, &qb, &qe);
         const int n = kv_length(kv, s, &clipped);
         any_clipped |= clipped;
         *q = qe - qb;

@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const RopeAppendArgs a
     long long off = -1;
     if (seq < kv.batch) {
       int b, e;
-      q_range(a.cu_q, seq, a.rows, &b, &e);
+      if (!q_range(a.cu_q, seq, a.rows, &b, &e)) atomicOr(err, kErrDecodeRange);
       if (t >= b && t < e) {
         pos = max(-1, __ldcg(kv.len + seq) - (e - b) + (t - b));
         if (pos >= 0) {  // outside the rotary table, the sequence's pages or the pool: skipped

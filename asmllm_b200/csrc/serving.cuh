@@ -183,18 +183,19 @@ __device__ __forceinline__ int kv_length(const KvArgs& kv, int s, bool* clipped)
   return *clipped ? 0 : e - b;
 }
 
-// Rows [begin, end) of sequence s in a packed query of `rows` rows (an
-// offset outside it gives an empty sequence).
-__device__ __forceinline__ void q_range(const int32_t* cu_q, int s, int rows, int* begin, int* end) {
+// Rows [begin, end) of sequence s in a packed query of `rows` rows; false
+// for offsets outside it, which give an empty sequence.
+__device__ __forceinline__ bool q_range(const int32_t* cu_q, int s, int rows, int* begin, int* end) {
   if (!cu_q) {
     *begin = s;
     *end = s + 1;
-    return;
+    return true;
   }
   const int b = __ldcg(cu_q + s), e = __ldcg(cu_q + s + 1);
   const bool ok = b >= 0 && e <= rows && b <= e;
   *begin = ok ? b : 0;
   *end = ok ? e : 0;
+  return ok;
 }
 
 // Element offset of position p of sequence s, head 0; negative when the page

@@ -712,6 +712,8 @@ def rope_append(qkv, rope_cs, kv_len, page_table, k_pages, v_pages, n_heads: int
         _check_dev(q_out, (dt,), "q_out")
         if q_out.shape != (T, n_heads, hd):
             raise ValueError(f"q_out {tuple(q_out.shape)}: expected {(T, n_heads, hd)}")
+    if T == 0 or batch == 0:
+        return q_out
     _call((native._lib or native.lib()).asm_rope_append_async(
         qkv.data_ptr(), _DT[qkv.dtype], qkv.stride(0) if T > 1 else qkv.shape[1], rope_cs.data_ptr(),
         rope_cs.shape[0], None if cu_q is None else cu_q.data_ptr(), T, n_heads, q_out.data_ptr(), kv,
@@ -736,6 +738,8 @@ def attention_prompt(q, k, v, cu_q, *, cu_k=None, kv_len=None, page_table=None, 
     _vector(cu_q, "cu_q", batch + 1, device)
     st, out = _query(q, k, out, out_dtype, stream)
     T, nh, hd = q.shape
+    if T == 0 or batch == 0:
+        return out
     _call((native._lib or native.lib()).asm_attention_prompt_async(
         q.data_ptr(), st[0], st[1], cu_q.data_ptr(), T, nh, hd ** -0.5 if scale is None else scale, out.data_ptr(),
         _DT[out.dtype], kv, _current_stream(device) if stream is None else stream.cuda_stream))
@@ -766,8 +770,13 @@ def attention_paged(q, k_pages, v_pages, page_table, kv_len, *, scale: float | N
     if B != batch:
         raise ValueError(f"q has {B} rows for {batch} sequences")
     lib = native._lib or native.lib()
+    if B == 0:
+        return out
     if workspace is None:
-        workspace = _empty(q, (lib.asm_attention_paged_workspace(B, nh, k_pages.shape[2], hd),), _U8, stream)
+        need = lib.asm_attention_paged_workspace(B, nh, k_pages.shape[2], hd)
+        if need < 0:
+            native.check()
+        workspace = _empty(q, (need,), _U8, stream)
     else:
         _check_dev(workspace, (_U8,), "workspace")
     _call(lib.asm_attention_paged_async(

@@ -659,7 +659,7 @@ ASMLLM_API int asm_rows_advance_async(const int64_t* keys, int32_t rows, int32_t
  *   Packed (table NULL): one page (n_pages 1) of page_size rows; sequence s
  *     holds rows cu[s] .. cu[s+1] - 1.
  * Lengths and page numbers live on the device.  A length above
- * table_width*page_size or below 0, packed offsets that are out of range, or a
+ * table_width*page_size or below 0, row offsets that are out of range, or a
  * page number outside [0, n_pages) sets ASM_DEVERR_DECODE_RANGE (see
  * asm_device_error): the length is clipped, the positions of a bad page count
  * as zero keys and values, and nothing is read outside the pool. */

@@ -511,6 +511,141 @@ def test_attention_prompt_bad_offsets_and_pages_are_reported(cuda):
     assert torch.equal(got[30:], good[30:]) and torch.isfinite(got).all()
 
 
+def test_attention_prompt_many_sequences_few_items(cuda):
+    # 100 sequences on one head, most without new rows: dealt out by key tiles over more than one warp of sequences
+    torch = cuda
+    rng = np.random.default_rng(3)
+    B, hd, page = 100, 128, 64
+    q_len = np.where(rng.random(B) < 0.2, rng.integers(1, 6, B), 0)
+    q_len[70] = 200
+    kv_len = np.maximum(q_len, rng.integers(0, 2500, B))
+    T = int(q_len.sum())
+    k = [rand(torch, int(n), 1, hd, dt=torch.float16, seed=100 + i) for i, n in enumerate(kv_len)]
+    v = [rand(torch, int(n), 1, hd, dt=torch.float16, seed=300 + i) for i, n in enumerate(kv_len)]
+    kp, vp, table = make_pages(torch, k, v, page)
+    q = rand(torch, T, 1, hd, dt=torch.float16, seed=1, scale=2.0)
+    cu_h = np.concatenate([[0], np.cumsum(q_len)])
+    got = ops.attention_prompt(q, kp, vp, torch.tensor(cu_h, dtype=torch.int32, device="cuda"), page_table=table,
+                               kv_len=torch.tensor(kv_len, dtype=torch.int32, device="cuda"))
+    for s in range(B):
+        a, b, n = int(cu_h[s]), int(cu_h[s + 1]), int(kv_len[s])
+        if b > a:
+            want, pv, serr = exact_attention(torch, q[a:b], k[s], v[s], hd ** -0.5, n - (b - a))
+            close(torch, got[a:b], want, pv, serr, n, prompt_weight(torch, torch.float16, n), torch.float16, f"{s}")
+
+
+def test_attention_paged_many_sequences(cuda):
+    # more sequences than a CTA has threads, many of them without positions
+    torch = cuda
+    rng = np.random.default_rng(4)
+    B, nh, nkv, hd, page = 700, 2, 1, 64, 16
+    lens = np.where(rng.random(B) < 0.3, 0, rng.integers(1, 90, B))
+    lens[650] = 3000
+    k = [rand(torch, int(n), nkv, hd, dt=torch.bfloat16, seed=i) for i, n in enumerate(lens)]
+    kp, vp, table = make_pages(torch, k, k, page)
+    q = rand(torch, B, nh, hd, dt=torch.bfloat16, seed=9)
+    got = ops.attention_paged(q, kp, vp, table, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    for s in list(range(0, B, 13)) + [650]:
+        n = int(lens[s])
+        want, pv, serr = exact_attention(torch, q[s:s + 1], k[s], k[s], hd ** -0.5, n - 1)
+        close(torch, got[s:s + 1], want, pv, serr, max(1, n), paged_weight(torch, torch.bfloat16, n), torch.bfloat16,
+              f"{s}")
+
+
+def test_calls_without_rows(cuda):
+    torch = cuda
+    kp = torch.zeros(2, 16, 1, 128, dtype=torch.float16, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    table = torch.zeros(0, 3, dtype=torch.int32, device="cuda")
+    q = torch.zeros(0, 4, 128, dtype=torch.float16, device="cuda")
+    assert ops.attention_paged(q, kp, kp, table, none).shape == (0, 4, 128)
+    cu = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert ops.attention_prompt(q, kp, kp, cu, kv_len=none, page_table=table).shape == (0, 4, 128)
+    rope = torch.from_numpy(D.rope_table(8, 128, 10000.0)).cuda()
+    x = torch.zeros(0, 6 * 128, device="cuda")
+    assert ops.rope_append(x, rope, none, table, kp, kp, 4).shape == (0, 4, 128)
+    logits = torch.zeros(0, 50, device="cuda")
+    assert ops.rows_sample(logits, torch.zeros(0, device="cuda")).shape == (0,)
+    two = torch.zeros(3, dtype=torch.int32, device="cuda")  # two sequences, none with a row
+    out = torch.full((5, 4, 128), 3.0, dtype=torch.float16, device="cuda")
+    rows = torch.zeros(5, 4, 128, dtype=torch.float16, device="cuda")
+    ops.attention_prompt(rows, kp[0], kp[0], two, out=out)
+    assert (out == 3.0).all()
+
+
+def test_refusals_of_the_python_layer(cuda):
+    torch = cuda
+    h = lambda *s, dt=torch.float16: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    kp, vp, table, n = h(4, 16, 2, 128), h(4, 16, 2, 128), i32(3, 2), i32(3)
+    q, cu = h(3, 4, 128), i32(4)
+    rope = torch.from_numpy(D.rope_table(8, 128, 10000.0)).cuda()
+    x = torch.zeros(3, 8 * 128, device="cuda")
+    sample = lambda **kw: ops.rows_sample(torch.zeros(3, 50, device="cuda"), torch.zeros(3, device="cuda"), **kw)  # noqa: E731
+    for error, call in [
+        (TypeError, lambda: ops.attention_paged(q.float(), kp, vp, table, n)),
+        (ValueError, lambda: ops.attention_paged(q.bfloat16(), kp, vp, table, n)),
+        (ValueError, lambda: ops.attention_paged(h(3, 5, 128), kp, vp, table, n)),          # 5 heads on 2
+        (ValueError, lambda: ops.attention_paged(h(2, 4, 128), kp, vp, table, n)),          # 2 rows, 3 sequences
+        (ValueError, lambda: ops.attention_paged(h(3, 4, 64), kp, vp, table, n)),
+        (ValueError, lambda: ops.attention_paged(q, kp, vp[:, :, :1], table, n)),
+        (ValueError, lambda: ops.attention_paged(q, kp, vp.transpose(1, 2).contiguous().transpose(1, 2), table, n)),
+        (TypeError, lambda: ops.attention_paged(q, kp, vp, table.long(), n)),
+        (TypeError, lambda: ops.attention_paged(q, kp, vp, table, n.long())),
+        (ValueError, lambda: ops.attention_paged(q, kp, vp, table, i32(2))),
+        (ValueError, lambda: ops.attention_paged(q, kp, vp, None, n)),
+        (ValueError, lambda: ops.attention_paged(q, kp, vp, i32(2, 3).T, n)),
+        (TypeError, lambda: ops.attention_paged(q, kp, vp, table, n, out_dtype=torch.bfloat16)),
+        (ValueError, lambda: ops.attention_paged(q, kp, vp, table, n, out=h(3, 4, 64))),
+        (ops.AsmError, lambda: ops.attention_paged(q, kp, vp, table, n, scale=0.0)),
+        (ops.AsmError, lambda: ops.attention_paged(q, kp, vp, table, n, scale=float("nan"))),
+        (ops.AsmError, lambda: ops.attention_paged(q, kp, vp, table, n, workspace=h(16, dt=torch.uint8))),
+        (ops.AsmError, lambda: ops.attention_paged(q, h(4, 24, 2, 128), h(4, 24, 2, 128), table, n)),
+        (ops.AsmError, lambda: ops.attention_paged(h(3, 4, 96), h(4, 16, 2, 96), h(4, 16, 2, 96), table, n)),
+        (ops.AsmError, lambda: ops.attention_paged(q[:, :1].expand(3, 4, 128), kp, vp, table, n)),
+        (ops.AsmError, lambda: ops.attention_paged(h(3, 4, 132)[..., 4:], kp, vp, table, n)),  # rows of 264 bytes
+        (ValueError, lambda: ops.attention_prompt(q, kp, vp, cu, kv_len=n)),
+        (ValueError, lambda: ops.attention_prompt(q, kp, vp, cu, page_table=table)),
+        (ValueError, lambda: ops.attention_prompt(q, kp, vp, cu, kv_len=n, page_table=table, cu_k=cu)),
+        (ValueError, lambda: ops.attention_prompt(q, kp, vp, i32(3), kv_len=n, page_table=table)),
+        (ValueError, lambda: ops.attention_prompt(q, kp, vp, cu)),                           # four axes, packed
+        (ops.AsmError, lambda: ops.attention_prompt(q, h(5, 2, 128), h(5, 2, 128), cu, scale=-1.0)),
+        (ValueError, lambda: ops.rope_append(x[:, :-128], rope, n, table, kp, vp, 4)),
+        (ValueError, lambda: ops.rope_append(x, rope[:, :32], n, table, kp, vp, 4)),
+        (ValueError, lambda: ops.rope_append(x[:2], rope, n, table, kp, vp, 4)),
+        (TypeError, lambda: ops.rope_append(x.bfloat16(), rope, n, table, kp, vp, 4)),
+        (ValueError, lambda: ops.rope_append(x, rope, n, table, kp, vp, 4, cu_q=i32(3))),
+        (ValueError, lambda: ops.rope_append(x, rope, n, table, kp, vp, 4, q_out=h(3, 5, 128))),
+        (TypeError, lambda: sample(temperature=torch.ones(3))),
+        (ValueError, lambda: sample(top_p=torch.ones(2, device="cuda"))),
+        (TypeError, lambda: sample(top_k=torch.ones(3, device="cuda"))),
+        (TypeError, lambda: ops.rows_sample(torch.zeros(3, 50, device="cuda").double(), torch.zeros(3, device="cuda"))),
+        (ops.AsmError, lambda: ops.rows_sample(h(1, 262145), torch.zeros(1, device="cuda"))),
+    ]:
+        with pytest.raises(error):
+            call()
+
+
+def test_two_streams_at_once(cuda):
+    torch = cuda
+    nh, nkv, hd, lens = 16, 2, 128, [3000, 17, 900]
+    k = [rand(torch, n, nkv, hd, dt=torch.bfloat16, seed=i) for i, n in enumerate(lens)]
+    kp, vp, table = make_pages(torch, k, k, 32)
+    kv = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = rand(torch, 3, nh, hd, dt=torch.bfloat16, seed=7)
+    cu = torch.arange(4, dtype=torch.int32, device="cuda")
+    logits, u = rand(torch, 3, 32000, dt=torch.float32, seed=8), torch.rand(3, device="cuda")
+    call = lambda st=None: (ops.attention_paged(q, kp, vp, table, kv, stream=st),  # noqa: E731
+                            ops.attention_prompt(q, kp, vp, cu, kv_len=kv, page_table=table, stream=st),
+                            ops.rows_sample(logits, u, stream=st))
+    want = call()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [call(streams[i % 2]) for i in range(20)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+
 # ------------------------------------------------------------------ sampling
 def sample_ref(x, u, T, k, p, mp):
     """One row in 64 bits: numpy, the definition word by word."""
