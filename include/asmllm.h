@@ -701,7 +701,9 @@ ASMLLM_API int asm_rope_append_async(const void* qkv, int32_t qkv_dtype, int64_t
  * maxima and sums are fp32; the weights are rounded to the 16-bit type for
  * the product with the values, which costs about as much as one rounding of
  * the output.  What a row does not attend to -- later positions, other
- * sequences, the rest of a page -- does not reach it, whatever it holds. */
+ * sequences, the rest of a page -- does not reach it, whatever it holds.
+ * Where the items may be fewer than the SMs and long, up to 40 MB of
+ * stream-ordered scratch are taken for the call. */
 ASMLLM_API int asm_attention_prompt_async(const void* q, int64_t q_row_stride, int64_t q_head_stride,
                                           const int32_t* cu_q, int32_t rows, int32_t n_heads, float scale, void* out,
                                           int32_t out_dtype, const asm_kv_t* kv, void* stream);
