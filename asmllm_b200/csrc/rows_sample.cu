@@ -276,14 +276,45 @@ struct Slice {
     u64 w = 0;
     if (c <= kList) {
       if (cluster.block_rank() == 0) {
-        for (int i = threadIdx.x; i < c; i += kThreads) sh.mass[i] = MASS ? row.mass(word_value(sh.list[i])) : 1ull;
+        // The bin once more in kThreads parts (comparing each of its words with each took 10 thousand cycles
+        // for 400 words); the words of the part that holds the border are then compared.
+        u64* part = reinterpret_cast<u64*>(sh.hist);  // all CTAs are past the histograms
+        u64* word = part + kThreads;                   // the words of the one part, and their masses
+        u64* weighs = word + kList;
+        static_assert((kThreads + 2 * kList) * sizeof(u64) <= sizeof(sh.hist), "room");
+        part[threadIdx.x] = 0;
+        if (threadIdx.x == 0) sh.found[2] = 0;
         __syncthreads();
+        auto part_of = [&](u64 x) {
+          const float t = (row.vtop - word_value(x)) * row.bin_scale - (float)b;
+          return word_value(x) == row.vtop ? 0 : min(kThreads - 1, max(0, (int)(t * (float)kThreads)));
+        };
         for (int i = threadIdx.x; i < c; i += kThreads) {
-          const u64 x = sh.list[i];
-          u64 s = before;
-          for (int j = 0; j < c; ++j)
-            if (sh.list[j] > x) s += sh.mass[j];
-          if (s < want && s + sh.mass[i] >= want) sh.cut = x;
+          const u64 m = MASS ? row.mass(word_value(sh.list[i])) : 1ull;
+          sh.mass[i] = m;
+          atomicAdd(part + part_of(sh.list[i]), m);
+        }
+        __syncthreads();
+        u64 all;
+        const u64 mine = part[threadIdx.x], run = before + block_scan(mine, sh, &all) - mine;
+        if (run < want && run + mine >= want) {
+          sh.found[0] = threadIdx.x;
+          sh.found[1] = run;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < c; i += kThreads)
+          if (part_of(sh.list[i]) == (int)sh.found[0]) {
+            const int at = (int)atomicAdd(&sh.found[2], 1ull);
+            word[at] = sh.list[i];
+            weighs[at] = sh.mass[i];
+          }
+        __syncthreads();
+        const int few = (int)sh.found[2];
+        for (int i = threadIdx.x; i < few; i += kThreads) {
+          u64 s = sh.found[1];
+          for (int j = 0; j < few; ++j)
+            if (word[j] > word[i]) s += weighs[j];
+          if (s < want && s + weighs[i] >= want) sh.cut = word[i];
         }
       }
       cluster.sync();
