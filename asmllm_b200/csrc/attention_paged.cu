@@ -24,6 +24,13 @@
 // hi + lo 16-bit parts, so it is as good as fp32; a group of up to 8 heads
 // fills rows 0-7 with hi and rows 8-15 with lo, and the product costs nothing
 // extra.
+//
+// Measured on one B200: 64 sequences of up to 16384 positions, 64 query on 8
+// KV heads of 128 values (2.26 GB), 355 us = 6.4 TB/s, 0.99 of the copy rate;
+// 32 sequences of up to 1024 (74 MB) 27.5 us, of which the streaming is 11
+// and the rest the lengths' prologue (2), first bytes and the join.  With one
+// CTA per unit (no split) one sequence of 131071 positions on one KV head
+// took 14 ms; now 25 to 30 us.
 #include "matvec.cuh"
 #include "mma16.cuh"
 #include "pipeline.cuh"

@@ -10,6 +10,10 @@
 // a row at p < 0 (a sequence with more rows than positions) gets a zero query
 // and appends nothing; so does one whose position or page is out of range,
 // which also sets the device error word.
+//
+// Bound by HBM: every input is read and every output written once.  8192 rows
+// of 32 query and 32 + 32 key and value heads of 128 values, fp32 to fp16,
+// take 93 us on one B200 = 6.5 TB/s, the copy rate; 32 rows 3.9 us, a launch.
 #include "matvec.cuh"
 #include "serving.cuh"
 

@@ -27,7 +27,13 @@
 // (m - x) / temperature, a scan over the bins finds the one that holds the
 // border, and only that bin's words are put in order.  A small top_k takes
 // the short way: the bins down to the border hold little more than top_k
-// words, which one CTA finishes alone (three barriers in all).
+// words, which one CTA finishes alone (four barriers in all).
+//
+// Measured on one B200: one row of 32000 words, top_k 40 and top_p 0.95, 8.9
+// us; 128 rows of 128256 words with mixed settings 111 us (the read alone
+// would take 10).  Radix selection straight from global memory, a CTA a row:
+// 835 and 3231 us.  64-bit histogram atomics in place of three 32-bit ones
+// and all CTAs reading all histograms: 39 and 374.
 #include <cooperative_groups.h>
 
 #include "matvec.cuh"

@@ -458,6 +458,26 @@ def test_attention_prompt_later_values_do_not_reach_earlier_rows(cuda, page, wid
     assert same(got[150:400, :2], good[150:400, :2]) and torch.isnan(got[400:, :2]).all()
 
 
+@pytest.mark.parametrize("split", [False, True])
+def test_attention_prompt_later_value_behind_a_long_prefix(cuda, split):
+    # the rows computed again have 20000 keys each, while the CTA's other roles wait
+    torch = cuda
+    nh, hd, page, prefix, n = (1, 128, 64, 20000, 100) if split else (160, 128, 64, 20000, 100)
+    k = rand(torch, prefix + n, 1, hd, dt=torch.float16, seed=2)
+    v = rand(torch, prefix + n, 1, hd, dt=torch.float16, seed=3)
+    v[prefix + 60, 0, 9] = float("nan")
+    kp, vp, table = make_pages(torch, [k], [v], page)
+    q = rand(torch, n, nh, hd, dt=torch.float16, seed=1)
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    kv = torch.tensor([prefix + n], dtype=torch.int32, device="cuda")
+    got = ops.attention_prompt(q, kp, vp, cu, kv_len=kv, page_table=table)
+    v[prefix + 60, 0, 9] = 0.0
+    heads = [0, nh - 1] if nh > 1 else [0]
+    want, pv, serr = exact_attention(torch, q[:60, heads], k, v, hd ** -0.5, prefix)
+    close(torch, got[:60, heads], want, pv, serr, prefix, prompt_weight(torch, torch.float16, prefix), torch.float16)
+    assert torch.isnan(got[60:, :, 9]).all() and torch.isfinite(got[:60]).all()
+
+
 def test_attention_prompt_rows_without_keys_and_strided_inputs(cuda):
     torch = cuda
     nh, nkv, hd = 4, 2, 128
