@@ -670,6 +670,8 @@ def _query(q, k, out, out_dtype, stream):
             raise TypeError(f"out_dtype {dt}: fp32 or q's type")
         return st, _empty(q, shape, dt, stream)
     _check_dev(out, (q.dtype, _F32), "out")
+    if out.data_ptr() == q.data_ptr() and q.numel():
+        raise ValueError("out must not be q: queries are read again after rows have been written")
     if out.shape != shape or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError(f"out: {tuple(out.shape)} {out.dtype}, expected {tuple(shape)} {out_dtype or q.dtype}")
     return st, out

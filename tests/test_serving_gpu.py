@@ -617,6 +617,8 @@ def test_refusals_of_the_python_layer(cuda):
         (ValueError, lambda: ops.attention_paged(q, kp, vp, i32(2, 3).T, n)),
         (TypeError, lambda: ops.attention_paged(q, kp, vp, table, n, out_dtype=torch.bfloat16)),
         (ValueError, lambda: ops.attention_paged(q, kp, vp, table, n, out=h(3, 4, 64))),
+        (ValueError, lambda: ops.attention_paged(q, kp, vp, table, n, out=q)),
+        (ValueError, lambda: ops.attention_prompt(q, kp, vp, cu, kv_len=n, page_table=table, out=q)),
         (ops.AsmError, lambda: ops.attention_paged(q, kp, vp, table, n, scale=0.0)),
         (ops.AsmError, lambda: ops.attention_paged(q, kp, vp, table, n, scale=float("nan"))),
         (ops.AsmError, lambda: ops.attention_paged(q, kp, vp, table, n, workspace=h(16, dt=torch.uint8))),
@@ -648,7 +650,7 @@ def test_refusals_of_the_python_layer(cuda):
 
 def test_two_streams_at_once(cuda):
     torch = cuda
-    nh, nkv, hd, lens = 16, 2, 128, [3000, 17, 900]
+    nh, nkv, hd, lens = 16, 2, 128, [2900, 17, 900]
     k = [rand(torch, n, nkv, hd, dt=torch.bfloat16, seed=i) for i, n in enumerate(lens)]
     kp, vp, table = make_pages(torch, k, k, 32)
     kv = torch.tensor(lens, dtype=torch.int32, device="cuda")
@@ -664,6 +666,18 @@ def test_two_streams_at_once(cuda):
     got = [call(streams[i % 2]) for i in range(20)]
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+    graphs = []  # the prompt's keys are dealt out here: its scratch belongs to each graph
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call()
+        graphs.append((g, out))
+    for _ in range(3):
+        for (g, out), st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for _, out in graphs for a, b in zip(out, want))
 
 
 # ------------------------------------------------------------------ sampling
