@@ -23,14 +23,18 @@
 // with the query heads as rows.  The weights enter the second product as
 // hi + lo 16-bit parts, so it is as good as fp32; a group of up to 8 heads
 // fills rows 0-7 with hi and rows 8-15 with lo, and the product costs nothing
-// extra.
+// extra.  Values that are infinite take another way (add_values): hi and lo
+// differ in sign, so their products with an infinity would add up to NaN.
+// Looking for them costs 1 us of the 28 below, nothing of the 355.
 //
 // Measured on one B200: 64 sequences of up to 16384 positions, 64 query on 8
 // KV heads of 128 values (2.26 GB), 355 us = 6.4 TB/s, 0.99 of the copy rate;
-// 32 sequences of up to 1024 (74 MB) 27.5 us, of which the streaming is 11
+// 32 sequences of up to 1024 (74 MB) 28.9 us, of which the streaming is 11
 // and the rest the lengths' prologue (2), first bytes and the join.  With one
 // CTA per unit (no split) one sequence of 131071 positions on one KV head
 // took 14 ms; now 25 to 30 us.
+#include <type_traits>
+
 #include "matvec.cuh"
 #include "mma16.cuh"
 #include "pipeline.cuh"
@@ -93,6 +97,35 @@ struct Deal {
     return x < big ? (int)(x / (each + 1)) : extra + (int)((x - big) / each);
   }
 };
+
+// o += p v in fp32 for D times 8 values from 8 d0 on and the first n of a warp's 16 positions of a tile (values at sv,
+// from row r0).  Weights that fp32 rounds to zero count as zero: times infinity that is NaN.  Lane: row
+// lane / 4 (and 8 more), values 2 (lane % 4) and the next of each eight; its weights are those of positions
+// 2 (lane % 4), the next, and both of these plus 8.
+template <class T, int HD, int R, int D>
+__device__ __forceinline__ void add_values(float (&o)[HD / 8][4], int d0, const float (&p)[R][4], uint32_t sv,
+                                           int r0, int n, int lane) {
+#pragma unroll 1
+  for (int j = 0; j < n; ++j) {
+    float w[R];
+#pragma unroll
+    for (int e = 0; e < R; ++e) {
+      const float odd = j < 8 ? p[e][1] : p[e][3], even = j < 8 ? p[e][0] : p[e][2];
+      w[e] = __shfl_sync(kFull, j & 1 ? odd : even, (lane & 28) | ((j & 7) >> 1));
+    }
+#pragma unroll
+    for (int d = d0; d < d0 + D; ++d) {
+      uint32_t x;
+      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(sv + tile_chunk<kTile>(r0 + j, d) + (lane & 3) * 4));
+      const float2 v = unpack16<T>(x);
+#pragma unroll
+      for (int e = 0; e < R; ++e) {
+        o[d][2 * e] = fmaf(w[e], v.x, o[d][2 * e]);
+        o[d][2 * e + 1] = fmaf(w[e], v.y, o[d][2 * e + 1]);
+      }
+    }
+  }
+}
 
 // A CTA's walk over its tiles: sequence, unit of the sequence, tile.
 struct Walk {
@@ -347,6 +380,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
           mma16816<T>(sc[1], qf[ks][0], qf[ks][Q1], qf[ks][1], qf[ks][Q3], b[2], b[3]);
         }
         uint32_t hi[4], lo[4];
+        float p[R][4];
 #pragma unroll
         for (int e = 0; e < R; ++e) {
           float x[4];
@@ -373,15 +407,14 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
             }
           }
           const float base = (m[e] == -INFINITY ? 0.0f : m[e]) - kShift;
-          float p[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) p[k] = ex2(x[k] - base);
-          l[e] += (p[0] + p[1]) + (p[2] + p[3]);
+          for (int k = 0; k < 4; ++k) p[e][k] = ex2(x[k] - base);
+          l[e] += (p[e][0] + p[e][1]) + (p[e][2] + p[e][3]);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            hi[2 * k + e] = pack16<T>(p[2 * k], p[2 * k + 1]);
+            hi[2 * k + e] = pack16<T>(p[e][2 * k], p[e][2 * k + 1]);
             const float2 q = unpack16<T>(hi[2 * k + e]);
-            lo[2 * k + e] = pack16<T>(p[2 * k] - q.x, p[2 * k + 1] - q.y);
+            lo[2 * k + e] = pack16<T>(p[e][2 * k] - q.x, p[e][2 * k + 1] - q.y);
           }
         }
         // the values of positions that do not exist are whatever the page or the ring holds: zeros instead
@@ -391,22 +424,38 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
           for (int k = 0; k < 2; ++k)
             keep[k] = (k * 8 + c2 < left ? 0xFFFFu : 0u) | (k * 8 + c2 + 1 < left ? 0xFFFF0000u : 0u);
         }
+        // The two parts of a weight differ in sign or one is zero, so an infinite value would come out as NaN:
+        // 16 N values of each position among which there is one (or a NaN) are summed weight by weight.
+        constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+        constexpr int N = ROWS == 8 ? HD / 16 : 2;  // registers: with 16 rows all at once spill
 #pragma unroll
-        for (int nt = 0; nt < HD / 16; ++nt) {
-          uint32_t b[4];
-          ldsm4_t(b, value_frag<kTile>(sv, r0, nt, lane));
-          b[0] &= keep[0];
-          b[1] &= keep[1];
-          b[2] &= keep[0];
-          b[3] &= keep[1];
-          if constexpr (ROWS == 8) {
-            mma16816<T>(o[2 * nt], hi[0], lo[0], hi[2], lo[2], b[0], b[1]);
-            mma16816<T>(o[2 * nt + 1], hi[0], lo[0], hi[2], lo[2], b[2], b[3]);
-          } else {
-            mma16816<T>(o[2 * nt], hi[0], hi[1], hi[2], hi[3], b[0], b[1]);
-            mma16816<T>(o[2 * nt], lo[0], lo[1], lo[2], lo[3], b[0], b[1]);
-            mma16816<T>(o[2 * nt + 1], hi[0], hi[1], hi[2], hi[3], b[2], b[3]);
-            mma16816<T>(o[2 * nt + 1], lo[0], lo[1], lo[2], lo[3], b[2], b[3]);
+        for (int n0 = 0; n0 < HD / 16; n0 += N) {
+          uint32_t b[N][4], big = 0u;
+#pragma unroll
+          for (int nt = 0; nt < N; ++nt) {
+            ldsm4_t(b[nt], value_frag<kTile>(sv, r0, n0 + nt, lane));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              b[nt][k] &= keep[k & 1];
+              big = __vmaxu2(big, b[nt][k] & 0x7FFF7FFFu);
+            }
+          }
+          if (__any_sync(kFull, (big & 0xFFFFu) >= kInf || (big >> 16) >= kInf)) {
+            add_values<T, HD, R, 2 * N>(o, 2 * n0, p, sv, r0, min(left, 16), lane);
+            continue;
+          }
+#pragma unroll
+          for (int nt = 0; nt < N; ++nt) {
+            float(&o0)[4] = o[2 * (n0 + nt)], (&o1)[4] = o[2 * (n0 + nt) + 1];
+            if constexpr (ROWS == 8) {
+              mma16816<T>(o0, hi[0], lo[0], hi[2], lo[2], b[nt][0], b[nt][1]);
+              mma16816<T>(o1, hi[0], lo[0], hi[2], lo[2], b[nt][2], b[nt][3]);
+            } else {
+              mma16816<T>(o0, hi[0], hi[1], hi[2], hi[3], b[nt][0], b[nt][1]);
+              mma16816<T>(o0, lo[0], lo[1], lo[2], lo[3], b[nt][0], b[nt][1]);
+              mma16816<T>(o1, hi[0], hi[1], hi[2], hi[3], b[nt][2], b[nt][3]);
+              mma16816<T>(o1, lo[0], lo[1], lo[2], lo[3], b[nt][2], b[nt][3]);
+            }
           }
         }
       }

@@ -284,6 +284,55 @@ def test_attention_nonfinite_inputs_of_attended_positions_show(cuda):
     assert torch.isfinite(got).all()           # ... unless it is behind the sequence's end
 
 
+def with_nonfinite(v, where):
+    """v with values set: {(position, head, column): value}."""
+    v = v.clone()
+    for at, x in where.items():
+        v[at] = x
+    return v
+
+
+def check_nonfinite(torch, got, q, k, v, scale, first, weight, dt, what):
+    """got [n, nh, hd] against the definition where v holds infinities and NaN: a column whose attended values
+    hold a NaN or infinities of both signs is NaN, one with an infinity is that infinity, the others are as ever."""
+    n, nh, _ = got.shape
+    m, g = k.shape[0], nh // k.shape[1]
+    want, pv, serr = exact_attention(torch, q, k, torch.nan_to_num(v, nan=0.0, posinf=0.0, neginf=0.0), scale, first)
+    keep = (torch.arange(m, device="cuda")[None] <= (first + torch.arange(n, device="cuda"))[:, None]).double()
+    seen = lambda x: torch.einsum("nm,mhd->nhd", keep, x.double()).repeat_interleave(g, 1) > 0  # noqa: E731
+    plus, minus, nan = seen(v == math.inf), seen(v == -math.inf), seen(v != v)
+    nan |= plus & minus
+    assert torch.isnan(got[nan]).all(), what
+    assert (got[plus & ~nan] == math.inf).all() and (got[minus & ~nan] == -math.inf).all(), what
+    rest = ~(plus | minus | nan)
+    close(torch, torch.where(rest, got, 0), torch.where(rest, want, 0), pv, serr, max(1, m), weight, dt, what)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("out", ["same", "float32"])
+@pytest.mark.parametrize("nh,nkv,hd,page", [(4, 4, 128, 16), (16, 2, 64, 64), (32, 2, 128, 32), (9, 1, 64, 16)])
+def test_attention_paged_infinite_values(cuda, dtype, out, nh, nkv, hd, page):
+    # an attended infinity comes out as itself whatever its weight's low part is
+    torch = cuda
+    dt = getattr(torch, dtype)
+    inf, nan = math.inf, math.nan
+    lens = [1, 40, 700, 33, 6000]  # whole units, and one whose positions are dealt out
+    k = [rand(torch, n, nkv, hd, dt=dt, seed=i) for i, n in enumerate(lens)]
+    v = [rand(torch, n, nkv, hd, dt=dt, seed=20 + i) for i, n in enumerate(lens)]
+    v[0] = with_nonfinite(v[0], {(0, 0, 0): inf, (0, nkv - 1, 3): -inf})
+    v[1] = with_nonfinite(v[1], {(i, 0, i): inf for i in range(40)})  # a weight each
+    v[2] = with_nonfinite(v[2], {(i, nkv - 1, i % 60): -inf for i in range(5, 700, 12)})
+    v[3] = with_nonfinite(v[3], {(32, 0, 1): inf, (3, 0, 1): -inf, (9, 0, 2): nan, (9, 0, 8): inf, (31, 0, 2): inf})
+    v[4] = with_nonfinite(v[4], {(p, nkv - 1, hd - 1 - i): inf for i, p in enumerate(range(0, 6000, 599))})
+    kp, vp, table = make_pages(torch, k, v, page)
+    q = rand(torch, len(lens), nh, hd, dt=dt, seed=99, scale=2.0)
+    kv = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    got = ops.attention_paged(q, kp, vp, table, kv, out_dtype=dt if out == "same" else torch.float32)
+    for i, n in enumerate(lens):
+        check_nonfinite(torch, got[i:i + 1], q[i:i + 1], k[i], v[i], hd ** -0.5, n - 1, paged_weight(torch, dt, n), dt,
+                        f"sequence {i} of {n}")
+
+
 def test_attention_paged_bad_pages_and_lengths_are_reported(cuda):
     torch = cuda
     k = [rand(torch, 64, 2, 128, dt=torch.float16, seed=i) for i in range(3)]
