@@ -431,6 +431,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_sample_kernel(const SampleAr
     return;
   }
   const float vtop = word_value(best);
+  const int top = word_index(best);  // the first word, which always stays
   Slice s{sh, s_val, n, first, cluster, ranks, Row{vtop, kBinsPerUnit / temp, 1.4426950408889634 / (double)temp, sh.pow2}};
   const double least = (double)mp;
   u64 total;
@@ -527,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_sample_kernel(const SampleAr
     const float v = s_val[i];
     if (!s.keep(v, i) || s.row.bin(v) == kBins - 1) return 0ull;
     const double w = s.row.weight(v);
-    return v == vtop || !(least > 0.0) || w >= least ? Row::fixed(w) : 0ull;
+    return first + i == top || !(least > 0.0) || w >= least ? Row::fixed(w) : 0ull;
   };
   u64 mine = 0;
 #pragma unroll 2

@@ -835,6 +835,25 @@ def test_rows_sample_ties_masks_and_infinities(cuda):
     assert got.tolist() == want
 
 
+@pytest.mark.parametrize("V", [300, 5000, 40000])  # one CTA a row, two, eight
+def test_rows_sample_min_p_above_one_keeps_the_first_word_alone(cuda, V):
+    # equal maxima: no weight reaches min_p, the first word stays, with and without top_k and top_p
+    torch = cuda
+    x = np.full(V, -2.0, np.float32)
+    ties = [V // 5, V // 3, V - 1]
+    x[ties] = 1.5
+    settings = [(k, p, mp) for k in (0, 2, 40, V - 1) for p in (1.0, 0.9, 0.0) for mp in (1.0, 1.5, math.inf)]
+    B = len(settings)
+    u = np.full(B, 0.999, np.float32)
+    got = ops.rows_sample(torch.from_numpy(np.tile(x, (B, 1))).cuda(), torch.from_numpy(u).cuda(),
+                          top_k=torch.tensor([s[0] for s in settings], dtype=torch.int32, device="cuda"),
+                          top_p=torch.tensor([s[1] for s in settings], device="cuda"),
+                          min_p=torch.tensor([s[2] for s in settings], device="cuda"))
+    want = [sample_ref(x.copy(), u[r], 1.0, k, f32(p), f32(mp)) for r, (k, p, mp) in enumerate(settings)]
+    assert got.tolist() == want
+    assert all(t == ties[0] for t, (_, _, mp) in zip(want, settings) if mp > 1.0)
+
+
 def test_rows_sample_greedy_is_rows_argmax_and_defaults(cuda):
     torch = cuda
     x = rand(torch, 9, 32000, dt=torch.float32, seed=4).mul_(4).round_()  # many equal maxima
