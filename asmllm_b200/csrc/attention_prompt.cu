@@ -57,10 +57,11 @@ constexpr int kThreads = 384;
 // 96 of 2048 36 / 33; the other way round 128 of 2048 37 / 39, 64 of 1024 22 / 26, 256 of 4096 63 / 97.
 constexpr int kSplitTiles = 16;
 
-// A row whose output is not finite, computed again key by key by one warp:
-// in a matrix product a later position's infinite or NaN value meets the
-// row's zero weight and turns its output to NaN, although the row does not
-// attend to that position.  Lane l holds values l, l + 32, ...; those from
+// A row whose output is not finite, computed again in fp32 key by key by one
+// warp: in a matrix product a later position's infinite or NaN value meets
+// the row's zero weight and turns its output to NaN, although the row does
+// not attend to that position; so does an infinity that it attends to with a
+// weight below the 16-bit type's smallest.  Lane l holds values l, l + 32, ...; those from
 // 32 e0 to 32 e1 are written.
 template <class T, class O, int HD>
 __device__ __forceinline__ void attend_row(const PromptArgs& a, const KvArgs& kv, int t, int h, int s, int last, int lane,
@@ -168,25 +169,51 @@ __device__ __forceinline__ int cta_of(long long x, long long total, int ctas) { 
   return (int)(((x + 1) * ctas - 1) / total);
 }
 
-// Rows `todo` of a warp's 32 (lane by lane) are not finite: computed again if that may be a later position's doing.
+// Whether values [32 e0, 32 e1) of positions [p, stop) hold an infinity, or (NAN_TOO) a NaN.  A position per lane.
+template <class T, bool NAN_TOO>
+__device__ __forceinline__ bool any_nonfinite(const KvArgs& kv, int s, long long ho, int p, int stop, int lane, int e0,
+                                              int e1) {
+#pragma unroll 1
+  for (; p < stop; p += 32) {
+    const long long off = p + lane < stop ? kv_offset(kv, s, p + lane) : -1;
+    bool found = false;
+    if (off >= 0) {
+#pragma unroll 4
+      for (int c = 32 * e0; c < 32 * e1; c += 8) {
+        float v[8];
+        load8(static_cast<const T*>(kv.v) + off + ho + c, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) found |= NAN_TOO ? !(fabsf(v[e]) < INFINITY) : fabsf(v[e]) == INFINITY;
+      }
+    }
+    if (__any_sync(kFull, found)) return true;
+  }
+  return false;
+}
+
+// Rows `todo` of a warp's 32 (lane by lane) are not finite although their weights are: computed again if that may be
+// the doing of a later position's value, or of an infinity whose weight a rounding made zero (NaN in place of it).
 template <class T, class O, int HD>
 __device__ __forceinline__ void mend_rows(const PromptArgs& a, const KvArgs& kv, const Item& it, int i, int pair, int tiles,
                                        int lrow, unsigned todo, int lane, int e0, int e1) {
   const int row = lrow + (pair ? 0 : i * kRows), head = it.head + (pair ? i : 0);
-  const int first = __shfl_sync(kFull, it.base + row, __ffs(todo) - 1) + 1, last = min(it.n, tiles * kRows);
+  const int first = max(0, __shfl_sync(kFull, it.base + row, __ffs(todo) - 1) + 1), last = min(it.n, tiles * kRows);
   const long long ho = (long long)(head / (a.n_heads / kv.n_kv)) * kv.head_stride;
-  bool later = false;
-#pragma unroll 1
-  for (int p = max(0, first); p < last; ++p) {
-    const long long o = kv_offset(kv, it.s, p);
-    if (o < 0) continue;
-    for (int e = lane + 32 * e0; e < 32 * e1; e += 32) later |= !(fabsf(to_f32(static_cast<const T*>(kv.v)[o + ho + e])) < INFINITY);
-  }
-  if (!__any_sync(kFull, later)) return;
+  const bool later = any_nonfinite<T, true>(kv, it.s, ho, first, last, lane, e0, e1);
+  if (!later && !any_nonfinite<T, false>(kv, it.s, ho, 0, min(first, it.n), lane, e0, e1)) return;
   __syncwarp();  // the rows' first stores come before the second ones
   while (todo) {
     const int rr = __shfl_sync(kFull, row, __ffs(todo) - 1);
     todo &= todo - 1;
+    if (!later) {  // an infinity that came through is right
+      const O* out = static_cast<const O*>(a.out) + ((long long)(it.t0 + rr) * a.n_heads + head) * HD + lane;
+      bool nan = false;
+      for (int e = e0; e < e1; ++e) {
+        const float v = to_f32(out[32 * e]);
+        nan |= v != v;
+      }
+      if (!__any_sync(kFull, nan)) continue;
+    }
     attend_row<T, O, HD>(a, kv, it.t0 + rr, head, it.s, min(it.base + rr, it.n - 1), lane, e0, e1);
   }
 }
@@ -884,8 +911,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(o_empty + i));
-      // Rows that are not finite: because of a later position's value?
-      const unsigned todo = __ballot_sync(kFull, bad && mine);
+      // Rows that are not finite: because of the values? (a NaN among the scores shows in the sum)
+      const unsigned todo = __ballot_sync(kFull, bad && mine && l == l);
       if (todo) {
         if (lane == 0) atomicAdd(s_mending, 1u);
         mend_rows<T, O, HD>(a, kv, it, i, pair, tiles, lrow, todo, lane, 0, HD / 32);
@@ -949,7 +976,7 @@ __global__ void __launch_bounds__(256) attention_prompt_join_kernel(const Prompt
   }
   // a row that is bad in either half is mended by the first (32 values from 32 z on)
   __shared__ unsigned s_bad[8];
-  const unsigned vote = __ballot_sync(kFull, bad && mine);
+  const unsigned vote = __ballot_sync(kFull, bad && mine && l == l);
   if ((threadIdx.x & 31) == 0) s_bad[threadIdx.x >> 5] = vote;
   __syncthreads();
   const int warp = threadIdx.x >> 5;

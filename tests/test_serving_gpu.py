@@ -507,6 +507,41 @@ def test_attention_prompt_later_values_do_not_reach_earlier_rows(cuda, page, wid
     assert same(got[150:400, :2], good[150:400, :2]) and torch.isnan(got[400:, :2]).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("out", ["same", "float32"])
+@pytest.mark.parametrize("nh,nkv,hd,page,width", [(4, 2, 128, 0, 0), (3, 1, 64, 16, 0), (2, 2, 128, 32, 300)])
+def test_attention_prompt_infinite_values(cuda, dtype, out, nh, nkv, hd, page, width):
+    # an attended infinity shows whatever is left of its weight in 16 bits; one behind the row does not
+    torch = cuda
+    dt = getattr(torch, dtype)
+    inf, nan = math.inf, math.nan
+    q_len = [200, 1, 150]
+    kv_len = [200, 90, 400] if page else q_len
+    k = [rand(torch, n, nkv, hd, dt=dt, seed=i) for i, n in enumerate(kv_len)]
+    v = [rand(torch, n, nkv, hd, dt=dt, seed=20 + i) for i, n in enumerate(kv_len)]
+    q = [rand(torch, n, nh, hd, dt=dt, seed=40 + i, scale=2.0) for i, n in enumerate(q_len)]
+    for x in q:
+        x[..., 0] = 4.0
+    faint = [10, 0, 77]  # a key some 40 below the others: e^-40 = 2^-58 of their weight
+    for x, j in zip(k, faint):
+        x[j, :, 0] = -10.0 * hd ** 0.5
+    v[0] = with_nonfinite(v[0], {(10, 0, 2): inf, (10, nkv - 1, 5): -inf, (60, 0, 5): inf, (150, 0, 7): nan})
+    v[1] = with_nonfinite(v[1], {(0, nkv - 1, 9): inf})
+    v[2] = with_nonfinite(v[2], {(77, 0, 11): -inf, (77, nkv - 1, 50): inf, (149, 0, 50): -inf, (3, 0, 12): inf})
+    cu_h = np.concatenate([[0], np.cumsum(q_len)])
+    cu = torch.tensor(cu_h, dtype=torch.int32, device="cuda")
+    odt = dt if out == "same" else torch.float32
+    if page:
+        kp, vp, table = make_pages(torch, k, v, page, width_extra=width)
+        got = ops.attention_prompt(torch.cat(q), kp, vp, cu, page_table=table, out_dtype=odt,
+                                   kv_len=torch.tensor(kv_len, dtype=torch.int32, device="cuda"))
+    else:
+        got = ops.attention_prompt(torch.cat(q), torch.cat(k), torch.cat(v), cu, out_dtype=odt)
+    for i, (n, m) in enumerate(zip(q_len, kv_len)):
+        check_nonfinite(torch, got[int(cu_h[i]):int(cu_h[i + 1])], q[i], k[i], v[i], hd ** -0.5, m - n,
+                        prompt_weight(torch, dt, m), dt, f"sequence {i}")
+
+
 @pytest.mark.parametrize("split", [False, True])
 def test_attention_prompt_later_value_behind_a_long_prefix(cuda, split):
     # the rows computed again have 20000 keys each, while the CTA's other roles wait
