@@ -12,12 +12,15 @@
 // 128-row query tiles that read the same keys: the same rows of two heads of
 // a group (even groups), or 256 rows of one head.  Per 128 keys and query
 // tile the tensor core computes S = Q K^T into tensor memory, one thread per
-// row takes maximum, exponentials and sum, writes the weights P (16 bits)
-// over S, and the tensor core adds P V to the output, which stays in tensor
-// memory.  While one tile's weights are computed the tensor core works on the
-// other's.  The output is rescaled only when a row's maximum has risen by
-// more than 2^kLazy since it was last set (the weights then still fit 16
-// bits and the division by the sum cancels the factor).
+// row takes maximum, exponentials and sum, writes the weights P over S, and
+// the tensor core adds P V to the output, which stays in tensor memory.  P is
+// rounded once to 16 bits where the output is: it adds an error of about the
+// output's own rounding.  For fp32 outputs it is two 16-bit parts (2^-22 of a
+// weight in fp16, 2^-16 in bf16), which fill the columns of S, and the second
+// product is done for both.  While one tile's weights are computed the tensor
+// core works on the other's.  The output is rescaled only when a row's
+// maximum has risen by more than 2^kLazy since it was last set (the weights
+// then still fit 16 bits and the division by the sum cancels the factor).
 //
 // CTA (one per SM, persistent), 12 warps:
 //   0-3, 4-7  softmax, rescale and output of query tile 0 and 1
@@ -30,7 +33,8 @@
 // an abort flag, all roles leave, and tensor memory is released.
 //
 // Measured on one B200: 8192 tokens on 32 heads of 128 values, bf16, 460 us =
-// 1.19 PFLOP/s, 0.71 of the cuBLAS rate.  A step (128 keys, both query tiles)
+// 1.19 PFLOP/s, 0.71 of the cuBLAS rate; 610 with an fp32 output (465 with
+// weights of one rounding there too).  A step (128 keys, both query tiles)
 // takes 3500 cycles; the tensor core's part of it, alone, 2049.  The rest is
 // one tile's chain -- scores, 1900 cycles of softmax, products -- which two
 // tiles in turn do not cover, and tensor memory (S 2 x 128 columns, outputs
@@ -263,6 +267,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                         unsigned* __restrict__ err) {
   using C = Cfg<HD>;
   constexpr int kHalves = HD / 64, S = C::kStages;
+  constexpr bool kTwo = sizeof(O) == 4;  // weights in two 16-bit parts: columns 0-63 and 64-127 of the scores
   constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
   constexpr uint32_t kIdescS = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((kRows >> 3) << 17) | ((kRows >> 4) << 24);
   constexpr uint32_t kIdescO =
@@ -734,9 +739,13 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
               if (!get(p_full + 2 * i + h, np >> i & 1)) break;
               tc_fence_after();
 #pragma unroll
-              for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
+              for (int ks = 4 * h; ks < 4 * h + 4; ++ks) {
                 umma_ts(tmem + C::kO + i * HD, tmem + i * kRows + ks * 8, desc64(vl + ks * (2048 >> 4), kDescHi),
                         kIdescO, ks > 0 || j > 0);
+                if constexpr (kTwo)
+                  umma_ts(tmem + C::kO + i * HD, tmem + i * kRows + kRows / 2 + ks * 8,
+                          desc64(vl + ks * (2048 >> 4), kDescHi), kIdescO, true);
+              }
             }
             if (!ok) break;
             np ^= 1u << i;
@@ -817,7 +826,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         unsigned long long sum[2] = {0ull, 0ull};
 #pragma unroll
         for (int b = 0; b < kRows; b += 64) {
-          uint32_t w[32];
+          uint32_t w[32], w2[32];
 #pragma unroll
           for (int e = 0; e < 64; e += 2) {
             float x0, x1;
@@ -826,8 +835,13 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
             x1 = ex2(x1);
             sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(x0, x1));
             w[e >> 1] = pack16<T>(x0, x1);
+            if constexpr (kTwo) {
+              const float2 y = unpack16<T>(w[e >> 1]);
+              w2[e >> 1] = pack16<T>(x0 - y.x, x1 - y.y);
+            }
           }
           tmem_st32(ts + (b >> 1), w);
+          if constexpr (kTwo) tmem_st32(ts + kRows / 2 + (b >> 1), w2);
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();

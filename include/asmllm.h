@@ -698,9 +698,11 @@ ASMLLM_API int asm_rope_append_async(const void* qkv, int32_t qkv_dtype, int64_t
  * keys), query head h on KV head h / (n_heads / n_kv_heads), scale > 0.  out
  * [rows][n_heads][head_dim], fp32 or the cache's type.  Rows without a key
  * give zeros; rows at or past cu_q[batch] are left as they are.  Scores,
- * maxima and sums are fp32; the weights are rounded to the 16-bit type for
- * the product with the values, which costs about as much as one rounding of
- * the output.  What a row does not attend to -- later positions, other
+ * maxima and sums are fp32; for a 16-bit output the weights are rounded to
+ * its type for the product with the values, which costs about as much as the
+ * rounding of the output, for an fp32 output they enter as two 16-bit parts
+ * (2^-22 of a weight in fp16 down to 2^-33 of the row's largest, 2^-16 in
+ * bf16).  What a row does not attend to -- later positions, other
  * sequences, the rest of a page -- does not reach it, whatever it holds.
  * Where the items may be fewer than the SMs and long, up to 40 MB of
  * stream-ordered scratch are taken for the call. */

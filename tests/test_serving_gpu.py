@@ -20,6 +20,7 @@ import pytest
 
 from asmllm_b200 import decode as D
 from asmllm_b200 import native, ops
+from test_serving_host import WEIGHT_CASES, one_value_case, one_value_exact
 
 pytestmark = pytest.mark.gpu
 
@@ -249,6 +250,28 @@ def test_attention_paged_long_tail_of_small_weights(cuda):
     got = ops.attention_prompt(q, kp, vp, cu, kv_len=kv, page_table=table, scale=1.0, out_dtype=torch.float32)
     # n weights of fp16 with 2^-32 of the largest as their step
     close(torch, got, want, pv, serr, n, prompt_weight(torch, torch.float16, n), torch.float16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", WEIGHT_CASES)
+@pytest.mark.parametrize("nkv,group,hd", [(4, 1, 128), (2, 12, 64)])
+def test_fp32_outputs_have_weights_of_two_parts(cuda, dtype, n, nkv, group, hd):
+    # exact scores, fp32 outputs, a bound that weights of one 16-bit rounding miss
+    torch = cuda
+    dt = getattr(torch, dtype)
+    q, k, v = one_value_case(torch, dt, n, nkv, hd, "cuda", n)
+    q = q.repeat_interleave(group, 1)
+    want, tol = (x.repeat_interleave(group, 1) for x in one_value_exact(torch, k, v))
+    kp, vp, table = make_pages(torch, [k], [v], 16)
+    kv = torch.tensor([n], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    wide = torch.zeros(1, 300, dtype=torch.int32, device="cuda")  # keys that may be many: dealt out by key tiles
+    wide[:, :table.shape[1]] = table
+    for got in (ops.attention_paged(q, kp, vp, table, kv, scale=1.0, out_dtype=torch.float32),
+                ops.attention_prompt(q, kp, vp, cu, kv_len=kv, page_table=table, scale=1.0, out_dtype=torch.float32),
+                ops.attention_prompt(q, kp, vp, cu, kv_len=kv, page_table=wide, scale=1.0, out_dtype=torch.float32)):
+        err = (got.double() - want).abs()
+        assert (err <= tol).all(), f"worst {float((err / tol).max()):.3g} of the bound"
 
 
 def test_attention_paged_strided_query_scale_and_out(cuda):

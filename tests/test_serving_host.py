@@ -146,3 +146,48 @@ def test_python_layer_refuses_host_tensors():
         ops.attention_paged(x.half(), h, h, t, n)
     with pytest.raises(TypeError):
         ops.rows_sample(x[:, 0], n)
+
+
+# ------------------------------------------------------------------ a bound that one 16-bit rounding of a weight exceeds
+# Scores that come out exactly (one value of q and of each key is not zero, both short) leave the weights' own errors:
+# the scaled score and maximum, at most 1.4427 each, are off by 1.5 * 2^-24 of themselves and their difference by half
+# a step, under 2^-21 in all, and the exponential by 2^-22; the two 16-bit parts by u^2 (and 2^-38 of the largest weight
+# where fp16 runs out of exponent); sums of n terms by n * 2^-23.  Twice, for the weighted sum and the sum of weights.
+WEIGHT_CASES = [1, 2, 3, 5, 9, 17, 33]  # keys
+
+
+def one_value_case(torch, dt, n, nkv, hd, device, seed):
+    """q [1, nkv, hd], k, v [n, nkv, hd]: scores k[:, :, 0] in eighths from -1 to 1, values of both signs."""
+    g = torch.Generator().manual_seed(seed)
+    q = torch.zeros(1, nkv, hd, dtype=dt)
+    q[..., 0] = 1.0
+    k = torch.zeros(n, nkv, hd, dtype=dt)
+    k[..., 0] = (torch.randint(-8, 9, (n, nkv), generator=g) / 8).to(dt)
+    v = torch.randn(n, nkv, hd, generator=g).to(dt)
+    return [t.to(device) for t in (q, k, v)]
+
+
+def one_value_exact(torch, k, v):
+    """Outputs [1, nkv, hd] in 64 bits and the bound above."""
+    p = torch.softmax(k[..., 0].double(), 0)
+    want, pv = (torch.einsum("nh,nhd->hd", p, x)[None] for x in (v.double(), v.double().abs()))
+    u = torch.finfo(v.dtype).eps / 2
+    part = u * u + (len(v) * 2.0 ** -38 if v.dtype == torch.float16 else 0.0)
+    return want, 2 * (2.0 ** -21 + 2.0 ** -22 + part + len(v) * 2.0 ** -23) * pv + 2.0 ** -24 * want.abs()
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_the_bound_on_two_part_weights_shows_a_missing_part(dtype):
+    torch = pytest.importorskip("torch")
+    dt = getattr(torch, dtype)
+    once = []
+    for n in WEIGHT_CASES:
+        _, k, v = one_value_case(torch, dt, n, 4, 128, "cpu", n)
+        want, tol = one_value_exact(torch, k, v)
+        w = 2.0 ** 14 * torch.exp(k[..., 0].double() - k[..., 0].double().amax(0))
+        hi = w.to(dt).double()
+        both = hi + (w - hi).to(dt).double()
+        got = [torch.einsum("nh,nhd->hd", x, v.double())[None] / w.sum(0)[None, :, None] for x in (both, hi)]
+        assert ((got[0] - want).abs() <= tol).all()
+        once.append(float(((got[1] - want).abs() / tol).max()))
+    assert min(once[1:]) > 5  # the second part left out: far outside at every length (a single weight is exact)
