@@ -921,6 +921,53 @@ int check_kv_pointers(const char* name, const KvArgs& kv) {
   return ASM_OK;
 }
 
+// An array of up to three strided axes (a stride in elements means nothing where there is one entry) of `inner`
+// dense elements of `size` bytes.
+struct Strided {
+  const void* p;
+  int size;
+  long long inner;
+  long long count[3], stride[3];
+};
+
+// Whether `bytes` bytes at `out` meet it.  Gaps of the outermost axis are seen (pages of other layers, rows of a
+// wider array); those further in count as taken.
+bool meets(const void* out, size_t bytes, const Strided& a) {
+  if (!a.p || bytes == 0 || a.inner <= 0) return false;
+  int outer = -1;
+  for (int i = 0; i < 3; ++i) {
+    if (a.count[i] <= 0) return false;
+    if (a.count[i] > 1 && (outer < 0 || a.stride[i] > a.stride[outer])) outer = i;
+  }
+  long long extent = a.inner;
+  for (int i = 0; i < 3; ++i)
+    if (i != outer && a.count[i] > 1) extent += (a.count[i] - 1) * a.stride[i];
+  extent *= a.size;
+  const long long n = outer < 0 ? 1 : a.count[outer], step = outer < 0 ? extent : a.stride[outer] * a.size;
+  const long long b = (long long)((intptr_t)out - (intptr_t)a.p), e = b + (long long)bytes;
+  if (e <= 0 || b >= (n - 1) * step + extent) return false;
+  if (b < 0 || extent >= step) return true;
+  const long long t = b / step;
+  return b < t * step + extent || (t + 1 < n && (t + 1) * step < e);
+}
+
+Strided flat(const void* p, int size, long long n) { return {p, size, n, {1, 1, 1}, {0, 0, 0}}; }
+
+// An output must not overlap the inputs: rows written early would be read as something else by rows still to come.
+int check_apart(const char* name, const char* what, const void* out, size_t bytes, const Strided* in, int n,
+                const KvArgs* kv) {
+  bool hit = false;
+  for (int i = 0; i < n; ++i) hit |= meets(out, bytes, in[i]);
+  if (kv) {
+    for (const void* p : {kv->k, kv->v})
+      hit |= meets(out, bytes, {p, 2, kv->head_dim, {kv->n_pages, kv->page_size, kv->n_kv},
+                                {kv->page_stride, kv->token_stride, kv->head_stride}});
+    hit |= meets(out, bytes, {kv->table, 4, kv->width, {kv->batch, 1, 1}, {kv->table_stride, 0, 0}});
+    hit |= meets(out, bytes, flat(kv->len, 4, kv->batch)) || meets(out, bytes, flat(kv->cu, 4, kv->batch + 1));
+  }
+  return hit ? set_error(ASM_E_INVALID, "%s: %s overlaps an input", name, what) : ASM_OK;
+}
+
 int check_heads(const char* name, int n_heads, int n_kv) {
   if (n_heads <= 0 || n_heads % n_kv || n_heads > 65535)
     return set_error(ASM_E_INVALID, "%s: n_heads %d is not a multiple of n_kv_heads %d", name, n_heads, n_kv);
@@ -961,6 +1008,14 @@ ASMLLM_API int asm_rope_append_async(const void* qkv, int32_t qkv_dtype, int64_t
       (rc = require_device(name, rope_cs, "rope_cs")) || (rc = require_device(name, q_out, "q_out")) ||
       (cu_q && (rc = require_device(name, cu_q, "cu_q"))))
     return rc;
+  const long long cols = (long long)(n_heads + 2 * kv.n_kv) * kv.head_dim;
+  const int wide = qkv_dtype == ASM_DT_F32 ? 4 : 2;
+  const Strided in[3] = {{qkv, wide, cols, {rows, 1, 1}, {qkv_stride, 0, 0}},
+                         flat(rope_cs, 4, (long long)rope_len * kv.head_dim), flat(cu_q, 4, kv.batch + 1)};
+  if ((rc = check_apart(name, "q_out", q_out, (size_t)rows * n_heads * kv.head_dim * 2, in, 3, &kv)) ||
+      (rc = check_apart(name, "qkv", qkv, ((size_t)(rows - 1) * qkv_stride + cols) * wide, nullptr, 0, &kv)))
+    return rc;
+  if (kv.k == kv.v) return set_error(ASM_E_INVALID, "%s: k and v are the same pages", name);
   RopeAppendArgs a;
   a.qkv = qkv;
   a.src_dtype = qkv_dtype;
@@ -991,6 +1046,11 @@ ASMLLM_API int asm_attention_prompt_async(const void* q, int64_t q_row_stride, i
   if (rows == 0 || kv.batch == 0) return ASM_OK;
   if ((rc = check_kv_pointers(name, kv)) || (rc = require_device(name, q, "q")) ||
       (rc = require_device(name, out, "out")) || (rc = require_device(name, cu_q, "cu_q")))
+    return rc;
+  const Strided in[2] = {{q, 2, kv.head_dim, {rows, n_heads, 1}, {q_row_stride, q_head_stride, 0}},
+                         flat(cu_q, 4, kv.batch + 1)};
+  if ((rc = check_apart(name, "out", out, (size_t)rows * n_heads * kv.head_dim * (out_dtype == ASM_DT_F32 ? 4 : 2), in,
+                        2, &kv)))
     return rc;
   PromptArgs a;
   a.q = q;
@@ -1035,6 +1095,12 @@ ASMLLM_API int asm_attention_paged_async(const void* q, int64_t q_row_stride, in
   if ((rc = check_kv_pointers(name, kv)) || (rc = require_device(name, q, "q")) ||
       (rc = require_device(name, out, "out")) || (need && (rc = require_device(name, workspace, "workspace"))))
     return rc;
+  const size_t out_bytes = (size_t)kv.batch * n_heads * kv.head_dim * (out_dtype == ASM_DT_F32 ? 4 : 2);
+  const Strided in[2] = {{q, 2, kv.head_dim, {kv.batch, n_heads, 1}, {q_row_stride, q_head_stride, 0}},
+                         flat(out, 1, (long long)out_bytes)};
+  if ((rc = check_apart(name, "out", out, out_bytes, in, 1, &kv)) ||
+      (rc = check_apart(name, "workspace", workspace, need, in, 2, &kv)))
+    return rc;
   PagedArgs a;
   a.q = q;
   a.q_row_stride = q_row_stride;
@@ -1069,6 +1135,9 @@ ASMLLM_API int asm_rows_sample_async(const void* logits, int32_t dtype, int32_t 
       (top_p && (rc = require_device(name, top_p, "top_p"))) ||
       (min_p && (rc = require_device(name, min_p, "min_p"))))
     return rc;
+  const Strided in[6] = {{logits, dtype == ASM_DT_F32 ? 4 : 2, n, {rows, 1, 1}, {stride, 0, 0}}, flat(u, 4, rows),
+                         flat(temperature, 4, rows), flat(top_k, 4, rows), flat(top_p, 4, rows), flat(min_p, 4, rows)};
+  if ((rc = check_apart(name, "tokens", tokens, (size_t)rows * 4, in, 6, nullptr))) return rc;
   SampleArgs a;
   a.logits = logits;
   a.dtype = dtype;

@@ -643,7 +643,8 @@ ASMLLM_API int asm_rows_advance_async(const int64_t* keys, int32_t rows, int32_t
  * argmax (src/runtime/generate.py:252-326, 410-411); these have no counterpart
  * there.  All are stream-ordered and capturable in CUDA graphs (after one eager
  * call per shape), take device pointers of the current device, and keep nothing
- * between calls.  Outputs must not overlap inputs. */
+ * between calls.  An output that overlaps an input is refused, as is a
+ * workspace that overlaps either. */
 #define ASM_DT_F32 0
 #define ASM_DT_F16 1
 #define ASM_DT_BF16 2

@@ -755,6 +755,64 @@ def test_refusals_of_the_python_layer(cuda):
             call()
 
 
+def test_outputs_over_inputs_are_refused(cuda):
+    torch = cuda
+    B, nh, nkv, hd, page = 3, 4, 2, 128, 16
+    row = nh * hd
+    arena = torch.zeros(1 << 16, dtype=torch.float16, device="cuda")
+    part = lambda at, *s: arena[at:at + math.prod(s)].view(s)  # noqa: E731
+    zeros = lambda *s, dt=torch.float16: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
+    kp, vp = zeros(4, page, nkv, hd), zeros(4, page, nkv, hd)
+    table, n, cu = (zeros(*s, dt=torch.int32) for s in ((B, 2), (B,), (B + 1,)))
+    rope = torch.from_numpy(D.rope_table(8, hd, 10000.0)).cuda()
+    x = zeros(B, (nh + 2 * nkv) * hd)
+    q = part(0, B, nh, hd)
+    paged = lambda q=q, k=kp, v=vp, **kw: ops.attention_paged(q, k, v, table, n, **kw)  # noqa: E731
+    prompt = lambda q=q, k=kp, v=vp, **kw: ops.attention_prompt(q, k, v, cu, kv_len=n, page_table=table, **kw)  # noqa: E731
+    append = lambda x=x, k=kp, v=vp, **kw: ops.rope_append(x, rope, n, table, k, v, nh, **kw)  # noqa: E731
+    pool = part(1 << 14, 4, page, nkv, hd)
+    behind = part((1 << 14) + 4 * page * nkv * hd, B, nh, hd)
+    inside = part((1 << 14) + 4 * page * nkv * hd - 8, B, nh, hd)  # begins in the pool's last key
+    before = part((1 << 14) - B * row + 8, B, nh, hd)              # ends in its first
+    wide = arena.view(4, -1)[:B, :row].view(B, nh, hd)             # rows with room between them
+    between = arena.view(4, -1)[0, row:2 * row].view(1, nh, hd)
+    packed = arena[:6 * nkv * hd].view(6, nkv, hd)
+    logits = torch.zeros(B, 64, device="cuda")
+    need = ops.attention_paged_workspace(B, nh, nkv, hd)
+    room = zeros(need + 4096, dt=torch.uint8)
+    refused = [
+        lambda: paged(out=part(8, B, nh, hd)), lambda: paged(out=part(B * row - 8, B, nh, hd)),
+        lambda: prompt(out=part(8, B, nh, hd)), lambda: prompt(out=part(B * row - 8, B, nh, hd)),
+        lambda: paged(k=pool, out=inside), lambda: paged(v=pool, out=inside), lambda: paged(k=pool, out=before),
+        lambda: prompt(k=pool, out=before), lambda: prompt(v=pool, out=inside),
+        lambda: ops.attention_prompt(zeros(3, nh, hd), packed, zeros(6, nkv, hd), cu, out=part(5 * nkv * hd, 3, nh, hd)),
+        lambda: paged(q=wide, out=part(1 << 14, B, nh, hd)),  # the second row of q
+        lambda: paged(out=room[-3 * row * 4:].view(torch.float32).view(B, nh, hd), workspace=room),
+        lambda: paged(q=room[:B * row * 2].view(torch.float16).view(B, nh, hd), workspace=room),
+        lambda: append(x=part(0, B, (nh + 2 * nkv) * hd), q_out=part(16, B, nh, hd)),
+        lambda: append(k=pool, q_out=inside), lambda: append(v=pool, q_out=before),
+        lambda: append(x=arena[1 << 14:][:B * 8 * hd].view(B, 8 * hd), v=pool),
+        lambda: append(v=kp),
+        lambda: ops.rows_sample(logits, logits[0, :B].clone(), tokens=logits.view(torch.int32)[1, 61:64]),
+        lambda: ops.rows_sample(logits, u := torch.zeros(B, device="cuda"), tokens=u.view(torch.int32)),
+    ]
+    for call in refused:
+        with pytest.raises(ops.AsmError, match="overlaps an input|same pages"):
+            call()
+    # beside an input, or between its rows, is not over it
+    paged(q=wide[:, :], out=part(row, B, nh, hd)[:0].new_zeros(B, nh, hd))
+    assert paged(k=pool, out=behind) is behind and prompt(v=pool, out=behind) is behind
+    one = wide[1:2]
+    ops.attention_paged(one, kp, vp, table[:1], n[:1], out=between)
+    ops.attention_prompt(wide, kp, vp, cu, kv_len=n, page_table=table, out=part((1 << 14) + row, B, nh, hd))
+    sliced = zeros(4, 3, page, nkv, hd)  # one layer's pages of a pool of three
+    assert paged(k=sliced[:, 0], v=sliced[:, 2], out=sliced[1, 1].view(-1)[:B * row].view(B, nh, hd)) is not None
+    append(k=sliced[:, 0], v=sliced[:, 1])
+    both = zeros(4, page, 2 * nkv, hd)  # keys and values side by side
+    append(k=both[:, :, :nkv], v=both[:, :, nkv:])
+    torch.cuda.synchronize()
+
+
 def test_two_streams_at_once(cuda):
     torch = cuda
     nh, nkv, hd, lens = 16, 2, 128, [2900, 17, 900]
