@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const RopeAppendArgs a
     long long off = -1;
     if (seq < kv.batch) {
       int b, e;
-      if (!q_range(a.cu_q, seq, a.rows, &b, &e)) atomicOr(err, kErrDecodeRange);
+      q_range(a.cu_q, seq, a.rows, &b, &e);
       if (t >= b && t < e) {
         pos = max(-1, __ldcg(kv.len + seq) - (e - b) + (t - b));
         if (pos >= 0) {  // outside the rotary table, the sequence's pages or the pool: skipped
@@ -60,6 +60,14 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const RopeAppendArgs a
     }
     s_pos = pos;
     s_off = off;
+  }
+  if (blockIdx.x == 0) {  // lengths and offsets out of range are reported whether a row meets them or not
+    for (int s = blockDim.x - 1 - threadIdx.x; s < kv.batch; s += blockDim.x) {
+      bool clipped;
+      int b, e;
+      kv_length(kv, s, &clipped);
+      if (clipped || !q_range(a.cu_q, s, a.rows, &b, &e)) atomicOr(err, kErrDecodeRange);
+    }
   }
   __syncthreads();
   const int pos = s_pos;

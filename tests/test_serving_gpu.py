@@ -194,6 +194,33 @@ def test_rope_append_refuses_positions_and_pages_on_the_device(cuda):
     assert (q == 0).all() and (kp == 0).all() and (vp == 0).all()
 
 
+def test_rope_append_reports_lengths_and_offsets_no_row_meets(cuda):
+    torch = cuda
+    nh, nkv, hd, B = 2, 1, 64, 300  # more sequences than a CTA has threads
+    x = rand(torch, B, (nh + 2 * nkv) * hd, dt=torch.float32, seed=3)
+    rope = torch.from_numpy(D.rope_table(32, hd, 10000.0)).cuda()
+    kp = torch.zeros(B, 16, nkv, hd, dtype=torch.float16, device="cuda")
+    vp = torch.zeros_like(kp)
+    table = torch.arange(B, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    lens = lambda **kw: torch.tensor([kw.get(f"s{i}", 1) for i in range(B)], dtype=torch.int32, device="cuda")  # noqa: E731
+    want = ops.rope_append(x, rope, lens(), table, kp, vp, nh)
+    assert ops.device_error() == 0
+    for bad in (dict(s0=-3), dict(s299=-1), dict(s280=17)):  # below zero; above the table's one page of 16
+        got = ops.rope_append(x, rope, lens(**bad), table, kp, vp, nh)
+        assert ops.device_error() == native.DEVERR_DECODE_RANGE
+        assert torch.equal(got[100:200], want[100:200])
+    cu = torch.arange(B + 1, dtype=torch.int32, device="cuda")
+    one = cu.clone()
+    one[B - 1:] = B + 5  # the last sequence begins and ends behind the rows
+    got = ops.rope_append(x, rope, lens(), table, kp, vp, nh, cu_q=one)
+    assert ops.device_error() == native.DEVERR_DECODE_RANGE
+    assert torch.equal(got[100:200], want[100:200])
+    none = lens(s7=40)  # a length past the table, without a new row
+    cu[8:] -= 1
+    ops.rope_append(x, rope, none, table, kp, vp, nh, cu_q=cu)
+    assert ops.device_error() == native.DEVERR_DECODE_RANGE
+
+
 # ------------------------------------------------------------------ paged attention
 PAGED = [
     # nh, nkv, hd, page, lengths
