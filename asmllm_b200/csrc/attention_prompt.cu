@@ -516,7 +516,13 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       }
       top = (__reduce_max_sync(kFull, top) + kRows - 1) / kRows;  // most key tiles of any item
       if (any_clipped && blockIdx.x == 0) atomicOr(err, kErrDecodeRange);
-      const long long count = (long long)total([&](int q, int) { return (q + R - 1) / R; }) * units;
+      const int tiles = total([&](int q, int) { return (q + R - 1) / R; });
+      const long long count = (long long)tiles * units;
+      // A CTA's ranks rise, so it goes on where its last item was: among tiles with `level` key tiles, the first of
+      // sequences `next` .. has rank `from`, and rank `upto` has fewer key tiles.  (From the start again for every
+      // item, a call's time grew with the square of the number of sequences: 1024 prompts of up to 100 tokens on
+      // 32 heads took 4957 us, now 570; 32768 of them take 18 ms.)
+      int level = top + 1, upto = 0, from = 0, next = 0;
       for (int k = 0;; ++k) {
         const long long G = gridDim.x, at = k * G + ((k & 1) ? G - 1 - blockIdx.x : blockIdx.x);
         if (k >= 2 && !wait(i_empty + (k & 1), ((k >> 1) - 1) & 1)) break;
@@ -524,25 +530,37 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         it.s = -1;
         if (at < count) {
           const int rank = (int)(at / units), unit = (int)(at % units);
-          // the largest w with more than `rank` tiles of at least w key tiles
-          int lo = 0, hi = top;
-          while (lo < hi) {
-            const int w = (lo + hi + 1) >> 1;
-            if (total([&](int q, int b) { return tiles_at_least(b, q, R, w); }) > rank) lo = w; else hi = w - 1;
+          if (rank >= upto) {  // the largest w with more than `rank` tiles of at least w key tiles
+            int lo = 0, hi = level - 1, most = tiles;  // tiles of at least lo key tiles; `upto`: of more than hi
+            for (int step = 1; lo < hi; step *= 2) {   // from the top: most often the next level
+              const int w = max((lo + hi + 1) >> 1, hi + 1 - step), x = total([&](int q, int b) { return tiles_at_least(b, q, R, w); });
+              if (x > rank) {
+                lo = w;
+                most = x;
+              } else {
+                hi = w - 1;
+                upto = x;
+              }
+            }
+            level = lo;
+            from = upto;
+            upto = most;
+            next = 0;
           }
-          int left = rank - total([&](int q, int b) { return tiles_at_least(b, q, R, lo + 1); });
-          // which of the tiles with exactly lo key tiles: true in every lane once it is among these sequences
+          // which of the tiles with exactly `level` key tiles: true in every lane once it is among these sequences
           auto pick = [&](int s0, int q, int b, int r) -> bool {
-            const int c1 = tiles_at_least(b, q, R, lo), c = c1 - tiles_at_least(b, q, R, lo + 1);
+            const int c1 = tiles_at_least(b, q, R, level), c = c1 - tiles_at_least(b, q, R, level + 1);
             int x = c;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
               const int y = __shfl_up_sync(kFull, x, o);
               if (lane >= o) x += y;
             }
+            const int left = rank - from;
             const unsigned hit = __ballot_sync(kFull, left < x);
             if (!hit) {
-              left -= __shfl_sync(kFull, x, 31);
+              from += __shfl_sync(kFull, x, 31);
+              next = s0 + 32;
               return false;
             }
             const int src = __ffs(hit) - 1, tile = (q + R - 1) / R - c1 + (left - (x - c));
@@ -556,15 +574,15 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
           bool found = false;
 #pragma unroll
           for (int e = 0; e < kHeld; ++e)
-            if (!found && 32 * e < kv.batch) found = pick(32 * e, hq[e], hb[e], hr[e]);
+            if (!found && 32 * e >= next && 32 * e < kv.batch) found = pick(32 * e, hq[e], hb[e], hr[e]);
 #pragma unroll 1
-          for (int s0 = 32 * kHeld; !found && s0 < kv.batch; s0 += 32) {
+          for (int s0 = max(next, 32 * kHeld); !found && s0 < kv.batch; s0 += 32) {
             int q = 0, b = 0, r = 0;
             if (s0 + lane < kv.batch) r = load(s0 + lane, &q, &b);
             found = pick(s0, q, b, r);
           }
           it.head = pair ? 2 * unit : unit;
-          it.key0 = kv.table ? 0 : __ldcg(kv.cu + it.s);
+          it.key0 = kv.table || !found ? 0 : __ldcg(kv.cu + it.s);
           it.j0 = 0;
           it.slot = -1;
           it.tiles[0] = tiles_in(it.base, it.rows, 0);

@@ -645,6 +645,49 @@ def test_attention_prompt_many_sequences(cuda):
               torch.bfloat16, f"sequence {s}")
 
 
+def test_attention_prompt_many_sequences_of_many_lengths(cuda):
+    # more sequences than the scheduler holds, many items a CTA: rows and keys of every count of key tiles, some none
+    torch = cuda
+    rng = np.random.default_rng(7)
+    B, nh, nkv, hd, page = 350, 4, 2, 64, 32
+    q_len = np.where(rng.random(B) < 0.1, 0, np.exp(rng.uniform(0, math.log(300), B)).astype(int))
+    kv_len = np.where(rng.random(B) < 0.1, q_len // 2, q_len + rng.integers(0, 900, B) * (rng.random(B) < 0.5))
+    T = int(q_len.sum())
+    k, v = ([rand(torch, int(n), nkv, hd, dt=torch.bfloat16, seed=c + i) for i, n in enumerate(kv_len)] for c in (0, 900))
+    kp, vp, table = make_pages(torch, k, v, page)
+    q = rand(torch, T, nh, hd, dt=torch.bfloat16, seed=1, scale=2.0)
+    cu_h = np.concatenate([[0], np.cumsum(q_len)])
+    got = ops.attention_prompt(q, kp, vp, torch.tensor(cu_h, dtype=torch.int32, device="cuda"), page_table=table,
+                               kv_len=torch.tensor(kv_len, dtype=torch.int32, device="cuda"))
+    for s in range(B):
+        a, b, n = int(cu_h[s]), int(cu_h[s + 1]), int(kv_len[s])
+        if b > a:
+            want, pv, serr = exact_attention(torch, q[a:b], k[s], v[s], hd ** -0.5, n - (b - a))
+            close(torch, got[a:b], want, pv, serr, max(1, n), prompt_weight(torch, torch.bfloat16, n), torch.bfloat16,
+                  f"sequence {s}")
+
+
+def test_attention_prompt_time_grows_with_the_sequences_not_their_square(cuda):
+    # four times the sequences are four times the work; where every item was looked for from the start it took 18
+    # times as long
+    torch = cuda
+    best = {}
+    for B in (256, 1024):
+        lens = torch.randint(1, 101, (B,), generator=torch.Generator().manual_seed(B))
+        cu = torch.cat([torch.zeros(1, dtype=torch.long), lens.cumsum(0)]).int().cuda()
+        q, k, v = (torch.randn(int(lens.sum()), n, 128, device="cuda").half() for n in (32, 8, 8))
+        times = []
+        for _ in range(6):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            ops.attention_prompt(q, k, v, cu)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        best[B] = min(times)
+    assert best[1024] < 8 * best[256], best
+
+
 def test_attention_prompt_bad_offsets_and_pages_are_reported(cuda):
     torch = cuda
     q = rand(torch, 60, 2, 128, dt=torch.float16, seed=1)
