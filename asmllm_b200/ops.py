@@ -652,6 +652,14 @@ def _kv_view(k, v, device, kv_len=None, page_table=None, cu_k=None):
                      shape[0], 0, shape[1], shape[2], _H16[k.dtype], 0), batch)
 
 
+def _no_keys(k, stream):
+    """One row in place of none: no sequence has a key, but a tensor without elements has no address."""
+    if stream is None:
+        return k.new_zeros((1, *k.shape[1:]))
+    with _torch().cuda.stream(stream):
+        return k.new_zeros((1, *k.shape[1:]))
+
+
 def _query(q, k, out, out_dtype, stream):
     """Checks q [rows, heads, head_dim] against k and returns (strides, out)."""
     if not _DT:
@@ -736,6 +744,8 @@ def attention_prompt(q, k, v, cu_q, *, cu_k=None, kv_len=None, page_table=None, 
     if (page_table is None) != (kv_len is None) or (page_table is not None and cu_k is not None):
         raise ValueError("pass page_table and kv_len (paged) or cu_k (packed)")
     device = q.get_device()
+    if page_table is None and device >= 0 and k.dim() == 3 and k.shape[0] == 0 == v.shape[0]:
+        k = v = _no_keys(k, stream)
     kv, batch = _kv_view(k, v, device, kv_len, page_table, cu_q if cu_k is None else cu_k)
     _vector(cu_q, "cu_q", batch + 1, device)
     st, out = _query(q, k, out, out_dtype, stream)

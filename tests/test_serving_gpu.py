@@ -627,6 +627,22 @@ def test_attention_prompt_rows_without_keys_and_strided_inputs(cuda):
         close(torch, got[a:b], want, pv, serr, kb - ka, prompt_weight(torch, torch.float16, 100), torch.float16)
 
 
+def test_attention_prompt_packed_without_any_key(cuda):
+    torch = cuda
+    q = rand(torch, 6, 4, 64, dt=torch.float16, seed=1)
+    none = q.new_empty(0, 2, 64)
+    cu = torch.tensor([0, 2, 5], dtype=torch.int32, device="cuda")
+    for stream in (None, torch.cuda.Stream()):
+        torch.cuda.synchronize()
+        out = torch.full((6, 4, 64), 7.0, device="cuda")
+        torch.cuda.synchronize()
+        ops.attention_prompt(q, none, none, cu, cu_k=torch.zeros_like(cu), out=out, stream=stream)
+        torch.cuda.synchronize()
+        assert (out[:5] == 0).all() and (out[5] == 7.0).all()
+    with pytest.raises(ValueError):
+        ops.attention_prompt(q, none, q.new_empty(1, 2, 64), cu, cu_k=torch.zeros_like(cu))
+
+
 def test_attention_prompt_many_sequences(cuda):
     torch = cuda
     nh, nkv, hd = 2, 1, 128
