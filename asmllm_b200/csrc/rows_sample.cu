@@ -105,30 +105,38 @@ struct Row {
   double exp_scale;  // log2(e) / temperature
   const double* pow2;
 
+  // Each step below is rounded as written.  The same word's bin, part of a bin and mass are computed at several
+  // places, and a multiplication fused with an addition at one of them alone would give a sum that no word reaches.
+  __device__ __forceinline__ float distance(float v) const { return __fmul_rn(__fsub_rn(vtop, v), bin_scale); }
   __device__ __forceinline__ int bin(float v) const {
-    const float t = (vtop - v) * bin_scale;
+    const float t = distance(v);
     return v == vtop ? 0 : t < (float)(kBins - 1) ? (int)t : kBins - 1;
+  }
+  // Which of kThreads parts of bin b.
+  __device__ __forceinline__ int part(float v, int b) const {
+    const float t = __fsub_rn(distance(v), (float)b);
+    return v == vtop ? 0 : min(kThreads - 1, max(0, (int)__fmul_rn(t, (float)kThreads)));
   }
   // w = exp((x - m) / temperature) for a word that is not in the last bin.
   // Table-driven (Tang 1989): x = (64 k + j) / 64 + r in powers of two, |r| <= 1/128, 2^(j/64) from the
   // table and 2^r from its Taylor polynomial; the remainder r^6 ln(2)^6 / 720 is below 2^-54.
   __device__ __forceinline__ double weight(float v) const {
     if (v == vtop) return 1.0;
-    const double y = ((double)v - (double)vtop) * exp_scale;
-    const double big = y + 105553116266496.0;  // 1.5 * 2^46: rounds to a multiple of 1/64
+    const double y = __dmul_rn(__dsub_rn((double)v, (double)vtop), exp_scale);
+    const double big = __dadd_rn(y, 105553116266496.0);  // 1.5 * 2^46: rounds to a multiple of 1/64
     const int n = __double2loint(big);
-    const double z = (y - (big - 105553116266496.0)) * 0.6931471805599453;
+    const double z = __dmul_rn(__dsub_rn(y, __dsub_rn(big, 105553116266496.0)), 0.6931471805599453);
     double p = fma(z, 1.0 / 120.0, 1.0 / 24.0);
     p = fma(z, p, 1.0 / 6.0);
     p = fma(z, p, 0.5);
     p = fma(z, p, 1.0);
     p = fma(z, p, 1.0);
     const double t = pow2[n & 63];
-    return __hiloint2double(__double2hiint(t) + (n >> 6) * 1048576, __double2loint(t)) * p;
+    return __dmul_rn(__hiloint2double(__double2hiint(t) + (n >> 6) * 1048576, __double2loint(t)), p);
   }
   // w <= 1 as a multiple of 2^-45: adding 2^7 leaves 45 bits behind the point, rounded to nearest even
   __device__ __forceinline__ static u64 fixed(double w) {
-    return (u64)__double_as_longlong(w + 128.0) - 0x4060000000000000ull;
+    return (u64)__double_as_longlong(__dadd_rn(w, 128.0)) - 0x4060000000000000ull;
   }
   __device__ __forceinline__ u64 mass(float v) const { return bin(v) == kBins - 1 ? 0ull : fixed(weight(v)); }
 };
@@ -291,10 +299,7 @@ struct Slice {
         part[threadIdx.x] = 0;
         if (threadIdx.x == 0) sh.found[2] = 0;
         __syncthreads();
-        auto part_of = [&](u64 x) {
-          const float t = (row.vtop - word_value(x)) * row.bin_scale - (float)b;
-          return word_value(x) == row.vtop ? 0 : min(kThreads - 1, max(0, (int)(t * (float)kThreads)));
-        };
+        auto part_of = [&](u64 x) { return row.part(word_value(x), b); };
         for (int i = threadIdx.x; i < c; i += kThreads) {
           const u64 m = MASS ? row.mass(word_value(sh.list[i])) : 1ull;
           sh.mass[i] = m;

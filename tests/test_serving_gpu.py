@@ -1069,6 +1069,64 @@ def test_rows_sample_greedy_is_rows_argmax_and_defaults(cuda):
     assert got.tolist() == [sample_ref(xs[r].copy(), u[r].item(), 1.0, 0, 1.0, 0.0) for r in range(9)]
 
 
+def test_rows_sample_borders_at_the_edge_of_a_part(cuda):
+    # The bin that holds a border is divided in 512 parts.  Words whose part is another one when (m - x) 32 / T - bin
+    # is rounded once, not twice: with each the last that top_p keeps, it has to be found all the same.
+    torch = cuda
+    rng = np.random.default_rng(11)
+    T = np.float32(1.1)
+    scale = np.float32(np.float32(32.0) / T)
+    v = -rng.uniform(0.05, 15.0, 200000).astype(np.float32)
+    twice = (-v) * scale
+    b = twice.astype(np.int64)
+    once = (-v.astype(np.float64) * np.float64(scale) - b).astype(np.float32)
+    part = lambda t: np.clip((t * np.float32(512)).astype(np.int64), 0, 511)  # noqa: E731
+    v = v[part(twice - b.astype(np.float32)) != part(once)][:600]
+    assert len(v) == 600
+    x = np.stack([np.zeros_like(v), v, v - 5, v - 6], 1)
+    w = np.exp(x.astype(np.float64) / np.float64(T))
+    p = ((1 + w[:, 1] / 2) / w.sum(1)).astype(np.float32)  # half way through the second word
+    for u, token in ((0.99999994, 1), (0.0, 0)):
+        for _ in range(3):
+            tokens = torch.full((600,), -77, dtype=torch.int32, device="cuda")
+            ops.rows_sample(torch.from_numpy(x).cuda(), torch.full((600,), u, device="cuda"),
+                            temperature=torch.full((600,), float(T), device="cuda"), top_p=torch.from_numpy(p).cuda(),
+                            tokens=tokens)
+            assert (tokens == token).all(), f"{int((tokens != token).sum())} of 600"
+
+
+def test_rows_sample_full_batches_give_the_definitions_tokens(cuda):
+    # large rows with settings of their own, beside each other: the borders lie anywhere
+    torch = cuda
+    B, V = 128, 128256
+    r = torch.arange(B, device="cuda")
+    for seed in range(12):
+        g = torch.Generator(device="cuda").manual_seed(1000 + seed)
+        x = torch.randn(B, V, generator=g, device="cuda") * 2.0
+        x += 6.0 * (torch.rand(B, V, generator=g, device="cuda") < 40.0 / V) * torch.randn(
+            B, V, generator=g, device="cuda").abs()
+        u = torch.rand(B, generator=g, device="cuda")
+        T = torch.where(r % 5 == 0, 0.0, 0.7 + 0.1 * (r % 7))
+        k = torch.where(r % 3 == 1, 50 + 40 * r, 0).int()
+        p = torch.where(r % 4 == 3, 1.0, 0.5 + 0.004 * (r % 120))
+        mp = torch.where(r % 6 == 1, 0.001, 0.0)
+        # the definition in 64 bits
+        v, order = torch.sort(x.double(), dim=-1, descending=True, stable=True)
+        w = torch.exp((v - v[:, :1]) / T.double().masked_fill(T == 0, 1.0)[:, None])
+        w = w * (torch.arange(V, device="cuda") < torch.where(k > 0, k, V)[:, None])
+        keep = (w.cumsum(-1) - w < p.double()[:, None] * w.sum(-1, keepdim=True)) | (p >= 1)[:, None]
+        keep &= w >= mp.double()[:, None]
+        keep[:, 0] = True
+        w = torch.zeros_like(w).scatter_(1, order, w * keep)
+        cum = w.cumsum(-1)
+        want = (cum > u.double()[:, None] * cum[:, -1:]).int().argmax(-1)
+        want = torch.where(T == 0, order[:, 0], want).int()
+        for _ in range(4):
+            tokens = torch.full((B,), -77, dtype=torch.int32, device="cuda")
+            ops.rows_sample(x, u, temperature=T, top_k=k, top_p=p, min_p=mp, tokens=tokens)
+            assert torch.equal(tokens, want), (seed, (tokens != want).nonzero().flatten().tolist())
+
+
 def test_rows_sample_frequencies(cuda):
     # 20000 evenly spaced numbers over one row: every word comes up as often as its probability says, to one
     torch = cuda
