@@ -684,17 +684,22 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
       uint32_t ph = 0;  // ring stage and its parity
       bool ok = true, issued = false;
       auto get = [&](uint64_t* bar, uint32_t parity) { return ok = ok && patient(bar, parity); };
-      // the next item with keys; false when there is none
-      auto next_item = [&](Item* it) -> bool {
-        for (;; ++k) {
+      bool ended = false;
+      // The next item with keys; false when there is none.  While products of the last item are outstanding
+      // (`ahead`) also where the very next item has no keys: the softmax warps come to that one, and make room for
+      // those behind it, only once they have these products.
+      auto next_item = [&](Item* it, bool ahead) -> bool {
+        for (;;) {
           if (!get(i_full + (k & 1), (k >> 1) & 1)) return false;
           *it = items[k & 1];
           mbar_arrive(smem_u32(i_empty + (k & 1)));
-          if (it->s < 0) return false;
-          if (max(it->tiles[0], it->tiles[1]) > 0) {
-            ++k;
-            return true;
+          ++k;
+          if (it->s < 0) {
+            ended = true;
+            return false;
           }
+          if (max(it->tiles[0], it->tiles[1]) > 0) return true;
+          if (ahead) return false;
         }
       };
       // S_i = Q_i K^T for key tile j of an item, its keys in ring stage st
@@ -724,7 +729,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         }
       };
       Item it, nx;
-      bool live = next_item(&it);
+      bool live = next_item(&it, false);
       nx = it;
       // Step j of an item: values of its key tile j into the outputs, then the scores of the next key tile,
       // of this item or the next.  Step -1 has no values: the first item's first scores.
@@ -743,8 +748,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
             ph ^= 1;
           }
         }
-        if (last) live = next_item(&nx);
-        const int jn = last ? 0 : j + 1;
+        if (last) live = next_item(&nx, true);
+        int jn = last ? 0 : j + 1;
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
           if (j >= 0 && j < (i ? it.tiles[1] : it.tiles[0])) {
@@ -774,6 +779,10 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         }
         if (!ok) break;
         if (live) release();
+        else if (!ended) {  // an item without keys was next: on from here, nothing outstanding
+          live = next_item(&nx, false);
+          jn = -1;
+        }
         it = nx;
         j = jn;
       }

@@ -643,6 +643,36 @@ def test_attention_prompt_packed_without_any_key(cuda):
         ops.attention_prompt(q, none, q.new_empty(1, 2, 64), cu, cu_k=torch.zeros_like(cu))
 
 
+@pytest.mark.parametrize("nh,nkv,hd,long,empty", [(64, 8, 64, 3, 0.5), (64, 8, 128, 300, 0.9), (32, 32, 128, 40, 1.0),
+                                                  (1, 1, 128, 60000, 0.9), (2, 1, 64, 30000, 0.7)])
+def test_attention_prompt_runs_of_sequences_without_keys(cuda, nh, nkv, hd, long, empty):
+    # rows of sequences that hold no position yet, several to a CTA behind one that has keys; the last two cases are
+    # dealt out by key tiles
+    torch = cuda
+    rng = np.random.default_rng(5)
+    B, page = (100 if nh < 4 else 300), 64
+    q_len = rng.integers(1, 4, B)
+    kv_len = np.where(rng.random(B) < empty, 0, q_len + rng.integers(0, 4, B))
+    kv_len[[0, B // 3]] = q_len[[0, B // 3]] + [long, 1]
+    if empty < 1.0:
+        q_len[B // 2], kv_len[B // 2] = 700, 150  # whole tiles of rows before the first key
+    T = int(q_len.sum())
+    k, v = ([rand(torch, int(n), nkv, hd, dt=torch.float16, seed=c + i) for i, n in enumerate(kv_len)] for c in (0, 900))
+    kp, vp, table = make_pages(torch, k, v, page)
+    q = rand(torch, T, nh, hd, dt=torch.float16, seed=1, scale=2.0)
+    cu_h = np.concatenate([[0], np.cumsum(q_len)])
+    out = torch.full((T, nh, hd), 99.0, dtype=torch.float16, device="cuda")
+    ops.attention_prompt(q, kp, vp, torch.tensor(cu_h, dtype=torch.int32, device="cuda"), page_table=table, out=out,
+                         kv_len=torch.tensor(kv_len, dtype=torch.int32, device="cuda"))
+    assert ops.device_error() == 0  # a role that waited for what could not come would have given up
+    for s in range(B):
+        a, b, n = int(cu_h[s]), int(cu_h[s + 1]), int(kv_len[s])
+        assert (out[a:max(a, b - n)] == 0).all(), f"sequence {s}"
+        if n:
+            want, pv, serr = exact_attention(torch, q[a:b], k[s], v[s], hd ** -0.5, n - (b - a))
+            close(torch, out[a:b], want, pv, serr, n, prompt_weight(torch, torch.float16, n), torch.float16, f"{s}")
+
+
 def test_attention_prompt_many_sequences(cuda):
     torch = cuda
     nh, nkv, hd = 2, 1, 128
