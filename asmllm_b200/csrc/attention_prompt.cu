@@ -803,7 +803,10 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
     Item it;
     for (int k = 0; take_item(k, &it); ++k) {
       const int row = lrow + (pair ? 0 : i * kRows), head = it.head + (pair ? i : 0), tiles = it.tiles[i];
-      const int pos = it.base + row;
+      // A row of the tile that is not the item's is masked like the last one that is (its query is another sequence's,
+      // or what lies behind them), and has no say in when the warp's rows are rescaled.
+      const bool mine = row < it.rows;
+      const int pos = it.base + min(row, it.rows - 1);
       float m = -INFINITY, l = 0.0f;
       bool ok = true;
       for (int j = 0; j < tiles; ++j) {
@@ -828,7 +831,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         const float mt = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
         if (j == 0) {
           m = mt;
-        } else if (__any_sync(kFull, (mt - m) * sl2 > kLazy || m == -INFINITY)) {
+        } else if (__any_sync(kFull, mine && (mt - m) * sl2 > kLazy)) {  // false for a row that has no key yet
           const float mn = fmaxf(m, mt), f = m == -INFINITY ? 0.0f : ex2((m - mn) * sl2);
           m = mn;
           l *= f;
@@ -879,7 +882,6 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         l += s0 + s1;
       }
       if (!ok) break;
-      const bool mine = row < it.rows;
       if (SPLIT && it.slot >= 0) {  // a part of an item: as it is, for the join
         float* part = parts + (size_t)it.slot * part_floats<HD>();
         __stcg(reinterpret_cast<float2*>(part + (size_t)2 * kRows * HD) + i * kRows + lrow, make_float2(m, l));

@@ -673,6 +673,28 @@ def test_attention_prompt_runs_of_sequences_without_keys(cuda, nh, nkv, hd, long
             close(torch, out[a:b], want, pv, serr, n, prompt_weight(torch, torch.float16, n), torch.float16, f"{s}")
 
 
+def test_attention_prompt_bits_do_not_depend_on_what_shared_memory_held(cuda):
+    # sequences of 3 rows and 200 keys, in tiles of 128 of each: the rest of a tile must not change a bit
+    torch = cuda
+    B, n, nh, hd, page = 200, 200, 2, 128, 16
+    k = [rand(torch, n, 1, hd, dt=torch.bfloat16, seed=i) for i in range(B)]
+    kp, vp, table = make_pages(torch, k, k, page)
+    q = rand(torch, 3 * B, nh, hd, dt=torch.bfloat16, seed=1, scale=2.0)
+    cu = torch.arange(B + 1, dtype=torch.int32, device="cuda") * 3
+    kv = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    other = torch.arange(65, dtype=torch.int32, device="cuda") * 512
+    got = []
+    for size in (0.0, 300.0, 0.01):  # keys that a call before this one leaves behind
+        x = rand(torch, 64 * 512, 4, hd, dt=torch.bfloat16, seed=5) * size
+        ops.attention_prompt(x, x, x, other)
+        got.append(ops.attention_prompt(q, kp, vp, cu, kv_len=kv, page_table=table, out_dtype=torch.float32))
+    for size in (0.0, 300.0, float("nan")):  # rows behind the last sequence
+        padded = torch.cat([q, torch.full_like(q[:100], 1.0) * size])
+        got.append(ops.attention_prompt(padded, kp, vp, cu, kv_len=kv, page_table=table, out_dtype=torch.float32)[:3 * B])
+    torch.cuda.synchronize()
+    assert all(torch.equal(got[0], g) for g in got[1:])
+
+
 def test_attention_prompt_many_sequences(cuda):
     torch = cuda
     nh, nkv, hd = 2, 1, 128
