@@ -34,11 +34,13 @@
 //
 // Measured on one B200: 8192 tokens on 32 heads of 128 values, bf16, 460 us =
 // 1.19 PFLOP/s, 0.71 of the cuBLAS rate; 610 with an fp32 output (465 with
-// weights of one rounding there too).  A step (128 keys, both query tiles)
-// takes 3500 cycles; the tensor core's part of it, alone, 2049.  The rest is
-// one tile's chain -- scores, 1900 cycles of softmax, products -- which two
-// tiles in turn do not cover, and tensor memory (S 2 x 128 columns, outputs
-// 2 x 128) has no room for a third.
+// weights of one rounding there too).  head_dim 64: 379 us and 444 with fp32.
+// A step (128 keys, both query tiles) takes 3500 cycles; the tensor core's
+// part of it, alone, 2049, the exponentials' 2048 (both pipes are busy 59 % of
+// the time).  The rest is one tile's chain -- scores, 1900 cycles of softmax,
+// products -- which two tiles in turn do not cover.  Columns 64 to 127 of S
+// are free from the softmax's read on with 16-bit outputs: the next scores of
+// 64 keys could start there.  Not done.
 #include <type_traits>
 
 #include "matvec.cuh"
@@ -57,8 +59,17 @@ constexpr float kLazy = 6.0f;
 constexpr float kPShift = 8.0f;  // weights are 2^kPShift exp(s - m): fp16 keeps those down to 2^-32 of the largest
 constexpr int kThreads = 384;
 // Items are dealt out by key tiles (and joined) where there may be fewer of them than SMs and one may have 16
-// key tiles or more.  Measured (us, by items / by key tiles): 64 items of 4096 keys 61 / 38, 128 of 8192 116 / 87,
-// 96 of 2048 36 / 33; the other way round 128 of 2048 37 / 39, 64 of 1024 22 / 26, 256 of 4096 63 / 97.
+// key tiles or more.  Lengths are on the device, so the rule goes by what the page table (or the packed rows) could
+// hold.  Measured, one packed sequence, bf16, 128 values a head (us, by items / by key tiles; the rule's choice *):
+//   keys   1 head        4            8            16           24           32           40
+//   512    *14.9/17.4   *15.2/18.7   *15.2/19.3   *15.5/19.9   *15.7/20.5   *15.9/22.3   *16.2/22.3
+//   1024   *21.5/21.2   *21.9/23.2   *22.3/25.5   *22.4/25.8   *23.3/28.0   *23.4/30.2   *23.7/35.0
+//   2048   34.5/*31.0   34.9/*27.4   35.4/*29.1   36.9/*39.3   *37.4/51.3   *39.7/62.6   *51.0/74.4
+//   4096   60.6/*36.3   61.4/*38.0   63.3/*55.6   *63.0/97.4   *98/139      *126/178     *159/225
+//   8192   112/*41.7    116/*87.3    *116/156     *228/296     *342/456     *463/636     *585/795
+// It loses at 2048 keys on 16 heads (2.4 us), and where a wide table holds short sequences: a table for 16384
+// positions costs prompts of 1 to 128 rows 3.4 us on 8/1 and 32/32 heads (8.2 -> 11.6 at 33 rows of 32 heads), 512
+// rows 3.2 and 6.4, and up to 40 MB of scratch.
 constexpr int kSplitTiles = 16;
 
 // A row whose output is not finite, computed again in fp32 key by key by one

@@ -111,10 +111,6 @@ inline cudaError_t kernel_setup(const void* kernel, int smem, std::atomic<unsign
 #ifdef __CUDACC__
 
 // ---- the two 16-bit types ----
-template <class T> struct Half2Of;
-template <> struct Half2Of<__half> { using type = __half2; };
-template <> struct Half2Of<__nv_bfloat16> { using type = __nv_bfloat162; };
-
 template <class T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }

@@ -739,8 +739,8 @@ def attention_prompt(q, k, v, cu_q, *, cu_k=None, kv_len=None, page_table=None, 
     [Tk, nkv, hd] with offsets cu_k (cu_q where they are the prompt's own), or the pages of a cache
     [pages, page_size, nkv, hd] with page_table int32 [B, n] and kv_len int32 [B].  The last row of a
     sequence sees all its keys; earlier rows one less each; a row without keys gives zeros.  scale
-    (positive) defaults to hd ** -0.5.  out [T, nh, hd] in q's type or fp32; rows at or past cu_q[B] are
-    not written."""
+    (positive) defaults to hd ** -0.5.  out [T, nh, hd] in q's type or fp32 (whose weights have two 16-bit
+    parts: about a third more time); rows at or past cu_q[B] are not written."""
     if (page_table is None) != (kv_len is None) or (page_table is not None and cu_k is not None):
         raise ValueError("pass page_table and kv_len (paged) or cu_k (packed)")
     device = q.get_device()

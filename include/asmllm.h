@@ -683,7 +683,8 @@ typedef struct asm_kv {
  * sits at position p = len[s] - (cu_q[s+1] - cu_q[s]) + (t - cu_q[s]); len
  * counts the new rows already.  Query and key heads are rotated in
  * interleaved pairs with rope_cs[p] (fp32 [rope_len][head_dim/2][2], as
- * asm_attention_decode_async), rounded to the cache's type and written to
+ * asm_attention_decode_async), rounded to the cache's type (in fp16 a value
+ * of 65520 or more becomes infinity, unreported) and written to
  * q_out [rows][n_heads][head_dim] and to the row's page; values are rounded
  * and written beside the keys.  p < 0: zero query, nothing appended.  p past
  * the table, the rotary table or the pool: the same, and
@@ -711,12 +712,19 @@ ASMLLM_API int asm_attention_prompt_async(const void* q, int64_t q_row_stride, i
                                           const int32_t* cu_q, int32_t rows, int32_t n_heads, float scale, void* out,
                                           int32_t out_dtype, const asm_kv_t* kv, void* stream);
 
-/* Attention of one new token per sequence over its pages: q [batch][n_heads]
+/* Both attentions take infinities and NaN in what a row attends to as fp32
+ * arithmetic does: an infinite value comes out as infinity unless fp32 rounds
+ * its weight to zero (NaN then).  The weights are kept up to 2^14 times their
+ * size, so bf16 values above about 2^96 may overflow the sums.
+ *
+ * Attention of one new token per sequence over its pages: q [batch][n_heads]
  * [head_dim] (strides as above), out [batch][n_heads][head_dim], fp32 or the
- * cache's type; len[s] == 0 gives zeros.  fp32 throughout (the weights enter
- * the product as two 16-bit parts).  workspace: asm_attention_paged_workspace
- * bytes of device memory, 16-byte aligned, whose content need not be set or
- * kept; calls that may overlap need one each. */
+ * cache's type; len[s] == 0 gives zeros.  Scores, maxima, sums and outputs
+ * are fp32; the weights enter the product with the values as two 16-bit parts
+ * (2^-22 of a weight in fp16 down to 2^-39 of the row's largest, 2^-16 in
+ * bf16).  workspace: asm_attention_paged_workspace bytes of device memory,
+ * 16-byte aligned, whose content need not be set or kept; calls that may
+ * overlap need one each. */
 ASMLLM_API int64_t asm_attention_paged_workspace(int32_t batch, int32_t n_heads, int32_t n_kv_heads,
                                                  int32_t head_dim);
 ASMLLM_API int asm_attention_paged_async(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t n_heads,
@@ -730,7 +738,11 @@ ASMLLM_API int asm_attention_paged_async(const void* q, int64_t q_row_stride, in
  * whose predecessors' mass is below top_p times the mass kept so far; min_p
  * keeps the words with w >= min_p; the first word always stays.  tokens[r] =
  * the first kept word, in index order, whose cumulative mass exceeds u[r]
- * times the kept mass.  temperature <= 0: the first maximum, as
+ * times the kept mass.  Masses are multiples of 2^-45 of the largest weight,
+ * computed in 64 bits and added up exactly; a word 32 temperatures or more
+ * below the maximum weighs nothing.  So a token is that of the definition
+ * unless a border lies nearer to a word than those steps, and it is the same
+ * in every call.  temperature <= 0: the first maximum, as
  * asm_rows_argmax_async.  NaN is never chosen; a row of NaN and -inf gives -1.
  * temperature, top_k, top_p, min_p: [rows] each, or NULL for 1, off, 1, 0. */
 ASMLLM_API int asm_rows_sample_async(const void* logits, int32_t dtype, int32_t rows, int32_t n, int64_t stride,
