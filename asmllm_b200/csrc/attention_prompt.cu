@@ -35,8 +35,8 @@
 // Measured on one B200: 8192 tokens on 32 heads of 128 values, bf16, 460 us =
 // 1.19 PFLOP/s, 0.71 of the cuBLAS rate; 610 with an fp32 output (465 with
 // weights of one rounding there too).  head_dim 64: 379 us and 444 with fp32.
-// A step (128 keys, both query tiles) takes 3500 cycles; the tensor core's
-// part of it, alone, 2049, the exponentials' 2048 (both pipes are busy 59 % of
+// A step (128 keys, both query tiles) takes 3400 to 3500 cycles; the tensor core's
+// part of it, alone, 2049, the exponentials' 2048 (both pipes are busy 60 % of
 // the time).  The rest is one tile's chain -- scores, 1900 cycles of softmax,
 // products -- which two tiles in turn do not cover.  Columns 64 to 127 of S
 // are free from the softmax's read on with 16-bit outputs: the next scores of
