@@ -23,9 +23,10 @@
 // with the query heads as rows.  The weights enter the second product as
 // hi + lo 16-bit parts, which leaves 2^-22 of a weight in fp16 (down to 2^-39
 // of the row's largest) and 2^-16 in bf16; a group of up to 8 heads fills rows
-// 0-7 with hi and rows 8-15 with lo, and the product costs nothing extra.  Values that are infinite take another way (add_values): hi and lo
-// differ in sign, so their products with an infinity would add up to NaN.
-// Looking for them costs 1 us of the 28 below, nothing of the 355.
+// 0-7 with hi and rows 8-15 with lo, and the product costs nothing extra.
+// Infinite values take another way (add_values): lo may be negative or zero,
+// and then its product with an infinity makes NaN of the sum.  Looking for
+// them costs 1 us of the 29 below, nothing of the 355.
 //
 // Measured on one B200: 64 sequences of up to 16384 positions, 64 query on 8
 // KV heads of 128 values (2.26 GB), 355 us = 6.4 TB/s, 0.99 of the copy rate;
@@ -428,7 +429,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
           for (int k = 0; k < 2; ++k)
             keep[k] = (k * 8 + c2 < left ? 0xFFFFu : 0u) | (k * 8 + c2 + 1 < left ? 0xFFFF0000u : 0u);
         }
-        // The two parts of a weight differ in sign or one is zero, so an infinite value would come out as NaN:
+        // The second part of a weight may be negative or zero, so an infinite value would come out as NaN:
         // 16 N values of each position among which there is one (or a NaN) are summed weight by weight.
         constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
         constexpr int N = ROWS == 8 ? HD / 16 : 2;  // registers: with 16 rows all at once spill
