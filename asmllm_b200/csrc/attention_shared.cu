@@ -1,0 +1,803 @@
+// asmllm_b200/csrc/attention_shared.cu -- attention of one new token per
+// sequence over a paged cache in which groups of sequences begin with the same
+// pages, read once for the whole group.
+//
+// The result is that of attention_paged.cu: softmax is split at the end of
+// the shared positions, and the two sides are joined by their maxima and sums.
+//   1. Shared pass (here): a group's query rows, (sequences x heads of a KV
+//      head), against its shared positions: a matrix product of up to 256 rows
+//      a key tile on the 5th-generation tensor cores.
+//   2. Own pass (attention_paged.cu): every sequence's positions behind those.
+//      It does not wait for the first, and runs on the SMs that has left.
+//   3. Join: a row's parts, in order.
+//
+// Shared pass.  A unit is (group, KV head, 256 rows); its positions are tiles
+// of 128, and the tiles of all units in a row are cut into one equal range per
+// CTA, one CTA an SM.  Two streams of four warps take maximum, exponentials
+// and sum, one thread a row, while the tensor core works for the other: with
+// more than 128 rows the streams have 128 rows each and the same keys, with
+// fewer the same rows and every other key tile.  Scores, weights (over the
+// scores) and outputs are in tensor memory.  Weights are rounded once to 16
+// bits where the output is, and are two 16-bit parts (2^-22 of a weight in
+// fp16, 2^-16 in bf16) for an fp32 output, as in attention_prompt.cu; the
+// output is rescaled only when a row's maximum has risen by more than 2^kLazy.
+//
+// CTA, 12 warps: 0-3 and 4-7 the streams (they also bring their queries into
+// shared memory), 8 tcgen05.mma issue by one elected thread, 9 tensor copies
+// of K and V tiles into a ring (a page behind the shared ones reads as zeros).
+// Every wait is bounded, as in attention_prompt.cu.
+#include <type_traits>
+
+#include "matvec.cuh"
+#include "mma16.cuh"
+#include "pipeline.cuh"
+#include "shared_prefix.cuh"
+#include "serving_q8.cuh"
+#include "tensor_map.cuh"
+#include "tmem.cuh"
+
+namespace asmllm {
+
+namespace {
+
+constexpr int kRows = 128;       // rows of a stream, positions of a key tile
+constexpr int kUnit = 2 * kRows; // rows of a unit
+constexpr float kLazy = 6.0f;
+constexpr float kPShift = 8.0f;  // weights are 2^kPShift exp(s - m)
+constexpr int kThreads = 384;
+constexpr int kMaxCtas = 160;
+
+// Where the shared pass leaves its results, unnormalised: whole units by row, twice (the streams of a unit of up to
+// 128 rows have a result each), parts in slots of kUnit rows.
+struct SharedParts {
+  float* o;       // [2][batch][n_heads][head_dim]
+  float2* ml;     // [2][batch][n_heads]: maximum in units of log2, sum
+  float* slots;   // [kMaxCtas][2] of kUnit x head_dim, then kUnit (maximum, sum)
+  Found* found;   // [n_kv][found_stride]: unit_index()
+  int found_stride;
+};
+template <int HD>
+__host__ __device__ constexpr size_t part_floats() { return (size_t)kUnit * HD + 2 * kUnit; }
+// Units of a KV head are numbered so that no two groups meet: rows before them / kUnit + groups before them.
+__device__ __forceinline__ int unit_index(int first_row, int group, int blk) { return first_row / kUnit + group + blk; }
+
+template <int HD>
+struct Cfg {
+  static constexpr int kTileBytes = kRows * HD * 2;
+  static constexpr int kStages = HD == 128 ? 5 : 8;
+  static constexpr int kRing = 2 * kTileBytes;
+  static constexpr int kBars = kRing + kStages * kTileBytes;
+  static constexpr int kNBars = 2 * kStages + 2 + 2 + 4 + 2 + 1;
+  static constexpr int kSum = kBars + kNBars * 8 + 16;
+  static constexpr int kSmem = kSum + 64 + 1024;
+  static constexpr uint32_t kO = 2 * kRows;  // tensor memory: S0, S1, then the two outputs
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+// Operand descriptors, 128-byte swizzle (as in attention_prompt.cu).
+constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
+constexpr uint32_t kLeading = ((kRows * 128) >> 4) << 16;
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr) { return ((addr >> 4) & 0x3FFFu) | kLeading; }
+__device__ __forceinline__ uint64_t desc64(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+
+// Exchange of 16-byte pieces within four lanes (lane = row, w = columns of a 4 x 4 matrix): its transpose.
+__device__ __forceinline__ float4 shfl_xor4(float4 v, int mask) {
+  return make_float4(__shfl_xor_sync(kFull, v.x, mask), __shfl_xor_sync(kFull, v.y, mask),
+                     __shfl_xor_sync(kFull, v.z, mask), __shfl_xor_sync(kFull, v.w, mask));
+}
+__device__ __forceinline__ void transpose4(float4 (&w)[4], int lane) {
+  const bool odd = lane & 1, high = lane & 2;
+#pragma unroll
+  for (int q = 0; q < 4; q += 2) {
+    const float4 t = shfl_xor4(odd ? w[q] : w[q + 1], 1);
+    if (odd) w[q] = t; else w[q + 1] = t;
+  }
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const float4 t = shfl_xor4(high ? w[q] : w[q + 2], 2);
+    if (high) w[q] = t; else w[q + 2] = t;
+  }
+}
+
+// A CTA's walk: group, unit (KV head, block of rows), key tile.
+struct Tour {
+  int grp, b, rows, shared;  // the group, its first sequence, its query rows of a KV head, its positions
+  int nb, nt, u, t;          // blocks a KV head, key tiles, unit of the group, tile of the unit
+  long long first, at, end;  // number of the unit's first tile; tiles [at, end) are left
+};
+
+struct Segment {
+  int head, blk, t0, n, rows;  // KV head, block, first tile, tiles, rows of the block
+  bool two, whole;             // streams of different rows; nothing of the unit is in another CTA
+};
+__device__ __forceinline__ Segment segment_of(const Tour& w) {
+  Segment x;
+  x.head = w.u / w.nb;
+  x.blk = w.u % w.nb;
+  x.t0 = w.t;
+  x.n = (int)min((long long)(w.nt - w.t), w.end - w.at);
+  x.rows = min(kUnit, w.rows - x.blk * kUnit);
+  x.two = x.rows > kRows;
+  x.whole = x.t0 == 0 && x.n == w.nt;
+  return x;
+}
+
+template <class T, bool TWO, int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                        const PagedArgs a, const KvArgs kv, const SharedView v, const SharedParts parts, int box_rows,
+                        unsigned* __restrict__ err) {
+  using C = Cfg<HD>;
+  constexpr int kHalves = HD / 64, S = C::kStages;
+  constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
+  constexpr uint32_t kIdescS = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((kRows >> 3) << 17) | ((kRows >> 4) << 24);
+  constexpr uint32_t kIdescO =
+      (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((kRows >> 4) << 24);
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBars);
+  uint64_t* kv_full = bars;
+  uint64_t* kv_empty = kv_full + S;
+  uint64_t* q_full = kv_empty + S;  // [2] a stream's queries are in shared memory
+  uint64_t* s_full = q_full + 2;    // [2] scores of a tile are in tensor memory
+  uint64_t* p_full = s_full + 2;    // [2][2] the weights of its first and second 64 keys are
+  uint64_t* o_full = p_full + 4;    // [2] the segment's output is complete
+  uint64_t* drain = o_full + 2;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile uint32_t* s_abort = s_tmem + 1;
+  long long* s_sum = reinterpret_cast<long long*>(smem);  // per-thread sums, before the queries come
+  long long* s_total = reinterpret_cast<long long*>(smem + C::kSum);
+  long long* s_first = s_total + 1;
+  int* s_group = reinterpret_cast<int*>(s_total + 2);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = a.n_heads / kv.n_kv;
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 0) {
+    prefetch_map(&kmap);
+    prefetch_map(&vmap);
+    for (int i = 0; i < S; ++i) {
+      mbar_init(smem_u32(kv_full + i), 1);
+      mbar_init(smem_u32(kv_empty + i), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(q_full + i), 4);
+      mbar_init(smem_u32(s_full + i), 1);
+      mbar_init(smem_u32(p_full + 2 * i), 4);
+      mbar_init(smem_u32(p_full + 2 * i + 1), 4);
+      mbar_init(smem_u32(o_full + i), 1);
+    }
+    mbar_init(smem_u32(drain), 1);
+    *s_abort = 0u;
+    fence_mbar_init();
+  }
+  // The next launch, the own pass, does not wait for this one: it may begin once everything before this one is over.
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- this CTA's range: the groups' tiles, a contiguous share of the groups per thread ----
+  auto load = [&](int grp, Tour* x, bool report) -> long long {
+    int b, e;
+    const bool ok = group_of(v, kv, grp, &b, &e, &x->shared);
+    if (!ok && report) atomicOr(err, kErrDecodeRange);
+    x->grp = grp;
+    x->b = b;
+    x->rows = (e - b) * g;
+    x->nb = (x->rows + kUnit - 1) / kUnit;
+    x->nt = (x->shared + kRows - 1) / kRows;
+    return (long long)x->nb * x->nt * kv.n_kv;
+  };
+  Tour w;
+  {
+    const int per = (v.groups + kThreads - 1) / kThreads, q0 = min(v.groups, tid * per), q1 = min(v.groups, q0 + per);
+    long long mine = 0;
+    for (int x = q0; x < q1; ++x) mine += load(x, &w, blockIdx.x == 0);
+    s_sum[tid] = mine;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 0) {
+      long long run = 0;
+      for (int c = 0; c < kThreads; c += 32) {
+        const long long y = s_sum[c + lane];
+        long long x = y;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long z = __shfl_up_sync(kFull, x, o);
+          if (lane >= o) x += z;
+        }
+        s_sum[c + lane] = run + x - y;  // exclusive
+        run += __shfl_sync(kFull, x, 31);
+      }
+      if (lane == 0) *s_total = run;
+    }
+    __syncthreads();
+    const int ctas = (int)min((long long)gridDim.x, *s_total);
+    const Deal deal(*s_total, max(1, ctas));
+    w.at = (int)blockIdx.x < ctas ? deal.start(blockIdx.x) : 0;
+    w.end = (int)blockIdx.x < ctas ? deal.start(blockIdx.x + 1) : 0;
+    const long long at = w.at, end = w.end;
+    if (at < end && s_sum[tid] <= at && at < s_sum[tid] + mine) {
+      long long x = s_sum[tid];
+      for (int y = q0; y < q1; ++y) {
+        const long long z = load(y, &w, false);
+        if (at < x + z) {
+          *s_group = y;
+          *s_first = x;
+          break;
+        }
+        x += z;
+      }
+    }
+    __syncthreads();
+    if (at < end) {
+      load(*s_group, &w, false);
+      w.u = (int)((at - *s_first) / w.nt);
+      w.first = *s_first + (long long)w.u * w.nt;
+      w.t = (int)(at - w.first);
+    }
+    w.at = at;
+    w.end = end;
+  }
+  const uint32_t tmem = *s_tmem;
+  // behind the segment of n tiles: the next unit, of this group or the next one that shares something
+  auto advance = [&](int n) {
+    w.at += n;
+    if (w.at >= w.end) return;
+    w.t = 0;
+    w.first += w.nt;
+    if (++w.u == w.nb * kv.n_kv) {
+      w.u = 0;
+      do {
+      } while (load(w.grp + 1, &w, false) == 0);
+    }
+  };
+  auto fail = [&]() {
+    *s_abort = 1u;
+    atomicOr(err, kErrRingTimeout);
+  };
+  // Warp-wide wait; false (in every lane) when the role has to leave.
+  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    if (__all_sync(kFull, mbar_try_wait(smem_u32(bar), parity))) return true;
+    const bool ok = mbar_wait_bounded(smem_u32(bar), parity);
+    if (!ok) fail();
+    return !__any_sync(kFull, !ok || *s_abort);
+  };
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 9) {
+      // ---------------- loader ----------------
+      const int pages = kRows / box_rows, my_page = lane / kHalves, half = lane % kHalves;
+      const uint32_t box_bytes = (uint32_t)box_rows * 128u;
+      int c = 0;
+      bool ok = true;
+      while (ok && w.at < w.end) {
+        const Segment x = segment_of(w);
+        // page of this lane's box in tile j of the segment; n_pages reads as zeros
+        auto lookup = [&](int j) -> int {
+          const int p = (x.t0 + j) * kRows + my_page * box_rows;
+          if (my_page >= pages || j >= x.n) return -1;
+          if (p >= w.shared) return kv.n_pages;
+          const int page = __ldcg(kv.table + (long long)w.b * kv.table_stride + (p >> kv.page_shift));
+          if ((unsigned)page < (unsigned)kv.n_pages) return page;
+          atomicOr(err, kErrDecodeRange);
+          return kv.n_pages;
+        };
+        int page = lookup(0);
+        for (int j = 0; j < x.n && ok; ++j) {
+          const int cur = page;
+          page = lookup(j + 1);
+          const int row = ((x.t0 + j) * kRows + my_page * box_rows) & (kv.page_size - 1);
+          for (int y = 0; y < 2; ++y, ++c) {
+            const int st = c % S;
+            if (c >= S && !(ok = wait(kv_empty + st, ((c / S) - 1) & 1))) break;
+            const uint32_t bar = smem_u32(kv_full + st);
+            if (lane == 0) mbar_arrive_expect_tx(bar, C::kTileBytes);
+            __syncwarp();
+            if (cur >= 0)
+              tma_load_4d(smem_u32(smem) + C::kRing + st * C::kTileBytes + half * (kRows * 128) + my_page * box_bytes,
+                          y ? &vmap : &kmap, half * 64, row, x.head, cur, bar);
+          }
+        }
+        advance(x.n);
+      }
+      // what was issued lands before the CTA may end (bounded)
+      for (int j = c - S < 0 ? 0 : c - S; j < c; ++j) mbar_wait_bounded(smem_u32(kv_full + j % S), (j / S) & 1);
+    } else if (warp == 8 && elect_one()) {
+      // ---------------- matrix products (one thread) ----------------
+      const uint32_t q_lo = desc_lo(smem_u32(smem)), ring_lo = desc_lo(smem_u32(smem) + C::kRing);
+      constexpr uint32_t kTileLo = C::kTileBytes >> 4;
+      uint32_t nq = 0, np = 0;  // parities, one bit a stream
+      int c = 0;                // ring entries before this segment
+      bool ok = true, issued = false;
+      auto get = [&](uint64_t* bar, uint32_t parity) { return ok = ok && mbar_wait_bounded(smem_u32(bar), parity); };
+      auto get_tile = [&](int e) { return get(kv_full + e % S, (e / S) & 1); };
+      auto release = [&](int e) { umma_commit(smem_u32(kv_empty + e % S)); };
+      // scores of stream i against the keys in ring entry e
+      auto scores = [&](int i, int e, bool first) {
+        if (first) {
+          if (!get(q_full + i, nq >> i & 1)) return;
+          nq ^= 1u << i;
+        }
+        if (!get_tile(e)) return;
+        tc_fence_after();
+        const uint32_t ql = q_lo + i * kTileLo, kl = ring_lo + (e % S) * kTileLo;
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * ((kRows * 128) >> 4) + (ks & 3) * 2;
+          umma_ss(tmem + i * kRows, desc64(ql + off, kDescHi), desc64(kl + off, kDescHi), kIdescS, ks > 0);
+        }
+        umma_commit(smem_u32(s_full + i));
+        issued = true;
+      };
+      // stream i's weights times the values in ring entry e
+      auto values = [&](int i, int e, bool first, bool last) {
+        if (!get_tile(e)) return;
+        const uint32_t vl = ring_lo + (e % S) * kTileLo;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // the first 64 keys while the weights of the others are computed
+          if (!get(p_full + 2 * i + h, np >> i & 1)) return;
+          tc_fence_after();
+#pragma unroll
+          for (int ks = 4 * h; ks < 4 * h + 4; ++ks) {
+            umma_ts(tmem + C::kO + i * HD, tmem + i * kRows + ks * 8, desc64(vl + ks * (2048 >> 4), kDescHi), kIdescO,
+                    ks > 0 || !first);
+            if constexpr (TWO)
+              umma_ts(tmem + C::kO + i * HD, tmem + i * kRows + kRows / 2 + ks * 8,
+                      desc64(vl + ks * (2048 >> 4), kDescHi), kIdescO, true);
+          }
+        }
+        np ^= 1u << i;
+        if (last) umma_commit(smem_u32(o_full + i));
+      };
+      while (ok && w.at < w.end) {
+        const Segment x = segment_of(w);
+        if (x.two) {  // both streams have all tiles
+          for (int j = 0; j <= x.n && ok; ++j) {
+#pragma unroll 1
+            for (int i = 0; i < 2 && ok; ++i) {
+              if (j > 0) values(i, c + 2 * j - 1, j == 1, j == x.n);
+              if (ok && j > 0 && i == 1) release(c + 2 * j - 1);
+              if (ok && j < x.n) scores(i, c + 2 * j, j == 0);
+              if (ok && j < x.n && i == 1) release(c + 2 * j);
+            }
+          }
+        } else {  // every other one
+          for (int j = 0; j < x.n + 2 && ok; ++j) {
+            if (j >= 2) {
+              values(j & 1, c + 2 * (j - 2) + 1, j < 4, j >= x.n);
+              if (ok) release(c + 2 * (j - 2) + 1);
+            }
+            if (ok && j < x.n) {
+              scores(j & 1, c + 2 * j, j < 2);
+              if (ok) release(c + 2 * j);
+            }
+          }
+        }
+        c += 2 * x.n;
+        advance(x.n);
+      }
+      if (!ok) fail();
+      if (issued) {  // the tensor core is done before tensor memory is released
+        umma_commit(smem_u32(drain));
+        if (!mbar_wait_bounded(smem_u32(drain), 0)) fail();
+      }
+    }
+  } else {
+    // ---------------- softmax ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    const int i = warp >> 2, lrow = 32 * (warp & 3) + lane;
+    const uint32_t ts = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + i * kRows;
+    const uint32_t to = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + C::kO + i * HD;
+    const float sl2 = a.scale * 1.4426950408889634f;
+    const long long begin = w.at;
+    int ns = 0, no = 0;
+    bool ok = true;
+    while (ok && w.at < w.end) {
+      const Segment x = segment_of(w);
+      const int row = lrow + (x.two ? i * kRows : 0), tiles = x.two ? x.n : (x.n + 1 - i) >> 1;
+      const bool mine = row < x.rows;
+      const int rr = x.blk * kUnit + row, seq = w.b + rr / g, head = x.head * g + rr % g;
+      const int slot = 2 * blockIdx.x + (w.at == begin ? 0 : 1);
+      if (x.t0 == 0 && tid == 0) {  // where the unit's results are
+        const int last = (int)blockIdx.x;
+        Found f;
+        f.parts = 1;
+        f.cta = last;
+        f.slot = slot;
+        f.pad = 0;
+        if (!x.whole) {
+          const int ctas = (int)min((long long)gridDim.x, *s_total);
+          f.parts = Deal(*s_total, ctas).cta_of(w.first + w.nt - 1) - last + 1;
+        }
+        __stcg(reinterpret_cast<int4*>(parts.found + (long long)x.head * parts.found_stride +
+                                       unit_index(w.b * g, w.grp, x.blk)),
+               make_int4(f.parts, f.cta, f.slot, 0));
+      }
+      float m = -INFINITY, l = 0.0f;
+      if (tiles > 0) {
+        // Queries: this warp's 32 rows, a row's pieces in consecutive lanes.  What was read from the buffer before has
+        // been: the last segment's last scores were waited for.
+        {
+          constexpr int P = HD / 8, N = 32 / P;  // pieces of a row, rows at a time
+          const long long mine_at = mine ? (long long)seq * a.q_row_stride + (long long)head * a.q_head_stride : -1;
+          unsigned char* sq = smem + i * C::kTileBytes;
+          uint4 y[32 / N];
+#pragma unroll
+          for (int k = 0; k < 32 / N; ++k) {
+            const int rw = k * N + lane / P;
+            const long long at = __shfl_sync(kFull, mine_at, rw);
+            y[k] = make_uint4(0u, 0u, 0u, 0u);
+            if (at >= 0) y[k] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at) + lane % P);
+          }
+#pragma unroll
+          for (int k = 0; k < 32 / N; ++k) {
+            const int rw = 32 * (warp & 3) + k * N + lane / P, ch = lane % P;
+            *reinterpret_cast<uint4*>(sq + (ch >> 3) * (kRows * 128) + rw * 128 + (((ch & 7) ^ (rw & 7)) << 4)) = y[k];
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(q_full + i));
+        }
+        for (int j = 0; j < tiles; ++j) {
+          if (!(ok = wait(s_full + i, ns & 1))) break;
+          ++ns;
+          tc_fence_after();
+          uint32_t y[kRows];
+#pragma unroll
+          for (int b = 0; b < kRows; b += 32) tmem_ld<32>(ts + b, *reinterpret_cast<uint32_t(*)[32]>(y + b));
+          tmem_wait_ld();
+          const int limit = w.shared - (x.t0 + (x.two ? j : 2 * j + i)) * kRows;  // columns below it exist
+          if (limit < kRows) {
+#pragma unroll
+            for (int e = 0; e < kRows; ++e)
+              if (e >= limit) y[e] = 0xFF800000u;
+          }
+          float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < kRows; e += 8)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              t[q] = max3(t[q], __uint_as_float(y[e + 2 * q]), __uint_as_float(y[e + 2 * q + 1]));
+          const float mt = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+          if (j == 0) {
+            m = mt;
+          } else if (__any_sync(kFull, mine && (mt - m) * sl2 > kLazy)) {
+            const float mn = fmaxf(m, mt), f = m == -INFINITY ? 0.0f : ex2((m - mn) * sl2);
+            m = mn;
+            l *= f;
+            const unsigned long long f2 = pack2(f, f);
+#pragma unroll 1
+            for (int b = 0; b < HD; b += 32) {
+              uint32_t z[32];
+              tmem_ld<32>(to + b, z);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                float z0, z1;
+                unpack2(mul2(pack2(__uint_as_float(z[e]), __uint_as_float(z[e + 1])), f2), z0, z1);
+                z[e] = __float_as_uint(z0);
+                z[e + 1] = __float_as_uint(z1);
+              }
+              tmem_st32(to + b, z);
+            }
+          }
+          const float off = kPShift - (m == -INFINITY ? 0.0f : m * sl2);
+          const unsigned long long sl22 = pack2(sl2, sl2), off2 = pack2(off, off);
+          unsigned long long sum[2] = {0ull, 0ull};
+#pragma unroll
+          for (int b = 0; b < kRows; b += 64) {
+            uint32_t p[32], p2[32];
+#pragma unroll
+            for (int e = 0; e < 64; e += 2) {
+              float x0, x1;
+              unpack2(fma2(pack2(__uint_as_float(y[b + e]), __uint_as_float(y[b + e + 1])), sl22, off2), x0, x1);
+              x0 = ex2(x0);
+              x1 = ex2(x1);
+              sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(x0, x1));
+              p[e >> 1] = pack16<T>(x0, x1);
+              if constexpr (TWO) {
+                const float2 q = unpack16<T>(p[e >> 1]);
+                p2[e >> 1] = pack16<T>(x0 - q.x, x1 - q.y);
+              }
+            }
+            tmem_st32(ts + (b >> 1), p);
+            if constexpr (TWO) tmem_st32(ts + kRows / 2 + (b >> 1), p2);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(p_full + 2 * i + (b >> 6)));
+          }
+          float s0, s1;
+          unpack2(add2(sum[0], sum[1]), s0, s1);
+          l += s0 + s1;
+        }
+        if (!ok) break;
+      }
+      // Results: o 2^ml.x is the sum of exp(s) v, l 2^ml.x of exp(s).  A thread holds a row; pieces of 16 bytes are
+      // exchanged within four lanes, so that a store writes 64 bytes of a row.
+      const long long at = ((long long)seq + (x.two ? 0 : (long long)i * kv.batch)) * a.n_heads + head;
+      float* slot_o = parts.slots + (size_t)slot * part_floats<HD>();
+      const float2 ml = make_float2(m == -INFINITY ? -INFINITY : m * sl2 - kPShift, l);
+      if (mine) {
+        if (x.whole) __stcg(parts.ml + at, ml);
+        else __stcg(reinterpret_cast<float2*>(slot_o + (size_t)kUnit * HD) + i * kRows + lrow, ml);
+      }
+      if (tiles > 0) {
+        if (!(ok = wait(o_full + i, no & 1))) break;
+        ++no;
+        tc_fence_after();
+        float* base = x.whole ? parts.o + at * HD : slot_o + (size_t)(i * kRows + lrow) * HD;
+        float* to4[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          to4[q] = reinterpret_cast<float*>(__shfl_sync(kFull, mine ? reinterpret_cast<unsigned long long>(base) : 0ull,
+                                                        (lane & ~3) + q));
+#pragma unroll 1
+        for (int b = 0; b < HD; b += 32) {
+          uint32_t z[32];
+          tmem_ld<32>(to + b, z);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; e += 16) {
+            float4 p[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              p[q] = make_float4(__uint_as_float(z[e + 4 * q]), __uint_as_float(z[e + 4 * q + 1]),
+                                 __uint_as_float(z[e + 4 * q + 2]), __uint_as_float(z[e + 4 * q + 3]));
+            transpose4(p, lane);  // p[q]: piece lane % 4 of the four lanes' row q
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (to4[q]) __stcg(reinterpret_cast<float4*>(to4[q] + b + e) + (lane & 3), p[q]);
+          }
+        }
+        tc_fence_before();
+      }
+      advance(x.n);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// Joins a row's parts: those of its own positions, then of the shared ones.  WARPS warps a row (8 or 1) take
+// every WARPS-th part.
+template <class O, int HD, int WARPS>
+__global__ void __launch_bounds__(256) attention_shared_join_kernel(const PagedArgs a, const KvArgs kv,
+                                                                    const SharedView v, const SharedParts parts,
+                                                                    int zs) {
+  constexpr int E = HD / 32;
+  __shared__ float s_o[8][HD];
+  __shared__ float2 s_ml[8];
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = a.n_heads / kv.n_kv;
+  const long long row = WARPS == 8 ? blockIdx.x : (long long)blockIdx.x * 8 + warp;
+  if (row >= (long long)kv.batch * a.n_heads) return;
+  const int s = (int)(row / a.n_heads), h = (int)(row % a.n_heads), j = h / g, in = h % g, R = g <= 8 ? 8 : 16;
+  bool clipped;
+  int grp, b = 0, e = 0, shared;
+  const int n = kv_length(kv, s, &clipped), base = shared_base(v, kv, s, n, &grp);
+  const Found own = [&] {
+    const int4 x = __ldcg(reinterpret_cast<const int4*>(v.own_found + ((long long)s * kv.n_kv + j) * zs + in / 16));
+    return Found{x.x, x.y, x.z, 0};
+  }();
+  Found f = {0, 0, 0, 0};
+  int local = 0, streams = 1;
+  if (base > 0) {
+    group_of(v, kv, grp, &b, &e, &shared);
+    const int rr = (s - b) * g + in, blk = rr / kUnit;
+    local = rr % kUnit;
+    streams = min(kUnit, (e - b) * g - blk * kUnit) > kRows ? 1 : 2;
+    const int4 x = __ldcg(reinterpret_cast<const int4*>(parts.found + (long long)j * parts.found_stride +
+                                                        unit_index(b * g, grp, blk)));
+    f = {x.x, x.y, x.z, 0};
+  }
+  const int total = own.parts + f.parts * streams;
+  // part p: its output row, and its (maximum, sum)
+  auto find = [&](int p, const float** o) -> float2 {
+    if (p < own.parts) {
+      if (own.parts == 1) {
+        *o = v.own_o + row * HD;
+        float2 ml = __ldcg(v.own_ml + row);
+        ml.x -= kShift;
+        return ml;
+      }
+      const float* slot = v.own_slots + (size_t)(p ? 2 * (own.cta + p) : own.slot) * (size_t)slot_floats(R, HD);
+      const int x = in % 16;
+      *o = slot + x * HD;
+      return make_float2(__ldcg(slot + R * HD + x) - kShift, __ldcg(slot + R * HD + R + x));
+    }
+    p -= own.parts;
+    const int i = streams == 2 ? p & 1 : 0, k = streams == 2 ? p >> 1 : p;
+    if (f.parts == 1) {
+      const long long at = row + (long long)i * kv.batch * a.n_heads;
+      *o = parts.o + at * HD;
+      return __ldcg(parts.ml + at);
+    }
+    const float* slot = parts.slots + (size_t)(k ? 2 * (f.cta + k) : f.slot) * part_floats<HD>();
+    *o = slot + (size_t)(local + i * kRows) * HD;
+    return __ldcg(reinterpret_cast<const float2*>(slot + (size_t)kUnit * HD) + local + i * kRows);
+  };
+  float m = -INFINITY, l = 0.0f, o[E] = {};
+  const int start = WARPS == 8 ? warp : 0;
+  for (int p0 = start; p0 < total; p0 += 32 * WARPS) {  // a part per lane for the maxima, then its output with all lanes
+    const float* at = nullptr;
+    const int p = p0 + lane * WARPS;
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (p < total) ml = find(p, &at);
+    float mn = ml.y == 0.0f ? -INFINITY : ml.x;  // nothing in it: there may be no output either
+    const bool live = p < total && !(ml.x == -INFINITY && ml.y == 0.0f);
+#pragma unroll
+    for (int q = 16; q > 0; q >>= 1) mn = fmaxf(mn, __shfl_xor_sync(kFull, mn, q));
+    mn = fmaxf(mn, m);
+    const float mz = mn == -INFINITY ? 0.0f : mn, f0 = ex2(m - mz), f1 = live ? ex2(ml.x - mz) : 0.0f;
+    m = mn;
+    l = l * f0 + warp_sum(f1 * ml.y);
+#pragma unroll
+    for (int q = 0; q < E; ++q) o[q] *= f0;
+    const int count = min(32, (total - p0 + WARPS - 1) / WARPS);
+#pragma unroll 8
+    for (int q = 0; q < count; ++q) {
+      const float* src = reinterpret_cast<const float*>(__shfl_sync(kFull, live ? reinterpret_cast<unsigned long long>(at) : 0ull, q));
+      const float wt = __shfl_sync(kFull, f1, q);
+      if (src) {
+#pragma unroll
+        for (int z = 0; z < E; z += 2) {
+          const float2 y = __ldcg(reinterpret_cast<const float2*>(src + lane * E + z));
+          o[z] = fmaf(wt, y.x, o[z]);
+          o[z + 1] = fmaf(wt, y.y, o[z + 1]);
+        }
+      }
+    }
+  }
+  if constexpr (WARPS == 8) {
+#pragma unroll
+    for (int q = 0; q < E; ++q) s_o[warp][lane * E + q] = o[q];
+    if (lane == 0) s_ml[warp] = make_float2(m, l);
+    __syncthreads();
+    if (warp) return;
+    m = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) m = fmaxf(m, s_ml[x].x);
+    const float mz = m == -INFINITY ? 0.0f : m;
+    l = 0.0f;
+#pragma unroll
+    for (int q = 0; q < E; ++q) o[q] = 0.0f;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const float fx = ex2(s_ml[x].x - mz);
+      l = fmaf(fx, s_ml[x].y, l);
+#pragma unroll
+      for (int q = 0; q < E; ++q) o[q] = fmaf(fx, s_o[x][lane * E + q], o[q]);
+    }
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  O* out = static_cast<O*>(a.out) + row * HD + lane * E;
+#pragma unroll
+  for (int z = 0; z < E; z += 2) {
+    if constexpr (sizeof(O) == 4) *reinterpret_cast<float2*>(out + z) = make_float2(o[z] * inv, o[z + 1] * inv);
+    else *reinterpret_cast<uint32_t*>(out + z) = pack16<O>(o[z] * inv, o[z + 1] * inv);
+  }
+}
+
+// Workspace: all parts, 16-byte aligned.
+struct Space {
+  size_t slots, o, ml, found, own_slots, own_o, own_ml, own_found, bytes;
+  int found_stride, zs;
+};
+Space space_of(int batch, int groups, int n_heads, int n_kv, int head_dim) {
+  Space x;
+  const size_t rows = (size_t)batch * n_heads;
+  const int g = n_heads / n_kv;
+  x.zs = (g + 15) / 16;
+  x.found_stride = (int)((long long)batch * g / kUnit) + groups + 1;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t was = at;
+    at += (bytes + 15) / 16 * 16;
+    return was;
+  };
+  x.slots = take((size_t)kMaxCtas * 2 * (head_dim == 128 ? part_floats<128>() : part_floats<64>()) * 4);
+  x.o = take(2 * rows * head_dim * 4);
+  x.ml = take(2 * rows * 8);
+  x.found = take((size_t)n_kv * x.found_stride * sizeof(Found));
+  x.own_slots = take(own_slots_floats(n_heads, n_kv, head_dim) * 4);
+  x.own_o = take(rows * head_dim * 4);
+  x.own_ml = take(rows * 8);
+  x.own_found = take((size_t)batch * n_kv * x.zs * sizeof(Found));
+  x.bytes = at;
+  return x;
+}
+
+template <class T, class O, int HD>
+cudaError_t launch_typed(const SharedArgs& sa, const KvArgs& kv, cudaStream_t stream, unsigned* err) {
+  using C = Cfg<HD>;
+  const PagedArgs& a = sa.paged;
+  auto kernel = attention_shared_kernel<T, sizeof(O) == 4, HD>;
+  const Space sp = space_of(kv.batch, sa.groups, a.n_heads, kv.n_kv, HD);
+  unsigned char* ws = static_cast<unsigned char*>(a.workspace);
+  SharedView v;
+  v.cu_group = sa.cu_group;
+  v.shared_len = sa.shared_len;
+  v.groups = sa.groups;
+  v.own_o = reinterpret_cast<float*>(ws + sp.own_o);
+  v.own_ml = reinterpret_cast<float2*>(ws + sp.own_ml);
+  v.own_found = reinterpret_cast<Found*>(ws + sp.own_found);
+  v.own_slots = reinterpret_cast<float*>(ws + sp.own_slots);
+  SharedParts parts;
+  parts.o = reinterpret_cast<float*>(ws + sp.o);
+  parts.ml = reinterpret_cast<float2*>(ws + sp.ml);
+  parts.slots = reinterpret_cast<float*>(ws + sp.slots);
+  parts.found = reinterpret_cast<Found*>(ws + sp.found);
+  parts.found_stride = sp.found_stride;
+  CUtensorMap kmap, vmap;
+  const int box_rows = kv.page_size < kRows ? kv.page_size : kRows;
+  if (!encode_kv_map(&kmap, kv, kv.k, box_rows) || !encode_kv_map(&vmap, kv, kv.v, box_rows))
+    return cudaErrorInvalidValue;
+  static std::atomic<unsigned long long> done{0};
+  int sms = 0;
+  cudaError_t e = kernel_setup(reinterpret_cast<const void*>(kernel), C::kSmem, done, &sms);
+  if (e != cudaSuccess) return e;
+  // What is known here bounds the tiles: units of all groups, key tiles by what the page table can hold.
+  const long long units = ((long long)kv.batch * (a.n_heads / kv.n_kv) / kUnit + sa.groups) * kv.n_kv;
+  const long long most = units * (((long long)kv.width * kv.page_size + kRows - 1) / kRows);
+  long long ctas = sms < kMaxCtas ? sms : kMaxCtas;
+  if (ctas > most) ctas = most < 1 ? 1 : most;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = g_opt_pdl.load() ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, kernel, kmap, vmap, a, kv, v, parts, box_rows, err);
+  if (e != cudaSuccess || (e = launch_attention_own(a, kv, v, stream)) != cudaSuccess) return e;
+  // Few rows may have many parts (a warp would read them one after the other): a block a row.
+  const long long rows = (long long)kv.batch * a.n_heads;
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  if (rows <= 2048) {
+    cfg.gridDim = dim3((unsigned)rows);
+    return cudaLaunchKernelEx(&cfg, attention_shared_join_kernel<O, HD, 8>, a, kv, v, parts, sp.zs);
+  }
+  cfg.gridDim = dim3((unsigned)((rows + 7) / 8));
+  return cudaLaunchKernelEx(&cfg, attention_shared_join_kernel<O, HD, 1>, a, kv, v, parts, sp.zs);
+}
+
+template <class T>
+cudaError_t launch_type(const SharedArgs& a, const KvArgs& kv, cudaStream_t stream, unsigned* err) {
+  const bool f32 = a.paged.out_dtype == kDtF32;
+  if (kv.head_dim == 128)
+    return f32 ? launch_typed<T, float, 128>(a, kv, stream, err) : launch_typed<T, T, 128>(a, kv, stream, err);
+  return f32 ? launch_typed<T, float, 64>(a, kv, stream, err) : launch_typed<T, T, 64>(a, kv, stream, err);
+}
+
+}  // namespace
+
+size_t attention_shared_workspace(int batch, int groups, int n_heads, int n_kv, int head_dim) {
+  return batch == 0 ? 0 : space_of(batch, groups, n_heads, n_kv, head_dim).bytes;
+}
+
+cudaError_t launch_attention_shared(const SharedArgs& a, const KvArgs& kv, cudaStream_t stream) {
+  unsigned* err = device_error_word();
+  if (!err) return cudaErrorUnknown;
+  return kv.dtype == kDtF16 ? launch_type<__half>(a, kv, stream, err)
+                            : launch_type<__nv_bfloat16>(a, kv, stream, err);
+}
+
+}  // namespace asmllm

@@ -29,6 +29,7 @@
 #include "decode_persistent.cuh"
 #include "matvec.cuh"
 #include "serving.cuh"
+#include "serving_q8.cuh"
 #include "tiles.cuh"
 
 using namespace asmllm;
@@ -1151,6 +1152,354 @@ ASMLLM_API int asm_rows_sample_async(const void* logits, int32_t dtype, int32_t 
   a.min_p = min_p;
   a.tokens = tokens;
   const cudaError_t e = launch_rows_sample(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_error(e, name);
+  return ASM_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Serving operators around an 8-bit cache, shared prefixes and logits
+// (cache_q8.cu, attention_paged_q8.cu, attention_shared.cu, rows_adjust.cu)
+// ---------------------------------------------------------------------------
+namespace {
+
+// The Q8_0 view's own arguments; pointers are looked at in check_kv_q8_pointers.
+int check_kv_q8(const char* name, const asm_kv_q8_t* d, KvQ8Args* out) {
+  if (!d) return set_error(ASM_E_INVALID, "%s: null key-value descriptor", name);
+  if (d->head_dim != 64 && d->head_dim != 128)
+    return set_error(ASM_E_UNSUPPORTED, "%s: head_dim %d (64 or 128)", name, d->head_dim);
+  if (d->batch < 0 || d->n_kv_heads <= 0 || d->n_pages <= 0 || d->page_size <= 0)
+    return set_error(ASM_E_INVALID, "%s: need batch >= 0 and n_kv_heads, n_pages, page_size > 0", name);
+  if (!d->table) return set_error(ASM_E_INVALID, "%s: null page table", name);
+  if (d->page_size < 16 || d->page_size > 256 || (d->page_size & (d->page_size - 1)))
+    return set_error(ASM_E_UNSUPPORTED, "%s: page_size %d (a power of two from 16 to 256)", name, d->page_size);
+  if (d->table_width <= 0 || d->table_stride < d->table_width)
+    return set_error(ASM_E_INVALID, "%s: need 0 < table_width <= table_stride", name);
+  KvQ8Args& c = *out;
+  KvArgs& kv = c.kv;
+  while ((1 << kv.page_shift) < d->page_size) ++kv.page_shift;
+  const int64_t s[3] = {d->page_stride, d->token_stride, d->head_stride};
+  for (int i = 0; i < 3; ++i)
+    if (s[i] <= 0 || s[i] % 16 || s[i] >= (1ll << 38))
+      return set_error(ASM_E_INVALID, "%s: key-value strides must be positive multiples of 16 bytes", name);
+  if (d->scale_page_stride <= 0 || d->scale_page_stride % 8 || d->scale_page_stride >= (1ll << 38) ||
+      d->scale_head_stride <= 0 || d->scale_head_stride % 8 || d->scale_head_stride >= (1ll << 38))
+    return set_error(ASM_E_INVALID, "%s: scale strides must be positive multiples of 8 elements", name);
+  if ((uintptr_t)d->k % 16 || (uintptr_t)d->v % 16 || (uintptr_t)d->k_scales % 16 || (uintptr_t)d->v_scales % 16)
+    return set_error(ASM_E_INVALID, "%s: k, v and their scales must be 16-byte aligned", name);
+  kv.k = d->k;
+  kv.v = d->v;
+  kv.page_stride = d->page_stride;
+  kv.token_stride = d->token_stride;
+  kv.head_stride = d->head_stride;
+  kv.table = d->table;
+  kv.table_stride = d->table_stride;
+  kv.len = d->len;
+  kv.batch = d->batch;
+  kv.n_pages = d->n_pages;
+  kv.page_size = d->page_size;
+  kv.width = d->table_width;
+  kv.n_kv = d->n_kv_heads;
+  kv.head_dim = d->head_dim;
+  c.ks = static_cast<__half*>(d->k_scales);
+  c.vs = static_cast<__half*>(d->v_scales);
+  c.scale_page_stride = d->scale_page_stride;
+  c.scale_head_stride = d->scale_head_stride;
+  return ASM_OK;
+}
+
+int check_kv_q8_pointers(const char* name, const KvQ8Args& c) {
+  int rc;
+  if ((rc = require_device(name, c.kv.k, "k")) || (rc = require_device(name, c.kv.v, "v")) ||
+      (rc = require_device(name, c.ks, "k scales")) || (rc = require_device(name, c.vs, "v scales")) ||
+      (rc = require_device(name, c.kv.table, "page table")) || (rc = require_device(name, c.kv.len, "lengths")))
+    return rc;
+  return ASM_OK;
+}
+
+// The cache's four arrays.
+struct Q8Arrays {
+  Strided a[4];
+  explicit Q8Arrays(const KvQ8Args& c) {
+    const KvArgs& kv = c.kv;
+    const long long scales = (long long)kv.page_size * (kv.head_dim / 32);
+    for (int i = 0; i < 2; ++i) {
+      a[i] = {i ? kv.v : kv.k, 1, kv.head_dim, {kv.n_pages, kv.page_size, kv.n_kv},
+              {kv.page_stride, kv.token_stride, kv.head_stride}};
+      a[2 + i] = {i ? c.vs : c.ks, 2, scales, {kv.n_pages, kv.n_kv, 1}, {c.scale_page_stride, c.scale_head_stride, 0}};
+    }
+  }
+};
+
+// check_apart with the cache, its table and its lengths as further inputs.
+int check_apart_q8(const char* name, const char* what, const void* out, size_t bytes, const Strided* in, int n,
+                   const KvQ8Args& c) {
+  const Q8Arrays q(c);
+  const Strided rest[2] = {{c.kv.table, 4, c.kv.width, {c.kv.batch, 1, 1}, {c.kv.table_stride, 0, 0}},
+                           flat(c.kv.len, 4, c.kv.batch)};
+  int rc;
+  if ((rc = check_apart(name, what, out, bytes, in, n, nullptr)) ||
+      (rc = check_apart(name, what, out, bytes, q.a, 4, nullptr)) ||
+      (rc = check_apart(name, what, out, bytes, rest, 2, nullptr)))
+    return rc;
+  return ASM_OK;
+}
+
+}  // namespace
+
+ASMLLM_API int asm_rope_append_q8_async(const void* qkv, int32_t qkv_dtype, int64_t qkv_stride, const float* rope_cs,
+                                        int32_t rope_len, const int32_t* cu_q, int32_t rows, int32_t n_heads,
+                                        void* q_out, int32_t q_dtype, const asm_kv_q8_t* kvd, void* stream) {
+  const char* name = "asm_rope_append_q8_async";
+  KvQ8Args c;
+  int rc;
+  if ((rc = check_kv_q8(name, kvd, &c)) || (rc = check_heads(name, n_heads, c.kv.n_kv))) return rc;
+  const KvArgs& kv = c.kv;
+  if (rows < 0 || rope_len <= 0 || (!cu_q && rows != kv.batch))
+    return set_error(ASM_E_INVALID, "%s: need rows >= 0 (the batch without cu_q) and rope_len > 0", name);
+  if (q_dtype != ASM_DT_F16 && q_dtype != ASM_DT_BF16)
+    return set_error(ASM_E_UNSUPPORTED, "%s: q_out is fp16 or bf16", name);
+  if (qkv_dtype != ASM_DT_F32 && qkv_dtype != q_dtype)
+    return set_error(ASM_E_UNSUPPORTED, "%s: qkv is fp32 or of q_out's type", name);
+  if (qkv_stride < (int64_t)(n_heads + 2 * kv.n_kv) * kv.head_dim || qkv_stride % 8)
+    return set_error(ASM_E_INVALID, "%s: qkv_stride %lld too small or not a multiple of 8", name, (long long)qkv_stride);
+  if ((uintptr_t)qkv % 16 || (uintptr_t)rope_cs % 16 || (uintptr_t)q_out % 16)
+    return set_error(ASM_E_INVALID, "%s: misaligned buffer", name);
+  if (rows == 0 || kv.batch == 0) return ASM_OK;
+  if ((rc = check_kv_q8_pointers(name, c)) || (rc = require_device(name, qkv, "qkv")) ||
+      (rc = require_device(name, rope_cs, "rope_cs")) || (rc = require_device(name, q_out, "q_out")) ||
+      (cu_q && (rc = require_device(name, cu_q, "cu_q"))))
+    return rc;
+  const long long cols = (long long)(n_heads + 2 * kv.n_kv) * kv.head_dim;
+  const int wide = qkv_dtype == ASM_DT_F32 ? 4 : 2;
+  const Strided in[3] = {{qkv, wide, cols, {rows, 1, 1}, {qkv_stride, 0, 0}},
+                         flat(rope_cs, 4, (long long)rope_len * kv.head_dim), flat(cu_q, 4, kv.batch + 1)};
+  if ((rc = check_apart_q8(name, "q_out", q_out, (size_t)rows * n_heads * kv.head_dim * 2, in, 3, c)) ||
+      (rc = check_apart_q8(name, "qkv", qkv, ((size_t)(rows - 1) * qkv_stride + cols) * wide, nullptr, 0, c)))
+    return rc;
+  if (kv.k == kv.v || c.ks == c.vs) return set_error(ASM_E_INVALID, "%s: k and v are the same pages", name);
+  RopeAppendArgs a;
+  a.qkv = qkv;
+  a.src_dtype = qkv_dtype;
+  a.qkv_stride = qkv_stride;
+  a.rope_cs = rope_cs;
+  a.rope_len = rope_len;
+  a.cu_q = cu_q;
+  a.rows = rows;
+  a.n_heads = n_heads;
+  a.q_out = q_out;
+  const cudaError_t e = launch_rope_append_q8(a, q_dtype, c, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_error(e, name);
+  return ASM_OK;
+}
+
+ASMLLM_API int asm_cache_read_q8_async(const asm_kv_q8_t* kvd, const int32_t* cu, int32_t rows, void* k_out,
+                                       void* v_out, int32_t dtype, void* stream) {
+  const char* name = "asm_cache_read_q8_async";
+  KvQ8Args c;
+  int rc;
+  if ((rc = check_kv_q8(name, kvd, &c))) return rc;
+  const KvArgs& kv = c.kv;
+  if (rows < 0) return set_error(ASM_E_INVALID, "%s: need rows >= 0", name);
+  if (dtype != ASM_DT_F16 && dtype != ASM_DT_BF16)
+    return set_error(ASM_E_UNSUPPORTED, "%s: rows are read back in fp16 or bf16", name);
+  if ((uintptr_t)k_out % 16 || (uintptr_t)v_out % 16) return set_error(ASM_E_INVALID, "%s: misaligned buffer", name);
+  if (rows == 0 || kv.batch == 0) return ASM_OK;
+  if ((rc = check_kv_q8_pointers(name, c)) || (rc = require_device(name, cu, "row offsets")) ||
+      (rc = require_device(name, k_out, "k_out")) || (rc = require_device(name, v_out, "v_out")))
+    return rc;
+  const size_t bytes = (size_t)rows * kv.n_kv * kv.head_dim * 2;
+  const Strided in[2] = {flat(cu, 4, kv.batch + 1), flat(v_out, 1, (long long)bytes)};
+  if ((rc = check_apart_q8(name, "k_out", k_out, bytes, in, 2, c)) ||
+      (rc = check_apart_q8(name, "v_out", v_out, bytes, in, 1, c)))
+    return rc;
+  CacheReadArgs a;
+  a.cu = cu;
+  a.rows = rows;
+  a.k = k_out;
+  a.v = v_out;
+  a.dtype = dtype;
+  const cudaError_t e = launch_cache_read_q8(a, c, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_error(e, name);
+  return ASM_OK;
+}
+
+ASMLLM_API int64_t asm_attention_paged_q8_workspace(int32_t batch, int32_t n_heads, int32_t n_kv_heads,
+                                                    int32_t head_dim) {
+  if (batch < 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || (head_dim != 64 && head_dim != 128)) {
+    set_error(ASM_E_INVALID, "asm_attention_paged_q8_workspace: need batch >= 0, n_heads a multiple of n_kv_heads, "
+                             "head_dim 64 or 128");
+    return -1;
+  }
+  return (int64_t)attention_paged_q8_workspace(batch, n_heads, n_kv_heads, head_dim);
+}
+
+ASMLLM_API int asm_attention_paged_q8_async(const void* q, int32_t q_dtype, int64_t q_row_stride, int64_t q_head_stride,
+                                            int32_t n_heads, float scale, void* out, int32_t out_dtype,
+                                            const asm_kv_q8_t* kvd, void* workspace, int64_t workspace_bytes,
+                                            void* stream) {
+  const char* name = "asm_attention_paged_q8_async";
+  KvQ8Args c;
+  int rc;
+  if ((rc = check_kv_q8(name, kvd, &c)) || (rc = check_heads(name, n_heads, c.kv.n_kv))) return rc;
+  if (q_dtype != ASM_DT_F16 && q_dtype != ASM_DT_BF16)
+    return set_error(ASM_E_UNSUPPORTED, "%s: q is fp16 or bf16", name);
+  if ((rc = check_query(name, q, q_row_stride, q_head_stride, out, out_dtype, q_dtype, scale))) return rc;
+  const KvArgs& kv = c.kv;
+  if (kv.batch > (1 << 15)) return set_error(ASM_E_UNSUPPORTED, "%s: batch %d (at most 2^15)", name, kv.batch);
+  const size_t need = attention_paged_q8_workspace(kv.batch, n_heads, kv.n_kv, kv.head_dim);
+  if (workspace_bytes < 0 || (size_t)workspace_bytes < need || (uintptr_t)workspace % 16)
+    return set_error(ASM_E_INVALID, "%s: workspace of %lld bytes, %zu needed (16-byte aligned)", name,
+                     (long long)workspace_bytes, need);
+  if (kv.batch == 0) return ASM_OK;
+  if ((rc = check_kv_q8_pointers(name, c)) || (rc = require_device(name, q, "q")) ||
+      (rc = require_device(name, out, "out")) || (rc = require_device(name, workspace, "workspace")))
+    return rc;
+  const size_t out_bytes = (size_t)kv.batch * n_heads * kv.head_dim * (out_dtype == ASM_DT_F32 ? 4 : 2);
+  const Strided in[2] = {{q, 2, kv.head_dim, {kv.batch, n_heads, 1}, {q_row_stride, q_head_stride, 0}},
+                         flat(out, 1, (long long)out_bytes)};
+  if ((rc = check_apart_q8(name, "out", out, out_bytes, in, 1, c)) ||
+      (rc = check_apart_q8(name, "workspace", workspace, need, in, 2, c)))
+    return rc;
+  PagedArgs a;
+  a.q = q;
+  a.q_row_stride = q_row_stride;
+  a.q_head_stride = q_head_stride;
+  a.out = out;
+  a.out_dtype = out_dtype;
+  a.n_heads = n_heads;
+  a.scale = scale;
+  a.workspace = workspace;
+  const cudaError_t e = launch_attention_paged_q8(a, q_dtype, c, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_error(e, name);
+  return ASM_OK;
+}
+
+ASMLLM_API int64_t asm_attention_shared_workspace(int32_t batch, int32_t groups, int32_t n_heads, int32_t n_kv_heads,
+                                                  int32_t head_dim) {
+  if (batch < 0 || groups < 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads ||
+      (head_dim != 64 && head_dim != 128)) {
+    set_error(ASM_E_INVALID, "asm_attention_shared_workspace: need batch, groups >= 0, n_heads a multiple of "
+                             "n_kv_heads, head_dim 64 or 128");
+    return -1;
+  }
+  return (int64_t)attention_shared_workspace(batch, groups, n_heads, n_kv_heads, head_dim);
+}
+
+ASMLLM_API int asm_attention_shared_async(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t n_heads,
+                                          float scale, void* out, int32_t out_dtype, const asm_kv_t* kvd,
+                                          const int32_t* cu_group, const int32_t* shared_len, int32_t groups,
+                                          void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* name = "asm_attention_shared_async";
+  KvArgs kv;
+  int rc;
+  if ((rc = check_kv(name, kvd, true, &kv)) || (rc = check_heads(name, n_heads, kv.n_kv)) ||
+      (rc = check_query(name, q, q_row_stride, q_head_stride, out, out_dtype, kv.dtype, scale)))
+    return rc;
+  if (groups < 0) return set_error(ASM_E_INVALID, "%s: need groups >= 0", name);
+  if (kv.batch > (1 << 15) || groups > (1 << 15) || (int64_t)kv.batch * n_heads > (1 << 22))
+    return set_error(ASM_E_UNSUPPORTED, "%s: batch %d, groups %d (at most 2^15, batch * n_heads 2^22)", name, kv.batch,
+                     groups);
+  const size_t need = attention_shared_workspace(kv.batch, groups, n_heads, kv.n_kv, kv.head_dim);
+  if (workspace_bytes < 0 || (size_t)workspace_bytes < need || (uintptr_t)workspace % 16)
+    return set_error(ASM_E_INVALID, "%s: workspace of %lld bytes, %zu needed (16-byte aligned)", name,
+                     (long long)workspace_bytes, need);
+  if (kv.batch == 0) return ASM_OK;
+  if ((rc = check_kv_pointers(name, kv)) || (rc = require_device(name, q, "q")) ||
+      (rc = require_device(name, out, "out")) || (rc = require_device(name, workspace, "workspace")) ||
+      (groups && ((rc = require_device(name, cu_group, "group offsets")) ||
+                  (rc = require_device(name, shared_len, "shared lengths")))))
+    return rc;
+  const size_t out_bytes = (size_t)kv.batch * n_heads * kv.head_dim * (out_dtype == ASM_DT_F32 ? 4 : 2);
+  const Strided in[4] = {{q, 2, kv.head_dim, {kv.batch, n_heads, 1}, {q_row_stride, q_head_stride, 0}},
+                         flat(groups ? cu_group : nullptr, 4, groups + 1), flat(groups ? shared_len : nullptr, 4, groups),
+                         flat(out, 1, (long long)out_bytes)};
+  if ((rc = check_apart(name, "out", out, out_bytes, in, 3, &kv)) ||
+      (rc = check_apart(name, "workspace", workspace, need, in, 4, &kv)))
+    return rc;
+  SharedArgs a;
+  a.paged.q = q;
+  a.paged.q_row_stride = q_row_stride;
+  a.paged.q_head_stride = q_head_stride;
+  a.paged.out = out;
+  a.paged.out_dtype = out_dtype;
+  a.paged.n_heads = n_heads;
+  a.paged.scale = scale;
+  a.paged.workspace = workspace;
+  a.cu_group = cu_group;
+  a.shared_len = shared_len;
+  a.groups = groups;
+  const cudaError_t e = launch_attention_shared(a, kv, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_error(e, name);
+  return ASM_OK;
+}
+
+ASMLLM_API int asm_rows_adjust_async(const asm_adjust_t* d, void* stream) {
+  const char* name = "asm_rows_adjust_async";
+  if (!d) return set_error(ASM_E_INVALID, "%s: null descriptor", name);
+  if (d->rows < 0 || d->n <= 0 || d->stride < d->n || d->out_stride < d->n)
+    return set_error(ASM_E_INVALID, "%s: need rows >= 0, n > 0, strides >= n", name);
+  if (d->rows > 65535) return set_error(ASM_E_UNSUPPORTED, "%s: rows %d (at most 65535)", name, d->rows);
+  if (d->dtype != ASM_DT_F32 && d->dtype != ASM_DT_F16 && d->dtype != ASM_DT_BF16)
+    return set_error(ASM_E_UNSUPPORTED, "%s: logits type %d", name, d->dtype);
+  const int size = d->dtype == ASM_DT_F32 ? 4 : 2;
+  if ((uintptr_t)d->logits % size || (uintptr_t)d->out % size)
+    return set_error(ASM_E_INVALID, "%s: misaligned buffer", name);
+  if (d->tokens && (d->held < 0 || d->token_stride < d->held))
+    return set_error(ASM_E_INVALID, "%s: need 0 <= held <= token_stride", name);
+  if (!d->tokens && (d->n_tokens || d->n_prompt || d->repetition || d->frequency || d->presence))
+    return set_error(ASM_E_INVALID, "%s: penalties without tokens", name);
+  if (d->n_bias < 0 || (d->n_bias > 0 && (!d->bias_tokens || !d->bias)))
+    return set_error(ASM_E_INVALID, "%s: need n_bias >= 0 and both arrays of biases", name);
+  if (d->n_bias > kAdjustMaxBias)
+    return set_error(ASM_E_UNSUPPORTED, "%s: %d biases a row (at most %d)", name, d->n_bias, kAdjustMaxBias);
+  if (d->allowed && d->allowed_stride < ((int64_t)d->n + 31) / 32)
+    return set_error(ASM_E_INVALID, "%s: allowed_stride %lld, a bit a word is needed", name, (long long)d->allowed_stride);
+  if (d->rows == 0) return ASM_OK;
+  const int32_t* bias_tokens = d->n_bias ? d->bias_tokens : nullptr;
+  const float* bias = d->n_bias ? d->bias : nullptr;
+  const int32_t* tokens = d->held ? d->tokens : nullptr;
+  struct { const void* p; const char* what; } given[] = {
+      {tokens, "tokens"}, {d->n_tokens, "n_tokens"}, {d->n_prompt, "n_prompt"}, {d->repetition, "repetition"},
+      {d->frequency, "frequency"}, {d->presence, "presence"}, {bias_tokens, "bias_tokens"}, {bias, "bias"},
+      {d->allowed, "allowed"}};
+  int rc;
+  if ((rc = require_device(name, d->logits, "logits")) || (rc = require_device(name, d->out, "out"))) return rc;
+  for (const auto& x : given)
+    if (x.p && (rc = require_device(name, x.p, x.what))) return rc;
+  const long long rows = d->rows;
+  const Strided in[10] = {{d->logits, size, d->n, {rows, 1, 1}, {d->stride, 0, 0}},
+                          {tokens, 4, d->held, {rows, 1, 1}, {d->token_stride, 0, 0}}, flat(d->n_tokens, 4, rows),
+                          flat(d->n_prompt, 4, rows), flat(d->repetition, 4, rows), flat(d->frequency, 4, rows),
+                          flat(d->presence, 4, rows), flat(bias_tokens, 4, rows * d->n_bias), flat(bias, 4, rows * d->n_bias),
+                          {d->allowed, 4, ((long long)d->n + 31) / 32, {rows, 1, 1}, {d->allowed_stride, 0, 0}}};
+  const bool in_place = d->out == d->logits && (d->rows == 1 || d->out_stride == d->stride);
+  for (long long r = 0; r < (d->out_stride == d->n ? 1 : rows); ++r) {  // dense rows are one piece
+    const char* out = static_cast<const char*>(d->out) + r * d->out_stride * size;
+    const size_t bytes = (size_t)d->n * size * (d->out_stride == d->n ? rows : 1);
+    if ((rc = check_apart(name, "out", out, bytes, in + in_place, 10 - in_place, nullptr))) return rc;
+  }
+  AdjustArgs a;
+  a.logits = d->logits;
+  a.out = d->out;
+  a.dtype = d->dtype;
+  a.stride = d->stride;
+  a.out_stride = d->out_stride;
+  a.rows = d->rows;
+  a.n = d->n;
+  a.tokens = tokens;
+  a.token_stride = d->token_stride;
+  a.held = d->held;
+  a.n_tokens = d->n_tokens;
+  a.n_prompt = d->n_prompt;
+  a.repetition = d->repetition;
+  a.frequency = d->frequency;
+  a.presence = d->presence;
+  a.bias_tokens = bias_tokens;
+  a.bias = bias;
+  a.n_bias = d->n_bias;
+  a.allowed = d->allowed;
+  a.allowed_stride = d->allowed_stride;
+  const cudaError_t e = launch_rows_adjust(a, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_error(e, name);
   return ASM_OK;
 }

@@ -1,0 +1,66 @@
+// asmllm_b200/csrc/shared_prefix.cuh -- groups of sequences that share their
+// first positions: what the two passes of attention_shared.cu and the paged
+// pass over the rest (attention_paged.cu) agree on.
+#pragma once
+
+#include "paged_deal.cuh"
+
+namespace asmllm {
+
+// One sequence's or group's result that is not split: 1 part, found by row; more: in slots.
+struct Found {
+  int parts;  // 0: no position, 1: whole, else CTAs cta .. cta + parts - 1 hold one part each
+  int cta;
+  int slot;   // slot of the first part (the others are in slot 2 c)
+  int pad;
+};
+
+struct SharedView {
+  const int32_t* cu_group = nullptr;
+  const int32_t* shared_len = nullptr;
+  int groups = 0;
+  // results of the positions that are not shared, unnormalised: [batch][n_heads][head_dim], (maximum in units of
+  // log2, sum) [batch][n_heads], and where each unit's are
+  float* own_o = nullptr;
+  float2* own_ml = nullptr;
+  Found* own_found = nullptr;  // [batch][n_kv * zs]
+  float* own_slots = nullptr;
+};
+
+#ifdef __CUDACC__
+
+// Sequences [*b, *e) of group g, and how many positions they share (whole pages); false for offsets out of range.
+__device__ __forceinline__ bool group_of(const SharedView& v, const KvArgs& kv, int g, int* b, int* e, int* shared) {
+  *b = __ldcg(v.cu_group + g);
+  *e = __ldcg(v.cu_group + g + 1);
+  const int n = __ldcg(v.shared_len + g);
+  const long long cap = (long long)kv.width << kv.page_shift;
+  *shared = n < 0 ? 0 : (int)(n > cap ? cap : n) & ~(kv.page_size - 1);
+  const bool ok = *b >= 0 && *e <= kv.batch && *b <= *e;
+  if (!ok) *b = *e = 0;
+  return ok && n >= 0 && n <= cap;
+}
+
+// Positions of sequence s, of n, that it shares with its group, and the group: none for a sequence without a group,
+// or with fewer positions than the group shares.
+__device__ __forceinline__ int shared_base(const SharedView& v, const KvArgs& kv, int s, int n, int* group) {
+  int lo = 0, hi = v.groups;
+  while (lo < hi) {  // the first group that ends behind s
+    const int mid = (lo + hi) >> 1;
+    if (__ldcg(v.cu_group + mid + 1) <= s) lo = mid + 1; else hi = mid;
+  }
+  *group = lo;
+  if (lo >= v.groups) return 0;
+  int b, e, shared;
+  group_of(v, kv, lo, &b, &e, &shared);
+  return s >= b && s < e && n >= shared ? shared : 0;
+}
+
+#endif  // __CUDACC__
+
+// The pass over the positions that are not shared (attention_paged.cu): results into `v`, none joined.
+constexpr int kOwnCtas = 320;
+size_t own_slots_floats(int n_heads, int n_kv, int head_dim);
+cudaError_t launch_attention_own(const PagedArgs& a, const KvArgs& kv, const SharedView& v, cudaStream_t stream);
+
+}  // namespace asmllm

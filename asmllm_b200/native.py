@@ -74,6 +74,25 @@ class Kv(ctypes.Structure):
                                       "reserved")])
 
 
+class KvQ8(ctypes.Structure):
+    """asm_kv_q8_t (include/asmllm.h): codes and scales of a paged Q8_0 cache."""
+    _fields_ = ([(n, vp) for n in ("k", "v", "k_scales", "v_scales")]
+                + [(n, i64) for n in ("page_stride", "token_stride", "head_stride", "scale_page_stride",
+                                      "scale_head_stride")]
+                + [("table", vp), ("table_stride", i64), ("len", vp)]
+                + [(n, i32) for n in ("batch", "n_pages", "page_size", "table_width", "n_kv_heads", "head_dim")])
+
+
+class Adjust(ctypes.Structure):
+    """asm_adjust_t (include/asmllm.h): penalties, biases and a mask on rows of logits."""
+    _fields_ = ([("logits", vp), ("out", vp), ("stride", i64), ("out_stride", i64)]
+                + [(n, i32) for n in ("dtype", "rows", "n", "held")]
+                + [("tokens", vp), ("token_stride", i64)]
+                + [(n, vp) for n in ("n_tokens", "n_prompt", "repetition", "frequency", "presence", "bias_tokens",
+                                     "bias", "allowed")]
+                + [("allowed_stride", i64), ("n_bias", i32), ("reserved", i32)])
+
+
 class Rows(ctypes.Structure):
     """asm_rows_t (include/asmllm.h): one batched RMSNorm / embed / residual step."""
     _fields_ = [("rows", i32), ("dim", i32), ("x", vp), ("delta", vp), ("embed", vp), ("tokens", vp), ("pos", vp),
@@ -117,6 +136,13 @@ SIGNATURES = {
     "asm_attention_paged_workspace": ([i32, i32, i32, i32], i64),
     "asm_attention_paged_async": ([vp, i64, i64, i32, f32, vp, i32, vp, vp, i64, vp], c_int),
     "asm_rows_sample_async": ([vp, i32, i32, i32, i64, vp, vp, vp, vp, vp, vp, vp], c_int),
+    "asm_rope_append_q8_async": ([vp, i32, i64, vp, i32, vp, i32, i32, vp, i32, vp, vp], c_int),
+    "asm_cache_read_q8_async": ([vp, vp, i32, vp, vp, i32, vp], c_int),
+    "asm_attention_paged_q8_workspace": ([i32, i32, i32, i32], i64),
+    "asm_attention_paged_q8_async": ([vp, i32, i64, i64, i32, f32, vp, i32, vp, vp, i64, vp], c_int),
+    "asm_attention_shared_workspace": ([i32, i32, i32, i32, i32], i64),
+    "asm_attention_shared_async": ([vp, i64, i64, i32, f32, vp, i32, vp, vp, vp, i32, vp, i64, vp], c_int),
+    "asm_rows_adjust_async": ([vp, vp], c_int),
     # additions
     "asm_matmul_q8q8": ([vp, vp, vp, vp, i64, i64], None),
     "asm_quantize_q8_0": ([vp, vp, vp, i64], None),

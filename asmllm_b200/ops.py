@@ -375,6 +375,8 @@ __all__ = [
     "block_sums_dev", "gguf_split_dev", "act_image_bytes", "act_image_dev", "matvec_image",
     "mark_static", "unmark_static", "device_error", "set_option",
     "rope_append", "attention_prompt", "attention_paged", "attention_paged_workspace", "rows_sample",
+    "rope_append_q8", "cache_read_q8", "attention_paged_q8", "attention_paged_q8_workspace", "attention_shared",
+    "attention_shared_workspace", "rows_adjust",
 ]
 
 
@@ -562,13 +564,16 @@ def key_index(keys):
 _DT: dict = {}   # torch dtype -> ASM_DT_*
 _H16: dict = {}  # the 16-bit ones alone
 _KV_PACK = struct.Struct("QQqqqQqQQiiiiiiii").pack  # asm_kv_t (native.Kv), field for field
-_F32 = _I32 = _U8 = _current_stream = None  # torch's, once it is imported
+_KV_Q8_PACK = struct.Struct("QQQQqqqqqQqQiiiiii").pack  # asm_kv_q8_t (native.KvQ8)
+_ADJUST_PACK = struct.Struct("QQqqiiiiQqQQQQQQQQqii").pack  # asm_adjust_t (native.Adjust)
+_F32 = _F16 = _I32 = _I8 = _U8 = _current_stream = None  # torch's, once it is imported
 
 
 def _dtypes():
-    global _F32, _I32, _U8, _current_stream
+    global _F32, _F16, _I32, _I8, _U8, _current_stream
     torch = _torch()
-    _F32, _I32, _U8, _current_stream = torch.float32, torch.int32, torch.uint8, torch._C._cuda_getCurrentRawStream
+    _F32, _F16, _I32, _I8, _U8 = torch.float32, torch.float16, torch.int32, torch.int8, torch.uint8
+    _current_stream = torch._C._cuda_getCurrentRawStream
     _H16.update({torch.float16: native.DT_F16, torch.bfloat16: native.DT_BF16})
     _DT.update({torch.float32: native.DT_F32, **_H16})
     return _DT
@@ -826,3 +831,292 @@ def rows_sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=No
     _call((native._lib or native.lib()).asm_rows_sample_async(logits.data_ptr(), _DT[logits.dtype], B, V,
                                              logits.stride(0) if B > 1 else V, *ptr, _current_stream(device) if stream is None else stream.cuda_stream))
     return tokens
+
+
+# --------------------------------------------------------------------------
+# Serving operators around an 8-bit cache, shared prefixes and logits
+# --------------------------------------------------------------------------
+
+
+def _kv_q8_view(k, v, k_scales, v_scales, device, kv_len, page_table):
+    """asm_kv_q8_t of codes k, v int8 [pages, page_size, heads, head_dim] and scales fp16
+    [pages, heads, page_size, head_dim / 32]."""
+    if not _DT:
+        _dtypes()
+    if page_table is None:
+        raise ValueError("page_table is required")
+    shape, st, ss = k.shape, _strides(k), _strides(k_scales)
+    if (k.dtype is not _I8 or v.dtype is not _I8 or k_scales.dtype is not _F16 or v_scales.dtype is not _F16
+            or len(st) != 4 or len(ss) != 4 or shape != v.shape or st != _strides(v) or st[-1] != 1
+            or k_scales.shape != v_scales.shape or ss != _strides(v_scales)
+            or not k.get_device() == v.get_device() == k_scales.get_device() == v_scales.get_device() == device >= 0):
+        for t, name, dt in ((k, "k", _I8), (v, "v", _I8), (k_scales, "k_scales", _F16), (v_scales, "v_scales", _F16)):
+            _dense(t, name, 4, (dt,))
+        if shape != v.shape or st != _strides(v) or k_scales.shape != v_scales.shape or ss != _strides(v_scales):
+            raise ValueError(f"k and v, and their scales, must agree in shape and strides: {tuple(k.shape)} {k.stride()}, "
+                             f"{tuple(v.shape)} {v.stride()}; {tuple(k_scales.shape)} {k_scales.stride()}, "
+                             f"{tuple(v_scales.shape)} {v_scales.stride()}")
+        raise ValueError("k, v, their scales and the rows are on different devices")
+    pages, size, heads, hd = shape
+    if k_scales.shape != (pages, heads, size, hd // 32) or hd % 32:
+        raise ValueError(f"k_scales {tuple(k_scales.shape)}: expected [pages, heads, page_size, head_dim / 32] of "
+                         f"k {tuple(shape)}")
+    if ss[3] != 1 or ss[2] != hd // 32:
+        raise ValueError(f"k_scales: a head's scales of a page must be dense, got strides {k_scales.stride()}")
+    batch, width = page_table.shape
+    if (page_table.dtype is not _I32 or page_table.get_device() != device
+            or (width > 1 and page_table.stride(1) != 1)):
+        _dense(page_table, "page_table", 2, (_I32,))
+        raise ValueError("page_table is on another device")
+    _vector(kv_len, "kv_len", batch, device)
+    return (_KV_Q8_PACK(k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), st[0], st[1], st[2],
+                        ss[0], ss[1], page_table.data_ptr(), page_table.stride(0) if batch > 1 else width,
+                        kv_len.data_ptr(), batch, pages, size, width, heads, hd), batch)
+
+
+def rope_append_q8(qkv, rope_cs, kv_len, page_table, k_pages, v_pages, k_scales, v_scales, n_heads: int, *, cu_q=None,
+                   q_dtype=None, q_out=None, stream=None):
+    """rope_append into a Q8_0 cache (asm_rope_append_q8_async): codes k_pages, v_pages int8
+    [pages, page_size, nkv, hd] (any strides, hd dense), scales fp16 [pages, nkv, page_size, hd / 32] (the
+    last two axes dense).
+
+    Keys are rotated in fp32, and keys and values quantized in blocks of 32 as quantize_q8_0 does it, the
+    scale rounded to fp16.  qkv fp32, or fp16 or bf16 (the queries' type then).  Returns the rotated queries
+    [T, nh, hd] in q_dtype (qkv's type; fp16 for fp32)."""
+    device = qkv.get_device()
+    if device < 0:
+        raise TypeError("qkv: expected a CUDA tensor")
+    kv, batch = _kv_q8_view(k_pages, v_pages, k_scales, v_scales, device, kv_len, page_table)
+    nkv, hd = k_pages.shape[2:]
+    if qkv.dtype not in _DT or qkv.dim() != 2 or qkv.stride(1) != 1:
+        _dense(qkv, "qkv", 2, _DT)
+    dt = q_dtype or (q_out.dtype if q_out is not None else _F16 if qkv.dtype is _F32 else qkv.dtype)
+    if dt not in _H16 or (qkv.dtype is not _F32 and qkv.dtype is not dt):
+        raise TypeError(f"queries of {dt} from qkv of {qkv.dtype}: fp16 or bf16, from fp32 or the same type")
+    T = qkv.shape[0]
+    if qkv.shape[1] != (n_heads + 2 * nkv) * hd:
+        raise ValueError(f"qkv has {qkv.shape[1]} columns, expected ({n_heads} + 2 * {nkv}) * {hd}")
+    if rope_cs.dtype is not _F32 or rope_cs.get_device() != device or not rope_cs.is_contiguous():
+        _check_dev(rope_cs, (_F32,), "rope_cs")
+        raise ValueError("rope_cs is on another device")
+    if rope_cs.shape[1:] != (hd // 2, 2):
+        raise ValueError(f"rope_cs {tuple(rope_cs.shape)}: expected [positions, {hd // 2}, 2]")
+    if cu_q is not None:
+        _vector(cu_q, "cu_q", batch + 1, device)
+    elif T != batch:
+        raise ValueError(f"{T} rows for {batch} sequences: pass cu_q")
+    if q_out is None:
+        q_out = _empty(qkv, (T, n_heads, hd), dt, stream)
+    else:
+        _check_dev(q_out, (dt,), "q_out")
+        if q_out.shape != (T, n_heads, hd) or q_out.get_device() != device:
+            raise ValueError(f"q_out {tuple(q_out.shape)} on device {q_out.get_device()}: expected {(T, n_heads, hd)} on {device}")
+    if T == 0 or batch == 0:
+        return q_out
+    _call((native._lib or native.lib()).asm_rope_append_q8_async(
+        qkv.data_ptr(), _DT[qkv.dtype], qkv.stride(0) if T > 1 else qkv.shape[1], rope_cs.data_ptr(),
+        rope_cs.shape[0], None if cu_q is None else cu_q.data_ptr(), T, n_heads, q_out.data_ptr(), _H16[dt], kv,
+        _current_stream(device) if stream is None else stream.cuda_stream))
+    return q_out
+
+
+def cache_read_q8(k_pages, v_pages, k_scales, v_scales, page_table, kv_len, cu, rows: int, *, dtype=None, out=None,
+                  stream=None):
+    """Keys and values of a Q8_0 cache as packed 16-bit rows (asm_cache_read_q8_async), for attention_prompt
+    with cu_k=cu.
+
+    Sequence s gets rows cu[s] .. cu[s + 1] - 1 (int32 [B + 1]) of `rows` in all: its last positions, as many
+    as it has rows (cu of the sums of kv_len reads everything, cu_q what a call has just appended).  Returns
+    (k, v) [rows, nkv, hd] in dtype (fp16 unless given) or in out=(k, v); rows before a sequence's first
+    position are zeros, rows at or past cu[B] are not written."""
+    device = k_pages.get_device()
+    kv, batch = _kv_q8_view(k_pages, v_pages, k_scales, v_scales, device, kv_len, page_table)
+    _vector(cu, "cu", batch + 1, device)
+    shape = (rows, *k_pages.shape[2:])
+    if rows < 0:
+        raise ValueError(f"rows {rows}")
+    if out is None:
+        dt = dtype or _F16
+        if dt not in _H16:
+            raise TypeError(f"dtype {dt}: fp16 or bf16")
+        k, v = _empty(k_pages, shape, dt, stream), _empty(k_pages, shape, dt, stream)
+    else:
+        k, v = out
+        dt = dtype or k.dtype
+        for t, name in ((k, "out[0]"), (v, "out[1]")):
+            _check_dev(t, (dt,) if dt in _H16 else tuple(_H16), name)
+            if t.shape != shape or t.get_device() != device:
+                raise ValueError(f"{name} {tuple(t.shape)} on device {t.get_device()}: expected {shape} on {device}")
+    if rows == 0 or batch == 0:
+        return k, v
+    _call((native._lib or native.lib()).asm_cache_read_q8_async(
+        kv, cu.data_ptr(), rows, k.data_ptr(), v.data_ptr(), _H16[dt],
+        _current_stream(device) if stream is None else stream.cuda_stream))
+    return k, v
+
+
+def _decode_query(q, nkv, hd, out, out_dtype, stream):
+    """Checks q [B, heads, head_dim] against the cache's heads and returns (strides, out)."""
+    shape, st = q.shape, _strides(q)
+    if q.dtype not in _H16 or not q.is_cuda or len(shape) != 3 or st[2] != 1:
+        _dense(q, "q", 3, _H16)
+    if shape[2] != hd:
+        raise ValueError(f"q of head_dim {shape[2]} against keys of {hd}")
+    if nkv == 0 or shape[1] == 0 or shape[1] % nkv:
+        raise ValueError(f"{shape[1]} query heads are not a multiple of {nkv} KV heads")
+    if out is None:
+        dt = out_dtype or q.dtype
+        if dt != q.dtype and dt != _F32:
+            raise TypeError(f"out_dtype {dt}: fp32 or q's type")
+        return st, _empty(q, shape, dt, stream)
+    _check_dev(out, (q.dtype, _F32), "out")
+    if out.shape != shape or out.get_device() != q.get_device() or (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError(f"out: {tuple(out.shape)} {out.dtype} on device {out.get_device()}, expected {tuple(shape)} "
+                         f"{out_dtype or q.dtype} on {q.get_device()}")
+    return st, out
+
+
+def _scratch(q, workspace, need, stream):
+    if need < 0:
+        native.check()
+    if workspace is None:
+        return _empty(q, (need,), _U8, stream)
+    _check_dev(workspace, (_U8,), "workspace")
+    if workspace.get_device() != q.get_device():
+        raise ValueError("workspace is on another device")
+    return workspace
+
+
+def attention_paged_q8_workspace(batch: int, n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    """Bytes of scratch one attention_paged_q8 call needs (asm_attention_paged_q8_workspace)."""
+    n = int(native.lib().asm_attention_paged_q8_workspace(batch, n_heads, n_kv_heads, head_dim))
+    if n < 0:
+        native.check()
+    return n
+
+
+def attention_paged_q8(q, k_pages, v_pages, k_scales, v_scales, page_table, kv_len, *, scale: float | None = None,
+                       out=None, out_dtype=None, workspace=None, stream=None):
+    """attention_paged over a Q8_0 cache (asm_attention_paged_q8_async): q [B, nh, hd] fp16 or bf16, the cache
+    as rope_append_q8 fills it, page_table int32 [B, n], kv_len int32 [B].  out [B, nh, hd] in q's type or
+    fp32.  workspace: uint8 of attention_paged_q8_workspace bytes, one per call that may overlap another."""
+    device = q.get_device()
+    kv, batch = _kv_q8_view(k_pages, v_pages, k_scales, v_scales, device, kv_len, page_table)
+    nkv, hd = k_pages.shape[2:]
+    st, out = _decode_query(q, nkv, hd, out, out_dtype, stream)
+    B, nh, _ = q.shape
+    if B != batch:
+        raise ValueError(f"q has {B} rows for {batch} sequences")
+    if B == 0:
+        return out
+    lib = native._lib or native.lib()
+    workspace = _scratch(q, workspace, lib.asm_attention_paged_q8_workspace(B, nh, nkv, hd), stream)
+    _call(lib.asm_attention_paged_q8_async(
+        q.data_ptr(), _H16[q.dtype], st[0], st[1], nh, hd ** -0.5 if scale is None else scale, out.data_ptr(),
+        _DT[out.dtype], kv, workspace.data_ptr(), workspace.numel(),
+        _current_stream(device) if stream is None else stream.cuda_stream))
+    return out
+
+
+def attention_shared_workspace(batch: int, groups: int, n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    """Bytes of scratch one attention_shared call needs (asm_attention_shared_workspace)."""
+    n = int(native.lib().asm_attention_shared_workspace(batch, groups, n_heads, n_kv_heads, head_dim))
+    if n < 0:
+        native.check()
+    return n
+
+
+def attention_shared(q, k_pages, v_pages, page_table, kv_len, cu_group, shared_len, *, scale: float | None = None,
+                     out=None, out_dtype=None, workspace=None, stream=None):
+    """attention_paged where groups of sequences begin with the same pages, which are read once for the whole
+    group (asm_attention_shared_async).
+
+    Sequences cu_group[i] .. cu_group[i + 1] - 1 (int32 [G + 1]) have their first shared_len[i] positions
+    (int32 [G], rounded down to whole pages) in common: their rows of page_table begin alike, kv_len counts
+    all positions.  A sequence in no group, or shorter than what its group shares, is on its own.  The rest is
+    attention_paged's.  workspace: uint8 of attention_shared_workspace bytes, one per call that may overlap
+    another."""
+    if page_table is None:
+        raise ValueError("page_table is required")
+    device = q.get_device()
+    kv, batch = _kv_view(k_pages, v_pages, device, kv_len, page_table)
+    nkv, hd = k_pages.shape[2:]
+    if q.dtype != k_pages.dtype:
+        raise ValueError(f"q {q.dtype} against keys {k_pages.dtype}")
+    st, out = _decode_query(q, nkv, hd, out, out_dtype, stream)
+    B, nh, _ = q.shape
+    if B != batch:
+        raise ValueError(f"q has {B} rows for {batch} sequences")
+    groups = shared_len.shape[0] if shared_len.dim() == 1 else -1
+    _vector(shared_len, "shared_len", groups, device)
+    _vector(cu_group, "cu_group", groups + 1, device)
+    if B == 0:
+        return out
+    lib = native._lib or native.lib()
+    workspace = _scratch(q, workspace, lib.asm_attention_shared_workspace(B, groups, nh, nkv, hd), stream)
+    _call(lib.asm_attention_shared_async(
+        q.data_ptr(), st[0], st[1], nh, hd ** -0.5 if scale is None else scale, out.data_ptr(), _DT[out.dtype], kv,
+        cu_group.data_ptr(), shared_len.data_ptr(), groups, workspace.data_ptr(), workspace.numel(),
+        _current_stream(device) if stream is None else stream.cuda_stream))
+    return out
+
+
+def rows_adjust(logits, *, tokens=None, n_tokens=None, n_prompt=None, repetition=None, frequency=None, presence=None,
+                bias_tokens=None, bias=None, allowed=None, out=None, stream=None):
+    """Logits [B, V] (fp32, fp16 or bf16) with penalties, biases and a mask, for rows_sample
+    (asm_rows_adjust_async).
+
+    In fp32: words among tokens [B, L] int32 (the first n_tokens[r] of a row) are divided by repetition where
+    they are above 0 and multiplied by it elsewhere; words that come c > 0 times from n_prompt[r] on lose
+    frequency * c + presence; words among bias_tokens int32 [B, N] (-1: unused; N <= 1024) gain their bias
+    fp32 [B, N], those of equal entries added up; words whose bit is 0 in allowed int32 [B, ceil(V / 32)] (bit
+    w % 32 of w / 32) become -inf.  n_tokens, n_prompt int32 [B] (L, 0) and repetition, frequency, presence
+    fp32 [B] (1, 0, 0) are optional.  Returns a new tensor, or out, which may be logits."""
+    if not _DT:
+        _dtypes()
+    if logits.dtype not in _DT or not logits.is_cuda or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        _dense(logits, "logits", 2, _DT)
+    B, V = shape = logits.shape
+    device = logits.get_device()
+    if out is None:
+        out = _empty(logits, shape, logits.dtype, stream)
+    elif out.dtype is not logits.dtype or out.shape != shape or out.get_device() != device or (V > 1 and out.stride(1) != 1):
+        _dense(out, "out", 2, (logits.dtype,))
+        raise ValueError(f"out: {tuple(out.shape)} on device {out.get_device()}, expected {tuple(shape)} on {device}")
+    ptr = []
+    for t, name, dt in ((n_tokens, "n_tokens", _I32), (n_prompt, "n_prompt", _I32), (repetition, "repetition", _F32),
+                        (frequency, "frequency", _F32), (presence, "presence", _F32)):
+        if t is None:
+            ptr.append(0)
+            continue
+        if tokens is None:
+            raise ValueError(f"{name} without tokens")
+        if t.dtype is not dt or t.get_device() != device or t.shape != shape[:1] or (B > 1 and t.stride(0) != 1):
+            _check_dev(t, (dt,), name)
+            raise ValueError(f"{name}: shape {tuple(t.shape)} on device {t.get_device()}, expected ({B},) on {device}")
+        ptr.append(t.data_ptr())
+    if (bias_tokens is None) != (bias is None):
+        raise ValueError("pass bias_tokens and bias together")
+    at = [(0, 0, 0)] * 4  # address, columns, row stride
+    for i, (t, name, dt) in enumerate(((tokens, "tokens", _I32), (bias_tokens, "bias_tokens", _I32), (bias, "bias", _F32),
+                                       (allowed, "allowed", _I32))):
+        if t is None:
+            continue
+        if t.dtype is not dt or t.get_device() != device or t.dim() != 2 or t.shape[0] != B or (
+                t.shape[1] > 1 and t.stride(1) != 1):
+            _dense(t, name, 2, (dt,))
+            raise ValueError(f"{name}: shape {tuple(t.shape)} on device {t.get_device()}, expected {B} rows on {device}")
+        n = t.shape[1]
+        at[i] = (t.data_ptr(), n, t.stride(0) if B > 1 else n)
+    if bias is not None and (bias.shape != bias_tokens.shape or not bias.is_contiguous() or not bias_tokens.is_contiguous()):
+        raise ValueError(f"bias_tokens {tuple(bias_tokens.shape)} and bias {tuple(bias.shape)}: expected equal, dense ones")
+    if allowed is not None and at[3][1] < (V + 31) // 32:
+        raise ValueError(f"allowed has {at[3][1]} words of 32 bits a row, {(V + 31) // 32} are needed")
+    if B == 0 or V == 0:
+        return out
+    _call((native._lib or native.lib()).asm_rows_adjust_async(
+        _ADJUST_PACK(logits.data_ptr(), out.data_ptr(), logits.stride(0) if B > 1 else V, out.stride(0) if B > 1 else V,
+                     _DT[logits.dtype], B, V, at[0][1], at[0][0], at[0][2], *ptr, at[1][0], at[2][0], at[3][0], at[3][2],
+                     at[1][1], 0),
+        _current_stream(device) if stream is None else stream.cuda_stream))
+    return out

@@ -749,6 +749,108 @@ ASMLLM_API int asm_rows_sample_async(const void* logits, int32_t dtype, int32_t 
                                      const float* u, const float* temperature, const int32_t* top_k,
                                      const float* top_p, const float* min_p, int32_t* tokens, void* stream);
 
+/* A paged cache in Q8_0: k and v hold int8 codes where asm_kv_t has 16-bit
+ * values (strides in bytes, multiples of 16; always paged), and a value is its
+ * code times the fp16 scale of its block of 32.  The head_dim/32 scales of
+ * (page, offset, head j) begin at k_scales[page*scale_page_stride +
+ * j*scale_head_stride + offset*head_dim/32]: those of a head's positions of a
+ * page lie side by side (strides in elements, multiples of 8).  All four
+ * arrays 16-byte aligned.  The rest is asm_kv_t's, its reports of lengths and
+ * page numbers out of range included. */
+typedef struct asm_kv_q8 {
+  int8_t* k;
+  int8_t* v;
+  void* k_scales;
+  void* v_scales;
+  int64_t page_stride, token_stride, head_stride;
+  int64_t scale_page_stride, scale_head_stride;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* len;
+  int32_t batch, n_pages, page_size, table_width;
+  int32_t n_kv_heads, head_dim;
+} asm_kv_q8_t;
+
+/* asm_rope_append_async into a Q8_0 cache: keys (rotated in fp32) and values
+ * are quantized as asm_quantize_q8_0 does it: a = max|x| of a block, codes
+ * rne(x * (127 / a)), scale a / 127, which is then rounded to fp16 (infinity
+ * from about 8.3e6 on).  A NaN or an infinity makes its whole block NaN to
+ * every reader.  q_out is of q_dtype (fp16 or bf16), qkv fp32 or of that. */
+ASMLLM_API int asm_rope_append_q8_async(const void* qkv, int32_t qkv_dtype, int64_t qkv_stride, const float* rope_cs,
+                                        int32_t rope_len, const int32_t* cu_q, int32_t rows, int32_t n_heads,
+                                        void* q_out, int32_t q_dtype, const asm_kv_q8_t* kv, void* stream);
+
+/* Rows of a Q8_0 cache in fp16 or bf16 (one rounding of code * scale), packed
+ * for asm_attention_prompt_async: row cu[s] + i of k_out and v_out [rows]
+ * [n_kv_heads][head_dim] is position len[s] - (cu[s+1] - cu[s]) + i of
+ * sequence s, so that cu decides how many of its last positions are read.
+ * Positions below 0 and those of a bad page give zeros; rows at or past
+ * cu[batch] are left as they are. */
+ASMLLM_API int asm_cache_read_q8_async(const asm_kv_q8_t* kv, const int32_t* cu, int32_t rows, void* k_out,
+                                       void* v_out, int32_t dtype, void* stream);
+
+/* asm_attention_paged_async over a Q8_0 cache, q fp16 or bf16, out fp32 or of
+ * q's type.  Codes enter the products as they are and scales multiply in
+ * fp32; the weights times a block's scale are two 16-bit parts (2^-22 of a
+ * weight, down to 2^-39 of the largest weight times the largest finite scale
+ * of the values).  A block of values whose scale is not finite gives NaN in its
+ * 32 outputs, whatever the weight is above zero. */
+ASMLLM_API int64_t asm_attention_paged_q8_workspace(int32_t batch, int32_t n_heads, int32_t n_kv_heads,
+                                                    int32_t head_dim);
+ASMLLM_API int asm_attention_paged_q8_async(const void* q, int32_t q_dtype, int64_t q_row_stride, int64_t q_head_stride,
+                                            int32_t n_heads, float scale, void* out, int32_t out_dtype,
+                                            const asm_kv_q8_t* kv, void* workspace, int64_t workspace_bytes,
+                                            void* stream);
+
+/* asm_attention_paged_async where sequences cu_group[i] .. cu_group[i+1] - 1
+ * have their first shared_len[i] positions in common (rounded down to whole
+ * pages: their tables begin with the same pages, and those of the first of
+ * them are read, once for the group).  Sequences in no group, and those with
+ * fewer positions than their group shares, have their own positions alone;
+ * lengths count all positions.  The weights over shared positions are those
+ * of asm_attention_prompt_async (one rounding for a 16-bit output, two 16-bit
+ * parts for fp32); a value there that is not finite gives an output that is
+ * not finite.  cu_group [groups + 1] and shared_len [groups] are on the
+ * device; offsets or lengths out of range set ASM_DEVERR_DECODE_RANGE (an
+ * offset: the group shares nothing; a length is clipped).  workspace as for
+ * asm_attention_paged_async (tens of MB); batch * n_heads at most 2^22. */
+ASMLLM_API int64_t asm_attention_shared_workspace(int32_t batch, int32_t groups, int32_t n_heads, int32_t n_kv_heads,
+                                                  int32_t head_dim);
+ASMLLM_API int asm_attention_shared_async(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t n_heads,
+                                          float scale, void* out, int32_t out_dtype, const asm_kv_t* kv,
+                                          const int32_t* cu_group, const int32_t* shared_len, int32_t groups,
+                                          void* workspace, int64_t workspace_bytes, void* stream);
+
+/* What is done to logits before asm_rows_sample_async: out = logits with, in
+ * fp32, each step rounded, and one rounding to their type at the end,
+ *   1. words among tokens[r][0 .. n_tokens[r]): x > 0 ? x / repetition : x * repetition;
+ *   2. words that occur c > 0 times from n_prompt[r] on: x - frequency * c - presence;
+ *   3. words among bias_tokens[r]: x + the sum of their biases (in 64 bits);
+ *   4. words whose bit in allowed[r] is 0 (bit w % 32 of word w / 32): -inf.
+ * tokens outside [0, n) are passed over, as are bias_tokens (-1: unused).
+ * n_tokens outside [0, held] is clipped and sets ASM_DEVERR_DECODE_RANGE.
+ * out may be logits itself; any other overlap with an input is refused. */
+typedef struct asm_adjust {
+  const void* logits;          /* [rows] x stride, dtype ASM_DT_* */
+  void* out;                   /* [rows] x out_stride, the same type */
+  int64_t stride, out_stride;
+  int32_t dtype, rows, n, held;
+  const int32_t* tokens;       /* [rows] x token_stride, `held` each; NULL: no penalties */
+  int64_t token_stride;
+  const int32_t* n_tokens;     /* [rows] or NULL (held) */
+  const int32_t* n_prompt;     /* [rows] or NULL (0) */
+  const float* repetition;     /* [rows] or NULL (1) */
+  const float* frequency;      /* [rows] or NULL (0) */
+  const float* presence;       /* [rows] or NULL (0) */
+  const int32_t* bias_tokens;  /* [rows][n_bias] */
+  const float* bias;           /* [rows][n_bias] */
+  const int32_t* allowed;      /* [rows] x allowed_stride, or NULL (all) */
+  int64_t allowed_stride;
+  int32_t n_bias;              /* at most 1024 */
+  int32_t reserved;
+} asm_adjust_t;
+ASMLLM_API int asm_rows_adjust_async(const asm_adjust_t* d, void* stream);
+
 /* Q5_0 x fp32 on device pointers (see asm_matmul_q5), stream ordered. */
 ASMLLM_API int asm_matmul_q5_async(const uint8_t* ql, const uint8_t* qh, const float* scales,
                                    const float* x, float* y, int64_t M, int64_t K, void* stream);
