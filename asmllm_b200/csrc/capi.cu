@@ -10,6 +10,7 @@
 //
 // The reference returns void and has no error channel; here a failure sets a
 // per-thread error (asm_get_last_error) and prints one line to stderr.
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <cuda_fp16.h>
 
@@ -19,6 +20,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <string>
@@ -1162,6 +1164,46 @@ ASMLLM_API int asm_rows_sample_async(const void* logits, int32_t dtype, int32_t 
 // ---------------------------------------------------------------------------
 namespace {
 
+// require_device for the pointers of a call at once (null ones are passed over unless `needed`): the driver's query of
+// just the memory's kind and device, 0.07 us a pointer where cudaPointerGetAttributes takes 0.13 with the device's.
+struct Given {
+  const void* p;
+  const char* what;
+  bool needed = true;
+};
+typedef CUresult (*PointerAttributes)(unsigned, CUpointer_attribute*, void**, CUdeviceptr);
+int require_devices(const char* name, const Given* x, int n) {
+  static PointerAttributes query = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPointByVersion("cuPointerGetAttributes", &p, 7000, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      query = reinterpret_cast<PointerAttributes>(p);
+    else
+      cudaGetLastError();
+  });
+  int cur = -1;
+  const bool fast = query && cudaGetDevice(&cur) == cudaSuccess;
+  for (int i = 0; i < n; ++i) {
+    if (!x[i].p && !x[i].needed) continue;
+    if (fast) {
+      unsigned kind = 0, managed = 0;
+      int dev = -1;
+      CUpointer_attribute what[3] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_IS_MANAGED,
+                                     CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL};
+      void* to[3] = {&kind, &managed, &dev};
+      if (query(3, what, to, (CUdeviceptr)(uintptr_t)x[i].p) == CUDA_SUCCESS && kind == CU_MEMORYTYPE_DEVICE &&
+          !managed && dev == cur)
+        continue;
+    }
+    const int rc = require_device(name, x[i].p, x[i].what);  // anything else: the long way, which says what is wrong
+    if (rc) return rc;
+  }
+  return ASM_OK;
+}
+
 // The Q8_0 view's own arguments; pointers are looked at in check_kv_q8_pointers.
 int check_kv_q8(const char* name, const asm_kv_q8_t* d, KvQ8Args* out) {
   if (!d) return set_error(ASM_E_INVALID, "%s: null key-value descriptor", name);
@@ -1207,13 +1249,13 @@ int check_kv_q8(const char* name, const asm_kv_q8_t* d, KvQ8Args* out) {
   return ASM_OK;
 }
 
-int check_kv_q8_pointers(const char* name, const KvQ8Args& c) {
-  int rc;
-  if ((rc = require_device(name, c.kv.k, "k")) || (rc = require_device(name, c.kv.v, "v")) ||
-      (rc = require_device(name, c.ks, "k scales")) || (rc = require_device(name, c.vs, "v scales")) ||
-      (rc = require_device(name, c.kv.table, "page table")) || (rc = require_device(name, c.kv.len, "lengths")))
-    return rc;
-  return ASM_OK;
+// The cache's pointers and up to six more.
+int check_kv_q8_pointers(const char* name, const KvQ8Args& c, std::initializer_list<Given> more) {
+  Given x[12] = {{c.kv.k, "k"}, {c.kv.v, "v"}, {c.ks, "k scales"}, {c.vs, "v scales"}, {c.kv.table, "page table"},
+                 {c.kv.len, "lengths"}};
+  int n = 6;
+  for (const Given& g : more) x[n++] = g;
+  return require_devices(name, x, n);
 }
 
 // The cache's four arrays.
@@ -1265,9 +1307,7 @@ ASMLLM_API int asm_rope_append_q8_async(const void* qkv, int32_t qkv_dtype, int6
   if ((uintptr_t)qkv % 16 || (uintptr_t)rope_cs % 16 || (uintptr_t)q_out % 16)
     return set_error(ASM_E_INVALID, "%s: misaligned buffer", name);
   if (rows == 0 || kv.batch == 0) return ASM_OK;
-  if ((rc = check_kv_q8_pointers(name, c)) || (rc = require_device(name, qkv, "qkv")) ||
-      (rc = require_device(name, rope_cs, "rope_cs")) || (rc = require_device(name, q_out, "q_out")) ||
-      (cu_q && (rc = require_device(name, cu_q, "cu_q"))))
+  if ((rc = check_kv_q8_pointers(name, c, {{qkv, "qkv"}, {rope_cs, "rope_cs"}, {q_out, "q_out"}, {cu_q, "cu_q", false}})))
     return rc;
   const long long cols = (long long)(n_heads + 2 * kv.n_kv) * kv.head_dim;
   const int wide = qkv_dtype == ASM_DT_F32 ? 4 : 2;
@@ -1304,9 +1344,7 @@ ASMLLM_API int asm_cache_read_q8_async(const asm_kv_q8_t* kvd, const int32_t* cu
     return set_error(ASM_E_UNSUPPORTED, "%s: rows are read back in fp16 or bf16", name);
   if ((uintptr_t)k_out % 16 || (uintptr_t)v_out % 16) return set_error(ASM_E_INVALID, "%s: misaligned buffer", name);
   if (rows == 0 || kv.batch == 0) return ASM_OK;
-  if ((rc = check_kv_q8_pointers(name, c)) || (rc = require_device(name, cu, "row offsets")) ||
-      (rc = require_device(name, k_out, "k_out")) || (rc = require_device(name, v_out, "v_out")))
-    return rc;
+  if ((rc = check_kv_q8_pointers(name, c, {{cu, "row offsets"}, {k_out, "k_out"}, {v_out, "v_out"}}))) return rc;
   const size_t bytes = (size_t)rows * kv.n_kv * kv.head_dim * 2;
   const Strided in[2] = {flat(cu, 4, kv.batch + 1), flat(v_out, 1, (long long)bytes)};
   if ((rc = check_apart_q8(name, "k_out", k_out, bytes, in, 2, c)) ||
@@ -1351,9 +1389,7 @@ ASMLLM_API int asm_attention_paged_q8_async(const void* q, int32_t q_dtype, int6
     return set_error(ASM_E_INVALID, "%s: workspace of %lld bytes, %zu needed (16-byte aligned)", name,
                      (long long)workspace_bytes, need);
   if (kv.batch == 0) return ASM_OK;
-  if ((rc = check_kv_q8_pointers(name, c)) || (rc = require_device(name, q, "q")) ||
-      (rc = require_device(name, out, "out")) || (rc = require_device(name, workspace, "workspace")))
-    return rc;
+  if ((rc = check_kv_q8_pointers(name, c, {{q, "q"}, {out, "out"}, {workspace, "workspace"}}))) return rc;
   const size_t out_bytes = (size_t)kv.batch * n_heads * kv.head_dim * (out_dtype == ASM_DT_F32 ? 4 : 2);
   const Strided in[2] = {{q, 2, kv.head_dim, {kv.batch, n_heads, 1}, {q_row_stride, q_head_stride, 0}},
                          flat(out, 1, (long long)out_bytes)};
@@ -1404,11 +1440,9 @@ ASMLLM_API int asm_attention_shared_async(const void* q, int64_t q_row_stride, i
     return set_error(ASM_E_INVALID, "%s: workspace of %lld bytes, %zu needed (16-byte aligned)", name,
                      (long long)workspace_bytes, need);
   if (kv.batch == 0) return ASM_OK;
-  if ((rc = check_kv_pointers(name, kv)) || (rc = require_device(name, q, "q")) ||
-      (rc = require_device(name, out, "out")) || (rc = require_device(name, workspace, "workspace")) ||
-      (groups && ((rc = require_device(name, cu_group, "group offsets")) ||
-                  (rc = require_device(name, shared_len, "shared lengths")))))
-    return rc;
+  const Given given[9] = {{kv.k, "k"}, {kv.v, "v"}, {kv.table, "page table"}, {kv.len, "lengths"}, {q, "q"}, {out, "out"},
+                          {workspace, "workspace"}, {cu_group, "group offsets"}, {shared_len, "shared lengths"}};
+  if ((rc = require_devices(name, given, groups ? 9 : 7))) return rc;
   const size_t out_bytes = (size_t)kv.batch * n_heads * kv.head_dim * (out_dtype == ASM_DT_F32 ? 4 : 2);
   const Strided in[4] = {{q, 2, kv.head_dim, {kv.batch, n_heads, 1}, {q_row_stride, q_head_stride, 0}},
                          flat(groups ? cu_group : nullptr, 4, groups + 1), flat(groups ? shared_len : nullptr, 4, groups),
@@ -1458,14 +1492,12 @@ ASMLLM_API int asm_rows_adjust_async(const asm_adjust_t* d, void* stream) {
   const int32_t* bias_tokens = d->n_bias ? d->bias_tokens : nullptr;
   const float* bias = d->n_bias ? d->bias : nullptr;
   const int32_t* tokens = d->held ? d->tokens : nullptr;
-  struct { const void* p; const char* what; } given[] = {
-      {tokens, "tokens"}, {d->n_tokens, "n_tokens"}, {d->n_prompt, "n_prompt"}, {d->repetition, "repetition"},
-      {d->frequency, "frequency"}, {d->presence, "presence"}, {bias_tokens, "bias_tokens"}, {bias, "bias"},
-      {d->allowed, "allowed"}};
-  int rc;
-  if ((rc = require_device(name, d->logits, "logits")) || (rc = require_device(name, d->out, "out"))) return rc;
-  for (const auto& x : given)
-    if (x.p && (rc = require_device(name, x.p, x.what))) return rc;
+  const Given given[] = {{d->logits, "logits"}, {d->out, "out"}, {tokens, "tokens", false}, {d->n_tokens, "n_tokens", false},
+                         {d->n_prompt, "n_prompt", false}, {d->repetition, "repetition", false},
+                         {d->frequency, "frequency", false}, {d->presence, "presence", false},
+                         {bias_tokens, "bias_tokens", false}, {bias, "bias", false}, {d->allowed, "allowed", false}};
+  int rc = require_devices(name, given, 11);
+  if (rc) return rc;
   const long long rows = d->rows;
   const Strided in[10] = {{d->logits, size, d->n, {rows, 1, 1}, {d->stride, 0, 0}},
                           {tokens, 4, d->held, {rows, 1, 1}, {d->token_stride, 0, 0}}, flat(d->n_tokens, 4, rows),

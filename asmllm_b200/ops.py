@@ -835,43 +835,112 @@ def rows_sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=No
 
 # --------------------------------------------------------------------------
 # Serving operators around an 8-bit cache, shared prefixes and logits
+#
+# Where a tensor is (which device, or none) is looked at by the library, once
+# a pointer; when it refuses a call, the tensors are gone through for the one
+# at fault.  Types, shapes and strides are only known here.
 # --------------------------------------------------------------------------
 
+_SPACE: dict = {}  # (function, sizes) -> bytes of workspace
+_cuda_empty = None
 
-def _kv_q8_view(k, v, k_scales, v_scales, device, kv_len, page_table):
-    """asm_kv_q8_t of codes k, v int8 [pages, page_size, heads, head_dim] and scales fp16
-    [pages, heads, page_size, head_dim / 32]."""
-    if not _DT:
-        _dtypes()
+
+def _setup():
+    """_dtypes, and torch's quickest way to an uninitialised tensor (0.9 us, new_empty takes 2) where it has it."""
+    global _cuda_empty
+    _dtypes()
+    try:
+        from torch._C._dynamo.guards import _empty_strided_cuda as _cuda_empty  # noqa: F811
+    except ImportError:
+        pass
+
+
+def _fresh(like, shape, dtype, stream):
+    """_empty on the current device (where the library wants its tensors), dense."""
+    if stream is not None or _cuda_empty is None:
+        return _empty(like, shape, dtype, stream)
+    if len(shape) == 3:
+        return _cuda_empty(shape, (shape[1] * shape[2], shape[2], 1), dtype)
+    return _cuda_empty(shape, (shape[1], 1) if len(shape) == 2 else (1,), dtype)
+
+
+def _place(t, name):
+    device = t.get_device()
+    if device < 0:
+        raise TypeError(f"{name}: expected a CUDA tensor")
+    return device
+
+
+def _ran(rc, tensors):
+    """Raises what the library refused: a TypeError or ValueError that names the tensor where it is one's place."""
+    if not rc:
+        return
+    code, message = native.last_error()
+    where = None
+    for t, name in tensors:
+        if t is None or not t.numel():
+            continue
+        if not t.is_cuda:
+            raise TypeError(f"{name}: expected a CUDA tensor")
+        where = t.get_device() if where is None else where
+        if t.get_device() != where:
+            raise ValueError(f"{name} is on device {t.get_device()}, {tensors[0][1]} on {where}")
+    raise AsmError(code or rc, message or "call failed")
+
+
+def _column(t, name, n, dtype):
+    """[n] of dtype, dense."""
+    if t.dtype is dtype and t.dim() == 1 and t.shape[0] == n and (n < 2 or t.is_contiguous()):
+        return t.data_ptr()
+    if t.dtype is not dtype:
+        raise TypeError(f"{name}: dtype {t.dtype}, expected {dtype}")
+    raise ValueError(f"{name}: shape {tuple(t.shape)} with strides {t.stride()}, expected ({n},), dense")
+
+
+def _table(page_table):
+    """Checked int32 [batch, width]: (address, row stride, batch, width)."""
     if page_table is None:
         raise ValueError("page_table is required")
-    shape, st, ss = k.shape, _strides(k), _strides(k_scales)
-    if (k.dtype is not _I8 or v.dtype is not _I8 or k_scales.dtype is not _F16 or v_scales.dtype is not _F16
-            or len(st) != 4 or len(ss) != 4 or shape != v.shape or st != _strides(v) or st[-1] != 1
-            or k_scales.shape != v_scales.shape or ss != _strides(v_scales)
-            or not k.get_device() == v.get_device() == k_scales.get_device() == v_scales.get_device() == device >= 0):
+    if page_table.dtype is not _I32 or page_table.dim() != 2:
+        raise TypeError(f"page_table: expected int32 with 2 axes, got {page_table.dtype} {tuple(page_table.shape)}")
+    batch, width = page_table.shape
+    row, col = page_table.stride()
+    if width > 1 and col != 1:
+        raise ValueError(f"page_table: rows must be dense, got strides {page_table.stride()}")
+    return page_table.data_ptr(), row if batch > 1 else width, batch, width
+
+
+def _kv_q8_view(k, v, k_scales, v_scales, kv_len, page_table):
+    """asm_kv_q8_t of codes k, v int8 [pages, page_size, heads, head_dim] and scales fp16
+    [pages, heads, page_size, head_dim / 32]."""
+    shape, st, ss = k.shape, k.stride(), k_scales.stride()
+    if not (k.dtype is v.dtype is _I8 and k_scales.dtype is v_scales.dtype is _F16 and len(st) == 4 == len(ss)
+            and v.shape == shape and (v.stride() == st or _strides(v) == _strides(k)) and v_scales.shape == k_scales.shape
+            and (v_scales.stride() == ss or _strides(v_scales) == _strides(k_scales))):
         for t, name, dt in ((k, "k", _I8), (v, "v", _I8), (k_scales, "k_scales", _F16), (v_scales, "v_scales", _F16)):
-            _dense(t, name, 4, (dt,))
-        if shape != v.shape or st != _strides(v) or k_scales.shape != v_scales.shape or ss != _strides(v_scales):
-            raise ValueError(f"k and v, and their scales, must agree in shape and strides: {tuple(k.shape)} {k.stride()}, "
-                             f"{tuple(v.shape)} {v.stride()}; {tuple(k_scales.shape)} {k_scales.stride()}, "
-                             f"{tuple(v_scales.shape)} {v_scales.stride()}")
-        raise ValueError("k, v, their scales and the rows are on different devices")
+            if t.dtype is not dt:
+                raise TypeError(f"{name}: dtype {t.dtype}, expected {dt}")
+        raise ValueError(f"k and v, and their scales, must have 4 axes and agree in shape and strides: {tuple(k.shape)} "
+                         f"{k.stride()}, {tuple(v.shape)} {v.stride()}; {tuple(k_scales.shape)} {k_scales.stride()}, "
+                         f"{tuple(v_scales.shape)} {v_scales.stride()}")
     pages, size, heads, hd = shape
-    if k_scales.shape != (pages, heads, size, hd // 32) or hd % 32:
+    per = hd // 32
+    if k_scales.shape != (pages, heads, size, per) or hd % 32:
         raise ValueError(f"k_scales {tuple(k_scales.shape)}: expected [pages, heads, page_size, head_dim / 32] of "
                          f"k {tuple(shape)}")
-    if ss[3] != 1 or ss[2] != hd // 32:
-        raise ValueError(f"k_scales: a head's scales of a page must be dense, got strides {k_scales.stride()}")
-    batch, width = page_table.shape
-    if (page_table.dtype is not _I32 or page_table.get_device() != device
-            or (width > 1 and page_table.stride(1) != 1)):
-        _dense(page_table, "page_table", 2, (_I32,))
-        raise ValueError("page_table is on another device")
-    _vector(kv_len, "kv_len", batch, device)
-    return (_KV_Q8_PACK(k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), st[0], st[1], st[2],
-                        ss[0], ss[1], page_table.data_ptr(), page_table.stride(0) if batch > 1 else width,
-                        kv_len.data_ptr(), batch, pages, size, width, heads, hd), batch)
+    page, token, head, one = st
+    if one != 1 or (per > 1 and ss[3] != 1) or (size > 1 and ss[2] != per):
+        raise ValueError(f"head_dim, and a head's scales of a page, must be dense: k {k.stride()}, k_scales "
+                         f"{k_scales.stride()}")
+    spage, shead = ss[0], ss[1]
+    if heads == 1:  # the stride of an axis with one entry means nothing
+        head, shead = hd, size * per
+    if pages == 1:
+        page, spage = token * size, heads * size * per
+    table, row, batch, width = _table(page_table)
+    return _KV_Q8_PACK(k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), page, token, head,
+                       spage, shead, table, row, _column(kv_len, "kv_len", batch, _I32), batch, pages, size, width,
+                       heads, hd), batch, heads, hd
 
 
 def rope_append_q8(qkv, rope_cs, kv_len, page_table, k_pages, v_pages, k_scales, v_scales, n_heads: int, *, cu_q=None,
@@ -883,40 +952,45 @@ def rope_append_q8(qkv, rope_cs, kv_len, page_table, k_pages, v_pages, k_scales,
     Keys are rotated in fp32, and keys and values quantized in blocks of 32 as quantize_q8_0 does it, the
     scale rounded to fp16.  qkv fp32, or fp16 or bf16 (the queries' type then).  Returns the rotated queries
     [T, nh, hd] in q_dtype (qkv's type; fp16 for fp32)."""
-    device = qkv.get_device()
-    if device < 0:
-        raise TypeError("qkv: expected a CUDA tensor")
-    kv, batch = _kv_q8_view(k_pages, v_pages, k_scales, v_scales, device, kv_len, page_table)
-    nkv, hd = k_pages.shape[2:]
-    if qkv.dtype not in _DT or qkv.dim() != 2 or qkv.stride(1) != 1:
-        _dense(qkv, "qkv", 2, _DT)
-    dt = q_dtype or (q_out.dtype if q_out is not None else _F16 if qkv.dtype is _F32 else qkv.dtype)
-    if dt not in _H16 or (qkv.dtype is not _F32 and qkv.dtype is not dt):
-        raise TypeError(f"queries of {dt} from qkv of {qkv.dtype}: fp16 or bf16, from fp32 or the same type")
-    T = qkv.shape[0]
-    if qkv.shape[1] != (n_heads + 2 * nkv) * hd:
-        raise ValueError(f"qkv has {qkv.shape[1]} columns, expected ({n_heads} + 2 * {nkv}) * {hd}")
-    if rope_cs.dtype is not _F32 or rope_cs.get_device() != device or not rope_cs.is_contiguous():
-        _check_dev(rope_cs, (_F32,), "rope_cs")
-        raise ValueError("rope_cs is on another device")
-    if rope_cs.shape[1:] != (hd // 2, 2):
-        raise ValueError(f"rope_cs {tuple(rope_cs.shape)}: expected [positions, {hd // 2}, 2]")
+    if _cuda_empty is None:
+        _setup()
+    device = _place(qkv, "qkv")
+    kv, batch, nkv, hd = _kv_q8_view(k_pages, v_pages, k_scales, v_scales, kv_len, page_table)
+    src = qkv.dtype
+    if src not in _DT:
+        raise TypeError(f"qkv: dtype {src} not in {tuple(_DT)}")
+    T, cols = qkv.shape
+    row, col = qkv.stride()
+    if cols != (n_heads + 2 * nkv) * hd or col != 1:
+        raise ValueError(f"qkv {tuple(qkv.shape)} with strides {qkv.stride()}, expected dense rows of ({n_heads} + "
+                         f"2 * {nkv}) * {hd}")
+    if rope_cs.dtype is not _F32 or rope_cs.shape[1:] != (hd // 2, 2) or not rope_cs.is_contiguous():
+        if rope_cs.dtype is not _F32:
+            raise TypeError(f"rope_cs: dtype {rope_cs.dtype}, expected fp32")
+        raise ValueError(f"rope_cs {tuple(rope_cs.shape)}: expected [positions, {hd // 2}, 2], dense")
+    cu = None
     if cu_q is not None:
-        _vector(cu_q, "cu_q", batch + 1, device)
+        cu = _column(cu_q, "cu_q", batch + 1, _I32)
     elif T != batch:
         raise ValueError(f"{T} rows for {batch} sequences: pass cu_q")
+    dt = q_dtype or (q_out.dtype if q_out is not None else _F16 if src is _F32 else src)
+    if dt not in _H16 or (src is not _F32 and src is not dt):
+        raise TypeError(f"queries of {dt} from qkv of {src}: fp16 or bf16, from fp32 or the same type")
     if q_out is None:
-        q_out = _empty(qkv, (T, n_heads, hd), dt, stream)
-    else:
-        _check_dev(q_out, (dt,), "q_out")
-        if q_out.shape != (T, n_heads, hd) or q_out.get_device() != device:
-            raise ValueError(f"q_out {tuple(q_out.shape)} on device {q_out.get_device()}: expected {(T, n_heads, hd)} on {device}")
+        q_out = _fresh(qkv, (T, n_heads, hd), dt, stream)
+    elif q_out.dtype is not dt or q_out.shape != (T, n_heads, hd) or not q_out.is_contiguous():
+        if q_out.dtype is not dt:
+            raise TypeError(f"q_out: dtype {q_out.dtype}, expected {dt}")
+        raise ValueError(f"q_out {tuple(q_out.shape)}: expected {(T, n_heads, hd)}, dense")
     if T == 0 or batch == 0:
         return q_out
-    _call((native._lib or native.lib()).asm_rope_append_q8_async(
-        qkv.data_ptr(), _DT[qkv.dtype], qkv.stride(0) if T > 1 else qkv.shape[1], rope_cs.data_ptr(),
-        rope_cs.shape[0], None if cu_q is None else cu_q.data_ptr(), T, n_heads, q_out.data_ptr(), _H16[dt], kv,
-        _current_stream(device) if stream is None else stream.cuda_stream))
+    rc = (native._lib or native.lib()).asm_rope_append_q8_async(
+        qkv.data_ptr(), _DT[src], row if T > 1 else cols, rope_cs.data_ptr(), rope_cs.shape[0], cu, T, n_heads,
+        q_out.data_ptr(), _H16[dt], kv,
+        _current_stream(device) if stream is None else stream.cuda_stream)
+    if rc:
+        _ran(rc, ((qkv, "qkv"), (rope_cs, "rope_cs"), (kv_len, "kv_len"), (page_table, "page_table"), (k_pages, "k_pages"),
+                  (v_pages, "v_pages"), (k_scales, "k_scales"), (v_scales, "v_scales"), (cu_q, "cu_q"), (q_out, "q_out")))
     return q_out
 
 
@@ -929,62 +1003,79 @@ def cache_read_q8(k_pages, v_pages, k_scales, v_scales, page_table, kv_len, cu, 
     as it has rows (cu of the sums of kv_len reads everything, cu_q what a call has just appended).  Returns
     (k, v) [rows, nkv, hd] in dtype (fp16 unless given) or in out=(k, v); rows before a sequence's first
     position are zeros, rows at or past cu[B] are not written."""
-    device = k_pages.get_device()
-    kv, batch = _kv_q8_view(k_pages, v_pages, k_scales, v_scales, device, kv_len, page_table)
-    _vector(cu, "cu", batch + 1, device)
-    shape = (rows, *k_pages.shape[2:])
+    if _cuda_empty is None:
+        _setup()
+    device = _place(k_pages, "k_pages")
+    kv, batch, nkv, hd = _kv_q8_view(k_pages, v_pages, k_scales, v_scales, kv_len, page_table)
+    at = _column(cu, "cu", batch + 1, _I32)
+    shape = (rows, nkv, hd)
     if rows < 0:
         raise ValueError(f"rows {rows}")
+    dt = dtype or (_F16 if out is None else out[0].dtype)
+    if dt not in _H16:
+        raise TypeError(f"dtype {dt}: fp16 or bf16")
     if out is None:
-        dt = dtype or _F16
-        if dt not in _H16:
-            raise TypeError(f"dtype {dt}: fp16 or bf16")
-        k, v = _empty(k_pages, shape, dt, stream), _empty(k_pages, shape, dt, stream)
+        k, v = _fresh(k_pages, shape, dt, stream), _fresh(k_pages, shape, dt, stream)
     else:
         k, v = out
-        dt = dtype or k.dtype
         for t, name in ((k, "out[0]"), (v, "out[1]")):
-            _check_dev(t, (dt,) if dt in _H16 else tuple(_H16), name)
-            if t.shape != shape or t.get_device() != device:
-                raise ValueError(f"{name} {tuple(t.shape)} on device {t.get_device()}: expected {shape} on {device}")
+            if t.dtype is not dt:
+                raise TypeError(f"{name}: dtype {t.dtype}, expected {dt}")
+            if t.shape != shape or not t.is_contiguous():
+                raise ValueError(f"{name} {tuple(t.shape)}: expected {shape}, dense")
     if rows == 0 or batch == 0:
         return k, v
-    _call((native._lib or native.lib()).asm_cache_read_q8_async(
-        kv, cu.data_ptr(), rows, k.data_ptr(), v.data_ptr(), _H16[dt],
-        _current_stream(device) if stream is None else stream.cuda_stream))
+    rc = (native._lib or native.lib()).asm_cache_read_q8_async(
+        kv, at, rows, k.data_ptr(), v.data_ptr(), _H16[dt],
+        _current_stream(device) if stream is None else stream.cuda_stream)
+    if rc:
+        _ran(rc, ((k_pages, "k_pages"), (v_pages, "v_pages"), (k_scales, "k_scales"), (v_scales, "v_scales"),
+                  (page_table, "page_table"), (kv_len, "kv_len"), (cu, "cu"), (k, "out[0]"), (v, "out[1]")))
     return k, v
 
 
-def _decode_query(q, nkv, hd, out, out_dtype, stream):
-    """Checks q [B, heads, head_dim] against the cache's heads and returns (strides, out)."""
-    shape, st = q.shape, _strides(q)
-    if q.dtype not in _H16 or not q.is_cuda or len(shape) != 3 or st[2] != 1:
-        _dense(q, "q", 3, _H16)
-    if shape[2] != hd:
-        raise ValueError(f"q of head_dim {shape[2]} against keys of {hd}")
-    if nkv == 0 or shape[1] == 0 or shape[1] % nkv:
-        raise ValueError(f"{shape[1]} query heads are not a multiple of {nkv} KV heads")
+def _decode_query(q, batch, nkv, hd, out, out_dtype, stream):
+    """Checks q [B, heads, head_dim] against the cache; (row stride, head stride, heads, out)."""
+    shape, st = q.shape, q.stride()
+    if q.dtype not in _H16 or len(st) != 3:
+        raise TypeError(f"q: expected fp16 or bf16 with 3 axes, got {q.dtype} {tuple(shape)}")
+    B, nh, d = shape
+    row, head, one = st
+    if B == 1:  # the stride of an axis with one entry means nothing
+        row = nh * hd
+    if nh == 1:
+        head = hd
+    if d != hd or one != 1 or B != batch:
+        raise ValueError(f"q {tuple(shape)} with strides {q.stride()}: expected {batch} sequences and head_dim {hd}, dense")
+    if nkv == 0 or nh == 0 or nh % nkv:
+        raise ValueError(f"{nh} query heads are not a multiple of {nkv} KV heads")
     if out is None:
         dt = out_dtype or q.dtype
-        if dt != q.dtype and dt != _F32:
+        if dt is not q.dtype and dt is not _F32:
             raise TypeError(f"out_dtype {dt}: fp32 or q's type")
-        return st, _empty(q, shape, dt, stream)
-    _check_dev(out, (q.dtype, _F32), "out")
-    if out.shape != shape or out.get_device() != q.get_device() or (out_dtype is not None and out.dtype != out_dtype):
-        raise ValueError(f"out: {tuple(out.shape)} {out.dtype} on device {out.get_device()}, expected {tuple(shape)} "
-                         f"{out_dtype or q.dtype} on {q.get_device()}")
-    return st, out
+        return row, head, nh, _fresh(q, (B, nh, hd), dt, stream)
+    if (out.dtype is not q.dtype and out.dtype is not _F32) or (out_dtype is not None and out.dtype is not out_dtype):
+        raise TypeError(f"out: dtype {out.dtype}, expected {out_dtype or q.dtype}")
+    if out.shape != shape or not out.is_contiguous():
+        raise ValueError(f"out {tuple(out.shape)}: expected {tuple(shape)}, dense")
+    return row, head, nh, out
 
 
-def _scratch(q, workspace, need, stream):
-    if need < 0:
-        native.check()
-    if workspace is None:
-        return _empty(q, (need,), _U8, stream)
-    _check_dev(workspace, (_U8,), "workspace")
-    if workspace.get_device() != q.get_device():
-        raise ValueError("workspace is on another device")
-    return workspace
+def _scratch(q, workspace, function, sizes, stream):
+    """The given workspace, or a new one of the bytes function(*sizes) asks for."""
+    if workspace is not None:
+        if workspace.dtype is not _U8 or not workspace.is_contiguous():
+            raise TypeError(f"workspace: expected dense uint8, got {workspace.dtype}")
+        return workspace
+    need = _SPACE.get((function, sizes))
+    if need is None:
+        need = int(getattr(native.lib(), function)(*sizes))
+        if need < 0:
+            native.check()
+        if len(_SPACE) > 4096:
+            _SPACE.clear()
+        _SPACE[function, sizes] = need
+    return _fresh(q, (need,), _U8, stream)
 
 
 def attention_paged_q8_workspace(batch: int, n_heads: int, n_kv_heads: int, head_dim: int) -> int:
@@ -1000,21 +1091,21 @@ def attention_paged_q8(q, k_pages, v_pages, k_scales, v_scales, page_table, kv_l
     """attention_paged over a Q8_0 cache (asm_attention_paged_q8_async): q [B, nh, hd] fp16 or bf16, the cache
     as rope_append_q8 fills it, page_table int32 [B, n], kv_len int32 [B].  out [B, nh, hd] in q's type or
     fp32.  workspace: uint8 of attention_paged_q8_workspace bytes, one per call that may overlap another."""
-    device = q.get_device()
-    kv, batch = _kv_q8_view(k_pages, v_pages, k_scales, v_scales, device, kv_len, page_table)
-    nkv, hd = k_pages.shape[2:]
-    st, out = _decode_query(q, nkv, hd, out, out_dtype, stream)
-    B, nh, _ = q.shape
-    if B != batch:
-        raise ValueError(f"q has {B} rows for {batch} sequences")
-    if B == 0:
+    if _cuda_empty is None:
+        _setup()
+    device = _place(q, "q")
+    kv, batch, nkv, hd = _kv_q8_view(k_pages, v_pages, k_scales, v_scales, kv_len, page_table)
+    row, head, nh, out = _decode_query(q, batch, nkv, hd, out, out_dtype, stream)
+    if batch == 0:
         return out
-    lib = native._lib or native.lib()
-    workspace = _scratch(q, workspace, lib.asm_attention_paged_q8_workspace(B, nh, nkv, hd), stream)
-    _call(lib.asm_attention_paged_q8_async(
-        q.data_ptr(), _H16[q.dtype], st[0], st[1], nh, hd ** -0.5 if scale is None else scale, out.data_ptr(),
-        _DT[out.dtype], kv, workspace.data_ptr(), workspace.numel(),
-        _current_stream(device) if stream is None else stream.cuda_stream))
+    workspace = _scratch(q, workspace, "asm_attention_paged_q8_workspace", (batch, nh, nkv, hd), stream)
+    rc = (native._lib or native.lib()).asm_attention_paged_q8_async(
+        q.data_ptr(), _H16[q.dtype], row, head, nh, hd ** -0.5 if scale is None else scale, out.data_ptr(),
+        _DT[out.dtype], kv, workspace.data_ptr(), workspace.shape[0],
+        _current_stream(device) if stream is None else stream.cuda_stream)
+    if rc:
+        _ran(rc, ((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages"), (k_scales, "k_scales"), (v_scales, "v_scales"),
+                  (page_table, "page_table"), (kv_len, "kv_len"), (out, "out"), (workspace, "workspace")))
     return out
 
 
@@ -1036,29 +1127,56 @@ def attention_shared(q, k_pages, v_pages, page_table, kv_len, cu_group, shared_l
     all positions.  A sequence in no group, or shorter than what its group shares, is on its own.  The rest is
     attention_paged's.  workspace: uint8 of attention_shared_workspace bytes, one per call that may overlap
     another."""
-    if page_table is None:
-        raise ValueError("page_table is required")
-    device = q.get_device()
-    kv, batch = _kv_view(k_pages, v_pages, device, kv_len, page_table)
-    nkv, hd = k_pages.shape[2:]
-    if q.dtype != k_pages.dtype:
-        raise ValueError(f"q {q.dtype} against keys {k_pages.dtype}")
-    st, out = _decode_query(q, nkv, hd, out, out_dtype, stream)
-    B, nh, _ = q.shape
-    if B != batch:
-        raise ValueError(f"q has {B} rows for {batch} sequences")
-    groups = shared_len.shape[0] if shared_len.dim() == 1 else -1
-    _vector(shared_len, "shared_len", groups, device)
-    _vector(cu_group, "cu_group", groups + 1, device)
-    if B == 0:
+    if _cuda_empty is None:
+        _setup()
+    device = _place(q, "q")
+    shape, st = k_pages.shape, k_pages.stride()
+    if not (k_pages.dtype is v_pages.dtype is q.dtype in _H16 and len(st) == 4 and v_pages.shape == shape
+            and (v_pages.stride() == st or _strides(v_pages) == _strides(k_pages)) and st[3] == 1):
+        if not k_pages.dtype is v_pages.dtype is q.dtype in _H16:
+            raise TypeError(f"q {q.dtype}, k_pages {k_pages.dtype}, v_pages {v_pages.dtype}: fp16 or bf16, all the same")
+        raise ValueError(f"k_pages and v_pages must have 4 axes, the last one dense, and agree in shape and strides: "
+                         f"{tuple(shape)} {k_pages.stride()}, {tuple(v_pages.shape)} {v_pages.stride()}")
+    pages, size, nkv, hd = shape
+    page, token, khead, _ = st
+    if nkv == 1:  # the stride of an axis with one entry means nothing
+        khead = hd
+    if pages == 1:
+        page = token * size
+    table, trow, batch, width = _table(page_table)
+    row, head, nh, out = _decode_query(q, batch, nkv, hd, out, out_dtype, stream)
+    if shared_len.dim() != 1:
+        raise ValueError(f"shared_len {tuple(shared_len.shape)}: expected one axis")
+    groups = shared_len.shape[0]
+    shared, cu = _column(shared_len, "shared_len", groups, _I32), _column(cu_group, "cu_group", groups + 1, _I32)
+    lens = _column(kv_len, "kv_len", batch, _I32)
+    if batch == 0:
         return out
-    lib = native._lib or native.lib()
-    workspace = _scratch(q, workspace, lib.asm_attention_shared_workspace(B, groups, nh, nkv, hd), stream)
-    _call(lib.asm_attention_shared_async(
-        q.data_ptr(), st[0], st[1], nh, hd ** -0.5 if scale is None else scale, out.data_ptr(), _DT[out.dtype], kv,
-        cu_group.data_ptr(), shared_len.data_ptr(), groups, workspace.data_ptr(), workspace.numel(),
-        _current_stream(device) if stream is None else stream.cuda_stream))
+    workspace = _scratch(q, workspace, "asm_attention_shared_workspace", (batch, groups, nh, nkv, hd), stream)
+    rc = (native._lib or native.lib()).asm_attention_shared_async(
+        q.data_ptr(), row, head, nh, hd ** -0.5 if scale is None else scale, out.data_ptr(), _DT[out.dtype],
+        _KV_PACK(k_pages.data_ptr(), v_pages.data_ptr(), page, token, khead, table, trow, lens, 0, batch, pages, size,
+                 width, nkv, hd, _H16[q.dtype], 0),
+        cu, shared, groups, workspace.data_ptr(), workspace.shape[0],
+        _current_stream(device) if stream is None else stream.cuda_stream)
+    if rc:
+        _ran(rc, ((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages"), (page_table, "page_table"), (kv_len, "kv_len"),
+                  (cu_group, "cu_group"), (shared_len, "shared_len"), (out, "out"), (workspace, "workspace")))
     return out
+
+
+def _rows2(t, name, rows, dtype):
+    """[rows, n] of dtype with dense rows: (address, n, row stride)."""
+    if t.dtype is not dtype:
+        raise TypeError(f"{name}: dtype {t.dtype}, expected {dtype}")
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != rows:
+        raise ValueError(f"{name}: shape {tuple(shape)}, expected {rows} rows")
+    row, col = t.stride()
+    n = shape[1]
+    if n > 1 and col != 1:
+        raise ValueError(f"{name}: rows must be dense, got strides {t.stride()}")
+    return t.data_ptr(), n, row if rows > 1 else n
 
 
 def rows_adjust(logits, *, tokens=None, n_tokens=None, n_prompt=None, repetition=None, frequency=None, presence=None,
@@ -1072,51 +1190,58 @@ def rows_adjust(logits, *, tokens=None, n_tokens=None, n_prompt=None, repetition
     fp32 [B, N], those of equal entries added up; words whose bit is 0 in allowed int32 [B, ceil(V / 32)] (bit
     w % 32 of w / 32) become -inf.  n_tokens, n_prompt int32 [B] (L, 0) and repetition, frequency, presence
     fp32 [B] (1, 0, 0) are optional.  Returns a new tensor, or out, which may be logits."""
-    if not _DT:
-        _dtypes()
-    if logits.dtype not in _DT or not logits.is_cuda or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        _dense(logits, "logits", 2, _DT)
-    B, V = shape = logits.shape
-    device = logits.get_device()
+    if _cuda_empty is None:
+        _setup()
+    device = _place(logits, "logits")
+    dt = logits.dtype
+    if dt not in _DT or logits.dim() != 2:
+        raise TypeError(f"logits: expected fp32, fp16 or bf16 with 2 axes, got {dt} {tuple(logits.shape)}")
+    B, V = logits.shape
+    at, _, row = _rows2(logits, "logits", B, dt)
     if out is None:
-        out = _empty(logits, shape, logits.dtype, stream)
-    elif out.dtype is not logits.dtype or out.shape != shape or out.get_device() != device or (V > 1 and out.stride(1) != 1):
-        _dense(out, "out", 2, (logits.dtype,))
-        raise ValueError(f"out: {tuple(out.shape)} on device {out.get_device()}, expected {tuple(shape)} on {device}")
-    ptr = []
-    for t, name, dt in ((n_tokens, "n_tokens", _I32), (n_prompt, "n_prompt", _I32), (repetition, "repetition", _F32),
-                        (frequency, "frequency", _F32), (presence, "presence", _F32)):
-        if t is None:
-            ptr.append(0)
-            continue
-        if tokens is None:
-            raise ValueError(f"{name} without tokens")
-        if t.dtype is not dt or t.get_device() != device or t.shape != shape[:1] or (B > 1 and t.stride(0) != 1):
-            _check_dev(t, (dt,), name)
-            raise ValueError(f"{name}: shape {tuple(t.shape)} on device {t.get_device()}, expected ({B},) on {device}")
-        ptr.append(t.data_ptr())
-    if (bias_tokens is None) != (bias is None):
+        out = _fresh(logits, (B, V), dt, stream)
+        to, n, to_row = out.data_ptr(), V, V
+    else:
+        to, n, to_row = _rows2(out, "out", B, dt)
+    if n != V:
+        raise ValueError(f"out {tuple(out.shape)}: expected {(B, V)}")
+    token = held = token_row = 0
+    n1 = n2 = rep = freq = pres = words = biases = bits = bits_row = n_bias = 0
+    if tokens is not None:
+        token, held, token_row = _rows2(tokens, "tokens", B, _I32)
+        if n_tokens is not None:
+            n1 = _column(n_tokens, "n_tokens", B, _I32)
+        if n_prompt is not None:
+            n2 = _column(n_prompt, "n_prompt", B, _I32)
+        if repetition is not None:
+            rep = _column(repetition, "repetition", B, _F32)
+        if frequency is not None:
+            freq = _column(frequency, "frequency", B, _F32)
+        if presence is not None:
+            pres = _column(presence, "presence", B, _F32)
+        if held == 0:  # nothing is read, and an array without elements has no address
+            token = n1 = n2 = rep = freq = pres = 0
+    elif not (n_tokens is n_prompt is repetition is frequency is presence is None):
+        raise ValueError("penalties without tokens")
+    if bias_tokens is not None and bias is not None:
+        words, n_bias, row1 = _rows2(bias_tokens, "bias_tokens", B, _I32)
+        biases, m, row2 = _rows2(bias, "bias", B, _F32)
+        if m != n_bias or row1 != m or row2 != m:
+            raise ValueError(f"bias_tokens {tuple(bias_tokens.shape)} and bias {tuple(bias.shape)}: expected equal, dense ones")
+    elif not (bias_tokens is bias is None):
         raise ValueError("pass bias_tokens and bias together")
-    at = [(0, 0, 0)] * 4  # address, columns, row stride
-    for i, (t, name, dt) in enumerate(((tokens, "tokens", _I32), (bias_tokens, "bias_tokens", _I32), (bias, "bias", _F32),
-                                       (allowed, "allowed", _I32))):
-        if t is None:
-            continue
-        if t.dtype is not dt or t.get_device() != device or t.dim() != 2 or t.shape[0] != B or (
-                t.shape[1] > 1 and t.stride(1) != 1):
-            _dense(t, name, 2, (dt,))
-            raise ValueError(f"{name}: shape {tuple(t.shape)} on device {t.get_device()}, expected {B} rows on {device}")
-        n = t.shape[1]
-        at[i] = (t.data_ptr(), n, t.stride(0) if B > 1 else n)
-    if bias is not None and (bias.shape != bias_tokens.shape or not bias.is_contiguous() or not bias_tokens.is_contiguous()):
-        raise ValueError(f"bias_tokens {tuple(bias_tokens.shape)} and bias {tuple(bias.shape)}: expected equal, dense ones")
-    if allowed is not None and at[3][1] < (V + 31) // 32:
-        raise ValueError(f"allowed has {at[3][1]} words of 32 bits a row, {(V + 31) // 32} are needed")
+    if allowed is not None:
+        bits, n, bits_row = _rows2(allowed, "allowed", B, _I32)
+        if n < (V + 31) // 32:
+            raise ValueError(f"allowed has {n} words of 32 bits a row, {(V + 31) // 32} are needed")
     if B == 0 or V == 0:
         return out
-    _call((native._lib or native.lib()).asm_rows_adjust_async(
-        _ADJUST_PACK(logits.data_ptr(), out.data_ptr(), logits.stride(0) if B > 1 else V, out.stride(0) if B > 1 else V,
-                     _DT[logits.dtype], B, V, at[0][1], at[0][0], at[0][2], *ptr, at[1][0], at[2][0], at[3][0], at[3][2],
-                     at[1][1], 0),
-        _current_stream(device) if stream is None else stream.cuda_stream))
+    rc = (native._lib or native.lib()).asm_rows_adjust_async(
+        _ADJUST_PACK(at, to, row, to_row, _DT[dt], B, V, held, token, token_row, n1, n2, rep, freq, pres, words, biases,
+                     bits, bits_row, n_bias, 0),
+        _current_stream(device) if stream is None else stream.cuda_stream)
+    if rc:
+        _ran(rc, ((logits, "logits"), (out, "out"), (tokens, "tokens"), (n_tokens, "n_tokens"), (n_prompt, "n_prompt"),
+                  (repetition, "repetition"), (frequency, "frequency"), (presence, "presence"),
+                  (bias_tokens, "bias_tokens"), (bias, "bias"), (allowed, "allowed")))
     return out
