@@ -8,10 +8,11 @@
 // fp16) and the scales stay outside: a score is the sum over the blocks of d
 // times the block's product in fp32, and a block of values is added with the
 // weights p d.  So nothing of the cache is rounded on the way.  The weights p
-// d enter as hi + lo 16-bit parts (2^-22 of a weight, down to 2^-39 of the
-// largest weight times the largest scale): d is held relative to a power of
-// two, the largest d a warp has met, and the output is rescaled when that
-// rises, as it is when the maximum does.  bf16 queries are scaled by a power
+// and their products with d are hi + lo 16-bit parts (2^-22 of a weight, down
+// to 2^-34 of the largest weight times its block's largest scale): d is held
+// relative to a power of two, the largest d of its block that a warp has met,
+// and the block's output is rescaled when that rises, as it is when the
+// maximum does.  bf16 queries are scaled by a power
 // of two per row into fp16's range, where their 8 bits are exact (those below
 // 2^-31 of the row's largest round).
 //
@@ -37,6 +38,9 @@ constexpr int kWarps = 4;  // consumer warps
 constexpr int kStages = 3;
 constexpr int kMaxCtas = 448;
 constexpr int kThreads = (kWarps + 1) * 32;
+// The output is rescaled only when a row's maximum has risen by more than 2^kLazy since it was last set; the weights,
+// 2^kPShift exp(s - m), stay below 2^15 then.
+constexpr float kLazy = 5.0f, kPShift = 9.0f;
 
 template <int ROWS, int HD>
 struct LayoutQ8 {
@@ -68,6 +72,30 @@ __device__ __forceinline__ uint32_t codes_even(uint32_t w) {
   return *reinterpret_cast<const uint32_t*>(&y);
 }
 __device__ __forceinline__ uint32_t codes_odd(uint32_t w) { return codes_even(w >> 8); }
+
+// c += a b, and c = a b, as mma16816 but free to be moved among the conversions.
+__device__ __forceinline__ void product(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void first_product(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// The transpose of an 8 x 8 matrix of 16-bit values (lane: row lane / 4, columns 2 (lane % 4) and the next).
+__device__ __forceinline__ uint32_t transposed8(uint32_t w) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
+  return r;
+}
+
+__device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
+__device__ __forceinline__ uint32_t as_word(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 
 template <class T, class O, int HD, int ROWS>
 __global__ void __launch_bounds__(kThreads, LayoutQ8<ROWS, HD>::kCtasPerSm)
@@ -179,22 +207,27 @@ attention_paged_q8_kernel(const __grid_constant__ CUtensorMap kmap, const __grid
   }
 
   // ---------------- consumers ----------------
+  constexpr int N = ROWS / 8;  // groups of 8 query heads
   const uint32_t ring = smem_u32(smem);
   const float sl2 = a.scale * 1.4426950408889634f;
-  const int r = lane >> 2, t4 = lane & 3, c2 = t4 * 2;
+  const int r = lane >> 2, t4 = lane & 3, c2 = t4 * 2, r0 = warp * 16;
   float* jbuf = reinterpret_cast<float*>(smem + L::kJoinOff);
   float2* jml = reinterpret_cast<float2*>(smem + L::kMlOff);
+  // Fragments' places in a tile: chunk 2 b of keys is at key_at ^ 32 b (positions 0-7, chunk + 1, positions 8-15, chunk
+  // + 1), values at value_at ^ 32 b (positions 0-7, 8-15, the same of chunk + 1).
+  const uint32_t key_at = code_chunk<HD>(r0 + (lane >> 4) * 8 + (lane & 7), (lane >> 3) & 1);
+  const uint32_t value_at = code_chunk<HD>(r0 + ((lane >> 3) & 1) * 8 + (lane & 7), lane >> 4);
   bool ok = true;
-  int i = 0, split_unit = -1, split_parts = 0, split_slot = 0;
+  int st = 0, phase = 0, split_unit = -1, split_parts = 0, split_slot = 0;
   bool next = true;
   while (next) {
     // one segment: tiles w.t .. of unit (w.s, w.u)
     const int j = w.u / zs, h0 = (w.u % zs) * 16, nh = min(16, g - h0);
     const int t0 = w.t, t1 = (int)min((long long)w.nt, w.t + (w.end - w.at));
-    constexpr int R = ROWS / 8;
-    // The unit's query rows in fp16, read once by the CTA, then as fragments.  Thread: 8 values of a row.
-    uint32_t qf[2 * B][2 * R];  // step 2 b + s: values 32 b + 16 s ..; [2 e]: 4 t4 and 4 t4 + 2 of row r + 8 e, [2 e + 1]: the next ones
-    float rs[R];                // a score is this times its row's product
+    // The unit's query rows in fp16, read once by the CTA (thread: 8 values of a row), then as fragments: those of head
+    // 8 n + r, values 32 b + 16 s + 4 t4 and + 2 in [0] of step 2 b + s, + 1 and + 3 in [1].
+    uint32_t qf[N][2 * B][2];
+    float rs[N][2];  // a score of head 8 n + c2 + e is this times its product
     {
       const T* qb = static_cast<const T*>(a.q) + w.s * a.q_row_stride + (long long)(j * g + h0) * a.q_head_stride;
       unsigned char* sq = smem + L::kJoinOff;
@@ -227,36 +260,37 @@ attention_paged_q8_kernel(const __grid_constant__ CUtensorMap kmap, const __grid
       }
       consumer_bar_sync(kWarps * 32);
 #pragma unroll
-      for (int e = 0; e < R; ++e) {
-        rs[e] = std::is_same<T, __half>::value ? sl2 : s_row[r + 8 * e];
+      for (int n = 0; n < N; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) rs[n][e] = std::is_same<T, __half>::value ? sl2 : s_row[8 * n + c2 + e];
 #pragma unroll
         for (int k = 0; k < 2 * B; ++k) {
-          const uint2 x = *reinterpret_cast<const uint2*>(sq + (r + 8 * e) * L::kQRow + k * 32 + t4 * 8);
-          qf[k][2 * e] = __byte_perm(x.x, x.y, 0x5410);
-          qf[k][2 * e + 1] = __byte_perm(x.x, x.y, 0x7632);
+          const uint2 x = *reinterpret_cast<const uint2*>(sq + (8 * n + r) * L::kQRow + k * 32 + t4 * 8);
+          qf[n][k][0] = __byte_perm(x.x, x.y, 0x5410);
+          qf[n][k][1] = __byte_perm(x.x, x.y, 0x7632);
         }
       }
       consumer_bar_sync(kWarps * 32);  // the buffer is the join's again
     }
-    // with ROWS == 8, rows 8-15 repeat rows 0-7: their scores are the same numbers
-    constexpr int Q1 = ROWS == 16 ? 2 : 0, Q3 = ROWS == 16 ? 3 : 1;
-    // o[x]: values 16 x + 4 t4 .. + 3 of rows r and r + 8: [0] and [2] the even ones of row r, [1] the odd ones'
-    float o[HD / 16][2][4], m[R], l[R];
-    unsigned top = 0x0400u;  // exponent of the largest scale met, as an fp16 power of two
-    float inv = 16384.0f;    // 1 / it
+    // o[n][x]: values 16 x + 2 r ([0], [1]) and the next ([2], [3]) of heads 8 n + c2 and the next
+    float o[N][HD / 16][4], m[N][2], l[N][2];
+    // largest scales met, as fp16 powers of two, and one over them: two blocks a word
+    unsigned top[B / 2], inv[B / 2];
 #pragma unroll
-    for (int e = 0; e < R; ++e) {
-      m[e] = -INFINITY;
-      l[e] = 0.0f;
+    for (int b = 0; b < B / 2; ++b) {
+      top[b] = 0x04000400u;
+      inv[b] = 0x74007400u;
     }
 #pragma unroll
-    for (int e = 0; e < HD / 16; ++e)
+    for (int n = 0; n < N; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) o[e][k][0] = o[e][k][1] = o[e][k][2] = o[e][k][3] = 0.0f;
+      for (int e = 0; e < HD / 16; ++e) o[n][e][0] = o[n][e][1] = o[n][e][2] = o[n][e][3] = 0.0f;
+    }
 
-    for (int t = t0; t < t1; ++t, ++i) {
-      const int st = i % kStages;
-      if (ok) ok = mbar_wait_bounded(smem_u32(full + st), (i / kStages) & 1) && !*s_abort;
+    for (int t = t0; t < t1; ++t) {
+      if (ok) ok = mbar_wait_bounded(smem_u32(full + st), phase) && !*s_abort;
       ok = __all_sync(kFull, ok);
       if (!ok) {  // give up: keep in step with the other warps, but touch no more tiles
         if (lane == 0) {
@@ -265,185 +299,243 @@ attention_paged_q8_kernel(const __grid_constant__ CUtensorMap kmap, const __grid
         }
         continue;
       }
-      const uint32_t sk = ring + st * L::kStageBytes, sv = sk + L::kCodes;
+      const uint32_t sk = ring + st * L::kStageBytes;
       const unsigned char* sc = smem + st * L::kStageBytes + 2 * L::kCodes;
-      const int r0 = warp * 16, left = w.n - t * kTile - r0;  // positions of this warp's 16 that exist
+      const int left = w.n - t * kTile - r0;  // positions of this warp's 16 that exist
       if (left > 0) {
-        // scales of positions c2, c2 + 1, c2 + 8, c2 + 9: B halves each
-        uint32_t ks[4][B / 2], vs[4][B / 2];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int p = r0 + c2 + (k & 1) + 8 * (k >> 1);
-          if constexpr (B == 4) {
-            const uint2 x = *reinterpret_cast<const uint2*>(sc + p * 8);
-            const uint2 y = *reinterpret_cast<const uint2*>(sc + L::kScales + p * 8);
-            ks[k][0] = x.x; ks[k][1] = x.y;
-            vs[k][0] = y.x; vs[k][1] = y.y;
-          } else {
-            ks[k][0] = *reinterpret_cast<const uint32_t*>(sc + p * 4);
-            vs[k][0] = *reinterpret_cast<const uint32_t*>(sc + L::kScales + p * 4);
-          }
-          if (left < 16 && c2 + (k & 1) + 8 * (k >> 1) >= left) {  // whatever the page or the ring holds
-#pragma unroll
-            for (int b = 0; b < B / 2; ++b) vs[k][b] = 0u;
-          }
-        }
-        float s[R][4] = {};
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-          uint32_t f[4];  // chunk 2 b of positions 0-7, chunk 2 b + 1; the same of positions 8-15
-          ldsm4(f, sk + code_chunk<HD>(r0 + (lane >> 4) * 8 + (lane & 7), 2 * b + ((lane >> 3) & 1)));
-          float x[2][4] = {};
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint32_t(&q)[2 * R] = qf[2 * b + u];
-            mma16816<__half>(x[0], q[0], q[Q1], q[1], q[Q3], codes_even(f[u]), codes_odd(f[u]));
-            mma16816<__half>(x[1], q[0], q[Q1], q[1], q[Q3], codes_even(f[2 + u]), codes_odd(f[2 + u]));
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 d2 = unpack16<__half>(ks[k][b >> 1]);
-            const float d = b & 1 ? d2.y : d2.x;
-#pragma unroll
-            for (int e = 0; e < R; ++e) s[e][k] = fmaf(x[k >> 1][2 * e + (k & 1)], d, s[e][k]);
-          }
-        }
-        // the largest finite scale so far: o is held in units of a power of two no larger than it
-        auto largest = [&](bool finite) -> unsigned {
-          unsigned x = 0u;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int b = 0; b < B / 2; ++b) {
-              unsigned y = vs[k][b] & 0x7FFF7FFFu;
-              if (finite) y &= ~__vcmpgeu2(y, 0x7C007C00u);
-              x = __vmaxu2(x, y);
-            }
-          x = max(x & 0xFFFFu, x >> 16);
-          x = max(x, __shfl_xor_sync(kFull, x, 1));
-          return max(x, __shfl_xor_sync(kFull, x, 2));
-        };
-        unsigned big = largest(false);
-        if (big >= 0x7C00u) big = largest(true);
-        big &= 0x7C00u;
-        if (big > top) {  // the same in every lane
-          const float f = __uint_as_float((127u << 23) - ((big - top) << 13));
-          top = big;
-          inv *= f;
-#pragma unroll
-          for (int e = 0; e < HD / 16; ++e)
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-              for (int z = 0; z < 4; ++z) o[e][k][z] *= f;
-        }
-        float p[R][4];
-#pragma unroll
-        for (int e = 0; e < R; ++e) {
-          float x[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            x[k] = s[e][k] * rs[e];
-            if (left < 16 && (k >> 1) * 8 + c2 + (k & 1) >= left) x[k] = -INFINITY;
-          }
-          float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-          mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 2));
-          if (__any_sync(kFull, mx > m[e])) {
-            const float mn = fmaxf(m[e], mx), f = mn == -INFINITY ? 1.0f : ex2(m[e] - mn);
-            m[e] = mn;
-            l[e] *= f;
-#pragma unroll
-            for (int d = 0; d < HD / 16; ++d)
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                o[d][k][2 * e] *= f;
-                o[d][k][2 * e + 1] *= f;
-                if constexpr (ROWS == 8) {
-                  o[d][k][2] *= f;
-                  o[d][k][3] *= f;
-                }
-              }
-          }
-          const float base = (m[e] == -INFINITY ? 0.0f : m[e]) - kShift;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) p[e][k] = ex2(x[k] - base);
-          l[e] += (p[e][0] + p[e][1]) + (p[e][2] + p[e][3]);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) p[e][k] *= inv;
-        }
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-          uint32_t hi[2 * R], lo[2 * R];  // [2 k + e] of rows r + 8 e
+        // scores of positions r ([0], [1]) and r + 8, heads 8 n + c2 and the next
+        float s[N][4] = {};
+        {
+          uint32_t d[2][B / 2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const float2 d0 = unpack16<__half>(vs[2 * k][b >> 1]), d1 = unpack16<__half>(vs[2 * k + 1][b >> 1]);
-            const float y0 = b & 1 ? d0.y : d0.x, y1 = b & 1 ? d1.y : d1.x;
-#pragma unroll
-            for (int e = 0; e < R; ++e) {
-              const float w0 = p[e][2 * k] * y0, w1 = p[e][2 * k + 1] * y1;
-              hi[R * k + e] = pack16<__half>(w0, w1);
-              const float2 q = unpack16<__half>(hi[R * k + e]);
-              lo[R * k + e] = pack16<__half>(w0 - q.x, w1 - q.y);
+            const unsigned char* at = sc + (r0 + r + 8 * k) * (2 * B);
+            if constexpr (B == 4) {
+              const uint2 x = *reinterpret_cast<const uint2*>(at);
+              d[k][0] = x.x;
+              d[k][1] = x.y;
+            } else {
+              d[k][0] = *reinterpret_cast<const uint32_t*>(at);
             }
           }
-          uint32_t f[4];  // chunk 2 b of positions 0-7 and 8-15, the same of chunk 2 b + 1
-          ldsm4_t(f, sv + code_chunk<HD>(r0 + ((lane >> 3) & 1) * 8 + (lane & 7), 2 * b + (lane >> 4)));
+          const uint32_t at = sk + key_at;
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            float(&o0)[4] = o[2 * b + x][0], (&o1)[4] = o[2 * b + x][1];
-            const uint32_t e0 = codes_even(f[2 * x]), e1 = codes_even(f[2 * x + 1]);
-            const uint32_t u0 = codes_odd(f[2 * x]), u1 = codes_odd(f[2 * x + 1]);
-            if constexpr (ROWS == 8) {
-              mma16816<__half>(o0, hi[0], lo[0], hi[1], lo[1], e0, e1);
-              mma16816<__half>(o1, hi[0], lo[0], hi[1], lo[1], u0, u1);
-            } else {
-              mma16816<__half>(o0, hi[0], hi[1], hi[2], hi[3], e0, e1);
-              mma16816<__half>(o0, lo[0], lo[1], lo[2], lo[3], e0, e1);
-              mma16816<__half>(o1, hi[0], hi[1], hi[2], hi[3], u0, u1);
-              mma16816<__half>(o1, lo[0], lo[1], lo[2], lo[3], u0, u1);
+          for (int b = 0; b < B; ++b) {
+            uint32_t f[4], c[8];
+            ldsm4(f, at ^ (32u * b));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              c[2 * k] = codes_even(f[k]);
+              c[2 * k + 1] = codes_odd(f[k]);
+            }
+            const float2 d0 = unpack16<__half>(d[0][b >> 1]), d1 = unpack16<__half>(d[1][b >> 1]);
+            const float y0 = b & 1 ? d0.y : d0.x, y1 = b & 1 ? d1.y : d1.x;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+              float x[4];
+              first_product(x, c[0], c[4], c[1], c[5], qf[n][2 * b][0], qf[n][2 * b][1]);
+              product(x, c[2], c[6], c[3], c[7], qf[n][2 * b + 1][0], qf[n][2 * b + 1][1]);
+              s[n][0] = fmaf(x[0], y0, s[n][0]);
+              s[n][1] = fmaf(x[1], y0, s[n][1]);
+              s[n][2] = fmaf(x[2], y1, s[n][2]);
+              s[n][3] = fmaf(x[3], y1, s[n][3]);
+            }
+          }
+        }
+        bool rises = false;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            s[n][k] *= rs[n][k & 1];
+            if (left < 16 && r + 8 * (k >> 1) >= left) s[n][k] = -INFINITY;
+          }
+          rises |= fmaxf(s[n][0], s[n][2]) > m[n][0] + kLazy || fmaxf(s[n][1], s[n][3]) > m[n][1] + kLazy;
+        }
+        if (__any_sync(kFull, rises)) {
+#pragma unroll
+          for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float mx = fmaxf(s[n][e], s[n][2 + e]);
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, x));
+              const float mn = fmaxf(m[n][e], mx), f = mn == -INFINITY ? 1.0f : ex2(m[n][e] - mn);
+              m[n][e] = mn;
+              l[n][e] *= f;
+#pragma unroll
+              for (int x = 0; x < HD / 16; ++x) {
+                o[n][x][e] *= f;
+                o[n][x][2 + e] *= f;
+              }
+            }
+        }
+        // weights as two fp16 parts: [k] of positions c2 + 8 k and the next, head 8 n + r (transposed by exchange)
+        uint32_t ph[N][2], pl[N][2];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          float base[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) base[e] = (m[n][e] == -INFINITY ? 0.0f : m[n][e]) - kPShift;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float p0 = ex2(s[n][2 * k] - base[0]), p1 = ex2(s[n][2 * k + 1] - base[1]);
+            l[n][0] += p0;
+            l[n][1] += p1;
+            const uint32_t hi = pack16<__half>(p0, p1);
+            const float2 q = unpack16<__half>(hi);
+            ph[n][k] = transposed8(hi);
+            pl[n][k] = transposed8(pack16<__half>(p0 - q.x, p1 - q.y));
+          }
+        }
+        // scales of the values of positions c2, c2 + 1, c2 + 8, c2 + 9
+        uint32_t vs[4][B / 2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const unsigned char* at = sc + L::kScales + (r0 + c2 + 8 * k) * (2 * B);
+          if constexpr (B == 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(at);
+            vs[2 * k][0] = x.x;
+            vs[2 * k][1] = x.y;
+            vs[2 * k + 1][0] = x.z;
+            vs[2 * k + 1][1] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(at);
+            vs[2 * k][0] = x.x;
+            vs[2 * k + 1][0] = x.y;
+          }
+        }
+        if (left < 16) {  // whatever the page or the ring holds there
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (c2 + (k & 1) + 8 * (k >> 1) >= left) {
+#pragma unroll
+              for (int b = 0; b < B / 2; ++b) vs[k][b] = 0u;
+            }
+        }
+        bool risen = false;
+#pragma unroll
+        for (int b = 0; b < B / 2; ++b) {  // below twice its power of two (a sign, infinities and NaN are above)
+          const unsigned big = __vmaxu2(__vmaxu2(vs[0][b], vs[1][b]), __vmaxu2(vs[2][b], vs[3][b]));
+          risen |= __vmaxu2(big, top[b] | 0x03FF03FFu) != (top[b] | 0x03FF03FFu);
+        }
+        if (__any_sync(kFull, risen)) {
+#pragma unroll
+          for (int b = 0; b < B; ++b) {
+            const int sh = 16 * (b & 1);
+            unsigned big = 0u;  // the largest finite one
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const unsigned y = vs[k][b >> 1] >> sh & 0x7FFFu;
+              big = y < 0x7C00u ? max(big, y) : big;
+            }
+            big = max(big, __shfl_xor_sync(kFull, big, 1));
+            big = max(big, __shfl_xor_sync(kFull, big, 2)) & 0x7C00u;
+            const unsigned was = top[b >> 1] >> sh & 0x7C00u;
+            if (big <= was) continue;
+            const unsigned one_over = big == 0x7800u ? 0x0200u : 0x7800u - big;
+            top[b >> 1] = (top[b >> 1] & ~(0xFFFFu << sh)) | big << sh;
+            inv[b >> 1] = (inv[b >> 1] & ~(0xFFFFu << sh)) | one_over << sh;
+            const float f = __uint_as_float((127u << 23) - ((big - was) << 13));
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+              for (int x = 2 * b; x < 2 * b + 2; ++x)
+#pragma unroll
+                for (int z = 0; z < 4; ++z) o[n][x][z] *= f;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int b = 0; b < B / 2; ++b) vs[k][b] = as_word(__hmul2(as_half2(vs[k][b]), as_half2(inv[b])));
+        const uint32_t at = sk + L::kCodes + value_at;
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+          uint32_t f[4], c[8];
+          ldsm4_t(f, at ^ (32u * b));
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            c[2 * k] = codes_even(f[k]);
+            c[2 * k + 1] = codes_odd(f[k]);
+          }
+          const __half2 d0 = as_half2(__byte_perm(vs[0][b >> 1], vs[1][b >> 1], b & 1 ? 0x7632 : 0x5410));
+          const __half2 d1 = as_half2(__byte_perm(vs[2][b >> 1], vs[3][b >> 1], b & 1 ? 0x7632 : 0x5410));
+#pragma unroll
+          for (int n = 0; n < N; ++n) {  // p d = hi + lo: the product's rounding is in lo
+            const __half2 x0 = as_half2(ph[n][0]), x1 = as_half2(ph[n][1]);
+            const __half2 h0 = __hmul2(x0, d0), h1 = __hmul2(x1, d1);
+            const __half2 l0 = __hfma2(as_half2(pl[n][0]), d0, __hfma2(x0, d0, __hneg2(h0)));
+            const __half2 l1 = __hfma2(as_half2(pl[n][1]), d1, __hfma2(x1, d1, __hneg2(h1)));
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              // The tensor core truncates its sums: 256 tiles in a row come out 5e-6 too small, which an fp32 output shows.
+              // There each tile starts from zero and is added with rounding.
+              if constexpr (sizeof(O) == 4) {
+                float y[4];
+                first_product(y, c[4 * x], c[4 * x + 1], c[4 * x + 2], c[4 * x + 3], as_word(h0), as_word(h1));
+                product(y, c[4 * x], c[4 * x + 1], c[4 * x + 2], c[4 * x + 3], as_word(l0), as_word(l1));
+#pragma unroll
+                for (int z = 0; z < 4; ++z) o[n][2 * b + x][z] += y[z];
+              } else {
+                product(o[n][2 * b + x], c[4 * x], c[4 * x + 1], c[4 * x + 2], c[4 * x + 3], as_word(h0), as_word(h1));
+                product(o[n][2 * b + x], c[4 * x], c[4 * x + 1], c[4 * x + 2], c[4 * x + 3], as_word(l0), as_word(l1));
+              }
             }
           }
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(empty + st));
+      if (++st == kStages) {
+        st = 0;
+        phase ^= 1;
+      }
     }
 
-    // Join the four warps, 8 rows at a time: 2 -> 0 and 3 -> 1, then 1 -> 0.
+    // Join the four warps, 8 heads at a time: 2 -> 0 and 3 -> 1, then 1 -> 0.
     const bool whole = t0 == 0 && t1 == w.nt;
     const int slot = 2 * cta + (w.at == begin ? 0 : 1);
-    const float unit = 1.0f / inv;
 #pragma unroll
-    for (int e = 0; e < R; ++e) {
-      float v[HD / 16][4];
+    for (int n = 0; n < N; ++n) {
+      float (&v)[HD / 16][4] = o[n];
 #pragma unroll
-      for (int d = 0; d < HD / 16; ++d)
+      for (int d = 0; d < HD / 16; ++d) {
+        const float unit = __half2float(__ushort_as_half((unsigned short)(top[d >> 2] >> 16 * (d >> 1 & 1))));
 #pragma unroll
-        for (int k = 0; k < 4; ++k)  // value 4 t4 + k
-          v[d][k] = unit * (ROWS == 8 ? o[d][k & 1][k >> 1] + o[d][k & 1][2 + (k >> 1)] : o[d][k & 1][2 * e + (k >> 1)]);
-      float mm = m[e], ll = l[e];
-      ll += __shfl_xor_sync(kFull, ll, 1);
-      ll += __shfl_xor_sync(kFull, ll, 2);
+        for (int k = 0; k < 4; ++k) v[d][k] *= unit;
+      }
+      float mm[2], ll[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        mm[e] = m[n][e];
+        ll[e] = l[n][e];
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) ll[e] += __shfl_xor_sync(kFull, ll[e], x);
+      }
       auto give = [&](int at) {
-        float* b = jbuf + (at * 8 + r) * L::kJoinRow + 4 * t4;
 #pragma unroll
-        for (int d = 0; d < HD / 16; ++d) *reinterpret_cast<float4*>(b + d * 16) = make_float4(v[d][0], v[d][1], v[d][2], v[d][3]);
-        if (t4 == 0) jml[at * 8 + r] = make_float2(mm, ll);
+        for (int e = 0; e < 2; ++e) {
+          float* b = jbuf + (at * 8 + c2 + e) * L::kJoinRow + 2 * r;
+#pragma unroll
+          for (int d = 0; d < HD / 16; ++d) *reinterpret_cast<float2*>(b + d * 16) = make_float2(v[d][e], v[d][2 + e]);
+          if (r == 0) jml[at * 8 + c2 + e] = make_float2(mm[e], ll[e]);
+        }
       };
       auto take = [&](int at) {
-        const float* b = jbuf + (at * 8 + r) * L::kJoinRow + 4 * t4;
-        const float2 x = jml[at * 8 + r];
-        const float mn = fmaxf(mm, x.x), mz = mn == -INFINITY ? 0.0f : mn, f0 = ex2(mm - mz), f1 = ex2(x.x - mz);
-        mm = mn;
-        ll = ll * f0 + x.y * f1;
 #pragma unroll
-        for (int d = 0; d < HD / 16; ++d) {
-          const float4 y = *reinterpret_cast<const float4*>(b + d * 16);
-          v[d][0] = v[d][0] * f0 + y.x * f1;
-          v[d][1] = v[d][1] * f0 + y.y * f1;
-          v[d][2] = v[d][2] * f0 + y.z * f1;
-          v[d][3] = v[d][3] * f0 + y.w * f1;
+        for (int e = 0; e < 2; ++e) {
+          const float* b = jbuf + (at * 8 + c2 + e) * L::kJoinRow + 2 * r;
+          const float2 x = jml[at * 8 + c2 + e];
+          const float mn = fmaxf(mm[e], x.x), mz = mn == -INFINITY ? 0.0f : mn, f0 = ex2(mm[e] - mz), f1 = ex2(x.x - mz);
+          mm[e] = mn;
+          ll[e] = ll[e] * f0 + x.y * f1;
+#pragma unroll
+          for (int d = 0; d < HD / 16; ++d) {
+            const float2 y = *reinterpret_cast<const float2*>(b + d * 16);
+            v[d][e] = v[d][e] * f0 + y.x * f1;
+            v[d][2 + e] = v[d][2 + e] * f0 + y.y * f1;
+          }
         }
       };
       if (warp >= 2) give(warp - 2);
@@ -454,28 +546,30 @@ attention_paged_q8_kernel(const __grid_constant__ CUtensorMap kmap, const __grid
       consumer_bar_sync(kWarps * 32);
       if (warp == 0) {
         take(0);
-        const int row = 8 * e + r;
-        if (whole) {
-          const float d = ll == 0.0f ? 0.0f : 1.0f / ll;
-          if (row < nh) {
-            O* out = static_cast<O*>(a.out) + ((long long)w.s * a.n_heads + j * g + h0 + row) * HD + 4 * t4;
 #pragma unroll
-            for (int x = 0; x < HD / 16; ++x) {
-              if constexpr (sizeof(O) == 4)
-                *reinterpret_cast<float4*>(out + x * 16) = make_float4(v[x][0] * d, v[x][1] * d, v[x][2] * d, v[x][3] * d);
-              else
-                *reinterpret_cast<uint2*>(out + x * 16) = make_uint2(pack16<O>(v[x][0] * d, v[x][1] * d),
-                                                                    pack16<O>(v[x][2] * d, v[x][3] * d));
+        for (int e = 0; e < 2; ++e) {
+          const int row = 8 * n + c2 + e;
+          if (whole) {
+            const float d = ll[e] == 0.0f ? 0.0f : 1.0f / ll[e];
+            if (row < nh) {
+              O* out = static_cast<O*>(a.out) + ((long long)w.s * a.n_heads + j * g + h0 + row) * HD + 2 * r;
+#pragma unroll
+              for (int x = 0; x < HD / 16; ++x) {
+                if constexpr (sizeof(O) == 4)
+                  *reinterpret_cast<float2*>(out + x * 16) = make_float2(v[x][e] * d, v[x][2 + e] * d);
+                else
+                  *reinterpret_cast<uint32_t*>(out + x * 16) = pack16<O>(v[x][e] * d, v[x][2 + e] * d);
+              }
             }
-          }
-        } else {
-          float* b = slots + (size_t)slot * slot_floats(ROWS, HD);
+          } else {
+            float* b = slots + (size_t)slot * slot_floats(ROWS, HD);
 #pragma unroll
-          for (int x = 0; x < HD / 16; ++x)
-            __stcg(reinterpret_cast<float4*>(b + row * HD + x * 16 + 4 * t4), make_float4(v[x][0], v[x][1], v[x][2], v[x][3]));
-          if (t4 == 0) {
-            __stcg(b + ROWS * HD + row, mm);
-            __stcg(b + ROWS * HD + ROWS + row, ll);
+            for (int x = 0; x < HD / 16; ++x)
+              __stcg(reinterpret_cast<float2*>(b + row * HD + x * 16 + 2 * r), make_float2(v[x][e], v[x][2 + e]));
+            if (r == 0) {
+              __stcg(b + ROWS * HD + row, mm[e]);
+              __stcg(b + ROWS * HD + ROWS + row, ll[e]);
+            }
           }
         }
       }
@@ -503,7 +597,7 @@ bool encode_codes(CUtensorMap* map, const KvArgs& kv, const void* base, int box_
   const cuuint32_t box[4] = {(cuuint32_t)HD, (cuuint32_t)box_rows, 1u, 1u}, step[4] = {1u, 1u, 1u, 1u};
   return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dim, stride, box, step,
                 CU_TENSOR_MAP_INTERLEAVE_NONE, HD == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                HD == 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_64B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <class T, class O, int HD, int ROWS>

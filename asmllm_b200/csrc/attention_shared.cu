@@ -46,6 +46,9 @@ constexpr float kLazy = 6.0f;
 constexpr float kPShift = 8.0f;  // weights are 2^kPShift exp(s - m)
 constexpr int kThreads = 384;
 constexpr int kMaxCtas = 160;
+// The tensor core truncates its sums: 128 tiles in a row come out 1e-5 too small, which an fp32 output shows.  There a
+// stream's output is added to what it has so far, in memory and with rounding, after every kChain tiles.
+constexpr int kChain = 16;
 
 // Where the shared pass leaves its results, unnormalised: whole units by row, twice (the streams of a unit of up to
 // 128 rows have a result each), parts in slots of kUnit rows.
@@ -360,11 +363,14 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       };
       while (ok && w.at < w.end) {
         const Segment x = segment_of(w);
+        // a stream's k-th tile begins, and ends, a chain of sums
+        auto begins = [&](int k) { return TWO ? k % kChain == 0 : k == 0; };
+        auto ends = [&](int k, int tiles) { return k == tiles - 1 || (TWO && k % kChain == kChain - 1); };
         if (x.two) {  // both streams have all tiles
           for (int j = 0; j <= x.n && ok; ++j) {
 #pragma unroll 1
             for (int i = 0; i < 2 && ok; ++i) {
-              if (j > 0) values(i, c + 2 * j - 1, j == 1, j == x.n);
+              if (j > 0) values(i, c + 2 * j - 1, begins(j - 1), ends(j - 1, x.n));
               if (ok && j > 0 && i == 1) release(c + 2 * j - 1);
               if (ok && j < x.n) scores(i, c + 2 * j, j == 0);
               if (ok && j < x.n && i == 1) release(c + 2 * j);
@@ -373,7 +379,8 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         } else {  // every other one
           for (int j = 0; j < x.n + 2 && ok; ++j) {
             if (j >= 2) {
-              values(j & 1, c + 2 * (j - 2) + 1, j < 4, j >= x.n);
+              const int k = (j - 2) >> 1;
+              values(j & 1, c + 2 * (j - 2) + 1, begins(k), ends(k, (x.n + 1 - (j & 1)) >> 1));
               if (ok) release(c + 2 * (j - 2) + 1);
             }
             if (ok && j < x.n) {
@@ -422,7 +429,61 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
                                        unit_index(w.b * g, w.grp, x.blk)),
                make_int4(f.parts, f.cta, f.slot, 0));
       }
-      float m = -INFINITY, l = 0.0f;
+      float m = -INFINITY, l = 0.0f, behind = 1.0f;  // behind: what the sums in memory are to be multiplied by
+      // Results: o 2^ml.x is the sum of exp(s) v, l 2^ml.x of exp(s).  A thread holds a row; pieces of 16 bytes are
+      // exchanged within four lanes, so that a store writes 64 bytes of a row.
+      const long long at = ((long long)seq + (x.two ? 0 : (long long)i * kv.batch)) * a.n_heads + head;
+      float* slot_o = parts.slots + (size_t)slot * part_floats<HD>();
+      float* to4[4];
+      {
+        float* base = x.whole ? parts.o + at * HD : slot_o + (size_t)(i * kRows + lrow) * HD;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          to4[q] = reinterpret_cast<float*>(__shfl_sync(kFull, mine ? reinterpret_cast<unsigned long long>(base) : 0ull,
+                                                        (lane & ~3) + q));
+      }
+      auto put = [&](bool add) -> bool {  // the chain's output, in place of or on top of what is in memory
+        if (!wait(o_full + i, no & 1)) return false;
+        ++no;
+        tc_fence_after();
+        float f4[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) f4[q] = TWO && add ? __shfl_sync(kFull, behind, (lane & ~3) + q) : 0.0f;
+#pragma unroll 1
+        for (int b = 0; b < HD; b += 32) {
+          float4 was[2][4];
+          if (TWO && add) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                if (to4[q]) was[e][q] = __ldcg(reinterpret_cast<const float4*>(to4[q] + b + 16 * e) + (lane & 3));
+          }
+          uint32_t z[32];
+          tmem_ld<32>(to + b, z);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float4 p[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              p[q] = make_float4(__uint_as_float(z[16 * e + 4 * q]), __uint_as_float(z[16 * e + 4 * q + 1]),
+                                 __uint_as_float(z[16 * e + 4 * q + 2]), __uint_as_float(z[16 * e + 4 * q + 3]));
+            transpose4(p, lane);  // p[q]: piece lane % 4 of the four lanes' row q
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              if (!to4[q]) continue;
+              if (TWO && add)
+                p[q] = make_float4(fmaf(was[e][q].x, f4[q], p[q].x), fmaf(was[e][q].y, f4[q], p[q].y),
+                                   fmaf(was[e][q].z, f4[q], p[q].z), fmaf(was[e][q].w, f4[q], p[q].w));
+              __stcg(reinterpret_cast<float4*>(to4[q] + b + 16 * e) + (lane & 3), p[q]);
+            }
+          }
+        }
+        behind = 1.0f;
+        tc_fence_before();
+        return true;
+      };
       if (tiles > 0) {
         // Queries: this warp's 32 rows, a row's pieces in consecutive lanes.  What was read from the buffer before has
         // been: the last segment's last scores were waited for.
@@ -474,9 +535,10 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             const float mn = fmaxf(m, mt), f = m == -INFINITY ? 0.0f : ex2((m - mn) * sl2);
             m = mn;
             l *= f;
+            behind *= f;
             const unsigned long long f2 = pack2(f, f);
 #pragma unroll 1
-            for (int b = 0; b < HD; b += 32) {
+            for (int b = 0; b < HD && !(TWO && j % kChain == 0); b += 32) {
               uint32_t z[32];
               tmem_ld<32>(to + b, z);
               tmem_wait_ld();
@@ -519,48 +581,16 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
           float s0, s1;
           unpack2(add2(sum[0], sum[1]), s0, s1);
           l += s0 + s1;
+          if (TWO && j % kChain == kChain - 1 && j < tiles - 1 && !(ok = put(j >= kChain))) break;
         }
         if (!ok) break;
       }
-      // Results: o 2^ml.x is the sum of exp(s) v, l 2^ml.x of exp(s).  A thread holds a row; pieces of 16 bytes are
-      // exchanged within four lanes, so that a store writes 64 bytes of a row.
-      const long long at = ((long long)seq + (x.two ? 0 : (long long)i * kv.batch)) * a.n_heads + head;
-      float* slot_o = parts.slots + (size_t)slot * part_floats<HD>();
-      const float2 ml = make_float2(m == -INFINITY ? -INFINITY : m * sl2 - kPShift, l);
       if (mine) {
+        const float2 ml = make_float2(m == -INFINITY ? -INFINITY : m * sl2 - kPShift, l);
         if (x.whole) __stcg(parts.ml + at, ml);
         else __stcg(reinterpret_cast<float2*>(slot_o + (size_t)kUnit * HD) + i * kRows + lrow, ml);
       }
-      if (tiles > 0) {
-        if (!(ok = wait(o_full + i, no & 1))) break;
-        ++no;
-        tc_fence_after();
-        float* base = x.whole ? parts.o + at * HD : slot_o + (size_t)(i * kRows + lrow) * HD;
-        float* to4[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          to4[q] = reinterpret_cast<float*>(__shfl_sync(kFull, mine ? reinterpret_cast<unsigned long long>(base) : 0ull,
-                                                        (lane & ~3) + q));
-#pragma unroll 1
-        for (int b = 0; b < HD; b += 32) {
-          uint32_t z[32];
-          tmem_ld<32>(to + b, z);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; e += 16) {
-            float4 p[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              p[q] = make_float4(__uint_as_float(z[e + 4 * q]), __uint_as_float(z[e + 4 * q + 1]),
-                                 __uint_as_float(z[e + 4 * q + 2]), __uint_as_float(z[e + 4 * q + 3]));
-            transpose4(p, lane);  // p[q]: piece lane % 4 of the four lanes' row q
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (to4[q]) __stcg(reinterpret_cast<float4*>(to4[q] + b + e) + (lane & 3), p[q]);
-          }
-        }
-        tc_fence_before();
-      }
+      if (tiles > 0 && !(ok = put(tiles > kChain))) break;
       advance(x.n);
     }
   }

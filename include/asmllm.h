@@ -792,7 +792,7 @@ ASMLLM_API int asm_cache_read_q8_async(const asm_kv_q8_t* kv, const int32_t* cu,
 /* asm_attention_paged_async over a Q8_0 cache, q fp16 or bf16, out fp32 or of
  * q's type.  Codes enter the products as they are and scales multiply in
  * fp32; the weights times a block's scale are two 16-bit parts (2^-22 of a
- * weight, down to 2^-39 of the largest weight times the largest finite scale
+ * weight, down to 2^-34 of the largest weight times the largest finite scale
  * of the values).  A block of values whose scale is not finite gives NaN in its
  * 32 outputs, whatever the weight is above zero. */
 ASMLLM_API int64_t asm_attention_paged_q8_workspace(int32_t batch, int32_t n_heads, int32_t n_kv_heads,
