@@ -134,17 +134,24 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
   if constexpr (!OWN) pdl_wait();
 
   // positions of sequence s, without those that it shares
+  int4 group;  // OWN: that of the sequence len() was last called for
   auto len = [&](int s, bool report) -> int {
     bool clipped;
-    int n = kv_length(kv, s, &clipped), group;
+    int n = kv_length(kv, s, &clipped);
     if (clipped && report) atomicOr(err, kErrDecodeRange);
     if constexpr (OWN) n -= shared_base(own, kv, s, n, &group);
     return n;
   };
+  // OWN: where unit u's result is, and the group it is joined with
+  auto leave = [&](int s, int u, int parts, int slot) {
+    int4* at = reinterpret_cast<int4*>(own.own_found + (long long)s * units + u);
+    __stcg(at, make_int4(parts, cta, slot, 0));
+    __stcg(at + 1, group);
+  };
   // a sequence without positions: zeros, written by one CTA
   auto none = [&](int s) {
     if constexpr (OWN) {
-      for (int u = 0; u < units; ++u) own.own_found[(long long)s * units + u].parts = 0;
+      for (int u = 0; u < units; ++u) leave(s, u, 0, 0);
     } else {
       O* out = static_cast<O*>(a.out) + (long long)s * a.n_heads * HD;
       const float z[8] = {};
@@ -179,7 +186,6 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
       if constexpr (OWN) {
         if (x.s != base_s) {
           bool clipped;
-          int group;
           base_s = x.s;
           base = shared_base(own, kv, x.s, kv_length(kv, x.s, &clipped), &group);
         }
@@ -233,6 +239,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
   bool ok = true;
   int i = 0, split_unit = -1, split_parts = 0, split_slot = 0;
   bool next = true;
+  if constexpr (OWN) len(w.s, false);
   while (next) {
     // one segment: tiles w.t .. of unit (w.s, w.u)
     const int j = w.u / zs, h0 = (w.u % zs) * 16, nh = min(16, g - h0);
@@ -454,8 +461,12 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
           for (int d = 0; d < HD / 8; ++d)
             __stcg(reinterpret_cast<float2*>(b + row * HD + d * 8 + c2), make_float2(v[d][0], v[d][1]));
           if ((lane & 3) == 0) {
-            __stcg(b + ROWS * HD + row, mm);
-            __stcg(b + ROWS * HD + ROWS + row, ll);
+            if constexpr (OWN) {
+              __stcg(reinterpret_cast<float2*>(b + ROWS * HD) + row, make_float2(mm, ll));
+            } else {
+              __stcg(b + ROWS * HD + row, mm);
+              __stcg(b + ROWS * HD + ROWS + row, ll);
+            }
           }
         }
       }
@@ -466,9 +477,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
       split_slot = slot;
       split_parts = deal.cta_of(w.first + w.nt - 1) - cta + 1;
     }
-    if (OWN && t0 == 0 && tid == 0)
-      __stcg(reinterpret_cast<int4*>(own.own_found + (long long)w.s * units + w.u),
-             whole ? make_int4(1, 0, 0, 0) : make_int4(split_parts, cta, slot, 0));
+    if (OWN && t0 == 0 && tid == 0) leave(w.s, w.u, whole ? 1 : split_parts, slot);
     w.at += t1 - t0;
     next = w.at < w.end;
     if (next) next_unit(w, units, len);

@@ -11,21 +11,29 @@
 //      It does not wait for the first, and runs on the SMs that has left.
 //   3. Join: a row's parts, in order.
 //
-// Shared pass.  A unit is (group, KV head, 256 rows); its positions are tiles
-// of 128, and the tiles of all units in a row are cut into one equal range per
-// CTA, one CTA an SM.  Two streams of four warps take maximum, exponentials
-// and sum, one thread a row, while the tensor core works for the other: with
-// more than 128 rows the streams have 128 rows each and the same keys, with
-// fewer the same rows and every other key tile.  Scores, weights (over the
-// scores) and outputs are in tensor memory.  Weights are rounded once to 16
-// bits where the output is, and are two 16-bit parts (2^-22 of a weight in
-// fp16, 2^-16 in bf16) for an fp32 output, as in attention_prompt.cu; the
-// output is rescaled only when a row's maximum has risen by more than 2^kLazy.
+// Shared pass.  A unit is (group, KV head, 256 rows); its positions are tiles,
+// and the tiles of all units in a row are cut into one equal range per CTA,
+// one CTA an SM.  Two streams of four warps take maximum, exponentials and
+// sum, one thread a row: with more than 128 rows the streams have 128 rows
+// each and the same keys, with fewer the same rows and every other key tile.
+//   16-bit output: tiles of 128 positions.  Weights are rounded once to 16
+//     bits and written over the scores; the output adds up in tensor memory and
+//     is rescaled only when a row's maximum has risen by more than 2^kLazy.
+//   fp32 output: tiles of 64.  Weights are two 16-bit parts (2^-22 of a weight
+//     in fp16, 2^-16 in bf16), in columns of their own, so that the next tile's
+//     scores are computed as soon as this one's have been read; the output adds
+//     up in registers.  (In tensor memory, which truncates its sums, 16384
+//     positions came out 1e-5 too small; added up in memory after every 16
+//     tiles of 128, 5e-6 and a third slower.)
 //
 // CTA, 12 warps: 0-3 and 4-7 the streams (they also bring their queries into
-// shared memory), 8 tcgen05.mma issue by one elected thread, 9 tensor copies
-// of K and V tiles into a ring (a page behind the shared ones reads as zeros).
-// Every wait is bounded, as in attention_prompt.cu.
+// shared memory), 8 tcgen05.mma issue by one elected thread (for an fp32 output
+// 8 and 10, a stream each), 9 tensor copies of K and V tiles into a ring (a page
+// behind the shared ones reads as zeros).  One thread that issues for both
+// streams in turn keeps them half a tile apart: with a thread each they ran in
+// step, waiting for the exponentials and for the tensor core at the same time
+// (306 us, not 220, for 256 sequences of 64 query and 8 KV heads that share
+// 32768 positions).  Every wait is bounded, as in attention_prompt.cu.
 #include <type_traits>
 
 #include "matvec.cuh"
@@ -40,15 +48,12 @@ namespace asmllm {
 
 namespace {
 
-constexpr int kRows = 128;       // rows of a stream, positions of a key tile
-constexpr int kUnit = 2 * kRows; // rows of a unit
+constexpr int kRows = 128;        // rows of a stream
+constexpr int kUnit = 2 * kRows;  // rows of a unit
 constexpr float kLazy = 6.0f;
 constexpr float kPShift = 8.0f;  // weights are 2^kPShift exp(s - m)
 constexpr int kThreads = 384;
 constexpr int kMaxCtas = 160;
-// The tensor core truncates its sums: 128 tiles in a row come out 1e-5 too small, which an fp32 output shows.  There a
-// stream's output is added to what it has so far, in memory and with rounding, after every kChain tiles.
-constexpr int kChain = 16;
 
 // Where the shared pass leaves its results, unnormalised: whole units by row, twice (the streams of a unit of up to
 // 128 rows have a result each), parts in slots of kUnit rows.
@@ -64,23 +69,26 @@ __host__ __device__ constexpr size_t part_floats() { return (size_t)kUnit * HD +
 // Units of a KV head are numbered so that no two groups meet: rows before them / kUnit + groups before them.
 __device__ __forceinline__ int unit_index(int first_row, int group, int blk) { return first_row / kUnit + group + blk; }
 
-template <int HD>
+template <bool TWO, int HD>
 struct Cfg {
-  static constexpr int kTileBytes = kRows * HD * 2;
-  static constexpr int kStages = HD == 128 ? 5 : 8;
-  static constexpr int kRing = 2 * kTileBytes;
+  static constexpr int kKeys = TWO ? 64 : 128;  // positions of a key tile
+  static constexpr int kQBytes = kRows * HD * 2;
+  static constexpr int kTileBytes = kKeys * HD * 2;
+  static constexpr int kStages = (HD == 128 ? 160 : 128) * 1024 / kTileBytes;
+  static constexpr int kRing = 2 * kQBytes;
   static constexpr int kBars = kRing + kStages * kTileBytes;
-  static constexpr int kNBars = 2 * kStages + 2 + 2 + 4 + 2 + 1;
+  static constexpr int kNBars = 2 * kStages + 7 * 2;
   static constexpr int kSum = kBars + kNBars * 8 + 16;
   static constexpr int kSmem = kSum + 64 + 1024;
-  static constexpr uint32_t kO = 2 * kRows;  // tensor memory: S0, S1, then the two outputs
+  // tensor memory: the streams' scores, weights (over the scores where the output has 16 bits), outputs
+  static constexpr uint32_t kP = TWO ? 128 : 0, kO = 256;
+  // Operand descriptors, 128-byte swizzle (as in attention_prompt.cu): V's leading offset, a half tile.
+  static constexpr uint32_t kLeading = ((kKeys * 128) >> 4) << 16;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
-// Operand descriptors, 128-byte swizzle (as in attention_prompt.cu).
 constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
-constexpr uint32_t kLeading = ((kRows * 128) >> 4) << 16;
-__device__ __forceinline__ uint32_t desc_lo(uint32_t addr) { return ((addr >> 4) & 0x3FFFu) | kLeading; }
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t leading) { return ((addr >> 4) & 0x3FFFu) | leading; }
 __device__ __forceinline__ uint64_t desc64(uint32_t lo, uint32_t hi) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
@@ -134,10 +142,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                         const PagedArgs a, const KvArgs kv, const SharedView v, const SharedParts parts, int box_rows,
                         unsigned* __restrict__ err) {
-  using C = Cfg<HD>;
-  constexpr int kHalves = HD / 64, S = C::kStages;
+  using C = Cfg<TWO, HD>;
+  constexpr int kHalves = HD / 64, S = C::kStages, kKeys = C::kKeys;
   constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
-  constexpr uint32_t kIdescS = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((kRows >> 3) << 17) | ((kRows >> 4) << 24);
+  constexpr uint32_t kIdescS = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((kKeys >> 3) << 17) | ((kRows >> 4) << 24);
   constexpr uint32_t kIdescO =
       (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((kRows >> 4) << 24);
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -147,10 +155,11 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   uint64_t* kv_empty = kv_full + S;
   uint64_t* q_full = kv_empty + S;  // [2] a stream's queries are in shared memory
   uint64_t* s_full = q_full + 2;    // [2] scores of a tile are in tensor memory
-  uint64_t* p_full = s_full + 2;    // [2][2] the weights of its first and second 64 keys are
-  uint64_t* o_full = p_full + 4;    // [2] the segment's output is complete
-  uint64_t* drain = o_full + 2;
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* s_free = s_full + 2;    // [2] and have been read (TWO)
+  uint64_t* p_full = s_free + 2;    // [2][2] its weights are there, of the first and second half of the keys (TWO: all)
+  uint64_t* o_full = p_full + 4;    // [2] the tile's (TWO) or the segment's output is there
+  uint64_t* drain = o_full + 2;     // [2]
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drain + 2);
   volatile uint32_t* s_abort = s_tmem + 1;
   long long* s_sum = reinterpret_cast<long long*>(smem);  // per-thread sums, before the queries come
   long long* s_total = reinterpret_cast<long long*>(smem + C::kSum);
@@ -168,16 +177,17 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     prefetch_map(&vmap);
     for (int i = 0; i < S; ++i) {
       mbar_init(smem_u32(kv_full + i), 1);
-      mbar_init(smem_u32(kv_empty + i), 1);
+      mbar_init(smem_u32(kv_empty + i), TWO ? 2 : 1);  // who issues the products that read it
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(q_full + i), 4);
       mbar_init(smem_u32(s_full + i), 1);
+      mbar_init(smem_u32(s_free + i), 4);
       mbar_init(smem_u32(p_full + 2 * i), 4);
       mbar_init(smem_u32(p_full + 2 * i + 1), 4);
       mbar_init(smem_u32(o_full + i), 1);
+      mbar_init(smem_u32(drain + i), 1);
     }
-    mbar_init(smem_u32(drain), 1);
     *s_abort = 0u;
     fence_mbar_init();
   }
@@ -194,7 +204,7 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     x->b = b;
     x->rows = (e - b) * g;
     x->nb = (x->rows + kUnit - 1) / kUnit;
-    x->nt = (x->shared + kRows - 1) / kRows;
+    x->nt = (x->shared + kKeys - 1) / kKeys;
     return (long long)x->nb * x->nt * kv.n_kv;
   };
   Tour w;
@@ -275,10 +285,11 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   };
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if constexpr (TWO) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");  // 8 x 216 + 4 x 72 = 12 x 168
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");                // 8 x 224 + 4 x 56
     if (warp == 9) {
       // ---------------- loader ----------------
-      const int pages = kRows / box_rows, my_page = lane / kHalves, half = lane % kHalves;
+      const int pages = kKeys / box_rows, my_page = lane / kHalves, half = lane % kHalves;
       const uint32_t box_bytes = (uint32_t)box_rows * 128u;
       int c = 0;
       bool ok = true;
@@ -286,7 +297,7 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         const Segment x = segment_of(w);
         // page of this lane's box in tile j of the segment; n_pages reads as zeros
         auto lookup = [&](int j) -> int {
-          const int p = (x.t0 + j) * kRows + my_page * box_rows;
+          const int p = (x.t0 + j) * kKeys + my_page * box_rows;
           if (my_page >= pages || j >= x.n) return -1;
           if (p >= w.shared) return kv.n_pages;
           const int page = __ldcg(kv.table + (long long)w.b * kv.table_stride + (p >> kv.page_shift));
@@ -298,7 +309,7 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         for (int j = 0; j < x.n && ok; ++j) {
           const int cur = page;
           page = lookup(j + 1);
-          const int row = ((x.t0 + j) * kRows + my_page * box_rows) & (kv.page_size - 1);
+          const int row = ((x.t0 + j) * kKeys + my_page * box_rows) & (kv.page_size - 1);
           for (int y = 0; y < 2; ++y, ++c) {
             const int st = c % S;
             if (c >= S && !(ok = wait(kv_empty + st, ((c / S) - 1) & 1))) break;
@@ -306,7 +317,7 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
             if (lane == 0) mbar_arrive_expect_tx(bar, C::kTileBytes);
             __syncwarp();
             if (cur >= 0)
-              tma_load_4d(smem_u32(smem) + C::kRing + st * C::kTileBytes + half * (kRows * 128) + my_page * box_bytes,
+              tma_load_4d(smem_u32(smem) + C::kRing + st * C::kTileBytes + half * (kKeys * 128) + my_page * box_bytes,
                           y ? &vmap : &kmap, half * 64, row, x.head, cur, bar);
           }
         }
@@ -314,29 +325,37 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       }
       // what was issued lands before the CTA may end (bounded)
       for (int j = c - S < 0 ? 0 : c - S; j < c; ++j) mbar_wait_bounded(smem_u32(kv_full + j % S), (j / S) & 1);
-    } else if (warp == 8 && elect_one()) {
-      // ---------------- matrix products (one thread) ----------------
-      const uint32_t q_lo = desc_lo(smem_u32(smem)), ring_lo = desc_lo(smem_u32(smem) + C::kRing);
-      constexpr uint32_t kTileLo = C::kTileBytes >> 4;
-      uint32_t nq = 0, np = 0;  // parities, one bit a stream
-      int c = 0;                // ring entries before this segment
+    } else if ((warp == 8 || (TWO && warp == 10)) && elect_one()) {
+      // ---------------- matrix products (one thread; TWO: one for each stream) ----------------
+      const uint32_t q_lo = desc_lo(smem_u32(smem), C::kLeading);
+      const uint32_t ring_lo = desc_lo(smem_u32(smem) + C::kRing, C::kLeading);
+      constexpr uint32_t kTileLo = C::kTileBytes >> 4, kQLo = C::kQBytes >> 4;
+      const int mine = warp == 8 ? 0 : 1;
+      uint32_t nq = 0, np = 0, nf = 0;  // parities, one bit a stream
+      int c = 0;                        // ring entries before this segment
       bool ok = true, issued = false;
       auto get = [&](uint64_t* bar, uint32_t parity) { return ok = ok && mbar_wait_bounded(smem_u32(bar), parity); };
       auto get_tile = [&](int e) { return get(kv_full + e % S, (e / S) & 1); };
-      auto release = [&](int e) { umma_commit(smem_u32(kv_empty + e % S)); };
+      auto release = [&](int e) {
+        if (ok) umma_commit(smem_u32(kv_empty + e % S));
+      };
       // scores of stream i against the keys in ring entry e
       auto scores = [&](int i, int e, bool first) {
         if (first) {
           if (!get(q_full + i, nq >> i & 1)) return;
           nq ^= 1u << i;
+        } else if (TWO) {  // the last ones have been read
+          if (!get(s_free + i, nf)) return;
+          nf ^= 1u;
         }
         if (!get_tile(e)) return;
         tc_fence_after();
-        const uint32_t ql = q_lo + i * kTileLo, kl = ring_lo + (e % S) * kTileLo;
+        const uint32_t ql = q_lo + i * kQLo, kl = ring_lo + (e % S) * kTileLo;
 #pragma unroll
         for (int ks = 0; ks < HD / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * ((kRows * 128) >> 4) + (ks & 3) * 2;
-          umma_ss(tmem + i * kRows, desc64(ql + off, kDescHi), desc64(kl + off, kDescHi), kIdescS, ks > 0);
+          const uint32_t in = (ks & 3) * 2;
+          umma_ss(tmem + i * kKeys, desc64(ql + (ks >> 2) * ((kRows * 128) >> 4) + in, kDescHi),
+                  desc64(kl + (ks >> 2) * ((kKeys * 128) >> 4) + in, kDescHi), kIdescS, ks > 0);
         }
         umma_commit(smem_u32(s_full + i));
         issued = true;
@@ -344,48 +363,65 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       // stream i's weights times the values in ring entry e
       auto values = [&](int i, int e, bool first, bool last) {
         if (!get_tile(e)) return;
-        const uint32_t vl = ring_lo + (e % S) * kTileLo;
+        const uint32_t vl = ring_lo + (e % S) * kTileLo, tp = tmem + C::kP + i * kKeys, to = tmem + C::kO + i * HD;
+        constexpr int kParts = TWO ? 1 : 2, kSteps = kKeys / 16 / kParts;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {  // the first 64 keys while the weights of the others are computed
+        for (int h = 0; h < kParts; ++h) {  // the first keys while the weights of the others are computed
           if (!get(p_full + 2 * i + h, np >> i & 1)) return;
           tc_fence_after();
 #pragma unroll
-          for (int ks = 4 * h; ks < 4 * h + 4; ++ks) {
-            umma_ts(tmem + C::kO + i * HD, tmem + i * kRows + ks * 8, desc64(vl + ks * (2048 >> 4), kDescHi), kIdescO,
-                    ks > 0 || !first);
-            if constexpr (TWO)
-              umma_ts(tmem + C::kO + i * HD, tmem + i * kRows + kRows / 2 + ks * 8,
-                      desc64(vl + ks * (2048 >> 4), kDescHi), kIdescO, true);
+          for (int ks = h * kSteps; ks < (h + 1) * kSteps; ++ks) {
+            umma_ts(to, tp + ks * 8, desc64(vl + ks * (2048 >> 4), kDescHi), kIdescO, ks > 0 || !(TWO || first));
+            if constexpr (TWO) umma_ts(to, tp + kKeys / 2 + ks * 8, desc64(vl + ks * (2048 >> 4), kDescHi), kIdescO, true);
           }
         }
         np ^= 1u << i;
-        if (last) umma_commit(smem_u32(o_full + i));
+        if (TWO || last) umma_commit(smem_u32(o_full + i));
       };
       while (ok && w.at < w.end) {
         const Segment x = segment_of(w);
-        // a stream's k-th tile begins, and ends, a chain of sums
-        auto begins = [&](int k) { return TWO ? k % kChain == 0 : k == 0; };
-        auto ends = [&](int k, int tiles) { return k == tiles - 1 || (TWO && k % kChain == kChain - 1); };
-        if (x.two) {  // both streams have all tiles
+        if constexpr (TWO) {
+          int passed = 0;  // tiles before this one are done with, as far as this stream goes
+          auto pass = [&](int tile) {  // those of the other stream: once they are there, this one does not need them
+            for (; ok && passed < tile; ++passed)
+              for (int y = 0; y < 2; ++y)
+                if (get_tile(c + 2 * passed + y)) mbar_arrive(smem_u32(kv_empty + (c + 2 * passed + y) % S));
+            ++passed;
+          };
+          const int step = x.two ? 1 : 2, begin = x.two ? 0 : mine;
+          for (int j = begin - step; ok && j < x.n; j += step) {
+            const int next = j + step;
+            if (next < x.n) {
+              pass(next);
+              if (ok) scores(mine, c + 2 * next, next == begin);
+              release(c + 2 * next);
+            }
+            if (ok && j >= begin) {
+              values(mine, c + 2 * j + 1, false, false);
+              release(c + 2 * j + 1);
+            }
+          }
+          if (ok && begin < x.n && get(s_free + mine, nf)) nf ^= 1u;
+          pass(x.n);
+        } else if (x.two) {  // both streams have all tiles
           for (int j = 0; j <= x.n && ok; ++j) {
 #pragma unroll 1
             for (int i = 0; i < 2 && ok; ++i) {
-              if (j > 0) values(i, c + 2 * j - 1, begins(j - 1), ends(j - 1, x.n));
-              if (ok && j > 0 && i == 1) release(c + 2 * j - 1);
+              if (j > 0) values(i, c + 2 * j - 1, j == 1, j == x.n);
+              if (j > 0 && i == 1) release(c + 2 * j - 1);
               if (ok && j < x.n) scores(i, c + 2 * j, j == 0);
-              if (ok && j < x.n && i == 1) release(c + 2 * j);
+              if (j < x.n && i == 1) release(c + 2 * j);
             }
           }
         } else {  // every other one
           for (int j = 0; j < x.n + 2 && ok; ++j) {
             if (j >= 2) {
-              const int k = (j - 2) >> 1;
-              values(j & 1, c + 2 * (j - 2) + 1, begins(k), ends(k, (x.n + 1 - (j & 1)) >> 1));
-              if (ok) release(c + 2 * (j - 2) + 1);
+              values(j & 1, c + 2 * j - 3, j < 4, j >= x.n);
+              release(c + 2 * j - 3);
             }
             if (ok && j < x.n) {
               scores(j & 1, c + 2 * j, j < 2);
-              if (ok) release(c + 2 * j);
+              release(c + 2 * j);
             }
           }
         }
@@ -394,151 +430,186 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       }
       if (!ok) fail();
       if (issued) {  // the tensor core is done before tensor memory is released
-        umma_commit(smem_u32(drain));
-        if (!mbar_wait_bounded(smem_u32(drain), 0)) fail();
+        umma_commit(smem_u32(drain + mine));
+        if (!mbar_wait_bounded(smem_u32(drain + mine), 0)) fail();
       }
     }
   } else {
     // ---------------- softmax ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    if constexpr (TWO) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int i = warp >> 2, lrow = 32 * (warp & 3) + lane;
-    const uint32_t ts = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + i * kRows;
-    const uint32_t to = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + C::kO + i * HD;
+    const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+    const uint32_t ts = lanes + i * kKeys, tp = lanes + C::kP + i * kKeys, to = lanes + C::kO + i * HD;
     const float sl2 = a.scale * 1.4426950408889634f;
     const long long begin = w.at;
-    int ns = 0, no = 0;
+    uint32_t ns = 0, no = 0;  // parities
     bool ok = true;
     while (ok && w.at < w.end) {
       const Segment x = segment_of(w);
       const int row = lrow + (x.two ? i * kRows : 0), tiles = x.two ? x.n : (x.n + 1 - i) >> 1;
-      const bool mine = row < x.rows;
+      const bool mine = row < x.rows, idle = row - lane >= x.rows;  // idle: the warp has no row
       const int rr = x.blk * kUnit + row, seq = w.b + rr / g, head = x.head * g + rr % g;
       const int slot = 2 * blockIdx.x + (w.at == begin ? 0 : 1);
       if (x.t0 == 0 && tid == 0) {  // where the unit's results are
-        const int last = (int)blockIdx.x;
-        Found f;
-        f.parts = 1;
-        f.cta = last;
-        f.slot = slot;
-        f.pad = 0;
+        int n = 1;
         if (!x.whole) {
           const int ctas = (int)min((long long)gridDim.x, *s_total);
-          f.parts = Deal(*s_total, ctas).cta_of(w.first + w.nt - 1) - last + 1;
+          n = Deal(*s_total, ctas).cta_of(w.first + w.nt - 1) - (int)blockIdx.x + 1;
         }
         __stcg(reinterpret_cast<int4*>(parts.found + (long long)x.head * parts.found_stride +
                                        unit_index(w.b * g, w.grp, x.blk)),
-               make_int4(f.parts, f.cta, f.slot, 0));
+               make_int4(n, (int)blockIdx.x, slot, 0));
       }
-      float m = -INFINITY, l = 0.0f, behind = 1.0f;  // behind: what the sums in memory are to be multiplied by
-      // Results: o 2^ml.x is the sum of exp(s) v, l 2^ml.x of exp(s).  A thread holds a row; pieces of 16 bytes are
-      // exchanged within four lanes, so that a store writes 64 bytes of a row.
-      const long long at = ((long long)seq + (x.two ? 0 : (long long)i * kv.batch)) * a.n_heads + head;
-      float* slot_o = parts.slots + (size_t)slot * part_floats<HD>();
-      float* to4[4];
-      {
-        float* base = x.whole ? parts.o + at * HD : slot_o + (size_t)(i * kRows + lrow) * HD;
+      if (tiles > 0) {
+        // Queries: this warp's 32 rows, a row's pieces in consecutive lanes.  What was read from the buffer before has
+        // been: the last segment's last scores were waited for.
+        constexpr int P = HD / 8, N = 32 / P;  // pieces of a row, rows at a time
+        const long long mine_at = mine ? (long long)seq * a.q_row_stride + (long long)head * a.q_head_stride : -1;
+        unsigned char* sq = smem + i * C::kQBytes;
+        uint4 y[32 / N];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          to4[q] = reinterpret_cast<float*>(__shfl_sync(kFull, mine ? reinterpret_cast<unsigned long long>(base) : 0ull,
-                                                        (lane & ~3) + q));
+        for (int k = 0; k < 32 / N; ++k) {
+          const int rw = k * N + lane / P;
+          const long long at = __shfl_sync(kFull, mine_at, rw);
+          y[k] = make_uint4(0u, 0u, 0u, 0u);
+          if (at >= 0) y[k] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at) + lane % P);
+        }
+#pragma unroll
+        for (int k = 0; k < 32 / N; ++k) {
+          const int rw = 32 * (warp & 3) + k * N + lane / P, ch = lane % P;
+          *reinterpret_cast<uint4*>(sq + (ch >> 3) * (kRows * 128) + rw * 128 + (((ch & 7) ^ (rw & 7)) << 4)) = y[k];
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(q_full + i));
       }
-      auto put = [&](bool add) -> bool {  // the chain's output, in place of or on top of what is in memory
-        if (!wait(o_full + i, no & 1)) return false;
-        ++no;
-        tc_fence_after();
-        float f4[4];
+      float m = -INFINITY, l = 0.0f;
+      float o[TWO ? HD : 1];  // fp32 outputs: the sums over the tiles
 #pragma unroll
-        for (int q = 0; q < 4; ++q) f4[q] = TWO && add ? __shfl_sync(kFull, behind, (lane & ~3) + q) : 0.0f;
-#pragma unroll 1
+      for (int e = 0; e < (TWO ? HD : 1); ++e) o[e] = 0.0f;
+      // the last tile's output on top of the sums, then times f if the row's maximum has risen
+      auto add_output = [&](bool rises, float f) {
+#pragma unroll
         for (int b = 0; b < HD; b += 32) {
-          float4 was[2][4];
-          if (TWO && add) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                if (to4[q]) was[e][q] = __ldcg(reinterpret_cast<const float4*>(to4[q] + b + 16 * e) + (lane & 3));
-          }
           uint32_t z[32];
           tmem_ld<32>(to + b, z);
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float4 p[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              p[q] = make_float4(__uint_as_float(z[16 * e + 4 * q]), __uint_as_float(z[16 * e + 4 * q + 1]),
-                                 __uint_as_float(z[16 * e + 4 * q + 2]), __uint_as_float(z[16 * e + 4 * q + 3]));
-            transpose4(p, lane);  // p[q]: piece lane % 4 of the four lanes' row q
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              if (!to4[q]) continue;
-              if (TWO && add)
-                p[q] = make_float4(fmaf(was[e][q].x, f4[q], p[q].x), fmaf(was[e][q].y, f4[q], p[q].y),
-                                   fmaf(was[e][q].z, f4[q], p[q].z), fmaf(was[e][q].w, f4[q], p[q].w));
-              __stcg(reinterpret_cast<float4*>(to4[q] + b + 16 * e) + (lane & 3), p[q]);
-            }
-          }
+          for (int e = 0; e < 32; ++e)
+            if constexpr (TWO) o[b + e] += __uint_as_float(z[e]);
         }
-        behind = 1.0f;
-        tc_fence_before();
+        if (rises) {
+#pragma unroll
+          for (int e = 0; e < (TWO ? HD : 1); ++e) o[e] *= f;
+        }
+      };
+      // What a warp does between having scores y of the stream's tile j and having to give their weights: the maximum, and
+      // whether the output so far is to be multiplied by *f.
+      auto mask = [&](uint32_t(&y)[kKeys], int j) {
+        const int limit = w.shared - (x.t0 + (x.two ? j : 2 * j + i)) * kKeys;  // columns below it exist
+        if (limit < kKeys) {
+#pragma unroll
+          for (int e = 0; e < kKeys; ++e)
+            if (e >= limit) y[e] = 0xFF800000u;
+        }
+      };
+      auto raise = [&](const uint32_t(&y)[kKeys], int j, float* f) -> bool {
+        float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < kKeys; e += 8)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            t[q] = max3(t[q], __uint_as_float(y[e + 2 * q]), __uint_as_float(y[e + 2 * q + 1]));
+        const float mt = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        if (j == 0) {
+          m = mt;
+          return false;
+        }
+        if (!__any_sync(kFull, mine && (mt - m) * sl2 > kLazy)) return false;
+        const float mn = fmaxf(m, mt);
+        *f = m == -INFINITY ? 0.0f : ex2((m - mn) * sl2);
+        m = mn;
+        l *= *f;
         return true;
       };
-      if (tiles > 0) {
-        // Queries: this warp's 32 rows, a row's pieces in consecutive lanes.  What was read from the buffer before has
-        // been: the last segment's last scores were waited for.
-        {
-          constexpr int P = HD / 8, N = 32 / P;  // pieces of a row, rows at a time
-          const long long mine_at = mine ? (long long)seq * a.q_row_stride + (long long)head * a.q_head_stride : -1;
-          unsigned char* sq = smem + i * C::kTileBytes;
-          uint4 y[32 / N];
+      // Weights of keys from .. from + 63 in place of their scores, and their sum.  First the exponentials, then what needs
+      // them: with the sum beside each, the in-order pipeline waited for it, and a warp alone took 1050 cycles for 64 of
+      // them where 550 are possible.
+      auto exponentials = [&](uint32_t(&y)[kKeys], int from) {
+        const float off = kPShift - (m == -INFINITY ? 0.0f : m * sl2);
+        const unsigned long long sl22 = pack2(sl2, sl2), off2 = pack2(off, off);
 #pragma unroll
-          for (int k = 0; k < 32 / N; ++k) {
-            const int rw = k * N + lane / P;
-            const long long at = __shfl_sync(kFull, mine_at, rw);
-            y[k] = make_uint4(0u, 0u, 0u, 0u);
-            if (at >= 0) y[k] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at) + lane % P);
-          }
-#pragma unroll
-          for (int k = 0; k < 32 / N; ++k) {
-            const int rw = 32 * (warp & 3) + k * N + lane / P, ch = lane % P;
-            *reinterpret_cast<uint4*>(sq + (ch >> 3) * (kRows * 128) + rw * 128 + (((ch & 7) ^ (rw & 7)) << 4)) = y[k];
-          }
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(q_full + i));
+        for (int e = from; e < from + 64; e += 2) {
+          float x0, x1;
+          unpack2(fma2(pack2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), sl22, off2), x0, x1);
+          y[e] = __float_as_uint(ex2(x0));
+          y[e + 1] = __float_as_uint(ex2(x1));
         }
-        for (int j = 0; j < tiles; ++j) {
-          if (!(ok = wait(s_full + i, ns & 1))) break;
-          ++ns;
-          tc_fence_after();
-          uint32_t y[kRows];
+        unsigned long long sum[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-          for (int b = 0; b < kRows; b += 32) tmem_ld<32>(ts + b, *reinterpret_cast<uint32_t(*)[32]>(y + b));
-          tmem_wait_ld();
-          const int limit = w.shared - (x.t0 + (x.two ? j : 2 * j + i)) * kRows;  // columns below it exist
-          if (limit < kRows) {
-#pragma unroll
-            for (int e = 0; e < kRows; ++e)
-              if (e >= limit) y[e] = 0xFF800000u;
+        for (int e = from; e < from + 64; e += 2)
+          sum[(e >> 1) & 3] = add2(sum[(e >> 1) & 3], pack2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])));
+        float s0, s1;
+        unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), s0, s1);
+        l += s0 + s1;
+      };
+      for (int j = 0; j < tiles; ++j) {
+        if (!(ok = wait(s_full + i, ns))) break;
+        ns ^= 1u;
+        if (idle) {
+          if (TWO) {
+            if (lane == 0) mbar_arrive(smem_u32(s_free + i));
+            if (j > 0) {
+              if (!(ok = wait(o_full + i, no))) break;
+              no ^= 1u;
+            }
           }
-          float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (lane == 0) {
+            mbar_arrive(smem_u32(p_full + 2 * i));
+            if (!TWO) mbar_arrive(smem_u32(p_full + 2 * i + 1));
+          }
+          continue;
+        }
+        tc_fence_after();
+        uint32_t y[kKeys];
 #pragma unroll
-          for (int e = 0; e < kRows; e += 8)
+        for (int b = 0; b < kKeys; b += 32) tmem_ld<32>(ts + b, *reinterpret_cast<uint32_t(*)[32]>(y + b));
+        tmem_wait_ld();
+        float f = 1.0f;
+        if constexpr (TWO) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(s_free + i));
+          mask(y, j);
+          const bool rises = raise(y, j, &f);
+          exponentials(y, 0);
+          uint32_t p[32], p2[32];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              t[q] = max3(t[q], __uint_as_float(y[e + 2 * q]), __uint_as_float(y[e + 2 * q + 1]));
-          const float mt = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-          if (j == 0) {
-            m = mt;
-          } else if (__any_sync(kFull, mine && (mt - m) * sl2 > kLazy)) {
-            const float mn = fmaxf(m, mt), f = m == -INFINITY ? 0.0f : ex2((m - mn) * sl2);
-            m = mn;
-            l *= f;
-            behind *= f;
+          for (int e = 0; e < 64; e += 2) {
+            const float x0 = __uint_as_float(y[e]), x1 = __uint_as_float(y[e + 1]);
+            p[e >> 1] = pack16<T>(x0, x1);
+            const float2 q = unpack16<T>(p[e >> 1]);
+            p2[e >> 1] = pack16<T>(x0 - q.x, x1 - q.y);
+          }
+          if (j > 0) {  // the last tile's weights have been read and its values added
+            if (!(ok = wait(o_full + i, no))) break;
+            no ^= 1u;
+            tc_fence_after();
+          }
+          tmem_st32(tp, p);
+          tmem_st32(tp + kKeys / 2, p2);
+          if (j > 0) add_output(rises, f);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(p_full + 2 * i));
+        } else {
+          mask(y, j);
+          if (raise(y, j, &f)) {  // the last tile's values have been added: its products came before these scores
             const unsigned long long f2 = pack2(f, f);
 #pragma unroll 1
-            for (int b = 0; b < HD && !(TWO && j % kChain == 0); b += 32) {
+            for (int b = 0; b < HD; b += 32) {
               uint32_t z[32];
               tmem_ld<32>(to + b, z);
               tmem_wait_ld();
@@ -552,45 +623,66 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
               tmem_st32(to + b, z);
             }
           }
-          const float off = kPShift - (m == -INFINITY ? 0.0f : m * sl2);
-          const unsigned long long sl22 = pack2(sl2, sl2), off2 = pack2(off, off);
-          unsigned long long sum[2] = {0ull, 0ull};
 #pragma unroll
-          for (int b = 0; b < kRows; b += 64) {
-            uint32_t p[32], p2[32];
+          for (int b = 0; b < kKeys; b += 64) {
+            exponentials(y, b);
+            uint32_t p[32];
 #pragma unroll
-            for (int e = 0; e < 64; e += 2) {
-              float x0, x1;
-              unpack2(fma2(pack2(__uint_as_float(y[b + e]), __uint_as_float(y[b + e + 1])), sl22, off2), x0, x1);
-              x0 = ex2(x0);
-              x1 = ex2(x1);
-              sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(x0, x1));
-              p[e >> 1] = pack16<T>(x0, x1);
-              if constexpr (TWO) {
-                const float2 q = unpack16<T>(p[e >> 1]);
-                p2[e >> 1] = pack16<T>(x0 - q.x, x1 - q.y);
-              }
-            }
-            tmem_st32(ts + (b >> 1), p);
-            if constexpr (TWO) tmem_st32(ts + kRows / 2 + (b >> 1), p2);
+            for (int e = 0; e < 64; e += 2) p[e >> 1] = pack16<T>(__uint_as_float(y[b + e]), __uint_as_float(y[b + e + 1]));
+            tmem_st32(tp + (b >> 1), p);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(p_full + 2 * i + (b >> 6)));
           }
-          float s0, s1;
-          unpack2(add2(sum[0], sum[1]), s0, s1);
-          l += s0 + s1;
-          if (TWO && j % kChain == kChain - 1 && j < tiles - 1 && !(ok = put(j >= kChain))) break;
         }
-        if (!ok) break;
       }
+      if (!ok) break;
+      // Results: o 2^ml.x is the sum of exp(s) v, l 2^ml.x of exp(s).  A thread holds a row; pieces of 16 bytes are
+      // exchanged within four lanes, so that a store writes 64 bytes of a row.
+      const long long at = ((long long)seq + (x.two ? 0 : (long long)i * kv.batch)) * a.n_heads + head;
+      float* slot_o = parts.slots + (size_t)slot * part_floats<HD>();
       if (mine) {
         const float2 ml = make_float2(m == -INFINITY ? -INFINITY : m * sl2 - kPShift, l);
         if (x.whole) __stcg(parts.ml + at, ml);
         else __stcg(reinterpret_cast<float2*>(slot_o + (size_t)kUnit * HD) + i * kRows + lrow, ml);
       }
-      if (tiles > 0 && !(ok = put(tiles > kChain))) break;
+      if (tiles > 0) {
+        if (!(ok = wait(o_full + i, no))) break;
+        no ^= 1u;
+        tc_fence_after();
+      }
+      if (tiles > 0 && !idle) {
+        float* base = x.whole ? parts.o + at * HD : slot_o + (size_t)(i * kRows + lrow) * HD;
+        float* to4[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          to4[q] = reinterpret_cast<float*>(__shfl_sync(kFull, mine ? reinterpret_cast<unsigned long long>(base) : 0ull,
+                                                        (lane & ~3) + q));
+#pragma unroll
+        for (int b = 0; b < HD; b += 32) {
+          uint32_t z[32];
+          tmem_ld<32>(to + b, z);
+          tmem_wait_ld();
+          if constexpr (TWO) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) z[e] = __float_as_uint(__uint_as_float(z[e]) + o[b + e]);
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e += 16) {
+            float4 p[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              p[q] = make_float4(__uint_as_float(z[e + 4 * q]), __uint_as_float(z[e + 4 * q + 1]),
+                                 __uint_as_float(z[e + 4 * q + 2]), __uint_as_float(z[e + 4 * q + 3]));
+            transpose4(p, lane);  // p[q]: piece lane % 4 of the four lanes' row q
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (to4[q]) __stcg(reinterpret_cast<float4*>(to4[q] + b + e) + (lane & 3), p[q]);
+          }
+        }
+        tc_fence_before();
+      }
       advance(x.n);
     }
   }
@@ -602,12 +694,13 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
 }
 
 // Joins a row's parts: those of its own positions, then of the shared ones.  WARPS warps a row (8 or 1) take
-// every WARPS-th part.
+// every WARPS-th part.  The own pass has left what leads to them (its parts, the group), so that three loads follow one
+// another: that, the shared pass's parts, and all parts' outputs, maxima and sums at once.
 template <class O, int HD, int WARPS>
 __global__ void __launch_bounds__(256) attention_shared_join_kernel(const PagedArgs a, const KvArgs kv,
                                                                     const SharedView v, const SharedParts parts,
                                                                     int zs) {
-  constexpr int E = HD / 32;
+  constexpr int E = HD / 32, U = WARPS == 8 ? 8 : 4;  // parts at a time
   __shared__ float s_o[8][HD];
   __shared__ float2 s_ml[8];
   pdl_trigger();
@@ -616,80 +709,75 @@ __global__ void __launch_bounds__(256) attention_shared_join_kernel(const PagedA
   const long long row = WARPS == 8 ? blockIdx.x : (long long)blockIdx.x * 8 + warp;
   if (row >= (long long)kv.batch * a.n_heads) return;
   const int s = (int)(row / a.n_heads), h = (int)(row % a.n_heads), j = h / g, in = h % g, R = g <= 8 ? 8 : 16;
-  bool clipped;
-  int grp, b = 0, e = 0, shared;
-  const int n = kv_length(kv, s, &clipped), base = shared_base(v, kv, s, n, &grp);
-  const Found own = [&] {
-    const int4 x = __ldcg(reinterpret_cast<const int4*>(v.own_found + ((long long)s * kv.n_kv + j) * zs + in / 16));
-    return Found{x.x, x.y, x.z, 0};
-  }();
-  Found f = {0, 0, 0, 0};
+  const int4* at_own = reinterpret_cast<const int4*>(v.own_found + ((long long)s * kv.n_kv + j) * zs + in / 16);
+  const int4 own = __ldcg(at_own), grp = __ldcg(at_own + 1);  // parts, CTA, slot; group (-1: none), its sequences
+  int4 f = make_int4(0, 0, 0, 0);
   int local = 0, streams = 1;
-  if (base > 0) {
-    group_of(v, kv, grp, &b, &e, &shared);
-    const int rr = (s - b) * g + in, blk = rr / kUnit;
+  if (grp.x >= 0) {
+    const int rr = (s - grp.y) * g + in, blk = rr / kUnit;
     local = rr % kUnit;
-    streams = min(kUnit, (e - b) * g - blk * kUnit) > kRows ? 1 : 2;
-    const int4 x = __ldcg(reinterpret_cast<const int4*>(parts.found + (long long)j * parts.found_stride +
-                                                        unit_index(b * g, grp, blk)));
-    f = {x.x, x.y, x.z, 0};
+    streams = min(kUnit, (grp.z - grp.y) * g - blk * kUnit) > kRows ? 1 : 2;
+    f = __ldcg(reinterpret_cast<const int4*>(parts.found + (long long)j * parts.found_stride +
+                                             unit_index(grp.y * g, grp.x, blk)));
   }
-  const int total = own.parts + f.parts * streams;
-  // part p: its output row, and its (maximum, sum)
-  auto find = [&](int p, const float** o) -> float2 {
-    if (p < own.parts) {
-      if (own.parts == 1) {
+  const int total = own.x + f.x * streams;
+  // where part p's output row is, and its (maximum, sum)
+  auto find = [&](int p, const float** o) -> const float2* {
+    if (p < own.x) {
+      if (own.x == 1) {
         *o = v.own_o + row * HD;
-        float2 ml = __ldcg(v.own_ml + row);
-        ml.x -= kShift;
-        return ml;
+        return v.own_ml + row;
       }
-      const float* slot = v.own_slots + (size_t)(p ? 2 * (own.cta + p) : own.slot) * (size_t)slot_floats(R, HD);
-      const int x = in % 16;
-      *o = slot + x * HD;
-      return make_float2(__ldcg(slot + R * HD + x) - kShift, __ldcg(slot + R * HD + R + x));
+      const float* slot = v.own_slots + (size_t)(p ? 2 * (own.y + p) : own.z) * (size_t)slot_floats(R, HD);
+      *o = slot + (in % 16) * HD;
+      return reinterpret_cast<const float2*>(slot + R * HD) + in % 16;
     }
-    p -= own.parts;
+    p -= own.x;
     const int i = streams == 2 ? p & 1 : 0, k = streams == 2 ? p >> 1 : p;
-    if (f.parts == 1) {
+    if (f.x == 1) {
       const long long at = row + (long long)i * kv.batch * a.n_heads;
       *o = parts.o + at * HD;
-      return __ldcg(parts.ml + at);
+      return parts.ml + at;
     }
-    const float* slot = parts.slots + (size_t)(k ? 2 * (f.cta + k) : f.slot) * part_floats<HD>();
+    const float* slot = parts.slots + (size_t)(k ? 2 * (f.y + k) : f.z) * part_floats<HD>();
     *o = slot + (size_t)(local + i * kRows) * HD;
-    return __ldcg(reinterpret_cast<const float2*>(slot + (size_t)kUnit * HD) + local + i * kRows);
+    return reinterpret_cast<const float2*>(slot + (size_t)kUnit * HD) + local + i * kRows;
   };
   float m = -INFINITY, l = 0.0f, o[E] = {};
-  const int start = WARPS == 8 ? warp : 0;
-  for (int p0 = start; p0 < total; p0 += 32 * WARPS) {  // a part per lane for the maxima, then its output with all lanes
-    const float* at = nullptr;
-    const int p = p0 + lane * WARPS;
-    float2 ml = make_float2(-INFINITY, 0.0f);
-    if (p < total) ml = find(p, &at);
-    float mn = ml.y == 0.0f ? -INFINITY : ml.x;  // nothing in it: there may be no output either
-    const bool live = p < total && !(ml.x == -INFINITY && ml.y == 0.0f);
+  for (int p0 = WARPS == 8 ? warp : 0; p0 < total; p0 += U * WARPS) {
+    float x[U][E];
+    float2 ml[U];
 #pragma unroll
-    for (int q = 16; q > 0; q >>= 1) mn = fmaxf(mn, __shfl_xor_sync(kFull, mn, q));
-    mn = fmaxf(mn, m);
-    const float mz = mn == -INFINITY ? 0.0f : mn, f0 = ex2(m - mz), f1 = live ? ex2(ml.x - mz) : 0.0f;
-    m = mn;
-    l = l * f0 + warp_sum(f1 * ml.y);
-#pragma unroll
-    for (int q = 0; q < E; ++q) o[q] *= f0;
-    const int count = min(32, (total - p0 + WARPS - 1) / WARPS);
-#pragma unroll 8
-    for (int q = 0; q < count; ++q) {
-      const float* src = reinterpret_cast<const float*>(__shfl_sync(kFull, live ? reinterpret_cast<unsigned long long>(at) : 0ull, q));
-      const float wt = __shfl_sync(kFull, f1, q);
-      if (src) {
+    for (int u = 0; u < U; ++u) {
+      const int p = p0 + u * WARPS;
+      ml[u] = make_float2(-INFINITY, 0.0f);
+      if (p < total) {
+        const float* src;
+        ml[u] = __ldcg(find(p, &src));
+        if (p < own.x) ml[u].x -= kShift;  // the two passes' weights have different factors
 #pragma unroll
         for (int z = 0; z < E; z += 2) {
           const float2 y = __ldcg(reinterpret_cast<const float2*>(src + lane * E + z));
-          o[z] = fmaf(wt, y.x, o[z]);
-          o[z + 1] = fmaf(wt, y.y, o[z + 1]);
+          x[u][z] = y.x;
+          x[u][z + 1] = y.y;
         }
       }
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
+    const float mz = mn == -INFINITY ? 0.0f : mn, f0 = ex2(m - mz);
+    m = mn;
+    l *= f0;
+#pragma unroll
+    for (int z = 0; z < E; ++z) o[z] *= f0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (ml[u].x == -INFINITY && ml[u].y == 0.0f) continue;  // nothing in it: there may be no output either
+      const float w = ex2(ml[u].x - mz);
+      l = fmaf(w, ml[u].y, l);
+#pragma unroll
+      for (int z = 0; z < E; ++z) o[z] = fmaf(w, x[u][z], o[z]);
     }
   }
   if constexpr (WARPS == 8) {
@@ -746,14 +834,15 @@ Space space_of(int batch, int groups, int n_heads, int n_kv, int head_dim) {
   x.own_slots = take(own_slots_floats(n_heads, n_kv, head_dim) * 4);
   x.own_o = take(rows * head_dim * 4);
   x.own_ml = take(rows * 8);
-  x.own_found = take((size_t)batch * n_kv * x.zs * sizeof(Found));
+  x.own_found = take((size_t)batch * n_kv * x.zs * sizeof(OwnFound));
   x.bytes = at;
   return x;
 }
 
 template <class T, class O, int HD>
 cudaError_t launch_typed(const SharedArgs& sa, const KvArgs& kv, cudaStream_t stream, unsigned* err) {
-  using C = Cfg<HD>;
+  using C = Cfg<sizeof(O) == 4, HD>;
+  constexpr int kKeys = C::kKeys;
   const PagedArgs& a = sa.paged;
   auto kernel = attention_shared_kernel<T, sizeof(O) == 4, HD>;
   const Space sp = space_of(kv.batch, sa.groups, a.n_heads, kv.n_kv, HD);
@@ -764,7 +853,7 @@ cudaError_t launch_typed(const SharedArgs& sa, const KvArgs& kv, cudaStream_t st
   v.groups = sa.groups;
   v.own_o = reinterpret_cast<float*>(ws + sp.own_o);
   v.own_ml = reinterpret_cast<float2*>(ws + sp.own_ml);
-  v.own_found = reinterpret_cast<Found*>(ws + sp.own_found);
+  v.own_found = reinterpret_cast<OwnFound*>(ws + sp.own_found);
   v.own_slots = reinterpret_cast<float*>(ws + sp.own_slots);
   SharedParts parts;
   parts.o = reinterpret_cast<float*>(ws + sp.o);
@@ -773,7 +862,7 @@ cudaError_t launch_typed(const SharedArgs& sa, const KvArgs& kv, cudaStream_t st
   parts.found = reinterpret_cast<Found*>(ws + sp.found);
   parts.found_stride = sp.found_stride;
   CUtensorMap kmap, vmap;
-  const int box_rows = kv.page_size < kRows ? kv.page_size : kRows;
+  const int box_rows = kv.page_size < kKeys ? kv.page_size : kKeys;
   if (!encode_kv_map(&kmap, kv, kv.k, box_rows) || !encode_kv_map(&vmap, kv, kv.v, box_rows))
     return cudaErrorInvalidValue;
   static std::atomic<unsigned long long> done{0};
@@ -782,7 +871,7 @@ cudaError_t launch_typed(const SharedArgs& sa, const KvArgs& kv, cudaStream_t st
   if (e != cudaSuccess) return e;
   // What is known here bounds the tiles: units of all groups, key tiles by what the page table can hold.
   const long long units = ((long long)kv.batch * (a.n_heads / kv.n_kv) / kUnit + sa.groups) * kv.n_kv;
-  const long long most = units * (((long long)kv.width * kv.page_size + kRows - 1) / kRows);
+  const long long most = units * (((long long)kv.width * kv.page_size + kKeys - 1) / kKeys);
   long long ctas = sms < kMaxCtas ? sms : kMaxCtas;
   if (ctas > most) ctas = most < 1 ? 1 : most;
   cudaLaunchConfig_t cfg = {};

@@ -7,11 +7,18 @@
 
 namespace asmllm {
 
-// One sequence's or group's result that is not split: 1 part, found by row; more: in slots.
+// Where a unit's result is.  1 part: found by row; more: in slots.
 struct Found {
   int parts;  // 0: no position, 1: whole, else CTAs cta .. cta + parts - 1 hold one part each
   int cta;
   int slot;   // slot of the first part (the others are in slot 2 c)
+  int pad;
+};
+// Of a sequence's own positions, and the group whose result is to be joined with it.
+struct OwnFound {
+  Found found;
+  int group;       // -1: none
+  int first, end;  // the group's sequences
   int pad;
 };
 
@@ -23,7 +30,7 @@ struct SharedView {
   // log2, sum) [batch][n_heads], and where each unit's are
   float* own_o = nullptr;
   float2* own_ml = nullptr;
-  Found* own_found = nullptr;  // [batch][n_kv * zs]
+  OwnFound* own_found = nullptr;  // [batch][n_kv * zs]
   float* own_slots = nullptr;
 };
 
@@ -41,19 +48,21 @@ __device__ __forceinline__ bool group_of(const SharedView& v, const KvArgs& kv, 
   return ok && n >= 0 && n <= cap;
 }
 
-// Positions of sequence s, of n, that it shares with its group, and the group: none for a sequence without a group,
-// or with fewer positions than the group shares.
-__device__ __forceinline__ int shared_base(const SharedView& v, const KvArgs& kv, int s, int n, int* group) {
+// Positions of sequence s, of n, that it shares with its group, and (group, its sequences): none, and -1, for a sequence
+// without a group, or with fewer positions than the group shares.
+__device__ __forceinline__ int shared_base(const SharedView& v, const KvArgs& kv, int s, int n, int4* group) {
   int lo = 0, hi = v.groups;
   while (lo < hi) {  // the first group that ends behind s
     const int mid = (lo + hi) >> 1;
     if (__ldcg(v.cu_group + mid + 1) <= s) lo = mid + 1; else hi = mid;
   }
-  *group = lo;
+  *group = make_int4(-1, 0, 0, 0);
   if (lo >= v.groups) return 0;
   int b, e, shared;
   group_of(v, kv, lo, &b, &e, &shared);
-  return s >= b && s < e && n >= shared ? shared : 0;
+  if (s < b || s >= e || n < shared || shared == 0) return 0;
+  *group = make_int4(lo, b, e, 0);
+  return shared;
 }
 
 #endif  // __CUDACC__
