@@ -1472,7 +1472,8 @@ ASMLLM_API int asm_rows_adjust_async(const asm_adjust_t* d, void* stream) {
   if (!d) return set_error(ASM_E_INVALID, "%s: null descriptor", name);
   if (d->rows < 0 || d->n <= 0 || d->stride < d->n || d->out_stride < d->n)
     return set_error(ASM_E_INVALID, "%s: need rows >= 0, n > 0, strides >= n", name);
-  if (d->rows > 65535) return set_error(ASM_E_UNSUPPORTED, "%s: rows %d (at most 65535)", name, d->rows);
+  if (d->rows > 65535 || d->n > kAdjustMaxN)
+    return set_error(ASM_E_UNSUPPORTED, "%s: rows %d (at most 65535) of %d words (at most %d)", name, d->rows, d->n, kAdjustMaxN);
   if (d->dtype != ASM_DT_F32 && d->dtype != ASM_DT_F16 && d->dtype != ASM_DT_BF16)
     return set_error(ASM_E_UNSUPPORTED, "%s: logits type %d", name, d->dtype);
   const int size = d->dtype == ASM_DT_F32 ? 4 : 2;
@@ -1480,6 +1481,7 @@ ASMLLM_API int asm_rows_adjust_async(const asm_adjust_t* d, void* stream) {
     return set_error(ASM_E_INVALID, "%s: misaligned buffer", name);
   if (d->tokens && (d->held < 0 || d->token_stride < d->held))
     return set_error(ASM_E_INVALID, "%s: need 0 <= held <= token_stride", name);
+  if (d->held > (1 << 28)) return set_error(ASM_E_UNSUPPORTED, "%s: %d tokens a row (at most 2^28)", name, d->held);
   if (!d->tokens && (d->n_tokens || d->n_prompt || d->repetition || d->frequency || d->presence))
     return set_error(ASM_E_INVALID, "%s: penalties without tokens", name);
   if (d->n_bias < 0 || (d->n_bias > 0 && (!d->bias_tokens || !d->bias)))
@@ -1518,6 +1520,7 @@ ASMLLM_API int asm_rows_adjust_async(const asm_adjust_t* d, void* stream) {
   a.out_stride = d->out_stride;
   a.rows = d->rows;
   a.n = d->n;
+  a.in_place = in_place;
   a.tokens = tokens;
   a.token_stride = d->token_stride;
   a.held = d->held;

@@ -42,6 +42,7 @@ struct AdjustArgs {
   int dtype = kDtF32;
   long long stride = 0, out_stride = 0;
   int rows = 0, n = 0;
+  bool in_place = false;  // out is logits
   const int32_t* tokens = nullptr;  // [rows] x token_stride, held tokens each; null: no penalties
   long long token_stride = 0;
   int held = 0;
@@ -56,7 +57,7 @@ struct AdjustArgs {
   const int32_t* allowed = nullptr;  // [rows] x allowed_stride words of 32 bits, or null
   long long allowed_stride = 0;
 };
-constexpr int kAdjustMaxBias = 1024;
+constexpr int kAdjustMaxBias = 1024, kAdjustMaxN = 1 << 18;
 
 cudaError_t launch_rope_append_q8(const RopeAppendArgs& a, int q_dtype, const KvQ8Args& c, cudaStream_t stream);
 cudaError_t launch_cache_read_q8(const CacheReadArgs& a, const KvQ8Args& c, cudaStream_t stream);

@@ -1181,7 +1181,7 @@ def _rows2(t, name, rows, dtype):
 
 def rows_adjust(logits, *, tokens=None, n_tokens=None, n_prompt=None, repetition=None, frequency=None, presence=None,
                 bias_tokens=None, bias=None, allowed=None, out=None, stream=None):
-    """Logits [B, V] (fp32, fp16 or bf16) with penalties, biases and a mask, for rows_sample
+    """Logits [B, V] (fp32, fp16 or bf16; V <= 262144) with penalties, biases and a mask, for rows_sample
     (asm_rows_adjust_async).
 
     In fp32: words among tokens [B, L] int32 (the first n_tokens[r] of a row) are divided by repetition where

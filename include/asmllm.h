@@ -823,11 +823,11 @@ ASMLLM_API int asm_attention_shared_async(const void* q, int64_t q_row_stride, i
 
 /* What is done to logits before asm_rows_sample_async: out = logits with, in
  * fp32, each step rounded, and one rounding to their type at the end,
- *   1. words among tokens[r][0 .. n_tokens[r]): x > 0 ? x / repetition : x * repetition;
+ *   1. words among tokens[r][0 .. n_tokens[r]): x > 0 ? x * (1 / repetition) : x * repetition;
  *   2. words that occur c > 0 times from n_prompt[r] on: x - frequency * c - presence;
  *   3. words among bias_tokens[r]: x + the sum of their biases (in 64 bits);
  *   4. words whose bit in allowed[r] is 0 (bit w % 32 of word w / 32): -inf.
- * tokens outside [0, n) are passed over, as are bias_tokens (-1: unused).
+ * n at most 262144.  tokens outside [0, n) are passed over, as are bias_tokens (-1: unused).
  * n_tokens outside [0, held] is clipped and sets ASM_DEVERR_DECODE_RANGE.
  * out may be logits itself; any other overlap with an input is refused. */
 typedef struct asm_adjust {
