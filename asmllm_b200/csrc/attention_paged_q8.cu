@@ -65,13 +65,15 @@ __device__ __forceinline__ uint32_t code_chunk(int r, int c) {
   return (uint32_t)(r * HD + ((HD == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4));
 }
 
-// Bytes 0 and 2 (odd: 1 and 3) of w, signed, as two fp16 values: 0x6400 + u is 1024 + u.
-__device__ __forceinline__ uint32_t codes_even(uint32_t w) {
-  const uint32_t x = (w & 0x00FF00FFu) ^ 0x64806480u;
-  const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
-  return *reinterpret_cast<const uint32_t*>(&y);
+// The four signed bytes of w as fp16: 0 and 2, and 1 and 3.  With the sign bit turned a byte is u = code + 128, and
+// 0x6400 + u is 1024 + u.
+__device__ __forceinline__ void codes_of(uint32_t w, uint32_t& even, uint32_t& odd) {
+  const uint32_t u = w ^ 0x80808080u, e = __byte_perm(u, 0x64646464u, 0x4240), o = __byte_perm(u, 0x64646464u, 0x4341);
+  const __half2 base = __half2half2(__ushort_as_half(0x6480));
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&e), base), y = __hsub2(*reinterpret_cast<const __half2*>(&o), base);
+  even = *reinterpret_cast<const uint32_t*>(&x);
+  odd = *reinterpret_cast<const uint32_t*>(&y);
 }
-__device__ __forceinline__ uint32_t codes_odd(uint32_t w) { return codes_even(w >> 8); }
 
 // c += a b, and c = a b, as mma16816 but free to be moved among the conversions.
 __device__ __forceinline__ void product(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -290,8 +292,10 @@ attention_paged_q8_kernel(const __grid_constant__ CUtensorMap kmap, const __grid
     }
 
     for (int t = t0; t < t1; ++t) {
-      if (ok) ok = mbar_wait_bounded(smem_u32(full + st), phase) && !*s_abort;
-      ok = __all_sync(kFull, ok);
+      if (!__all_sync(kFull, ok && mbar_try_wait(smem_u32(full + st), phase))) {
+        if (ok) ok = mbar_wait_bounded(smem_u32(full + st), phase) && !*s_abort;
+        ok = __all_sync(kFull, ok);
+      }
       if (!ok) {  // give up: keep in step with the other warps, but touch no more tiles
         if (lane == 0) {
           *s_abort = 1;
@@ -325,8 +329,7 @@ attention_paged_q8_kernel(const __grid_constant__ CUtensorMap kmap, const __grid
             ldsm4(f, at ^ (32u * b));
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              c[2 * k] = codes_even(f[k]);
-              c[2 * k + 1] = codes_odd(f[k]);
+              codes_of(f[k], c[2 * k], c[2 * k + 1]);
             }
             const float2 d0 = unpack16<__half>(d[0][b >> 1]), d1 = unpack16<__half>(d[1][b >> 1]);
             const float y0 = b & 1 ? d0.y : d0.x, y1 = b & 1 ? d1.y : d1.x;
@@ -346,9 +349,11 @@ attention_paged_q8_kernel(const __grid_constant__ CUtensorMap kmap, const __grid
 #pragma unroll
         for (int n = 0; n < N; ++n) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            s[n][k] *= rs[n][k & 1];
-            if (left < 16 && r + 8 * (k >> 1) >= left) s[n][k] = -INFINITY;
+          for (int k = 0; k < 4; ++k) s[n][k] *= rs[n][k & 1];
+          if (left < 16) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (r + 8 * (k >> 1) >= left) s[n][k] = -INFINITY;
           }
           rises |= fmaxf(s[n][0], s[n][2]) > m[n][0] + kLazy || fmaxf(s[n][1], s[n][3]) > m[n][1] + kLazy;
         }
@@ -456,8 +461,7 @@ attention_paged_q8_kernel(const __grid_constant__ CUtensorMap kmap, const __grid
           ldsm4_t(f, at ^ (32u * b));
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            c[2 * k] = codes_even(f[k]);
-            c[2 * k + 1] = codes_odd(f[k]);
+            codes_of(f[k], c[2 * k], c[2 * k + 1]);
           }
           const __half2 d0 = as_half2(__byte_perm(vs[0][b >> 1], vs[1][b >> 1], b & 1 ? 0x7632 : 0x5410));
           const __half2 d1 = as_half2(__byte_perm(vs[2][b >> 1], vs[3][b >> 1], b & 1 ? 0x7632 : 0x5410));
