@@ -23,7 +23,8 @@ LIB_PATH = LIB_DIR / "libasmllm.so"
 
 SOURCES = ["matvec.cu", "tma_matvec.cu", "decode.cu", "decode_persistent.cu", "q5_matvec.cu", "prefill_gemm.cu",
            "batch_decode.cu", "rope_append.cu", "attention_prompt.cu", "attention_paged.cu", "rows_sample.cu",
-           "cache_q8.cu", "attention_paged_q8.cu", "attention_shared.cu", "rows_adjust.cu", "glue.cu", "capi.cu"]
+           "cache_q8.cu", "attention_paged_q8.cu", "attention_shared.cu", "attention_own.cu",
+           "rows_adjust.cu", "glue.cu", "capi.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -45,7 +45,6 @@
 #include "paged_deal.cuh"
 #include "pipeline.cuh"
 #include "serving.cuh"
-#include "shared_prefix.cuh"
 #include "tensor_map.cuh"
 
 namespace asmllm {
@@ -54,7 +53,7 @@ namespace {
 
 constexpr int kWarps = 4;   // consumer warps
 constexpr int kStages = 3;
-constexpr int kMaxCtas = kOwnCtas;
+constexpr int kMaxCtas = 320;
 constexpr int kThreads = (kWarps + 1) * 32;
 
 template <int ROWS, int HD>
@@ -100,12 +99,10 @@ __device__ __forceinline__ void add_values(float (&o)[HD / 8][4], int d0, const 
   }
 }
 
-// OWN: the positions behind those that a group shares alone, and all results left unnormalised for another join.
-template <class T, class O, int HD, int ROWS, bool OWN>
+template <class T, class O, int HD, int ROWS>
 __global__ void __launch_bounds__(kThreads, 2)
 attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                       const PagedArgs a, const KvArgs kv, int zs, int box_rows, unsigned* __restrict__ err,
-                       const SharedView own) {
+                       const PagedArgs a, const KvArgs kv, int zs, int box_rows, unsigned* __restrict__ err) {
   using L = Layout<ROWS, HD>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -129,44 +126,27 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
     fence_mbar_init();
   }
   pdl_trigger();
-  // OWN: the launch before this one is the shared pass, which nothing here reads; it began behind whatever wrote the
-  // queries and the cache.  Its end is waited for at this kernel's, so that the join behind has both.
-  if constexpr (!OWN) pdl_wait();
+  pdl_wait();
 
-  // positions of sequence s, without those that it shares
-  int4 group;  // OWN: that of the sequence len() was last called for
   auto len = [&](int s, bool report) -> int {
     bool clipped;
-    int n = kv_length(kv, s, &clipped);
+    const int n = kv_length(kv, s, &clipped);
     if (clipped && report) atomicOr(err, kErrDecodeRange);
-    if constexpr (OWN) n -= shared_base(own, kv, s, n, &group);
     return n;
   };
-  // OWN: where unit u's result is, and the group it is joined with
-  auto leave = [&](int s, int u, int parts, int slot) {
-    int4* at = reinterpret_cast<int4*>(own.own_found + (long long)s * units + u);
-    __stcg(at, make_int4(parts, cta, slot, 0));
-    __stcg(at + 1, group);
-  };
-  // a sequence without positions: zeros, written by one CTA
-  auto none = [&](int s) {
-    if constexpr (OWN) {
-      for (int u = 0; u < units; ++u) leave(s, u, 0, 0);
-    } else {
-      O* out = static_cast<O*>(a.out) + (long long)s * a.n_heads * HD;
-      const float z[8] = {};
-      for (int i = 0; i < a.n_heads * HD; i += 8) store8(out + i, z);
-    }
+  auto none = [&](int s) {  // a sequence without positions: zeros, written by one CTA
+    O* out = static_cast<O*>(a.out) + (long long)s * a.n_heads * HD;
+    const float z[8] = {};
+    for (int i = 0; i < a.n_heads * HD; i += 8) store8(out + i, z);
   };
   Walk w;
   Deal deal(0, 1);
   const bool any = deal_range<kThreads>(kv.batch, units, s_part, s_first, s_start, len, none, &w, &deal);
 
-  float* slots = OWN ? own.own_slots : static_cast<float*>(a.workspace);
+  float* slots = static_cast<float*>(a.workspace);
   Split* splits = reinterpret_cast<Split*>(slots + (size_t)kMaxCtas * 2 * slot_floats(ROWS, HD));
   if (!any) {
-    if constexpr (OWN) pdl_wait();
-    else if (tid == 0) splits[cta].unit = -1;
+    if (tid == 0) splits[cta].unit = -1;
     return;
   }
   const long long begin = w.at;
@@ -180,18 +160,10 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
     const bool worker = my_page < pages_tile;
     const uint32_t box_bytes = (uint32_t)box_rows * 128u;
     // page number of this lane's box in tile t of sequence s; n_pages (filled with zeros) for a bad one
-    int base_s = -1, base = 0;  // OWN: where a sequence's positions begin (a multiple of the page)
     auto lookup = [&](const Walk& x) -> int {
       const int p = x.t * kTile + my_page * box_rows;
-      if constexpr (OWN) {
-        if (x.s != base_s) {
-          bool clipped;
-          base_s = x.s;
-          base = shared_base(own, kv, x.s, kv_length(kv, x.s, &clipped), &group);
-        }
-      }
       if (!worker || p >= x.n) return -1;
-      const int page = __ldcg(kv.table + (long long)x.s * kv.table_stride + ((base + p) >> kv.page_shift));
+      const int page = __ldcg(kv.table + (long long)x.s * kv.table_stride + (p >> kv.page_shift));
       if ((unsigned)page < (unsigned)kv.n_pages) return page;
       atomicOr(err, kErrDecodeRange);
       return kv.n_pages;
@@ -226,7 +198,6 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
     // every issued copy lands before the CTA may end (bounded)
     for (int j = i - kStages < 0 ? 0 : i - kStages; j < i; ++j)
       mbar_wait_bounded(smem_u32(full + j % kStages), (j / kStages) & 1);
-    if constexpr (OWN) pdl_wait();
     return;
   }
 
@@ -239,7 +210,6 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
   bool ok = true;
   int i = 0, split_unit = -1, split_parts = 0, split_slot = 0;
   bool next = true;
-  if constexpr (OWN) len(w.s, false);
   while (next) {
     // one segment: tiles w.t .. of unit (w.s, w.u)
     const int j = w.u / zs, h0 = (w.u % zs) * 16, nh = min(16, g - h0);
@@ -435,15 +405,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
       if (warp == 0) {
         take(0);
         const int row = 8 * e + r;
-        if (OWN && whole) {
-          if (row < nh) {
-            const long long at = (long long)w.s * a.n_heads + j * g + h0 + row;
-#pragma unroll
-            for (int d = 0; d < HD / 8; ++d)
-              __stcg(reinterpret_cast<float2*>(own.own_o + at * HD + d * 8 + c2), make_float2(v[d][0], v[d][1]));
-            if ((lane & 3) == 0) __stcg(own.own_ml + at, make_float2(mm, ll));
-          }
-        } else if (whole) {
+        if (whole) {
           const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
           if (row < nh) {
             O* out = static_cast<O*>(a.out) + ((long long)w.s * a.n_heads + j * g + h0 + row) * HD;
@@ -461,12 +423,8 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
           for (int d = 0; d < HD / 8; ++d)
             __stcg(reinterpret_cast<float2*>(b + row * HD + d * 8 + c2), make_float2(v[d][0], v[d][1]));
           if ((lane & 3) == 0) {
-            if constexpr (OWN) {
-              __stcg(reinterpret_cast<float2*>(b + ROWS * HD) + row, make_float2(mm, ll));
-            } else {
-              __stcg(b + ROWS * HD + row, mm);
-              __stcg(b + ROWS * HD + ROWS + row, ll);
-            }
+            __stcg(b + ROWS * HD + row, mm);
+            __stcg(b + ROWS * HD + ROWS + row, ll);
           }
         }
       }
@@ -477,14 +435,11 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
       split_slot = slot;
       split_parts = deal.cta_of(w.first + w.nt - 1) - cta + 1;
     }
-    if (OWN && t0 == 0 && tid == 0) leave(w.s, w.u, whole ? 1 : split_parts, slot);
     w.at += t1 - t0;
     next = w.at < w.end;
     if (next) next_unit(w, units, len);
   }
-  if constexpr (OWN) {
-    pdl_wait();
-  } else if (tid == 0) {
+  if (tid == 0) {
     Split x;
     x.unit = split_unit;
     x.parts = split_parts;
@@ -494,11 +449,10 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
   }
 }
 
-template <class T, class O, int HD, int ROWS, bool OWN>
-cudaError_t launch_typed(const PagedArgs& a, const KvArgs& kv, cudaStream_t stream, unsigned* err,
-                         const SharedView& own) {
+template <class T, class O, int HD, int ROWS>
+cudaError_t launch_typed(const PagedArgs& a, const KvArgs& kv, cudaStream_t stream, unsigned* err) {
   using L = Layout<ROWS, HD>;
-  auto kernel = attention_paged_kernel<T, O, HD, ROWS, OWN>;
+  auto kernel = attention_paged_kernel<T, O, HD, ROWS>;
   CUtensorMap kmap, vmap;
   const int box_rows = kv.page_size < kTile ? kv.page_size : kTile;
   if (!encode_kv_map(&kmap, kv, kv.k, box_rows) || !encode_kv_map(&vmap, kv, kv.v, box_rows))
@@ -519,8 +473,8 @@ cudaError_t launch_typed(const PagedArgs& a, const KvArgs& kv, cudaStream_t stre
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = g_opt_pdl.load() ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, kernel, kmap, vmap, a, kv, zs, box_rows, err, own);
-  if (e != cudaSuccess || OWN) return e;
+  e = cudaLaunchKernelEx(&cfg, kernel, kmap, vmap, a, kv, zs, box_rows, err);
+  if (e != cudaSuccess) return e;
   cfg.gridDim = dim3((unsigned)ctas, (unsigned)(g < 16 ? g : 16));
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
@@ -529,14 +483,8 @@ cudaError_t launch_typed(const PagedArgs& a, const KvArgs& kv, cudaStream_t stre
 
 template <class T, class O, int HD>
 cudaError_t launch_rows(const PagedArgs& a, const KvArgs& kv, cudaStream_t stream, unsigned* err) {
-  return a.n_heads / kv.n_kv <= 8 ? launch_typed<T, O, HD, 8, false>(a, kv, stream, err, SharedView())
-                                  : launch_typed<T, O, HD, 16, false>(a, kv, stream, err, SharedView());
-}
-
-template <class T, int HD>
-cudaError_t launch_own(const PagedArgs& a, const KvArgs& kv, const SharedView& v, cudaStream_t stream, unsigned* err) {
-  return a.n_heads / kv.n_kv <= 8 ? launch_typed<T, float, HD, 8, true>(a, kv, stream, err, v)
-                                  : launch_typed<T, float, HD, 16, true>(a, kv, stream, err, v);
+  return a.n_heads / kv.n_kv <= 8 ? launch_typed<T, O, HD, 8>(a, kv, stream, err)
+                                  : launch_typed<T, O, HD, 16>(a, kv, stream, err);
 }
 
 template <class T>
@@ -560,19 +508,6 @@ cudaError_t launch_attention_paged(const PagedArgs& a, const KvArgs& kv, cudaStr
   if (!err) return cudaErrorUnknown;
   return kv.dtype == kDtF16 ? launch_type<__half>(a, kv, stream, err)
                             : launch_type<__nv_bfloat16>(a, kv, stream, err);
-}
-
-size_t own_slots_floats(int n_heads, int n_kv, int head_dim) {
-  return (size_t)kMaxCtas * 2 * slot_floats(n_heads / n_kv <= 8 ? 8 : 16, head_dim);
-}
-
-cudaError_t launch_attention_own(const PagedArgs& a, const KvArgs& kv, const SharedView& v, cudaStream_t stream) {
-  unsigned* err = device_error_word();
-  if (!err) return cudaErrorUnknown;
-  if (kv.dtype == kDtF16)
-    return kv.head_dim == 128 ? launch_own<__half, 128>(a, kv, v, stream, err) : launch_own<__half, 64>(a, kv, v, stream, err);
-  return kv.head_dim == 128 ? launch_own<__nv_bfloat16, 128>(a, kv, v, stream, err)
-                            : launch_own<__nv_bfloat16, 64>(a, kv, v, stream, err);
 }
 
 }  // namespace asmllm

@@ -89,13 +89,6 @@ __device__ __forceinline__ void first_product(float (&c)[4], uint32_t a0, uint32
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
-// The transpose of an 8 x 8 matrix of 16-bit values (lane: row lane / 4, columns 2 (lane % 4) and the next).
-__device__ __forceinline__ uint32_t transposed8(uint32_t w) {
-  uint32_t r;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
-  return r;
-}
-
 __device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
 __device__ __forceinline__ uint32_t as_word(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 

@@ -7,7 +7,7 @@
 //   1. Shared pass (here): a group's query rows, (sequences x heads of a KV
 //      head), against its shared positions: a matrix product of up to 256 rows
 //      a key tile on the 5th-generation tensor cores.
-//   2. Own pass (attention_paged.cu): every sequence's positions behind those.
+//   2. Own pass (attention_own.cu): every sequence's positions behind those.
 //      It does not wait for the first, and runs on the SMs that has left.
 //   3. Join: a row's parts, in order.
 //
@@ -59,7 +59,7 @@ constexpr int kMaxCtas = 160;
 // 128 rows have a result each), parts in slots of kUnit rows.
 struct SharedParts {
   float* o;       // [2][batch][n_heads][head_dim]
-  float2* ml;     // [2][batch][n_heads]: maximum in units of log2, sum
+  float2* ml;     // [2][batch][n_heads]: (maximum in units of log2, sum); o 2^maximum is the sum of exp(s) v
   float* slots;   // [kMaxCtas][2] of kUnit x head_dim, then kUnit (maximum, sum)
   Found* found;   // [n_kv][found_stride]: unit_index()
   int found_stride;
@@ -710,7 +710,7 @@ __global__ void __launch_bounds__(256) attention_shared_join_kernel(const PagedA
   if (row >= (long long)kv.batch * a.n_heads) return;
   const int s = (int)(row / a.n_heads), h = (int)(row % a.n_heads), j = h / g, in = h % g, R = g <= 8 ? 8 : 16;
   const int4* at_own = reinterpret_cast<const int4*>(v.own_found + ((long long)s * kv.n_kv + j) * zs + in / 16);
-  const int4 own = __ldcg(at_own), grp = __ldcg(at_own + 1);  // parts, CTA, slot; group (-1: none), its sequences
+  const int4 own = __ldcg(at_own), grp = __ldcg(at_own + 1);  // parts, range, slot; group (-1: none), its sequences
   int4 f = make_int4(0, 0, 0, 0);
   int local = 0, streams = 1;
   if (grp.x >= 0) {
@@ -754,7 +754,6 @@ __global__ void __launch_bounds__(256) attention_shared_join_kernel(const PagedA
       if (p < total) {
         const float* src;
         ml[u] = __ldcg(find(p, &src));
-        if (p < own.x) ml[u].x -= kShift;  // the two passes' weights have different factors
 #pragma unroll
         for (int z = 0; z < E; z += 2) {
           const float2 y = __ldcg(reinterpret_cast<const float2*>(src + lane * E + z));

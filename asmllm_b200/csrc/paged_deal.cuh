@@ -48,6 +48,13 @@ struct Deal {
   }
 };
 
+// The transpose of an 8 x 8 matrix of 16-bit values (lane: row lane / 4, columns 2 (lane % 4) and the next).
+__device__ __forceinline__ uint32_t transposed8(uint32_t w) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
+  return r;
+}
+
 // A CTA's walk over its tiles: sequence, unit of the sequence, tile.
 struct Walk {
   int s, u, t, n, nt;      // n positions, nt tiles of sequence s

@@ -1,6 +1,6 @@
 // asmllm_b200/csrc/shared_prefix.cuh -- groups of sequences that share their
-// first positions: what the two passes of attention_shared.cu and the paged
-// pass over the rest (attention_paged.cu) agree on.
+// first positions: what the pass over those (attention_shared.cu) and the pass
+// over the rest (attention_own.cu) agree on.
 #pragma once
 
 #include "paged_deal.cuh"
@@ -9,9 +9,9 @@ namespace asmllm {
 
 // Where a unit's result is.  1 part: found by row; more: in slots.
 struct Found {
-  int parts;  // 0: no position, 1: whole, else CTAs cta .. cta + parts - 1 hold one part each
-  int cta;
-  int slot;   // slot of the first part (the others are in slot 2 c)
+  int parts;  // 0: no position, 1: whole, else ranges first .. first + parts - 1 hold one part each
+  int first;
+  int slot;   // slot of the first part (the others are in slot 2 r of range r)
   int pad;
 };
 // Of a sequence's own positions, and the group whose result is to be joined with it.
@@ -67,8 +67,8 @@ __device__ __forceinline__ int shared_base(const SharedView& v, const KvArgs& kv
 
 #endif  // __CUDACC__
 
-// The pass over the positions that are not shared (attention_paged.cu): results into `v`, none joined.
-constexpr int kOwnCtas = 320;
+// The pass over the positions that are not shared (attention_own.cu): results into `v`, none joined.
+constexpr int kOwnRanges = 1280;  // at most, one a warp
 size_t own_slots_floats(int n_heads, int n_kv, int head_dim);
 cudaError_t launch_attention_own(const PagedArgs& a, const KvArgs& kv, const SharedView& v, cudaStream_t stream);
 
