@@ -1184,8 +1184,8 @@ def rows_adjust(logits, *, tokens=None, n_tokens=None, n_prompt=None, repetition
     """Logits [B, V] (fp32, fp16 or bf16; V <= 262144) with penalties, biases and a mask, for rows_sample
     (asm_rows_adjust_async).
 
-    In fp32: words among tokens [B, L] int32 (the first n_tokens[r] of a row) are divided by repetition where
-    they are above 0 and multiplied by it elsewhere; words that come c > 0 times from n_prompt[r] on lose
+    In fp32: words among tokens [B, L] int32 (the first n_tokens[r] of a row) are multiplied by 1 / repetition
+    where they are above 0 and by repetition elsewhere; words that come c > 0 times from n_prompt[r] on lose
     frequency * c + presence; words among bias_tokens int32 [B, N] (-1: unused; N <= 1024) gain their bias
     fp32 [B, N], those of equal entries added up; words whose bit is 0 in allowed int32 [B, ceil(V / 32)] (bit
     w % 32 of w / 32) become -inf.  n_tokens, n_prompt int32 [B] (L, 0) and repetition, frequency, presence

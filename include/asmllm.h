@@ -809,8 +809,9 @@ ASMLLM_API int asm_attention_paged_q8_async(const void* q, int32_t q_dtype, int6
  * fewer positions than their group shares, have their own positions alone;
  * lengths count all positions.  The weights over shared positions are those
  * of asm_attention_prompt_async (one rounding for a 16-bit output, two 16-bit
- * parts for fp32); a value there that is not finite gives an output that is
- * not finite.  cu_group [groups + 1] and shared_len [groups] are on the
+ * parts for fp32), those over a sequence's own are two 16-bit parts; a value
+ * among what a row attends to that is not finite gives an output that is not
+ * finite.  cu_group [groups + 1] and shared_len [groups] are on the
  * device; offsets or lengths out of range set ASM_DEVERR_DECODE_RANGE (an
  * offset: the group shares nothing; a length is clipped).  workspace as for
  * asm_attention_paged_async (tens of MB); batch * n_heads at most 2^22. */
