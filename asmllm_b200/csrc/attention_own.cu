@@ -16,6 +16,12 @@
 // exchange within the warp, and enter as two 16-bit parts (2^-22 of a weight in
 // fp16, 2^-16 in bf16).  The output is rescaled only when a maximum has risen
 // by more than 2^kLazy.
+//
+// Measured on one B200: 256 sequences of 8 KV heads with 1 to 1023 positions of
+// 128 values each, 113 us (4.8 TB/s; issue at 70 % of what the SMs can do); 48
+// sequences of 32 KV heads with 1 to 299, 38 us.  With a CTA's four warps on one
+// ring and tiles of 64 positions, and the join in them, a call with the latter
+// took 95 us, not 80.
 #include <type_traits>
 
 #include "matvec.cuh"
@@ -376,7 +382,9 @@ attention_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     // every issued copy lands before the CTA may end (bounded)
     for (int i = done; i < asked; ++i) mbar_wait_bounded(smem_u32(full + i % S), (i / S) & 1);
   }
-  pdl_wait();
+  // The join may begin once every CTA here has ended: one that waits for the shared pass is enough, and the others leave
+  // their SM to the next ones.
+  if (blockIdx.x == gridDim.x - 1) pdl_wait();
 }
 
 template <class T, int HD, int ROWS, bool EXACT>

@@ -23,6 +23,14 @@
 // one position (keys), or two values of two positions (values, transposed),
 // and is split into its even and odd bytes.  The order of the values within a
 // product is free as long as the query's is the same.
+//
+// Measured on one B200, 64 sequences of 64 query and 8 KV heads of 128 values
+// that hold up to 16384 positions: 235 us (5.1 TB/s; the copy takes 184).  Codes
+// to fp16 and the scales are most of its instructions, 505 for 16 positions and
+// a warp, which issue in 55 % of the cycles.  355 for the fp16 cache of twice the
+// bytes (attention_paged.cu).  With positions as the right side, padded to 8
+// rows of heads as the left, 341; with 4 CTAs an SM of 2 stages 273, not 3 of 3.
+// 32 sequences of 1 to 1024: 22 us.  One of 32 heads and 512 positions: 10.
 #include "matvec.cuh"
 #include "mma16.cuh"
 #include "paged_deal.cuh"

@@ -31,9 +31,18 @@
 // 8 and 10, a stream each), 9 tensor copies of K and V tiles into a ring (a page
 // behind the shared ones reads as zeros).  One thread that issues for both
 // streams in turn keeps them half a tile apart: with a thread each they ran in
-// step, waiting for the exponentials and for the tensor core at the same time
-// (306 us, not 220, for 256 sequences of 64 query and 8 KV heads that share
-// 32768 positions).  Every wait is bounded, as in attention_prompt.cu.
+// step, waiting for the exponentials and for the tensor core at the same time.
+// Every wait is bounded, as in attention_prompt.cu.
+//
+// Measured on one B200, 256 sequences of 64 query and 8 KV heads of 128 values
+// in bf16 that share 32768 positions and have up to 1023 of their own: 360 us,
+// of which this pass takes 257 (1.07 PFLOP/s; matrix products alone would take
+// 165, exponentials 119), the own pass 85 to 113 and the join 16.  The shared
+// pass took 276 with two issuing threads and 296 with tiles of 64 positions.
+// Three groups of 48 sequences, 32 heads, fp32 outputs: 80 us.  8 sequences of
+// 8 heads that share 1024 positions: 12 us.  Giving this pass fewer SMs, so
+// that the own pass runs beside it, gained 5 % in the first of these and lost
+// up to 25 % elsewhere: a few SMs do not read the own positions fast enough.
 #include <type_traits>
 
 #include "matvec.cuh"
@@ -161,7 +170,7 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
   uint64_t* drain = o_full + 2;     // [2]
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drain + 2);
   volatile uint32_t* s_abort = s_tmem + 1;
-  long long* s_sum = reinterpret_cast<long long*>(smem);  // per-thread sums, before the queries come
+  long long* s_sum = reinterpret_cast<long long*>(smem);  // per-warp sums, before the queries come
   long long* s_total = reinterpret_cast<long long*>(smem + C::kSum);
   long long* s_first = s_total + 1;
   int* s_group = reinterpret_cast<int*>(s_total + 2);
@@ -212,33 +221,31 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     const int per = (v.groups + kThreads - 1) / kThreads, q0 = min(v.groups, tid * per), q1 = min(v.groups, q0 + per);
     long long mine = 0;
     for (int x = q0; x < q1; ++x) mine += load(x, &w, blockIdx.x == 0);
-    s_sum[tid] = mine;
+    long long x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long z = __shfl_up_sync(kFull, x, o);
+      if (lane >= o) x += z;
+    }
+    if (lane == 31) s_sum[warp] = x;  // the warps' sums
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 0) {
-      long long run = 0;
-      for (int c = 0; c < kThreads; c += 32) {
-        const long long y = s_sum[c + lane];
-        long long x = y;
+    long long before = x - mine, total = 0;  // tiles of the groups before this thread's; of all
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long z = __shfl_up_sync(kFull, x, o);
-          if (lane >= o) x += z;
-        }
-        s_sum[c + lane] = run + x - y;  // exclusive
-        run += __shfl_sync(kFull, x, 31);
-      }
-      if (lane == 0) *s_total = run;
+    for (int i = 0; i < kThreads / 32; ++i) {
+      const long long y = s_sum[i];
+      before += i < warp ? y : 0;
+      total += y;
     }
-    __syncthreads();
-    const int ctas = (int)min((long long)gridDim.x, *s_total);
-    const Deal deal(*s_total, max(1, ctas));
+    if (tid == 0) *s_total = total;
+    const int ctas = (int)min((long long)gridDim.x, total);
+    const Deal deal(total, max(1, ctas));
     w.at = (int)blockIdx.x < ctas ? deal.start(blockIdx.x) : 0;
     w.end = (int)blockIdx.x < ctas ? deal.start(blockIdx.x + 1) : 0;
     const long long at = w.at, end = w.end;
-    if (at < end && s_sum[tid] <= at && at < s_sum[tid] + mine) {
-      long long x = s_sum[tid];
+    if (at < end && before <= at && at < before + mine) {
+      x = before;
       for (int y = q0; y < q1; ++y) {
         const long long z = load(y, &w, false);
         if (at < x + z) {
@@ -534,8 +541,7 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         return true;
       };
       // Weights of keys from .. from + 63 in place of their scores, and their sum.  First the exponentials, then what needs
-      // them: with the sum beside each, the in-order pipeline waited for it, and a warp alone took 1050 cycles for 64 of
-      // them where 550 are possible.
+      // them: with the sum beside each, a warp by itself waits for each in turn.
       auto exponentials = [&](uint32_t(&y)[kKeys], int from) {
         const float off = kPShift - (m == -INFINITY ? 0.0f : m * sl2);
         const unsigned long long sl22 = pack2(sl2, sl2), off2 = pack2(off, off);

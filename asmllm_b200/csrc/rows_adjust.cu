@@ -22,7 +22,7 @@
 //     one's logits (asked for a slice ahead), two sets of counters in turn.
 //   A small batch: a CTA a slice of 2048 words, as many as there are.
 // Measured on one B200, 128 rows of 128256 words, 8192 tokens, 64 biases and a
-// mask: 42 us (the copy alone takes 21); instructions, of which the words'
+// mask: 44 us (the copy alone takes 21); instructions, of which the words'
 // penalties are the most, issue in 58 % of the cycles.  56 where every CTA
 // counts and then streams; 49 with a row's tokens in a hash table that is
 // applied to a copy of the logits (its scattered accesses take one cycle of an
