@@ -18,10 +18,13 @@
 // by more than 2^kLazy.
 //
 // Measured on one B200: 256 sequences of 8 KV heads with 1 to 1023 positions of
-// 128 values each, 113 us (4.8 TB/s; issue at 70 % of what the SMs can do); 48
-// sequences of 32 KV heads with 1 to 299, 38 us.  With a CTA's four warps on one
-// ring and tiles of 64 positions, and the join in them, a call with the latter
-// took 95 us, not 80.
+// 128 values each, about 105 us (5.2 TB/s), where a quarter of the cycles issue
+// an instruction: a tile is one chain of copy, products, softmax, products.  So
+// as many warps as registers allow, with one tile each: 128 sequences of up to
+// 8000 positions of their own take 398 us, 444 with half the warps and three
+// tiles each, 409 with two.  48 sequences of 32 KV heads with 1 to 299 behind
+// three prefixes: 74 us a call, 95 with a CTA's warps on one ring of tiles of 64
+// and their join.
 #include <type_traits>
 
 #include "matvec.cuh"
@@ -34,15 +37,16 @@ namespace asmllm {
 
 namespace {
 
-constexpr int kWarps = 4;
 constexpr int kSmall = 16;  // positions per tile
-constexpr int kThreads = kWarps * 32;
+constexpr int kLeast = 2;   // tiles of a warp, where there are few
 constexpr float kLazy = 5.0f, kPShift = 9.0f;  // weights 2^kPShift exp(s - m) stay below 2^15
 
-template <int HD>
+template <int HD, int ROWS>
 struct LayoutOwn {
+  static constexpr int kWarps = ROWS == 8 ? 8 : 6;    // two CTAs an SM: what the registers allow
+  static constexpr int kThreads = kWarps * 32;
   static constexpr int kTileBytes = kSmall * HD * 2;  // keys or values of a tile
-  static constexpr int kStages = HD == 128 ? 3 : 6;
+  static constexpr int kStages = 128 / HD;
   static constexpr int kRing = kStages * 2 * kTileBytes;  // of a warp
   static constexpr int kBarOff = kWarps * kRing;
   static constexpr int kSmem = kBarOff + kWarps * kStages * 8 + 1024;
@@ -75,11 +79,11 @@ struct Steps {
 
 // EXACT: fp32 outputs: each tile is added with rounding (the tensor core truncates its sums).
 template <class T, int HD, int ROWS, bool EXACT>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(LayoutOwn<HD, ROWS>::kThreads, 2)
 attention_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                      const PagedArgs a, const KvArgs kv, const SharedView v, int zs, unsigned* __restrict__ err) {
-  using L = LayoutOwn<HD>;
-  constexpr int S = L::kStages, N = ROWS / 8, kHalves = HD / 64;
+  using L = LayoutOwn<HD, ROWS>;
+  constexpr int kWarps = L::kWarps, kThreads = L::kThreads, S = L::kStages, N = ROWS / 8, kHalves = HD / 64;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ long long s_part[kThreads + 1];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -151,7 +155,10 @@ attention_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     __syncthreads();
   }
   const long long total = s_part[kThreads];
-  const int count = (int)min((long long)gridDim.x * kWarps, total);  // every range in use holds a tile
+  // A range has kLeast tiles, but for the shortest: a part costs the join more than the second tile its warp (100
+  // sequences of one KV head, 512 positions of their own: 31.7 us, 34.2 with one tile; 8 sequences of 64: 16 us with 4
+  // tiles, 12 with 2).
+  const int count = (int)min((long long)gridDim.x * kWarps, (total + kLeast - 1) / kLeast);
   // neighbouring ranges lie in different CTAs: few units spread over all SMs
   const int index = warp * gridDim.x + blockIdx.x;
   const Deal deal(total, max(1, count));
@@ -389,7 +396,7 @@ attention_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 
 template <class T, int HD, int ROWS, bool EXACT>
 cudaError_t launch_typed(const PagedArgs& a, const KvArgs& kv, const SharedView& v, cudaStream_t stream, unsigned* err) {
-  using L = LayoutOwn<HD>;
+  using L = LayoutOwn<HD, ROWS>;
   auto kernel = attention_own_kernel<T, HD, ROWS, EXACT>;
   CUtensorMap kmap, vmap;
   if (!encode_kv_map(&kmap, kv, kv.k, kSmall) || !encode_kv_map(&vmap, kv, kv.v, kSmall)) return cudaErrorInvalidValue;
@@ -397,10 +404,10 @@ cudaError_t launch_typed(const PagedArgs& a, const KvArgs& kv, const SharedView&
   int sms = 0;
   const cudaError_t e = kernel_setup(reinterpret_cast<const void*>(kernel), L::kSmem, done, &sms);
   if (e != cudaSuccess) return e;
-  const int ctas = 2 * sms * kWarps < kOwnRanges ? 2 * sms : kOwnRanges / kWarps;
+  const int ctas = 2 * sms * L::kWarps < kOwnRanges ? 2 * sms : kOwnRanges / L::kWarps;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(L::kThreads);
   cfg.dynamicSmemBytes = L::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

@@ -35,11 +35,11 @@
 // Every wait is bounded, as in attention_prompt.cu.
 //
 // Measured on one B200, 256 sequences of 64 query and 8 KV heads of 128 values
-// in bf16 that share 32768 positions and have up to 1023 of their own: 360 us,
+// in bf16 that share 32768 positions and have up to 1023 of their own: 354 us,
 // of which this pass takes 257 (1.07 PFLOP/s; matrix products alone would take
-// 165, exponentials 119), the own pass 85 to 113 and the join 16.  The shared
+// 165, exponentials 119), the own pass 105 and the join 16.  The shared
 // pass took 276 with two issuing threads and 296 with tiles of 64 positions.
-// Three groups of 48 sequences, 32 heads, fp32 outputs: 80 us.  8 sequences of
+// Three groups of 48 sequences, 32 heads, fp32 outputs: 74 us.  8 sequences of
 // 8 heads that share 1024 positions: 12 us.  Giving this pass fewer SMs, so
 // that the own pass runs beside it, gained 5 % in the first of these and lost
 // up to 25 % elsewhere: a few SMs do not read the own positions fast enough.

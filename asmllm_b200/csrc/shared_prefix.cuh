@@ -68,7 +68,7 @@ __device__ __forceinline__ int shared_base(const SharedView& v, const KvArgs& kv
 #endif  // __CUDACC__
 
 // The pass over the positions that are not shared (attention_own.cu): results into `v`, none joined.
-constexpr int kOwnRanges = 1280;  // at most, one a warp
+constexpr int kOwnRanges = 2400;  // at most, one a warp
 size_t own_slots_floats(int n_heads, int n_kv, int head_dim);
 cudaError_t launch_attention_own(const PagedArgs& a, const KvArgs& kv, const SharedView& v, cudaStream_t stream);
 
