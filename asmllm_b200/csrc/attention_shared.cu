@@ -298,24 +298,41 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       // ---------------- loader ----------------
       const int pages = kKeys / box_rows, my_page = lane / kHalves, half = lane % kHalves;
       const uint32_t box_bytes = (uint32_t)box_rows * 128u;
-      int c = 0;
+      int c = 0, grp = -1, from = -1;  // from: the sequence whose table is read, -1: none of the group has the positions
       bool ok = true;
       while (ok && w.at < w.end) {
         const Segment x = segment_of(w);
-        // page of this lane's box in tile j of the segment; n_pages reads as zeros
-        auto lookup = [&](int j) -> int {
+        // page of this lane's box in tile j of the segment: as sequence s has it, and for the copy (n_pages: zeros)
+        auto number = [&](int j, int s) -> int {
+          const int p = (x.t0 + j) * kKeys + my_page * box_rows;
+          if (my_page >= pages || j >= x.n || p >= w.shared || s < 0) return 0;
+          return __ldcg(kv.table + (long long)s * kv.table_stride + (p >> kv.page_shift));
+        };
+        auto box = [&](int j, int page) -> int {
           const int p = (x.t0 + j) * kKeys + my_page * box_rows;
           if (my_page >= pages || j >= x.n) return -1;
-          if (p >= w.shared) return kv.n_pages;
-          const int page = __ldcg(kv.table + (long long)w.b * kv.table_stride + (p >> kv.page_shift));
+          if (p >= w.shared || from < 0) return kv.n_pages;
           if ((unsigned)page < (unsigned)kv.n_pages) return page;
           atomicOr(err, kErrDecodeRange);
           return kv.n_pages;
         };
-        int page = lookup(0);
+        int page;
+        if (w.grp == grp) {
+          page = number(0, from);
+        } else {  // the group's first sequence that is as long, most often its first
+          grp = w.grp;
+          page = number(0, w.b);
+          const int members = w.rows / g;
+          from = -1;
+          for (int i = 0; i < members && from < 0; i += 32) {
+            const unsigned hit = __ballot_sync(kFull, i + lane < members && __ldcg(kv.len + w.b + i + lane) >= w.shared);
+            if (hit) from = w.b + i + __ffs(hit) - 1;
+          }
+          if (from != w.b) page = number(0, from);
+        }
         for (int j = 0; j < x.n && ok; ++j) {
-          const int cur = page;
-          page = lookup(j + 1);
+          const int cur = box(j, page);
+          page = number(j + 1, from);
           const int row = ((x.t0 + j) * kKeys + my_page * box_rows) & (kv.page_size - 1);
           for (int y = 0; y < 2; ++y, ++c) {
             const int st = c % S;

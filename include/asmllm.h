@@ -805,7 +805,7 @@ ASMLLM_API int asm_attention_paged_q8_async(const void* q, int32_t q_dtype, int6
 /* asm_attention_paged_async where sequences cu_group[i] .. cu_group[i+1] - 1
  * have their first shared_len[i] positions in common (rounded down to whole
  * pages: their tables begin with the same pages, and those of the first of
- * them are read, once for the group).  Sequences in no group, and those with
+ * them that holds as many are read, once for the group).  Sequences in no group, and those with
  * fewer positions than their group shares, have their own positions alone;
  * lengths count all positions.  The weights over shared positions are those
  * of asm_attention_prompt_async (one rounding for a 16-bit output, two 16-bit

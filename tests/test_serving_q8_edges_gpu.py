@@ -155,3 +155,29 @@ def test_logits_rows_more_than_2_31_apart(cuda, B, V):
     ops.rows_adjust(x, tokens=tokens, n_prompt=ints(torch, *[10] * B), repetition=1.5 * ones, frequency=0.5 * ones,
                     presence=0.25 * ones, out=x)
     check_adjust(torch, x, want, size)
+
+
+def test_shared_groups_that_begin_with_padding(cuda):
+    """Slots without a sequence, and short ones, before those that hold the prefix: their tables are not read for it."""
+    torch = cuda
+    nh, nkv, hd, page = 8, 2, 128, 16
+    k, v = (rand(torch, 40, page, nkv, hd, dt=torch.float16, seed=s) for s in (2, 3))
+    for empty in (1, 31, 32, 40, 70):
+        B = empty + 3
+        table = torch.full((B + 2, 6), -7, dtype=torch.int32)
+        table[empty:B, :4] = torch.tensor([30, 4, 17, 9])
+        table[empty:B, 4] = torch.tensor([5, 6, 7])
+        table[0, 0] = 39
+        table[B:, :2] = torch.tensor([[1, 2], [3, 8]])
+        lens = [9] + [0] * (empty - 1) + [64, 70, 80, 20, 32]  # the last two: a group whose prefix neither holds
+        table = table.cuda()
+        q = rand(torch, B + 2, nh, hd, dt=torch.float16, seed=4)
+        for odt in (torch.float16, torch.float32):
+            got = ops.attention_shared(q, k, v, table, ints(torch, *lens), ints(torch, 0, B, B + 2), ints(torch, 64, 48),
+                                       out_dtype=odt)
+            assert ops.device_error() == 0
+            dense = [[t[table[s].clamp_min(0).long()].flatten(0, 1)[:lens[s]] for s in range(B + 2)] for t in (k, v)]
+            some = [0, *range(empty, B + 2)]
+            assert (got[1:empty] == 0).all()
+            check_shared(torch, got[some], q[some], [dense[0][s] for s in some], [dense[1][s] for s in some], hd ** -0.5,
+                         torch.float16)
