@@ -38,7 +38,9 @@ namespace asmllm {
 namespace {
 
 constexpr int kSmall = 16;  // positions per tile
-constexpr int kLeast = 2;   // tiles of a warp, where there are few
+// Tiles of a warp at least, where there are few: a part costs the join more than the second tile its warp (100 sequences of
+// one KV head, 512 positions of their own: 31.7 us, 34.2 with one tile; 8 sequences of 64: 16 us with 4 tiles, 12 with 2).
+constexpr int kLeast = 2;
 constexpr float kLazy = 5.0f, kPShift = 9.0f;  // weights 2^kPShift exp(s - m) stay below 2^15
 
 template <int HD, int ROWS>
@@ -83,7 +85,7 @@ __global__ void __launch_bounds__(LayoutOwn<HD, ROWS>::kThreads, 2)
 attention_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                      const PagedArgs a, const KvArgs kv, const SharedView v, int zs, unsigned* __restrict__ err) {
   using L = LayoutOwn<HD, ROWS>;
-  constexpr int kWarps = L::kWarps, kThreads = L::kThreads, S = L::kStages, N = ROWS / 8, kHalves = HD / 64;
+  constexpr int kThreads = L::kThreads, S = L::kStages, N = ROWS / 8, kHalves = HD / 64;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ long long s_part[kThreads + 1];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -122,69 +124,13 @@ attention_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     __stcg(at + 1, x.group);
   };
 
-  // ---- the warps' ranges: all tiles, a contiguous share of the sequences per thread ----
   Steps w;
-  {
-    const int per = (kv.batch + kThreads - 1) / kThreads, q0 = min(kv.batch, tid * per), q1 = min(kv.batch, q0 + per);
-    long long mine = 0;
-    for (int s = q0; s < q1; ++s) {
-      const int nt = load(s, &w, blockIdx.x == 0);
-      mine += nt;
-      if (nt == 0 && s % gridDim.x == blockIdx.x)
-        for (int u = 0; u < units; ++u) leave(w, u, 0, 0, 0);
-    }
-    mine *= units;
-    long long x = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(kFull, x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 31) s_part[warp] = x;  // the warps' sums, then every thread's first tile
-    __syncthreads();
-    long long before = 0, total = 0;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      const long long y = s_part[i];
-      before += i < warp ? y : 0;
-      total += y;
-    }
-    __syncthreads();
-    s_part[tid] = before + x - mine;
-    if (tid == 0) s_part[kThreads] = total;
-    __syncthreads();
-  }
-  const long long total = s_part[kThreads];
-  // A range has kLeast tiles, but for the shortest: a part costs the join more than the second tile its warp (100
-  // sequences of one KV head, 512 positions of their own: 31.7 us, 34.2 with one tile; 8 sequences of 64: 16 us with 4
-  // tiles, 12 with 2).
-  const int count = (int)min((long long)gridDim.x * kWarps, (total + kLeast - 1) / kLeast);
-  // neighbouring ranges lie in different CTAs: few units spread over all SMs
-  const int index = warp * gridDim.x + blockIdx.x;
-  const Deal deal(total, max(1, count));
-  const long long begin = index < count ? deal.start(index) : 0, end = index < count ? deal.start(index + 1) : 0;
-  if (begin < end) {
-    // the last thread whose sequences begin at or before the range (those behind it with the same number have none)
-    int lo = 0;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      const unsigned hit = __ballot_sync(kFull, s_part[32 * i + lane] <= begin);
-      if (hit) lo = 32 * i + 31 - __clz(hit);
-    }
-    const int per = (kv.batch + kThreads - 1) / kThreads;
-    long long x = s_part[lo];
-    for (int s = lo * per;; ++s) {
-      const long long t = (long long)load(s, &w, false) * units;
-      if (begin < x + t) break;
-      x += t;
-    }
-    const long long into = begin - x;
-    w.u = (int)(into / w.nt);
-    w.first = x + (long long)w.u * w.nt;
-    w.t = (int)(begin - w.first);
-    w.at = begin;
-    w.end = end;
-
+  Deal deal(0, 1);
+  const int index = deal_warps<kThreads>(kv.batch, units, kLeast, s_part, load, [&](const Steps& x) {
+    for (int u = 0; u < units; ++u) leave(x, u, 0, 0, 0);
+  }, &w, &deal);
+  if (index >= 0) {
+    const long long begin = w.at;
     auto next_unit = [&](Steps& x) {
       x.first += x.nt;
       x.t = 0;

@@ -2,9 +2,10 @@
 // deal out their work, and the join of units that lie in several CTAs.
 //
 // A unit is one (sequence, KV head, up to 16 of its query heads); its
-// positions are tiles of kTile.  The tiles of all units in a row are cut into
-// one equal range per CTA; a range covers whole units and at most two parts
-// of units.  Lengths live on the device, so each CTA sums them itself.
+// positions are tiles.  The tiles of all units in a row are cut into one equal
+// range per CTA (attention_paged.cu, tiles of kTile) or per warp; a range
+// covers whole units and at most two parts of units.  Lengths live on the
+// device, so each CTA sums them itself.
 #pragma once
 
 #include "matvec.cuh"
@@ -61,6 +62,71 @@ struct Walk {
   long long first;         // number of the unit's first tile
   long long at, end;       // tiles [at, end) are left
 };
+
+// The range of this warp where every warp of the grid has its own (W: a walk; its n and nt are load's).  load(s, w, report)
+// gives a sequence's tiles, empty(w) is called in one thread of one CTA for a sequence without any.  Neighbouring ranges
+// lie in different CTAs, so that few units spread over all SMs; a range has `least` tiles, but for the shortest, and there
+// are at most kMostParts for each unit, whose parts the join reads (one unit of 131071 positions: 33 us, 58 with one for
+// each of 2368 warps).
+// s_part: THREADS + 1 values in shared memory.  Gives the range's number, or -1 where the warp has none.
+constexpr int kMostParts = 1024;
+template <int THREADS, class W, class Load, class Empty>
+__device__ __forceinline__ int deal_warps(int batch, int units, int least, long long* s_part, Load load, Empty empty, W* w,
+                                          Deal* deal) {
+  constexpr int kWarps = THREADS / 32;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int per = (batch + THREADS - 1) / THREADS, q0 = min(batch, tid * per), q1 = min(batch, q0 + per);
+  long long mine = 0;
+  for (int s = q0; s < q1; ++s) {
+    const int nt = load(s, w, blockIdx.x == 0);
+    mine += nt;
+    if (nt == 0 && s % gridDim.x == blockIdx.x) empty(*w);
+  }
+  mine *= units;
+  long long x = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(kFull, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) s_part[warp] = x;  // the warps' sums, then every thread's first tile
+  __syncthreads();
+  long long before = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    const long long y = s_part[i];
+    before += i < warp ? y : 0;
+    total += y;
+  }
+  __syncthreads();
+  s_part[tid] = before + x - mine;
+  __syncthreads();
+  const int count = (int)min(min((long long)gridDim.x * kWarps, (long long)batch * units * kMostParts), (total + least - 1) / least);
+  const int index = warp * gridDim.x + blockIdx.x;
+  *deal = Deal(total, max(1, count));
+  const long long begin = index < count ? deal->start(index) : 0, end = index < count ? deal->start(index + 1) : 0;
+  if (begin >= end) return -1;
+  // the last thread whose sequences begin at or before the range (those behind it with the same number have none)
+  int lo = 0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    const unsigned hit = __ballot_sync(kFull, s_part[32 * i + lane] <= begin);
+    if (hit) lo = 32 * i + 31 - __clz(hit);
+  }
+  x = s_part[lo];
+  for (int s = lo * per;; ++s) {
+    const long long t = (long long)load(s, w, false) * units;
+    if (begin < x + t) break;
+    x += t;
+  }
+  const long long into = begin - x;
+  w->u = (int)(into / w->nt);
+  w->first = x + (long long)w->u * w->nt;
+  w->t = (int)(begin - w->first);
+  w->at = begin;
+  w->end = end;
+  return index;
+}
 
 // The range of this CTA (of THREADS threads): false when it has none.  len(s, report) is a sequence's positions
 // (report: bad lengths are to be reported), empty(s) is called in one thread of one CTA for a sequence without any.
