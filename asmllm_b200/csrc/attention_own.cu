@@ -23,7 +23,7 @@
 // as many warps as registers allow, with one tile each: 128 sequences of up to
 // 8000 positions of their own take 398 us, 444 with half the warps and three
 // tiles each, 409 with two.  48 sequences of 32 KV heads with 1 to 299 behind
-// three prefixes: 74 us a call, 95 with a CTA's warps on one ring of tiles of 64
+// three prefixes: 71 us a call, 95 with a CTA's warps on one ring of tiles of 64
 // and their join.
 #include <type_traits>
 

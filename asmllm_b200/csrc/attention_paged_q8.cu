@@ -559,13 +559,13 @@ __device__ __forceinline__ float2 join_parts(const Parts& parts, int4 f, long lo
   return make_float2(m, l);
 }
 
-// ROWS rows a CTA: 1, by 16 warps, or 8, by a warp each, or one after the other by all where one of them has more than kFew
+// ROWS rows a CTA of W warps: 1, by all of them, or 8, by a warp each, or one after the other by all where one of them has more than kFew
 // parts.
 constexpr int kFew = 64;
-template <class O, int HD, int ROWS>
-__global__ void __launch_bounds__(ROWS == 8 ? 256 : 512, ROWS == 8 ? 4 : 1) attention_paged_q8_join_kernel(const PagedArgs a, const Parts parts, int batch, int n_kv,
+template <class O, int HD, int ROWS, int W>
+__global__ void __launch_bounds__(W * 32, ROWS == 8 ? 4 : W == 16 ? 1 : 3) attention_paged_q8_join_kernel(const PagedArgs a, const Parts parts, int batch, int n_kv,
                                                                       int zs) {
-  constexpr int E = HD / 32, W = ROWS == 8 ? 8 : 16;  // warps
+  constexpr int E = HD / 32;
   __shared__ float s_o[W][HD];
   __shared__ float2 s_ml[W];
   pdl_trigger();
@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(ROWS == 8 ? 256 : 512, ROWS == 8 ? 4 : 1) atte
   for (int i = 0; i < ROWS; ++i) {
     const long long row = row0 + i;
     if (row >= rows) return;
-    const float2 ml = join_parts<HD, 4>(parts, found(row), row, (int)(row % a.n_heads) % g % 16, R, warp, W, o);
+    const float2 ml = join_parts<HD, 64 / W / (ROWS == 8 ? 2 : 1)>(parts, found(row), row, (int)(row % a.n_heads) % g % 16, R, warp, W, o);
 #pragma unroll
     for (int q = 0; q < E; ++q) s_o[warp][lane * E + q] = o[q];
     if (lane == 0) s_ml[warp] = ml;
@@ -693,17 +693,21 @@ cudaError_t launch_typed(const PagedArgs& a, const KvQ8Args& c, cudaStream_t str
   e = cudaLaunchKernelEx(&cfg, kernel, kmap, vmap, a, c, parts, zs, err);
   if (e != cudaSuccess) return e;
   // Few rows may have many parts each.  (2048 rows of 9 parts: a block a row makes the call 24.7 us, not 21; 640 rows of 37
-  // parts: eight rows a block 24, not 16.6.)
+  // parts: eight rows a block 24, not 15; 8 rows of 1024 parts: blocks of 8 warps 39, not 33.)
   const long long rows = (long long)kv.batch * a.n_heads;
-  cfg.blockDim = dim3(512);
   cfg.dynamicSmemBytes = 0;
-  if (rows <= 1184) {
+  if (rows <= sms) {
+    cfg.blockDim = dim3(512);
     cfg.gridDim = dim3((unsigned)rows);
-    return cudaLaunchKernelEx(&cfg, attention_paged_q8_join_kernel<O, HD, 1>, a, parts, kv.batch, kv.n_kv, zs);
+    return cudaLaunchKernelEx(&cfg, attention_paged_q8_join_kernel<O, HD, 1, 16>, a, parts, kv.batch, kv.n_kv, zs);
   }
   cfg.blockDim = dim3(256);
+  if (rows <= 1184) {
+    cfg.gridDim = dim3((unsigned)rows);
+    return cudaLaunchKernelEx(&cfg, attention_paged_q8_join_kernel<O, HD, 1, 8>, a, parts, kv.batch, kv.n_kv, zs);
+  }
   cfg.gridDim = dim3((unsigned)((rows + 7) / 8));
-  return cudaLaunchKernelEx(&cfg, attention_paged_q8_join_kernel<O, HD, 8>, a, parts, kv.batch, kv.n_kv, zs);
+  return cudaLaunchKernelEx(&cfg, attention_paged_q8_join_kernel<O, HD, 8, 8>, a, parts, kv.batch, kv.n_kv, zs);
 }
 
 template <class T, class O, int HD>

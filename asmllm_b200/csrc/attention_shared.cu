@@ -35,11 +35,11 @@
 // Every wait is bounded, as in attention_prompt.cu.
 //
 // Measured on one B200, 256 sequences of 64 query and 8 KV heads of 128 values
-// in bf16 that share 32768 positions and have up to 1023 of their own: 354 us,
+// in bf16 that share 32768 positions and have up to 1023 of their own: 350 us,
 // of which this pass takes 257 (1.07 PFLOP/s; matrix products alone would take
 // 165, exponentials 119), the own pass 105 and the join 16.  The shared
 // pass took 276 with two issuing threads and 296 with tiles of 64 positions.
-// Three groups of 48 sequences, 32 heads, fp32 outputs: 74 us.  8 sequences of
+// Three groups of 48 sequences, 32 heads, fp32 outputs: 71 us.  8 sequences of
 // 8 heads that share 1024 positions: 12 us.  Giving this pass fewer SMs, so
 // that the own pass runs beside it, gained 5 % in the first of these and lost
 // up to 25 % elsewhere: a few SMs do not read the own positions fast enough.
@@ -716,119 +716,153 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
-// Joins a row's parts: those of its own positions, then of the shared ones.  WARPS warps a row (8 or 1) take
-// every WARPS-th part.  The own pass has left what leads to them (its parts, the group), so that three loads follow one
-// another: that, the shared pass's parts, and all parts' outputs, maxima and sums at once.
-template <class O, int HD, int WARPS>
-__global__ void __launch_bounds__(256) attention_shared_join_kernel(const PagedArgs a, const KvArgs kv,
-                                                                    const SharedView v, const SharedParts parts,
-                                                                    int zs) {
-  constexpr int E = HD / 32, U = WARPS == 8 ? 8 : 4;  // parts at a time
-  __shared__ float s_o[8][HD];
-  __shared__ float2 s_ml[8];
+// Joins a row's parts: those of its own positions, then of the shared ones.  The own pass has left what leads to them (its
+// parts, the group), so that three loads follow one another: that, the shared pass's parts, and all parts' outputs, maxima
+// and sums at once.  ROWS rows a CTA: 1, by all warps, or 8, by a warp each, or one after the other by all where one of them
+// has more than kFew parts.
+constexpr int kFew = 64;
+template <class O, int HD, int ROWS>
+__global__ void __launch_bounds__(256, ROWS == 8 ? 4 : 3)
+attention_shared_join_kernel(const PagedArgs a, const KvArgs kv, const SharedView v, const SharedParts parts, int zs) {
+  constexpr int E = HD / 32, W = 8, U = ROWS == 8 ? 4 : 8;  // values of a lane, warps, parts at a time
+  __shared__ float s_o[W][HD];
+  __shared__ float2 s_ml[W];
   pdl_trigger();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = a.n_heads / kv.n_kv;
-  const long long row = WARPS == 8 ? blockIdx.x : (long long)blockIdx.x * 8 + warp;
-  if (row >= (long long)kv.batch * a.n_heads) return;
-  const int s = (int)(row / a.n_heads), h = (int)(row % a.n_heads), j = h / g, in = h % g, R = g <= 8 ? 8 : 16;
-  const int4* at_own = reinterpret_cast<const int4*>(v.own_found + ((long long)s * kv.n_kv + j) * zs + in / 16);
-  const int4 own = __ldcg(at_own), grp = __ldcg(at_own + 1);  // parts, range, slot; group (-1: none), its sequences
-  int4 f = make_int4(0, 0, 0, 0);
-  int local = 0, streams = 1;
-  if (grp.x >= 0) {
-    const int rr = (s - grp.y) * g + in, blk = rr / kUnit;
-    local = rr % kUnit;
-    streams = min(kUnit, (grp.z - grp.y) * g - blk * kUnit) > kRows ? 1 : 2;
-    f = __ldcg(reinterpret_cast<const int4*>(parts.found + (long long)j * parts.found_stride +
-                                             unit_index(grp.y * g, grp.x, blk)));
-  }
-  const int total = own.x + f.x * streams;
-  // where part p's output row is, and its (maximum, sum)
-  auto find = [&](int p, const float** o) -> const float2* {
-    if (p < own.x) {
-      if (own.x == 1) {
-        *o = v.own_o + row * HD;
-        return v.own_ml + row;
-      }
-      const float* slot = v.own_slots + (size_t)(p ? 2 * (own.y + p) : own.z) * (size_t)slot_floats(R, HD);
-      *o = slot + (in % 16) * HD;
-      return reinterpret_cast<const float2*>(slot + R * HD) + in % 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = a.n_heads / kv.n_kv, R = g <= 8 ? 8 : 16;
+  const long long rows = (long long)kv.batch * a.n_heads, row0 = (long long)blockIdx.x * ROWS;
+  struct Way {  // to a row's parts
+    int4 own, shared;  // parts, range, slot
+    int in, local, streams, total;
+    long long row;
+  };
+  auto way = [&](long long row) -> Way {
+    Way x = {};
+    x.row = row;
+    if (row >= rows) return x;
+    const int s = (int)(row / a.n_heads), h = (int)(row % a.n_heads), j = h / g;
+    x.in = h % g;
+    const int4* at_own = reinterpret_cast<const int4*>(v.own_found + ((long long)s * kv.n_kv + j) * zs + x.in / 16);
+    x.own = __ldcg(at_own);
+    const int4 grp = __ldcg(at_own + 1);  // group (-1: none), its sequences
+    x.streams = 1;
+    if (grp.x >= 0) {
+      const int rr = (s - grp.y) * g + x.in, blk = rr / kUnit;
+      x.local = rr % kUnit;
+      x.streams = min(kUnit, (grp.z - grp.y) * g - blk * kUnit) > kRows ? 1 : 2;
+      x.shared = __ldcg(reinterpret_cast<const int4*>(parts.found + (long long)j * parts.found_stride +
+                                                      unit_index(grp.y * g, grp.x, blk)));
     }
-    p -= own.x;
-    const int i = streams == 2 ? p & 1 : 0, k = streams == 2 ? p >> 1 : p;
-    if (f.x == 1) {
-      const long long at = row + (long long)i * kv.batch * a.n_heads;
+    x.total = x.own.x + x.shared.x * x.streams;
+    return x;
+  };
+  // where part p's output row is, and its (maximum, sum)
+  auto find = [&](const Way& x, int p, const float** o) -> const float2* {
+    if (p < x.own.x) {
+      if (x.own.x == 1) {
+        *o = v.own_o + x.row * HD;
+        return v.own_ml + x.row;
+      }
+      const float* slot = v.own_slots + (size_t)(p ? 2 * (x.own.y + p) : x.own.z) * (size_t)slot_floats(R, HD);
+      *o = slot + (x.in % 16) * HD;
+      return reinterpret_cast<const float2*>(slot + R * HD) + x.in % 16;
+    }
+    p -= x.own.x;
+    const int i = x.streams == 2 ? p & 1 : 0, k = x.streams == 2 ? p >> 1 : p;
+    if (x.shared.x == 1) {
+      const long long at = x.row + (long long)i * kv.batch * a.n_heads;
       *o = parts.o + at * HD;
       return parts.ml + at;
     }
-    const float* slot = parts.slots + (size_t)(k ? 2 * (f.y + k) : f.z) * part_floats<HD>();
-    *o = slot + (size_t)(local + i * kRows) * HD;
-    return reinterpret_cast<const float2*>(slot + (size_t)kUnit * HD) + local + i * kRows;
+    const float* slot = parts.slots + (size_t)(k ? 2 * (x.shared.y + k) : x.shared.z) * part_floats<HD>();
+    *o = slot + (size_t)(x.local + i * kRows) * HD;
+    return reinterpret_cast<const float2*>(slot + (size_t)kUnit * HD) + x.local + i * kRows;
   };
-  float m = -INFINITY, l = 0.0f, o[E] = {};
-  for (int p0 = WARPS == 8 ? warp : 0; p0 < total; p0 += U * WARPS) {
-    float x[U][E];
-    float2 ml[U];
+  float m, l, o[E];
+  auto join = [&](const Way& w, int first, int warps) {  // every `warps`-th part
+    m = -INFINITY;
+    l = 0.0f;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int p = p0 + u * WARPS;
-      ml[u] = make_float2(-INFINITY, 0.0f);
-      if (p < total) {
-        const float* src;
-        ml[u] = __ldcg(find(p, &src));
+    for (int z = 0; z < E; ++z) o[z] = 0.0f;
+    for (int p0 = first; p0 < w.total; p0 += U * warps) {
+      float x[U][E];
+      float2 ml[U];
 #pragma unroll
-        for (int z = 0; z < E; z += 2) {
-          const float2 y = __ldcg(reinterpret_cast<const float2*>(src + lane * E + z));
-          x[u][z] = y.x;
-          x[u][z + 1] = y.y;
+      for (int u = 0; u < U; ++u) {
+        const int p = p0 + u * warps;
+        ml[u] = make_float2(-INFINITY, 0.0f);
+        if (p < w.total) {
+          const float* src;
+          ml[u] = __ldcg(find(w, p, &src));
+#pragma unroll
+          for (int z = 0; z < E; z += 2) {
+            const float2 y = __ldcg(reinterpret_cast<const float2*>(src + lane * E + z));
+            x[u][z] = y.x;
+            x[u][z + 1] = y.y;
+          }
         }
       }
+      float mn = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
+      const float mz = mn == -INFINITY ? 0.0f : mn, f0 = ex2(m - mz);
+      m = mn;
+      l *= f0;
+#pragma unroll
+      for (int z = 0; z < E; ++z) o[z] *= f0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (ml[u].x == -INFINITY && ml[u].y == 0.0f) continue;  // nothing in it: there may be no output either
+        const float by = ex2(ml[u].x - mz);
+        l = fmaf(by, ml[u].y, l);
+#pragma unroll
+        for (int z = 0; z < E; ++z) o[z] = fmaf(by, x[u][z], o[z]);
+      }
     }
-    float mn = m;
+  };
+  auto put = [&](long long row) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    O* out = static_cast<O*>(a.out) + row * HD + lane * E;
 #pragma unroll
-    for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
-    const float mz = mn == -INFINITY ? 0.0f : mn, f0 = ex2(m - mz);
-    m = mn;
-    l *= f0;
-#pragma unroll
-    for (int z = 0; z < E; ++z) o[z] *= f0;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (ml[u].x == -INFINITY && ml[u].y == 0.0f) continue;  // nothing in it: there may be no output either
-      const float w = ex2(ml[u].x - mz);
-      l = fmaf(w, ml[u].y, l);
-#pragma unroll
-      for (int z = 0; z < E; ++z) o[z] = fmaf(w, x[u][z], o[z]);
+    for (int z = 0; z < E; z += 2) {
+      if constexpr (sizeof(O) == 4) *reinterpret_cast<float2*>(out + z) = make_float2(o[z] * inv, o[z + 1] * inv);
+      else *reinterpret_cast<uint32_t*>(out + z) = pack16<O>(o[z] * inv, o[z + 1] * inv);
+    }
+  };
+  if constexpr (ROWS == 8) {
+    const Way w = way(row0 + warp);
+    if (!__syncthreads_or(w.total > kFew)) {
+      if (w.row >= rows) return;
+      join(w, 0, 1);
+      put(w.row);
+      return;
     }
   }
-  if constexpr (WARPS == 8) {
+  for (int i = 0; i < ROWS; ++i) {
+    if (row0 + i >= rows) return;
+    join(way(row0 + i), warp, W);
 #pragma unroll
     for (int q = 0; q < E; ++q) s_o[warp][lane * E + q] = o[q];
     if (lane == 0) s_ml[warp] = make_float2(m, l);
     __syncthreads();
-    if (warp) return;
-    m = -INFINITY;
+    if (warp == 0) {
+      m = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < 8; ++x) m = fmaxf(m, s_ml[x].x);
-    const float mz = m == -INFINITY ? 0.0f : m;
-    l = 0.0f;
+      for (int x = 0; x < W; ++x) m = fmaxf(m, s_ml[x].x);
+      const float mz = m == -INFINITY ? 0.0f : m;
+      l = 0.0f;
 #pragma unroll
-    for (int q = 0; q < E; ++q) o[q] = 0.0f;
+      for (int q = 0; q < E; ++q) o[q] = 0.0f;
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const float fx = ex2(s_ml[x].x - mz);
-      l = fmaf(fx, s_ml[x].y, l);
+      for (int x = 0; x < W; ++x) {
+        const float fx = ex2(s_ml[x].x - mz);
+        l = fmaf(fx, s_ml[x].y, l);
 #pragma unroll
-      for (int q = 0; q < E; ++q) o[q] = fmaf(fx, s_o[x][lane * E + q], o[q]);
+        for (int q = 0; q < E; ++q) o[q] = fmaf(fx, s_o[x][lane * E + q], o[q]);
+      }
+      put(row0 + i);
     }
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  O* out = static_cast<O*>(a.out) + row * HD + lane * E;
-#pragma unroll
-  for (int z = 0; z < E; z += 2) {
-    if constexpr (sizeof(O) == 4) *reinterpret_cast<float2*>(out + z) = make_float2(o[z] * inv, o[z + 1] * inv);
-    else *reinterpret_cast<uint32_t*>(out + z) = pack16<O>(o[z] * inv, o[z + 1] * inv);
+    __syncthreads();
   }
 }
 
@@ -908,16 +942,17 @@ cudaError_t launch_typed(const SharedArgs& sa, const KvArgs& kv, cudaStream_t st
   cfg.numAttrs = g_opt_pdl.load() ? 1 : 0;
   e = cudaLaunchKernelEx(&cfg, kernel, kmap, vmap, a, kv, v, parts, box_rows, err);
   if (e != cudaSuccess || (e = launch_attention_own(a, kv, v, stream)) != cudaSuccess) return e;
-  // Few rows may have many parts (a warp would read them one after the other): a block a row.
+  // Few rows may have many parts each.  (1536 rows: a block a row makes the call 74 us, not 71; 800 rows of 46 parts: eight
+  // rows a block 38, not 31.)
   const long long rows = (long long)kv.batch * a.n_heads;
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
-  if (rows <= 2048) {
+  if (rows <= 1184) {
     cfg.gridDim = dim3((unsigned)rows);
-    return cudaLaunchKernelEx(&cfg, attention_shared_join_kernel<O, HD, 8>, a, kv, v, parts, sp.zs);
+    return cudaLaunchKernelEx(&cfg, attention_shared_join_kernel<O, HD, 1>, a, kv, v, parts, sp.zs);
   }
   cfg.gridDim = dim3((unsigned)((rows + 7) / 8));
-  return cudaLaunchKernelEx(&cfg, attention_shared_join_kernel<O, HD, 1>, a, kv, v, parts, sp.zs);
+  return cudaLaunchKernelEx(&cfg, attention_shared_join_kernel<O, HD, 8>, a, kv, v, parts, sp.zs);
 }
 
 template <class T>
