@@ -87,7 +87,7 @@ attention_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   using L = LayoutOwn<HD, ROWS>;
   constexpr int kThreads = L::kThreads, S = L::kStages, N = ROWS / 8, kHalves = HD / 64;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  __shared__ long long s_part[kThreads + 1];
+  __shared__ long long s_part[kThreads];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff) + warp * S;
@@ -328,7 +328,7 @@ attention_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
           if (r == 0)
             __stcg(whole ? v.own_ml + at : reinterpret_cast<float2*>(part + ROWS * HD) + row, make_float2(m[n][e] - kPShift, sum));
         }
-      if (t0 == 0 && lane == 0) leave(w, w.u, whole ? 1 : deal.cta_of(w.first + w.nt - 1) - index + 1, index, slot);
+      if (t0 == 0 && lane == 0) leave(w, w.u, whole ? 1 : deal.range_of(w.first + w.nt - 1) - index + 1, index, slot);
       w.at += t1 - t0;
       if (w.at < w.end) next_unit(w);
     }

@@ -42,7 +42,6 @@
 
 #include "matvec.cuh"
 #include "mma16.cuh"
-#include "paged_deal.cuh"
 #include "pipeline.cuh"
 #include "serving.cuh"
 #include "tensor_map.cuh"
@@ -51,10 +50,22 @@ namespace asmllm {
 
 namespace {
 
+constexpr int kTile = 64;   // positions per tile, 16 per consumer warp
 constexpr int kWarps = 4;   // consumer warps
 constexpr int kStages = 3;
 constexpr int kMaxCtas = 320;
 constexpr int kThreads = (kWarps + 1) * 32;
+
+// Parts of split units: [kMaxCtas][2] slots of ROWS x (HD outputs, maximum,
+// sum), then one Split per CTA: the split unit that begins in its range.
+struct Split {
+  int unit;   // -1: none
+  int parts;  // CTAs c .. c + parts - 1 hold one each
+  int slot;   // slot of the first part (the others are in slot 2 c)
+  int pad;
+};
+
+__host__ __device__ constexpr size_t slot_floats(int rows, int hd) { return (size_t)rows * hd + 2 * rows; }
 
 template <int ROWS, int HD>
 struct Layout {
@@ -68,6 +79,28 @@ struct Layout {
   // A unit's query rows pass through the join buffer: padded by 16 bytes for ldmatrix.
   static constexpr int kQRow = HD * 2 + 16;
   static_assert(16 * kQRow <= 2 * 8 * kJoinRow * 4, "the query rows fit the join buffer");
+};
+
+__device__ __forceinline__ int tiles_of(int n) { return (n + kTile - 1) / kTile; }
+
+// `total` tiles over `ctas` ranges: the first `extra` have one more than the others.
+struct Deal {
+  long long each;
+  int extra;
+  __device__ __forceinline__ Deal(long long total, int ctas) {
+    if (total < (1ll << 32)) {  // a 64-bit division costs hundreds of cycles
+      each = (unsigned)total / (unsigned)ctas;
+      extra = (int)((unsigned)total % (unsigned)ctas);
+    } else {
+      each = total / ctas;
+      extra = (int)(total % ctas);
+    }
+  }
+  __device__ __forceinline__ long long start(int c) const { return c * each + min(c, extra); }
+  __device__ __forceinline__ int cta_of(long long x) const {  // whose range holds tile x
+    const long long big = (each + 1) * extra;
+    return x < big ? (int)(x / (each + 1)) : extra + (int)((x - big) / each);
+  }
 };
 
 // o += p v in fp32 for D times 8 values from 8 d0 on and the first n of a warp's 16 positions of a tile (values at sv,
@@ -99,6 +132,13 @@ __device__ __forceinline__ void add_values(float (&o)[HD / 8][4], int d0, const 
   }
 }
 
+// A CTA's walk over its tiles: sequence, unit of the sequence, tile.
+struct Walk {
+  int s, u, t, n, nt;      // n positions, nt tiles of sequence s
+  long long first;         // number of the unit's first tile
+  long long at, end;       // tiles [at, end) are left
+};
+
 template <class T, class O, int HD, int ROWS>
 __global__ void __launch_bounds__(kThreads, 2)
 attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -128,28 +168,93 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
   pdl_trigger();
   pdl_wait();
 
-  auto len = [&](int s, bool report) -> int {
+  // Sum of all tiles and the sequence this range begins in: a contiguous share of the sequences per thread.
+  const int per = (kv.batch + kThreads - 1) / kThreads, q0 = min(kv.batch, tid * per), q1 = min(kv.batch, q0 + per);
+  long long mine = 0;
+  int held = 0;  // positions of the thread's first sequence
+  for (int s = q0; s < q1; ++s) {
     bool clipped;
     const int n = kv_length(kv, s, &clipped);
-    if (clipped && report) atomicOr(err, kErrDecodeRange);
-    return n;
-  };
-  auto none = [&](int s) {  // a sequence without positions: zeros, written by one CTA
-    O* out = static_cast<O*>(a.out) + (long long)s * a.n_heads * HD;
-    const float z[8] = {};
-    for (int i = 0; i < a.n_heads * HD; i += 8) store8(out + i, z);
-  };
-  Walk w;
-  Deal deal(0, 1);
-  const bool any = deal_range<kThreads>(kv.batch, units, s_part, s_first, s_start, len, none, &w, &deal);
+    if (s == q0) held = n;
+    if (clipped && cta == 0) atomicOr(err, kErrDecodeRange);
+    mine += tiles_of(n);
+    // a sequence without positions: zeros, written by one CTA
+    if (n == 0 && s % gridDim.x == cta) {
+      O* out = static_cast<O*>(a.out) + (long long)s * a.n_heads * HD;
+      const float z[8] = {};
+      for (int i = 0; i < a.n_heads * HD; i += 8) store8(out + i, z);
+    }
+  }
+  mine *= units;
+  s_part[tid] = mine;
+  __syncthreads();
+  if (warp == 0) {
+    long long run = 0;
+    for (int b = 0; b < kThreads; b += 32) {
+      const long long v = s_part[b + lane];
+      long long x = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(kFull, x, o);
+        if (lane >= o) x += y;
+      }
+      s_part[b + lane] = run + x - v;  // exclusive
+      run += __shfl_sync(kFull, x, 31);
+    }
+    if (lane == 0) s_first[1] = run;
+  }
+  __syncthreads();
+  const long long total = s_first[1];
+  const int ctas = (int)min((long long)gridDim.x, total);  // every range in use holds a tile; the other CTAs have none
+  const Deal deal(total, max(1, ctas));
+  const long long begin = cta < ctas ? deal.start(cta) : 0, end = cta < ctas ? deal.start(cta + 1) : 0;
+  if (begin < end && s_part[tid] <= begin && begin < s_part[tid] + mine) {
+    long long x = s_part[tid];
+    for (int s = q0; s < q1; ++s) {
+      bool clipped;
+      const int n = s == q0 ? held : kv_length(kv, s, &clipped);
+      const long long w = (long long)tiles_of(n) * units;
+      if (begin < x + w) {
+        s_start[0] = s;
+        s_start[1] = n;
+        s_first[0] = x;
+        break;
+      }
+      x += w;
+    }
+  }
+  __syncthreads();
 
   float* slots = static_cast<float*>(a.workspace);
   Split* splits = reinterpret_cast<Split*>(slots + (size_t)kMaxCtas * 2 * slot_floats(ROWS, HD));
-  if (!any) {
+  if (begin >= end) {
     if (tid == 0) splits[cta].unit = -1;
     return;
   }
-  const long long begin = w.at;
+  Walk w;
+  w.s = s_start[0];
+  bool clipped;
+  w.n = s_start[1];
+  w.nt = tiles_of(w.n);
+  const long long into = begin - s_first[0];
+  w.u = into < (1ll << 32) ? (int)((unsigned)into / (unsigned)w.nt) : (int)(into / w.nt);
+  w.first = s_first[0] + (long long)w.u * w.nt;
+  w.t = (int)(begin - w.first);
+  w.at = begin;
+  w.end = end;
+  // the next unit, of this sequence or the next one that holds positions
+  auto next_unit = [&](Walk& x) {
+    x.first += x.nt;
+    x.t = 0;
+    if (++x.u == units) {
+      x.u = 0;
+      do {
+        ++x.s;
+        x.n = kv_length(kv, x.s, &clipped);
+      } while (x.n == 0);
+      x.nt = tiles_of(x.n);
+    }
+  };
 
   if (warp == kWarps) {
     // ---------------- producer ----------------
@@ -175,7 +280,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
       const Walk cur = w;
       const int cur_page = page;
       if (++w.at < w.end) {  // the next tile's page number is on its way while this one waits for its stage
-        if (++w.t == w.nt) next_unit(w, units, len);
+        if (++w.t == w.nt) next_unit(w);
         page = lookup(w);
       }
       if (i >= kStages) ok = mbar_wait_bounded(smem_u32(empty + st), ((i / kStages) - 1) & 1);
@@ -437,7 +542,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
     }
     w.at += t1 - t0;
     next = w.at < w.end;
-    if (next) next_unit(w, units, len);
+    if (next) next_unit(w);
   }
   if (tid == 0) {
     Split x;
@@ -447,6 +552,113 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_co
     x.pad = 0;
     __stcg(reinterpret_cast<int4*>(splits + cta), *reinterpret_cast<int4*>(&x));
   }
+}
+
+// Joins the parts of the split unit that began in CTA blockIdx.x.  Up to four parts (ordinary batches have two
+// or three): block y = 0 takes all rows, a warp each.  More (a few long sequences): block y takes row y, its
+// warps every eighth part, all maxima and sums first so that the outputs are independent loads.
+template <class O, int HD, int ROWS>
+__global__ void __launch_bounds__(256) attention_paged_join_kernel(const PagedArgs a, int n_kv, int zs) {
+  constexpr int E = HD / 32;
+  __shared__ float s_o[8][HD], s_f[kMaxCtas], s_red[8], s_sum[8];
+  pdl_trigger();
+  pdl_wait();
+  const float* slots = static_cast<const float*>(a.workspace);
+  const Split* splits = reinterpret_cast<const Split*>(slots + (size_t)kMaxCtas * 2 * slot_floats(ROWS, HD));
+  const int c = blockIdx.x, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int4 raw = __ldcg(reinterpret_cast<const int4*>(splits + c));
+  if (raw.x < 0) return;
+  const int g = a.n_heads / n_kv, units = n_kv * zs, s = raw.x / units, u = raw.x % units, n = raw.y;
+  const int h0 = (u % zs) * 16;
+  auto part = [&](int p) { return slots + (size_t)(p ? 2 * (c + p) : raw.z) * slot_floats(ROWS, HD); };
+  if (n <= 4) {
+    if (blockIdx.y) return;
+    for (int r = warp; r < min(16, g - h0); r += 8) {
+      const float pm = lane < n ? __ldcg(part(lane) + ROWS * HD + r) : -INFINITY;
+      const float pl = lane < n ? __ldcg(part(lane) + ROWS * HD + ROWS + r) : 0.0f;
+      float m = pm;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+      const float f = ex2(pm - (m == -INFINITY ? 0.0f : m)), sum = warp_sum(f * pl);
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      float o[E] = {};
+#pragma unroll 4
+      for (int p = 0; p < n; ++p) {
+        const float w = __shfl_sync(kFull, f, p);
+        const float* b = part(p) + r * HD + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(b + e));
+          o[e] = fmaf(w, v.x, o[e]);
+          o[e + 1] = fmaf(w, v.y, o[e + 1]);
+        }
+      }
+      O* out = static_cast<O*>(a.out) + ((long long)s * a.n_heads + (u / zs) * g + h0 + r) * HD + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        if constexpr (sizeof(O) == 4) *reinterpret_cast<float2*>(out + e) = make_float2(o[e] * inv, o[e + 1] * inv);
+        else *reinterpret_cast<uint32_t*>(out + e) = pack16<O>(o[e] * inv, o[e + 1] * inv);
+      }
+    }
+    return;
+  }
+  if (row >= g - h0) return;
+  // weights 2^(m_p - max) of the parts (at most two a thread) and the weighted sum
+  float pm[2] = {-INFINITY, -INFINITY}, pl[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int p = threadIdx.x + 256 * e;
+    if (p < n) {
+      pm[e] = __ldcg(part(p) + ROWS * HD + row);
+      pl[e] = __ldcg(part(p) + ROWS * HD + ROWS + row);
+    }
+  }
+  float m = fmaxf(pm[0], pm[1]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+  if (lane == 0) s_red[warp] = m;
+  __syncthreads();
+  m = s_red[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = fmaxf(m, s_red[i]);
+  const float mz = m == -INFINITY ? 0.0f : m;
+  float sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int p = threadIdx.x + 256 * e;
+    if (p < n) {
+      const float f = ex2(pm[e] - mz);
+      s_f[p] = f;
+      sum += f * pl[e];
+    }
+  }
+  sum = warp_sum(sum);
+  if (lane == 0) s_sum[warp] = sum;
+  __syncthreads();
+  float o[E] = {};
+#pragma unroll 8
+  for (int p = warp; p < n; p += 8) {
+    const float* b = part(p) + row * HD + lane;
+    const float f = s_f[p];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = fmaf(f, __ldcg(b + 32 * e), o[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) s_o[warp][lane + 32 * e] = o[e];
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d >= HD) return;
+  float v = 0.0f;
+  sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v += s_o[i][d];
+    sum += s_sum[i];
+  }
+  v *= sum == 0.0f ? 0.0f : 1.0f / sum;
+  O* out = static_cast<O*>(a.out) + ((long long)s * a.n_heads + (u / zs) * g + h0 + row) * HD;
+  if constexpr (sizeof(O) == 4) out[d] = v;
+  else reinterpret_cast<unsigned short*>(out)[d] = (unsigned short)pack16<O>(v, 0.0f);
 }
 
 template <class T, class O, int HD, int ROWS>
@@ -478,7 +690,7 @@ cudaError_t launch_typed(const PagedArgs& a, const KvArgs& kv, cudaStream_t stre
   cfg.gridDim = dim3((unsigned)ctas, (unsigned)(g < 16 ? g : 16));
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<O, HD, ROWS, kMaxCtas>, a, kv.n_kv, zs);
+  return cudaLaunchKernelEx(&cfg, attention_paged_join_kernel<O, HD, ROWS>, a, kv.n_kv, zs);
 }
 
 template <class T, class O, int HD>

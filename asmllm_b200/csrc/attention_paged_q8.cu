@@ -122,7 +122,7 @@ attention_paged_q8_kernel(const __grid_constant__ CUtensorMap kmap, const __grid
   constexpr int B = HD / 32, S = L::kStages, N = ROWS / 8;  // blocks of a position, tiles under way, groups of 8 heads
   const KvArgs& kv = c.kv;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  __shared__ long long s_part[L::kThreads + 1];
+  __shared__ long long s_part[L::kThreads];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff) + warp * S;
@@ -502,7 +502,7 @@ attention_paged_q8_kernel(const __grid_constant__ CUtensorMap kmap, const __grid
           __stcg(whole ? parts.ml + at : reinterpret_cast<float2*>(part + ROWS * HD) + row, make_float2(m[n][e] - kPShift, sum));
       }
     }
-    if (t0 == 0 && lane == 0) leave(w, w.u, whole ? 1 : deal.cta_of(w.first + w.nt - 1) - index + 1, index, slot);
+    if (t0 == 0 && lane == 0) leave(w, w.u, whole ? 1 : deal.range_of(w.first + w.nt - 1) - index + 1, index, slot);
     w.at += t1 - t0;
     if (w.at < w.end) next_unit(w);
   }

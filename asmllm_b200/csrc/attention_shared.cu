@@ -479,7 +479,7 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
         int n = 1;
         if (!x.whole) {
           const int ctas = (int)min((long long)gridDim.x, *s_total);
-          n = Deal(*s_total, ctas).cta_of(w.first + w.nt - 1) - (int)blockIdx.x + 1;
+          n = Deal(*s_total, ctas).range_of(w.first + w.nt - 1) - (int)blockIdx.x + 1;
         }
         __stcg(reinterpret_cast<int4*>(parts.found + (long long)x.head * parts.found_stride +
                                        unit_index(w.b * g, w.grp, x.blk)),
