@@ -12,7 +12,9 @@
 // to 2^-34 of the largest weight times its block's largest scale): d is held
 // relative to a power of two, the largest d of its block that a warp has met,
 // and the block's output is rescaled when that rises, as it is when the
-// maximum does.  bf16 queries are scaled by a power
+// maximum does.  A tile with scales below 2^-14 of that, which would lose bits
+// in fp16, is added up by itself, in three passes (the code for it costs the
+// others 1 to 2 %, a call of 32 sequences 1 us: registers).  bf16 queries are scaled by a power
 // of two per row into fp16's range, where their 8 bits are exact (those below
 // 2^-31 of the row's largest round).
 //
@@ -107,6 +109,18 @@ __device__ __forceinline__ void first_product(float (&c)[4], uint32_t a0, uint32
 
 __device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
 __device__ __forceinline__ uint32_t as_word(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+
+// hi + lo = weights p = h + l of positions c2, c2 + 1 ([0]) and 8 behind times their scales d0, d1: the product's rounding is
+// in lo.
+__device__ __forceinline__ void weighted(const uint32_t (&h)[2], const uint32_t (&l)[2], __half2 d0, __half2 d1,
+                                         uint32_t (&hi)[2], uint32_t (&lo)[2]) {
+  const __half2 x0 = as_half2(h[0]), x1 = as_half2(h[1]);
+  const __half2 h0 = __hmul2(x0, d0), h1 = __hmul2(x1, d1);
+  hi[0] = as_word(h0);
+  hi[1] = as_word(h1);
+  lo[0] = as_word(__hfma2(as_half2(l[0]), d0, __hfma2(x0, d0, __hneg2(h0))));
+  lo[1] = as_word(__hfma2(as_half2(l[1]), d1, __hfma2(x1, d1, __hneg2(h1))));
+}
 
 struct Steps {  // a warp's walk over its tiles
   int s, n, nt, u, t;
@@ -400,72 +414,121 @@ attention_paged_q8_kernel(const __grid_constant__ CUtensorMap kmap, const __grid
             for (int b = 0; b < B / 2; ++b) vs[k][b] = 0u;
           }
       }
-      bool risen = false;
+      // One word of the tile's scales a lane: has one risen to twice its block's power of two (infinities and NaN are
+      // above it), or is one, other than zero, so far below that fp16 would lose bits of it relative to that?
+      bool apart = false;
+      {
+        const int word = B == 4 ? lane : lane & 15;
+        unsigned y = *reinterpret_cast<const uint32_t*>(sc + L::kScales + 4 * word) & 0x7FFF7FFFu;
+        y = word / (B / 2) < left ? y : 0u;
+        auto unit = [&]() { return B == 4 && (lane & 1) ? top[B / 2 - 1] : top[0]; };
+        auto far_below = [&]() {
+          const unsigned least = __vmaxu2(unit(), 0x38013801u) - 0x38013801u;
+          return __vminu2(__vsub2(y, 0x00010001u), least) != least;
+        };
+        const unsigned most = unit() | 0x03FF03FFu;
+        if (__any_sync(kFull, __vmaxu2(y, most) != most || far_below())) {
 #pragma unroll
-      for (int b = 0; b < B / 2; ++b) {  // below twice its power of two (a sign, infinities and NaN are above)
-        const unsigned big = __vmaxu2(__vmaxu2(vs[0][b], vs[1][b]), __vmaxu2(vs[2][b], vs[3][b]));
-        risen |= __vmaxu2(big, top[b] | 0x03FF03FFu) != (top[b] | 0x03FF03FFu);
+          for (int b = 0; b < B; ++b) {
+            const int sh = 16 * (b & 1);
+            unsigned big = 0u;  // the largest finite one
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const unsigned z = vs[k][b >> 1] >> sh & 0x7FFFu;
+              big = z < 0x7C00u ? max(big, z) : big;
+            }
+            big = max(big, __shfl_xor_sync(kFull, big, 1));
+            big = max(big, __shfl_xor_sync(kFull, big, 2)) & 0x7C00u;
+            const unsigned was = top[b >> 1] >> sh & 0x7C00u;
+            if (big <= was) continue;
+            const unsigned one_over = big == 0x7800u ? 0x0200u : 0x7800u - big;
+            top[b >> 1] = (top[b >> 1] & ~(0xFFFFu << sh)) | big << sh;
+            inv[b >> 1] = (inv[b >> 1] & ~(0xFFFFu << sh)) | one_over << sh;
+            const float f = __uint_as_float((127u << 23) - ((big - was) << 13));
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+              for (int x = 2 * b; x < 2 * b + 2; ++x)
+#pragma unroll
+                for (int z = 0; z < 4; ++z) o[n][x][z] *= f;
+          }
+          apart = __any_sync(kFull, far_below());
+        }
       }
-      if (__any_sync(kFull, risen)) {
+      const uint32_t at = sk + L::kCodes + value_at;
+      if (!apart) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int b = 0; b < B / 2; ++b) vs[k][b] = as_word(__hmul2(as_half2(vs[k][b]), as_half2(inv[b])));
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+          uint32_t f[4], c[8];
+          ldsm4_t(f, at ^ (32u * b));
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            codes_of(f[k], c[2 * k], c[2 * k + 1]);
+          }
+          const __half2 d0 = as_half2(__byte_perm(vs[0][b >> 1], vs[1][b >> 1], b & 1 ? 0x7632 : 0x5410));
+          const __half2 d1 = as_half2(__byte_perm(vs[2][b >> 1], vs[3][b >> 1], b & 1 ? 0x7632 : 0x5410));
+#pragma unroll
+          for (int n = 0; n < N; ++n) {
+            uint32_t hi[2], lo[2];
+            weighted(ph[n], pl[n], d0, d1, hi, lo);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              // The tensor core truncates its sums: 256 tiles in a row come out 5e-6 too small, which an fp32 output shows.
+              // There each tile starts from zero and is added with rounding.
+              if constexpr (EXACT) {
+                float y[4];
+                first_product(y, c[4 * x], c[4 * x + 1], c[4 * x + 2], c[4 * x + 3], hi[0], hi[1]);
+                product(y, c[4 * x], c[4 * x + 1], c[4 * x + 2], c[4 * x + 3], lo[0], lo[1]);
+#pragma unroll
+                for (int z = 0; z < 4; ++z) o[n][2 * b + x][z] += y[z];
+              } else {
+                product(o[n][2 * b + x], c[4 * x], c[4 * x + 1], c[4 * x + 2], c[4 * x + 3], hi[0], hi[1]);
+                product(o[n][2 * b + x], c[4 * x], c[4 * x + 1], c[4 * x + 2], c[4 * x + 3], lo[0], lo[1]);
+              }
+            }
+          }
+        }
+      } else {
+        // Scales 2^-14 and more below their block's power of two: three passes, with those from 2^-14 of it on, those from
+        // 2^-28 on, 2^14 times as large, and the rest (2^-24 beside 2^15), 2^28 times; the products come back in fp32.
 #pragma unroll
         for (int b = 0; b < B; ++b) {
           const int sh = 16 * (b & 1);
-          unsigned big = 0u;  // the largest finite one
+          const unsigned unit = top[b >> 1] >> sh & 0x7C00u, over = inv[b >> 1] >> sh & 0xFFFFu;
+          uint32_t f[4], c[8];
+          ldsm4_t(f, at ^ (32u * b));
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const unsigned y = vs[k][b >> 1] >> sh & 0x7FFFu;
-            big = y < 0x7C00u ? max(big, y) : big;
-          }
-          big = max(big, __shfl_xor_sync(kFull, big, 1));
-          big = max(big, __shfl_xor_sync(kFull, big, 2)) & 0x7C00u;
-          const unsigned was = top[b >> 1] >> sh & 0x7C00u;
-          if (big <= was) continue;
-          const unsigned one_over = big == 0x7800u ? 0x0200u : 0x7800u - big;
-          top[b >> 1] = (top[b >> 1] & ~(0xFFFFu << sh)) | big << sh;
-          inv[b >> 1] = (inv[b >> 1] & ~(0xFFFFu << sh)) | one_over << sh;
-          const float f = __uint_as_float((127u << 23) - ((big - was) << 13));
+          for (int k = 0; k < 4; ++k) codes_of(f[k], c[2 * k], c[2 * k + 1]);
+#pragma unroll 1
+          for (unsigned by = 0u; by < 0xA800u; by += 0x3800u) {
+            const float back = __uint_as_float((127u << 23) - (by << 13));
+            const unsigned above = by ? max(unit, by) - by : 0x8000u, least = max(unit, by + 0x3800u) - (by + 0x3800u);
+            __half d[4];
 #pragma unroll
-          for (int n = 0; n < N; ++n)
+            for (int k = 0; k < 4; ++k) {
+              const int p = c2 + (k & 1) + 8 * (k >> 1);
+              const unsigned y = p < left ? *reinterpret_cast<const unsigned short*>(sc + L::kScales + 2 * (p * B + b)) : 0u;
+              const unsigned z = y & 0x7FFFu;
+              const __half y14 = __hmul(__ushort_as_half((unsigned short)y), __ushort_as_half(by ? 0x7400 : 0x3C00));
+              const __half y28 = __hmul(y14, __ushort_as_half(by > 0x3800u ? 0x7400 : 0x3C00));
+              d[k] = z >= least && z < above ? __hmul(y28, __ushort_as_half((unsigned short)over)) : __ushort_as_half(0);
+            }
 #pragma unroll
-            for (int x = 2 * b; x < 2 * b + 2; ++x)
+            for (int n = 0; n < N; ++n) {
+              uint32_t hi[2], lo[2];
+              weighted(ph[n], pl[n], __halves2half2(d[0], d[1]), __halves2half2(d[2], d[3]), hi, lo);
 #pragma unroll
-              for (int z = 0; z < 4; ++z) o[n][x][z] *= f;
-        }
-      }
+              for (int x = 0; x < 2; ++x) {
+                float y[4];
+                first_product(y, c[4 * x], c[4 * x + 1], c[4 * x + 2], c[4 * x + 3], hi[0], hi[1]);
+                product(y, c[4 * x], c[4 * x + 1], c[4 * x + 2], c[4 * x + 3], lo[0], lo[1]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int b = 0; b < B / 2; ++b) vs[k][b] = as_word(__hmul2(as_half2(vs[k][b]), as_half2(inv[b])));
-      const uint32_t at = sk + L::kCodes + value_at;
-#pragma unroll
-      for (int b = 0; b < B; ++b) {
-        uint32_t f[4], c[8];
-        ldsm4_t(f, at ^ (32u * b));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          codes_of(f[k], c[2 * k], c[2 * k + 1]);
-        }
-        const __half2 d0 = as_half2(__byte_perm(vs[0][b >> 1], vs[1][b >> 1], b & 1 ? 0x7632 : 0x5410));
-        const __half2 d1 = as_half2(__byte_perm(vs[2][b >> 1], vs[3][b >> 1], b & 1 ? 0x7632 : 0x5410));
-#pragma unroll
-        for (int n = 0; n < N; ++n) {  // p d = hi + lo: the product's rounding is in lo
-          const __half2 x0 = as_half2(ph[n][0]), x1 = as_half2(ph[n][1]);
-          const __half2 h0 = __hmul2(x0, d0), h1 = __hmul2(x1, d1);
-          const __half2 l0 = __hfma2(as_half2(pl[n][0]), d0, __hfma2(x0, d0, __hneg2(h0)));
-          const __half2 l1 = __hfma2(as_half2(pl[n][1]), d1, __hfma2(x1, d1, __hneg2(h1)));
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            // The tensor core truncates its sums: 256 tiles in a row come out 5e-6 too small, which an fp32 output shows.
-            // There each tile starts from zero and is added with rounding.
-            if constexpr (EXACT) {
-              float y[4];
-              first_product(y, c[4 * x], c[4 * x + 1], c[4 * x + 2], c[4 * x + 3], as_word(h0), as_word(h1));
-              product(y, c[4 * x], c[4 * x + 1], c[4 * x + 2], c[4 * x + 3], as_word(l0), as_word(l1));
-#pragma unroll
-              for (int z = 0; z < 4; ++z) o[n][2 * b + x][z] += y[z];
-            } else {
-              product(o[n][2 * b + x], c[4 * x], c[4 * x + 1], c[4 * x + 2], c[4 * x + 3], as_word(h0), as_word(h1));
-              product(o[n][2 * b + x], c[4 * x], c[4 * x + 1], c[4 * x + 2], c[4 * x + 3], as_word(l0), as_word(l1));
+                for (int z = 0; z < 4; ++z) o[n][2 * b + x][z] = fmaf(y[z], back, o[n][2 * b + x][z]);
+              }
             }
           }
         }
