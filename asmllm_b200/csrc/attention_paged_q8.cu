@@ -317,6 +317,10 @@ attention_paged_q8_kernel(const __grid_constant__ CUtensorMap kmap, const __grid
           } else {
             d[k][0] = *reinterpret_cast<const uint32_t*>(at);
           }
+          // An infinite scale stands for infinities of both signs and 0 times infinity: NaN, where its product with the
+          // block's sum could be a score of minus infinity, which has no weight.
+#pragma unroll
+          for (int b = 0; b < B / 2; ++b) d[k][b] = as_word(__hfma2(as_half2(d[k][b]), as_half2(0u), as_half2(d[k][b])));
         }
         const uint32_t at = sk + key_at;
 #pragma unroll

@@ -794,7 +794,8 @@ ASMLLM_API int asm_cache_read_q8_async(const asm_kv_q8_t* kv, const int32_t* cu,
  * fp32; the weights times a block's scale are two 16-bit parts (2^-22 of a
  * weight, down to 2^-34 of the largest weight times the largest finite scale
  * of the values).  A block of values whose scale is not finite gives NaN in its
- * 32 outputs, whatever the weight is above zero. */
+ * 32 outputs, whatever the weight is above zero; a block of keys, in all
+ * outputs of the heads that read it. */
 ASMLLM_API int64_t asm_attention_paged_q8_workspace(int32_t batch, int32_t n_heads, int32_t n_kv_heads,
                                                     int32_t head_dim);
 ASMLLM_API int asm_attention_paged_q8_async(const void* q, int32_t q_dtype, int64_t q_row_stride, int64_t q_head_stride,

@@ -76,3 +76,37 @@ def test_scales_over_the_whole_range_beside_a_large_one(cuda, nh, nkv, hd):
     w = torch.ones(n, dtype=torch.float64, device="cuda")
     w[at] = math.exp(-60.0)
     check_flat(torch, got[0], values(vc, vd), w / w.sum(), 2.0 ** 15)
+
+
+@pytest.mark.parametrize("nh,nkv,hd,dtype", [(8, 2, 128, "float16"), (40, 2, 64, "bfloat16")])
+@pytest.mark.parametrize("code", [-1, 0, 1])
+def test_key_scale_that_is_not_finite_shows_in_its_rows_alone(cuda, nh, nkv, hd, dtype, code):
+    """A key block with an infinite scale holds infinities of its codes' signs and NaN: no score, whatever their sum's sign."""
+    torch = cuda
+    n = 40
+    for bad in (float("inf"), float("nan")):
+        for at, block in ((0, 0), (20, 1), (n - 1, hd // 32 - 1)):
+            dense = [list(random8(torch, n, nkv, hd, s)) for s in range(3)]
+            q = rand(torch, 3, nh, hd, dt=getattr(torch, dtype), seed=5).abs()
+            lens = ints(torch, n, n, n)
+            args = make_pages8(torch, dense, 16)
+            want = ops.attention_paged_q8(q, *args, lens, out_dtype=torch.float32)
+            dense[1][0][at, 1, 32 * block:32 * block + 32] = code
+            dense[1][1][at, 1, block] = bad
+            got = ops.attention_paged_q8(q, *make_pages8(torch, dense, 16), lens, out_dtype=torch.float32)
+            hit = torch.zeros_like(got, dtype=torch.bool)
+            hit[1, nh // 2:] = True
+            assert torch.isnan(got[hit]).all()
+            assert torch.equal(got[~hit], want[~hit])
+
+
+def test_key_beyond_a_scale_of_16_bits_is_nan(cuda):
+    """Finite keys past what an fp16 scale holds (about 8.3e6): their row has no answer, instead of one without them."""
+    torch = cuda
+    x = rand(torch, 1, 3 * 64, dt=torch.float32, seed=3).abs()
+    x[0, 64:96] = -1e7
+    rope = torch.zeros(32, 32, 2, device="cuda")
+    rope[..., 0] = 1.0
+    k, v, ks, vs, table = make_pages8(torch, [random8(torch, 20, 1, 64, 0)], 16)
+    q = ops.rope_append_q8(x, rope, ints(torch, 20), table, k, v, ks, vs, 1)
+    assert torch.isnan(ops.attention_paged_q8(q, k, v, ks, vs, table, ints(torch, 20))).all()
