@@ -140,6 +140,10 @@ attention_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         }
       }
     };
+    auto advance = [&](int n) {
+      w.at += n;
+      if (w.at < w.end) next_unit(w);
+    };
     // ---- copies, S tiles ahead; the page number of the next one is on its way ----
     Steps ahead = w;
     int asked = 0, page = 0;
@@ -329,9 +333,9 @@ attention_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             __stcg(whole ? v.own_ml + at : reinterpret_cast<float2*>(part + ROWS * HD) + row, make_float2(m[n][e] - kPShift, sum));
         }
       if (t0 == 0 && lane == 0) leave(w, w.u, whole ? 1 : deal.range_of(w.first + w.nt - 1) - index + 1, index, slot);
-      w.at += t1 - t0;
-      if (w.at < w.end) next_unit(w);
+      advance(t1 - t0);
     }
+    if (!ok) abandon(w, [&]() { if (lane == 0) leave(w, w.u, 0, 0, 0); }, advance);
     // every issued copy lands before the CTA may end (bounded)
     for (int i = done; i < asked; ++i) mbar_wait_bounded(smem_u32(full + i % S), (i / S) & 1);
   }

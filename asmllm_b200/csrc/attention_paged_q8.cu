@@ -36,6 +36,7 @@
 // fp32 outputs: 161.  With a CTA's four warps on one ring of tiles of 64, fed by
 // a fifth, and their join: 232, 22, 10.1, 32 and 202; with positions as the
 // right side, padded to 8 rows of heads as the left, 341 in the first.
+#include "found.cuh"
 #include "matvec.cuh"
 #include "mma16.cuh"
 #include "paged_deal.cuh"
@@ -73,7 +74,7 @@ struct LayoutQ8 {
 struct Parts {
   float* o;       // [batch][n_heads][head_dim]
   float2* ml;     // [batch][n_heads]: (maximum in units of log2, sum); o 2^maximum is the sum of exp(s) v
-  int4* found;    // [batch][units]: parts (0: no position, 1: whole), range of the first, its slot
+  int4* found;    // [batch][units]: a Found
   float* slots;
 };
 
@@ -180,6 +181,10 @@ attention_paged_q8_kernel(const __grid_constant__ CUtensorMap kmap, const __grid
       while (load(x.s + 1, &x, false) == 0) {
       }
     }
+  };
+  auto advance = [&](int n) {
+    w.at += n;
+    if (w.at < w.end) next_unit(w);
   };
 
   // ---- copies, S tiles ahead, by four lanes: codes of keys and values, their scales; the page number of the next one is on
@@ -570,9 +575,9 @@ attention_paged_q8_kernel(const __grid_constant__ CUtensorMap kmap, const __grid
       }
     }
     if (t0 == 0 && lane == 0) leave(w, w.u, whole ? 1 : deal.range_of(w.first + w.nt - 1) - index + 1, index, slot);
-    w.at += t1 - t0;
-    if (w.at < w.end) next_unit(w);
+    advance(t1 - t0);
   }
+  if (!ok) abandon(w, [&]() { if (lane == 0) leave(w, w.u, 0, 0, 0); }, advance);
   // every issued copy lands before the CTA may end (bounded)
   for (int i = done; i < asked; ++i) mbar_wait_bounded(smem_u32(full + i % S), (i / S) & 1);
 }
@@ -642,7 +647,9 @@ __global__ void __launch_bounds__(W * 32, ROWS == 8 ? 4 : W == 16 ? 1 : 3) atten
   auto found = [&](long long row) -> int4 {
     if (row >= rows) return make_int4(0, 0, 0, 0);
     const int s = (int)(row / a.n_heads), h = (int)(row % a.n_heads);
-    return __ldcg(parts.found + ((long long)s * n_kv + h / g) * zs + h % g / 16);
+    int4 f = __ldcg(parts.found + ((long long)s * n_kv + h / g) * zs + h % g / 16);
+    f.x = parts_of({f.x, f.y, f.z, 0}, kRanges);
+    return f;
   };
   auto put = [&](long long row, float l, const float (&o)[E]) {
     const float by = l == 0.0f ? 0.0f : 1.0f / l;

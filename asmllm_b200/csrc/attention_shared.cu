@@ -469,21 +469,23 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
     const long long begin = w.at;
     uint32_t ns = 0, no = 0;  // parities
     bool ok = true;
+    auto leave = [&](const Segment& x, int n, int slot) {  // where the unit's results are
+      __stcg(reinterpret_cast<int4*>(parts.found + (long long)x.head * parts.found_stride + unit_index(w.b * g, w.grp, x.blk)),
+             make_int4(n, (int)blockIdx.x, slot, 0));
+    };
     while (ok && w.at < w.end) {
       const Segment x = segment_of(w);
       const int row = lrow + (x.two ? i * kRows : 0), tiles = x.two ? x.n : (x.n + 1 - i) >> 1;
       const bool mine = row < x.rows, idle = row - lane >= x.rows;  // idle: the warp has no row
       const int rr = x.blk * kUnit + row, seq = w.b + rr / g, head = x.head * g + rr % g;
       const int slot = 2 * blockIdx.x + (w.at == begin ? 0 : 1);
-      if (x.t0 == 0 && tid == 0) {  // where the unit's results are
+      if (x.t0 == 0 && tid == 0) {
         int n = 1;
         if (!x.whole) {
           const int ctas = (int)min((long long)gridDim.x, *s_total);
           n = Deal(*s_total, ctas).range_of(w.first + w.nt - 1) - (int)blockIdx.x + 1;
         }
-        __stcg(reinterpret_cast<int4*>(parts.found + (long long)x.head * parts.found_stride +
-                                       unit_index(w.b * g, w.grp, x.blk)),
-               make_int4(n, (int)blockIdx.x, slot, 0));
+        leave(x, n, slot);
       }
       if (tiles > 0) {
         // Queries: this warp's 32 rows, a row's pieces in consecutive lanes.  What was read from the buffer before has
@@ -708,6 +710,7 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_c
       }
       advance(x.n);
     }
+    if (!ok && tid == 0) abandon(w, [&]() { leave(segment_of(w), 0, 0); }, advance);
   }
   tc_fence_before();
   __syncthreads();
@@ -745,13 +748,15 @@ attention_shared_join_kernel(const PagedArgs a, const KvArgs kv, const SharedVie
     const int4* at_own = reinterpret_cast<const int4*>(v.own_found + ((long long)s * kv.n_kv + j) * zs + x.in / 16);
     x.own = __ldcg(at_own);
     const int4 grp = __ldcg(at_own + 1);  // group (-1: none), its sequences
+    x.own.x = parts_of({x.own.x, x.own.y, x.own.z, 0}, kOwnRanges);
     x.streams = 1;
-    if (grp.x >= 0) {
+    if (in_group(grp.x, grp.y, grp.z, s, v.groups, kv.batch)) {
       const int rr = (s - grp.y) * g + x.in, blk = rr / kUnit;
       x.local = rr % kUnit;
       x.streams = min(kUnit, (grp.z - grp.y) * g - blk * kUnit) > kRows ? 1 : 2;
       x.shared = __ldcg(reinterpret_cast<const int4*>(parts.found + (long long)j * parts.found_stride +
                                                       unit_index(grp.y * g, grp.x, blk)));
+      x.shared.x = parts_of({x.shared.x, x.shared.y, x.shared.z, 0}, kMaxCtas);
     }
     x.total = x.own.x + x.shared.x * x.streams;
     return x;

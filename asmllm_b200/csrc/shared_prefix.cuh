@@ -3,17 +3,11 @@
 // over the rest (attention_own.cu) agree on.
 #pragma once
 
+#include "found.cuh"
 #include "paged_deal.cuh"
 
 namespace asmllm {
 
-// Where a unit's result is.  1 part: found by row; more: in slots.
-struct Found {
-  int parts;  // 0: no position, 1: whole, else ranges first .. first + parts - 1 hold one part each
-  int first;
-  int slot;   // slot of the first part (the others are in slot 2 r of range r)
-  int pad;
-};
 // Of a sequence's own positions, and the group whose result is to be joined with it.
 struct OwnFound {
   Found found;
