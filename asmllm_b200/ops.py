@@ -1226,8 +1226,10 @@ def rows_adjust(logits, *, tokens=None, n_tokens=None, n_prompt=None, repetition
     if bias_tokens is not None and bias is not None:
         words, n_bias, row1 = _rows2(bias_tokens, "bias_tokens", B, _I32)
         biases, m, row2 = _rows2(bias, "bias", B, _F32)
-        if m != n_bias or row1 != m or row2 != m:
+        if m != n_bias or m and (row1 != m or row2 != m):
             raise ValueError(f"bias_tokens {tuple(bias_tokens.shape)} and bias {tuple(bias.shape)}: expected equal, dense ones")
+        if m == 0:
+            words = biases = 0
     elif not (bias_tokens is bias is None):
         raise ValueError("pass bias_tokens and bias together")
     if allowed is not None:
