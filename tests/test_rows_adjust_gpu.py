@@ -28,3 +28,37 @@ def test_a_step_where_no_row_has_a_bias_or_a_token(cuda, B, V):
     check_adjust(torch, got, want, size)
     with pytest.raises(ValueError, match="equal, dense"):
         ops.rows_adjust(x, bias_tokens=words, bias=torch.zeros(B, 1, device="cuda"))
+
+
+def test_rows_with_padding_are_looked_at_together(cuda):
+    """What lies between the rows of out may hold an input; and a call's time does not grow with the rows there."""
+    torch = cuda
+    B, V = 300, 1000
+    wide = torch.zeros(B, V + 32, device="cuda")
+    x = wide[:, :V]
+    x.copy_(rand(torch, B, V, dt=torch.float32, seed=1))
+    allowed = wide.view(torch.int32)[:, V:V + 32]  # in the padding of the rows it masks
+    allowed.copy_(torch.randint(-2 ** 31, 2 ** 31, (B, 32), generator=torch.Generator().manual_seed(2)).int())
+    bits = (allowed[:, :, None] >> torch.arange(32, device="cuda") & 1).flatten(1)[:, :V]
+    want = torch.where(bits == 1, x, float("-inf"))
+    assert torch.equal(ops.rows_adjust(x, allowed=allowed), want)
+    keep = allowed.clone()
+    ops.rows_adjust(x, allowed=allowed, out=x)
+    assert torch.equal(x, want) and torch.equal(allowed, keep)
+    for first in (V - 1, 1):  # one word of a row is a word of the mask
+        with pytest.raises(ops.AsmError, match="overlaps"):
+            ops.rows_adjust(x, allowed=wide.view(torch.int32)[:, first:first + 32], out=x)
+    with pytest.raises(ops.AsmError, match="overlaps"):
+        ops.rows_adjust(torch.zeros(1, V, device="cuda"), out=x[:1], tokens=wide.view(torch.int32)[:1, :4])
+
+    def host(rows, padding):
+        y = torch.zeros(rows, 64 + padding, device="cuda")[:, :64]
+        best = 1.0
+        for _ in range(20):
+            torch.cuda.synchronize()
+            begin = time.perf_counter()
+            ops.rows_adjust(y, out=y)
+            best = min(best, time.perf_counter() - begin)
+        return best
+
+    assert host(60000, 8) < 5 * host(60000, 0) + 50e-6
