@@ -843,15 +843,22 @@ def rows_sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=No
 
 _SPACE: dict = {}  # (function, sizes) -> bytes of workspace
 _cuda_empty = None
+_ready = False
 
 
 def _setup():
-    """_dtypes, and torch's quickest way to an uninitialised tensor (0.9 us, new_empty takes 2) where it has it."""
-    global _cuda_empty
+    """_dtypes, and torch's quickest way to an uninitialised tensor (0.9 us, new_empty takes 2) where it has it.
+
+    The name is not a public one: it is used where it does what is expected of it, once a process."""
+    global _cuda_empty, _ready
     _dtypes()
+    _ready = True
     try:
-        from torch._C._dynamo.guards import _empty_strided_cuda as _cuda_empty  # noqa: F811
-    except ImportError:
+        from torch._C._dynamo.guards import _empty_strided_cuda as quick
+        t = quick((2, 3), (3, 1), _I8)
+        if t.is_cuda and t.dtype is _I8 and tuple(t.shape) == (2, 3) and t.stride() == (3, 1):
+            _cuda_empty = quick
+    except Exception:  # whatever another release of torch does there: new_empty then
         pass
 
 
@@ -952,9 +959,9 @@ def rope_append_q8(qkv, rope_cs, kv_len, page_table, k_pages, v_pages, k_scales,
     Keys are rotated in fp32, and keys and values quantized in blocks of 32 as quantize_q8_0 does it, the
     scale rounded to fp16.  qkv fp32, or fp16 or bf16 (the queries' type then).  Returns the rotated queries
     [T, nh, hd] in q_dtype (qkv's type; fp16 for fp32)."""
-    if _cuda_empty is None:
-        _setup()
     device = _place(qkv, "qkv")
+    if not _ready:
+        _setup()
     kv, batch, nkv, hd = _kv_q8_view(k_pages, v_pages, k_scales, v_scales, kv_len, page_table)
     src = qkv.dtype
     if src not in _DT:
@@ -1003,9 +1010,9 @@ def cache_read_q8(k_pages, v_pages, k_scales, v_scales, page_table, kv_len, cu, 
     as it has rows (cu of the sums of kv_len reads everything, cu_q what a call has just appended).  Returns
     (k, v) [rows, nkv, hd] in dtype (fp16 unless given) or in out=(k, v); rows before a sequence's first
     position are zeros, rows at or past cu[B] are not written."""
-    if _cuda_empty is None:
-        _setup()
     device = _place(k_pages, "k_pages")
+    if not _ready:
+        _setup()
     kv, batch, nkv, hd = _kv_q8_view(k_pages, v_pages, k_scales, v_scales, kv_len, page_table)
     at = _column(cu, "cu", batch + 1, _I32)
     shape = (rows, nkv, hd)
@@ -1091,9 +1098,9 @@ def attention_paged_q8(q, k_pages, v_pages, k_scales, v_scales, page_table, kv_l
     """attention_paged over a Q8_0 cache (asm_attention_paged_q8_async): q [B, nh, hd] fp16 or bf16, the cache
     as rope_append_q8 fills it, page_table int32 [B, n], kv_len int32 [B].  out [B, nh, hd] in q's type or
     fp32.  workspace: uint8 of attention_paged_q8_workspace bytes, one per call that may overlap another."""
-    if _cuda_empty is None:
-        _setup()
     device = _place(q, "q")
+    if not _ready:
+        _setup()
     kv, batch, nkv, hd = _kv_q8_view(k_pages, v_pages, k_scales, v_scales, kv_len, page_table)
     row, head, nh, out = _decode_query(q, batch, nkv, hd, out, out_dtype, stream)
     if batch == 0:
@@ -1127,9 +1134,9 @@ def attention_shared(q, k_pages, v_pages, page_table, kv_len, cu_group, shared_l
     all positions.  A sequence in no group, or shorter than what its group shares, is on its own.  The rest is
     attention_paged's.  workspace: uint8 of attention_shared_workspace bytes, one per call that may overlap
     another."""
-    if _cuda_empty is None:
-        _setup()
     device = _place(q, "q")
+    if not _ready:
+        _setup()
     shape, st = k_pages.shape, k_pages.stride()
     if not (k_pages.dtype is v_pages.dtype is q.dtype in _H16 and len(st) == 4 and v_pages.shape == shape
             and (v_pages.stride() == st or _strides(v_pages) == _strides(k_pages)) and st[3] == 1):
@@ -1190,9 +1197,9 @@ def rows_adjust(logits, *, tokens=None, n_tokens=None, n_prompt=None, repetition
     fp32 [B, N], those of equal entries added up; words whose bit is 0 in allowed int32 [B, ceil(V / 32)] (bit
     w % 32 of w / 32) become -inf.  n_tokens, n_prompt int32 [B] (L, 0) and repetition, frequency, presence
     fp32 [B] (1, 0, 0) are optional.  Returns a new tensor, or out, which may be logits."""
-    if _cuda_empty is None:
-        _setup()
     device = _place(logits, "logits")
+    if not _ready:
+        _setup()
     dt = logits.dtype
     if dt not in _DT or logits.dim() != 2:
         raise TypeError(f"logits: expected fp32, fp16 or bf16 with 2 axes, got {dt} {tuple(logits.shape)}")

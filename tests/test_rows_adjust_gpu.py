@@ -62,3 +62,14 @@ def test_rows_with_padding_are_looked_at_together(cuda):
         return best
 
     assert host(60000, 8) < 5 * host(60000, 0) + 50e-6
+
+
+def test_calls_without_torchs_quick_allocation(cuda, monkeypatch):
+    torch = cuda
+    x = rand(torch, 2, 100, dt=torch.float32, seed=1)
+    monkeypatch.setattr(ops, "_ready", False)
+    monkeypatch.setattr(ops, "_cuda_empty", None)
+    monkeypatch.setattr(torch._C._dynamo.guards, "_empty_strided_cuda", None)
+    got = ops.rows_adjust(x)
+    assert ops._ready and ops._cuda_empty is None
+    assert torch.equal(got, x) and got.data_ptr() != x.data_ptr()
