@@ -1526,7 +1526,6 @@ ASMLLM_API int asm_rows_adjust_async(const asm_adjust_t* d, void* stream) {
   a.out_stride = d->out_stride;
   a.rows = d->rows;
   a.n = d->n;
-  a.in_place = in_place;
   a.tokens = tokens;
   a.token_stride = d->token_stride;
   a.held = d->held;

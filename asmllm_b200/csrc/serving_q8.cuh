@@ -42,7 +42,6 @@ struct AdjustArgs {
   int dtype = kDtF32;
   long long stride = 0, out_stride = 0;
   int rows = 0, n = 0;
-  bool in_place = false;  // out is logits
   const int32_t* tokens = nullptr;  // [rows] x token_stride, held tokens each; null: no penalties
   long long token_stride = 0;
   int held = 0;
