@@ -45,9 +45,10 @@ __device__ __forceinline__ uint32_t transposed8(uint32_t w) {
 
 // The range of this warp (W: a walk, whose sequence, positions and tiles load fills in).  load(s, w, report)
 // gives a sequence's tiles, empty(w) is called in one thread of one CTA for a sequence without any.  Neighbouring ranges
-// lie in different CTAs, so that few units spread over all SMs; a range has `least` tiles, but for the shortest, and there
-// are at most kMostParts for each unit, whose parts the join reads (one unit of 131071 positions: 33 us, 58 with one for
-// each of 2368 warps).
+// lie in different CTAs, so that few units spread over all SMs; a range has `least` tiles, but for the shortest, and as many
+// more as it takes to cut no unit into more than about kMostParts, which its join reads one after the other (one unit of
+// 131071 positions: 33 us, 58 with a part for each of 2368 warps; with one more sequence of a single position 33, 45 with
+// twice the parts).
 // s_part: THREADS values in shared memory.  Gives the range's number, or -1 where the warp has none.
 constexpr int kMostParts = 1024;
 template <int THREADS, class W, class Load, class Empty>
@@ -57,9 +58,11 @@ __device__ __forceinline__ int deal_warps(int batch, int units, int least, long 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int per = (batch + THREADS - 1) / THREADS, q0 = min(batch, tid * per), q1 = min(batch, q0 + per);
   long long mine = 0;
+  int longest = 0;
   for (int s = q0; s < q1; ++s) {
     const int nt = load(s, w, blockIdx.x == 0);
     mine += nt;
+    longest = max(longest, nt);
     if (nt == 0 && s % gridDim.x == blockIdx.x) empty(*w);
   }
   mine *= units;
@@ -69,7 +72,11 @@ __device__ __forceinline__ int deal_warps(int batch, int units, int least, long 
     const long long y = __shfl_up_sync(kFull, x, o);
     if (lane >= o) x += y;
   }
-  if (lane == 31) s_part[warp] = x;  // the warps' sums, then every thread's first tile
+  longest = __reduce_max_sync(kFull, longest);
+  if (lane == 31) {  // the warps' sums, then every thread's first tile
+    s_part[warp] = x;
+    s_part[kWarps + warp] = longest;
+  }
   __syncthreads();
   long long before = 0, total = 0;
 #pragma unroll
@@ -77,13 +84,19 @@ __device__ __forceinline__ int deal_warps(int batch, int units, int least, long 
     const long long y = s_part[i];
     before += i < warp ? y : 0;
     total += y;
+    longest = max(longest, (int)s_part[kWarps + i]);
   }
   __syncthreads();
   s_part[tid] = before + x - mine;
   __syncthreads();
-  const int count = (int)min(min((long long)gridDim.x * kWarps, (long long)batch * units * kMostParts), (total + least - 1) / least);
+  long long count = (total + least - 1) / least;
+  if (longest > kMostParts * least) {
+    const int n = (longest + kMostParts - 1) / kMostParts;
+    count = total < (1ll << 31) ? (long long)((unsigned)(total + n - 1) / (unsigned)n) : (total + n - 1) / n;
+  }
+  count = min((long long)gridDim.x * kWarps, count);
   const int index = warp * gridDim.x + blockIdx.x;
-  *deal = Deal(total, max(1, count));
+  *deal = Deal(total, (int)max(1ll, count));
   const long long begin = index < count ? deal->start(index) : 0, end = index < count ? deal->start(index + 1) : 0;
   if (begin >= end) return -1;
   // the last thread whose sequences begin at or before the range (those behind it with the same number have none)
