@@ -13,10 +13,10 @@
 // relative to a power of two, the largest d of its block that a warp has met,
 // and the block's output is rescaled when that rises, as it is when the
 // maximum does.  A tile with scales below 2^-14 of that, which would lose bits
-// in fp16, is added up by itself, in three passes (the code for it costs the
-// others 1 to 2 %, a call of 32 sequences 1 us: registers).  bf16 queries are scaled by a power
-// of two per row into fp16's range, where their 8 bits are exact (those below
-// 2^-31 of the row's largest round).
+// in fp16, is added up by itself, in three passes; the registers of that code
+// cost the other tiles 1 to 2 %, a call of 32 short sequences 1 us.  bf16
+// queries are scaled by a power of two per row into fp16's range, where their 8
+// bits are exact (those below 2^-31 of the row's largest round).
 //
 // 2 head_dim (1 + 1/16) bytes a position and KV head, read once.  The warps work
 // alone, as in attention_own.cu: each has an equal range of all tiles of 16
@@ -28,14 +28,16 @@
 // values within a product is free as long as the query's is the same.
 //
 // Measured on one B200, 64 sequences of 64 query and 8 KV heads of 128 values
-// in bf16 that hold up to 16384 positions: 236 us (5.1 TB/s; the copy takes
-// 184; the fp16 cache of twice the bytes 355).  Codes to fp16 and the scales are
-// most of a warp's 590 instructions for 16 positions, and 62 % of the cycles
-// issue one.  32 sequences of up to 1024: 21 us; one of 32 heads and 512
-// positions: 9.4; one of 8 heads and 131071: 33; 32 of 32 heads, up to 4096,
-// fp32 outputs: 161.  With a CTA's four warps on one ring of tiles of 64, fed by
-// a fifth, and their join: 232, 22, 10.1, 32 and 202; with positions as the
-// right side, padded to 8 rows of heads as the left, 341 in the first.
+// in bf16 that hold up to 16384 positions: 239 us (5.0 TB/s; the copy takes
+// 184; the 16-bit cache of twice the bytes 356).  Called for a second and more,
+// under the power cap, 268 (364).  571 where every tile takes three passes.
+// Codes to fp16 and the scales are most of a warp's 600 instructions for 16
+// positions, and 63 % of the cycles issue one.  32 sequences of up to 1024: 22
+// us; one of 32 heads and 512 positions: 9.5; one of 8 heads and 131071: 33; 32
+// of 32 heads, up to 4096, fp32 outputs: 165.  Before there were three passes:
+// 236, 21, 9.4, 33 and 161; with a CTA's four warps on one ring of tiles of 64,
+// fed by a fifth, and their join: 232, 22, 10.1, 32 and 202; with positions as
+// the right side, padded to 8 rows of heads as the left, 341 in the first.
 #include "found.cuh"
 #include "matvec.cuh"
 #include "mma16.cuh"

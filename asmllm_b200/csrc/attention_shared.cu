@@ -35,9 +35,13 @@
 // Every wait is bounded, as in attention_prompt.cu.
 //
 // Measured on one B200, 256 sequences of 64 query and 8 KV heads of 128 values
-// in bf16 that share 32768 positions and have up to 1023 of their own: 350 us,
-// of which this pass takes 257 (1.07 PFLOP/s; matrix products alone would take
-// 165, exponentials 119), the own pass 105 and the join 16.  The shared
+// in bf16 that share 32768 positions and have up to 1023 of their own: 350 us
+// (410 under the power cap), of which this pass takes 257 (1.07 PFLOP/s; matrix
+// products alone would take 165, exponentials 119), the own pass 105 and the
+// join 16.  With fp32 outputs 600 to 650: twice the products of the weights,
+// and every 64 positions the 128 sums of a row are added up in registers, which
+// do not hold them beside 64 scores and 64 weights (690 bytes are spilled, 300
+// for 16-bit outputs).  The shared
 // pass took 276 with two issuing threads and 296 with tiles of 64 positions.
 // Three groups of 48 sequences, 32 heads, fp32 outputs: 71 us.  8 sequences of
 // 8 heads that share 1024 positions: 12 us.  Giving this pass fewer SMs, so

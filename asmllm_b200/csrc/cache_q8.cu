@@ -13,6 +13,8 @@
 // Both are bound by HBM: every input is read and every output written once.
 // At 8192 rows of 32 heads of 128 values the append of fp32 rows takes 96 us
 // (5.7 TB/s) and the read 36 us (5.7 TB/s); for 32 single tokens 3.7 and 3.4.
+// 2048 rows of 64 + 2 x 8 heads in 16 bits, half the bytes for the same
+// arithmetic, 18.6 (4.3 TB/s: the quantizer's instructions).
 #include "matvec.cuh"
 #include "serving_q8.cuh"
 

@@ -28,7 +28,10 @@
 // applied to a copy of the logits (its scattered accesses take one cycle of an
 // SM each, three a word); 150 and more where the counting threads change the
 // words that have come by themselves.  32 rows of bf16, 1024 tokens, 300
-// biases: 15 us.  One row of 32000 words: 4 us.
+// biases: 15 us.  One row of 32000 words: 4 us.  Rows that are not aligned in
+// fours of words (a dense vocabulary of 50257) go by slices of 2048 with single
+// accesses, each of which looks at all of the row's tokens: 128 rows of 50257
+// words 32 us where 50256 take 23, of 128257 words 73 where 128256 take 45.
 #include "matvec.cuh"
 #include "serving_q8.cuh"
 
@@ -362,7 +365,10 @@ __global__ void __launch_bounds__(kBoth, 1) rows_adjust_stream_kernel(const Adju
   }
 }
 
-// Words of a batch from which on the second kernel is faster.
+// Words of a batch from which on the second kernel is the faster one, where its rows are aligned (both, the first one
+// first; fp32 and bf16, us).  1024 tokens a row: 0.5 M words 4.1 and 4.7, 4.2 and 4.1; 1 M 6.2 and 6.2, 6.2 and 5.8 (32 rows),
+// 5.3 and 5.7, 5.4 and 5.3 (8); 2 M 7.9 and 8.0, 8.0 and 7.3; 3.9 M 12.3 and 10.9, 12.3 and 9.7.  8192 tokens: 0.5 M 5.3 and
+// 6.2, 5.4 and 5.9; 1 M 7.1 and 7.4, 7.2 and 6.4 (8 rows); 2 M 10.8 and 10.5, 10.9 and 10.3.
 constexpr long long kSmallBatch = 1 << 20;
 
 template <class... Args>

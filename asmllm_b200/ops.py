@@ -1132,8 +1132,9 @@ def attention_shared(q, k_pages, v_pages, page_table, kv_len, cu_group, shared_l
     Sequences cu_group[i] .. cu_group[i + 1] - 1 (int32 [G + 1]) have their first shared_len[i] positions
     (int32 [G], rounded down to whole pages) in common: their rows of page_table begin alike, kv_len counts
     all positions.  A sequence in no group, or shorter than what its group shares, is on its own.  The rest is
-    attention_paged's.  workspace: uint8 of attention_shared_workspace bytes, one per call that may overlap
-    another."""
+    attention_paged's, but for one rounding: with 16-bit outputs the weights over shared positions are rounded once
+    to 16 bits, as attention_prompt's are (attention_paged and out_dtype=torch.float32 have two parts of them).
+    workspace: uint8 of attention_shared_workspace bytes, one per call that may overlap another."""
     device = _place(q, "q")
     if not _ready:
         _setup()

@@ -814,7 +814,9 @@ ASMLLM_API int asm_attention_paged_q8_async(const void* q, int32_t q_dtype, int6
  * among what a row attends to that is not finite gives an output that is not
  * finite.  cu_group [groups + 1] and shared_len [groups] are on the
  * device; offsets or lengths out of range set ASM_DEVERR_DECODE_RANGE (an
- * offset: the group shares nothing; a length is clipped).  workspace as for
+ * offset: the group shares nothing; a length is clipped).  Offsets that fall
+ * set it too, and what the groups that overlap there get is not defined, as it
+ * is not where tables differ.  workspace as for
  * asm_attention_paged_async (tens of MB); batch * n_heads at most 2^22. */
 ASMLLM_API int64_t asm_attention_shared_workspace(int32_t batch, int32_t groups, int32_t n_heads, int32_t n_kv_heads,
                                                   int32_t head_dim);
@@ -830,7 +832,8 @@ ASMLLM_API int asm_attention_shared_async(const void* q, int64_t q_row_stride, i
  *   3. words among bias_tokens[r]: x + the sum of their biases (in 64 bits);
  *   4. words whose bit in allowed[r] is 0 (bit w % 32 of word w / 32): -inf.
  * n at most 262144.  tokens outside [0, n) are passed over, as are bias_tokens (-1: unused).
- * n_tokens outside [0, held] is clipped and sets ASM_DEVERR_DECODE_RANGE.
+ * n_tokens outside [0, held] is clipped and sets ASM_DEVERR_DECODE_RANGE (not
+ * where held is 0: nothing is read then).
  * out may be logits itself; any other overlap with an input is refused. */
 typedef struct asm_adjust {
   const void* logits;          /* [rows] x stride, dtype ASM_DT_* */
